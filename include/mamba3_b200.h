@@ -529,6 +529,113 @@ M3B_API int m3b_scaled_add(const void* x, const void* h, float scale, void* out,
                            void* stream);
 
 /* ------------------------------------------------------------------------
+ * Gated feed-forward block (the blocks' SwiGLU, mamba3/block.py:16-26, with the scaled residual
+ * of mamba3/block.py:79-107), forward and backward, on the tensor cores:
+ *   g = x w_gate^T + b_gate, u = x w_up^T + b_up, act = silu(g) * u,
+ *   out = residual + residual_scale * (act w_down^T + b_down).
+ * x, residual, out and their gradients (rows, d_model), w_gate / w_up (d_ff, d_model), w_down
+ * (d_model, d_ff), all of `dtype`; x, residual and dout with rows *_stride elements apart, the
+ * rest contiguous; biases and residual may be null.  Sums are kept in fp32; act, and in the
+ * backward dg and du, are rounded to 16-bit `dtype` once (operands of the next product); fp32
+ * operands travel as three bf16 planes, which keeps 24 bits.
+ *
+ * saved_act (m3b_gated_ffn_act_bytes) is always written.  saved_gu (m3b_gated_ffn_gu_bytes; g and
+ * u in fp32, private layout) is written when not null; the backward needs both as the forward
+ * left them.  Backward outputs may be null where no gradient is wanted.  16-byte aligned
+ * workspace of m3b_gated_ffn_{fwd,bwd}_workspace bytes (may be 0).
+ * ------------------------------------------------------------------------ */
+typedef struct m3b_gated_ffn_args {
+  int64_t rows, x_stride, residual_stride, dout_stride;
+  int32_t d_model, d_ff, dtype;
+  float residual_scale;
+  const void* x;
+  const void* w_gate;
+  const void* w_up;
+  const void* w_down;
+  const void* b_gate;    /* (d_ff) or NULL; b_gate and b_up together */
+  const void* b_up;
+  const void* b_down;    /* (d_model) or NULL */
+  const void* residual;  /* (rows, d_model) or NULL */
+  void* saved_act;
+  void* saved_gu;
+  void* out;             /* forward */
+  const void* dout;      /* backward: */
+  void* dx;
+  void* dw_gate;
+  void* dw_up;
+  void* dw_down;
+  void* db_gate;
+  void* db_up;
+  void* db_down;
+  int* err;
+} m3b_gated_ffn_args;
+M3B_API size_t m3b_gated_ffn_act_bytes(const m3b_gated_ffn_args* a);
+M3B_API size_t m3b_gated_ffn_gu_bytes(const m3b_gated_ffn_args* a);
+M3B_API size_t m3b_gated_ffn_fwd_workspace(const m3b_gated_ffn_args* a);
+M3B_API int m3b_gated_ffn_fwd(const m3b_gated_ffn_args* a, void* workspace, size_t workspace_bytes, void* stream);
+M3B_API size_t m3b_gated_ffn_bwd_workspace(const m3b_gated_ffn_args* a);
+M3B_API int m3b_gated_ffn_bwd(const m3b_gated_ffn_args* a, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Cross entropy of the language-model head (KulaMambaLM's loss, mamba3/block.py:186-193) straight
+ * from the hidden states, without the (rows, vocab) logits in memory:
+ *   z = hidden weight^T; loss_i = logsumexp(z_i) - z_i[target_i]; rows with target == ignore_index
+ *   are left out (their values are not used, their gradient is zero).
+ * reduction 0: loss (rows), 0 for ignored rows; 1: the mean over the kept rows (NaN with none);
+ * 2: their sum.  hidden (rows, d_model; rows hidden_stride apart), weight (vocab, d_model) of
+ * `dtype`; target (rows) int64; loss and dloss fp32.  A target outside [0, vocab) that is not
+ * ignore_index records M3B_ERR_INVALID_ARG in *err and makes the loss and the gradients NaN.
+ * Sums and softmax statistics are fp32; in the backward the logits are computed again, a piece of
+ * the vocabulary at a time, and softmax - onehot is rounded to 16-bit `dtype` once (an operand of
+ * the two gradient products); fp32 operands travel as three bf16 planes.
+ *
+ * saved (m3b_linear_xent_saved bytes, 16-byte aligned): the kept rows in operand form, their row
+ * numbers, targets and log-sums; the backward needs it as the forward left it.  Backward
+ * outputs may be null.  Workspaces as the query functions say.
+ * ------------------------------------------------------------------------ */
+typedef struct m3b_linear_xent_args {
+  int64_t rows, hidden_stride, ignore_index;
+  int32_t d_model, vocab, dtype, reduction;
+  const void* hidden;
+  const void* weight;
+  const int64_t* target;
+  void* saved;
+  float* loss;
+  const float* dloss;  /* backward: (rows) for reduction 0, else one value */
+  void* dhidden;       /* (rows, d_model) contiguous */
+  void* dweight;       /* (vocab, d_model) contiguous */
+  int* err;
+} m3b_linear_xent_args;
+M3B_API size_t m3b_linear_xent_saved(const m3b_linear_xent_args* a);
+M3B_API size_t m3b_linear_xent_fwd_workspace(const m3b_linear_xent_args* a);
+M3B_API int m3b_linear_xent_fwd(const m3b_linear_xent_args* a, void* workspace, size_t workspace_bytes, void* stream);
+M3B_API size_t m3b_linear_xent_bwd_workspace(const m3b_linear_xent_args* a);
+M3B_API int m3b_linear_xent_bwd(const m3b_linear_xent_args* a, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Global gradient norm over many tensors, and clipping.
+ *   norm = (sum over tensors of sum |g|^2)^(1/2)   (norm_type 2), or max |g| (norm_type 0: infinity)
+ *   out_i = g_i * min(1, max_norm / (norm + 1e-6)), computed in fp32 and rounded to out_dtype once.
+ * grads / outs: HOST arrays of n device pointers, numel and dtype codes; outs[i] may equal
+ * grads[i] (same dtype), in which case a tensor that keeps its values is not written.  outs null:
+ * the norm alone.  norm: one fp32 value on the device.  No host synchronisation; sums in a fixed
+ * order (fp32 partial sums over at most 32 values per lane, fp64 above).
+ * ------------------------------------------------------------------------ */
+typedef struct m3b_grad_clip_args {
+  int64_t n;
+  const void* const* grads;
+  void* const* outs;
+  const int64_t* numel;
+  const int32_t* grad_dtype;
+  const int32_t* out_dtype;
+  int32_t norm_type;
+  float max_norm;
+  float* norm;
+} m3b_grad_clip_args;
+M3B_API size_t m3b_grad_clip_workspace(const m3b_grad_clip_args* a);
+M3B_API int m3b_grad_clip(const m3b_grad_clip_args* a, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
  * Tensor-core self-test (diagnostic; no counterpart in the reference).
  * D (128 x 64, fp32) = A (128 x 128 bf16, row-major) x B (64 x 128 bf16, row-major)^T,
  * staged through the same shared-memory layouts and UMMA descriptors as the chunk

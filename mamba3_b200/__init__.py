@@ -12,6 +12,9 @@ from .block import KulaMambaBlock, KulaMambaLM, SwiGLU  # noqa: E402
 from .ssd import SSDOutput, chunked_ssd  # noqa: E402
 from .scan import ssd_scan  # noqa: E402
 from .decode import GraphDecoder  # noqa: E402  (extension: CUDA-graph decode loop)
+from .ffn import gated_ffn  # noqa: E402  (extension: the blocks' MLP as one operator)
+from .loss import linear_cross_entropy  # noqa: E402  (extension: the LM loss without the logits)
+from .clip import clip_grad_norm_, clip_grads  # noqa: E402  (extension: global-norm clipping)
 from ._lib import M3bError, check_device_errors  # noqa: E402  (status codes, device error word)
 
 __all__ = [
@@ -24,6 +27,10 @@ __all__ = [
     "chunked_ssd",
     "ssd_scan",
     "GraphDecoder",
+    "gated_ffn",
+    "linear_cross_entropy",
+    "clip_grads",
+    "clip_grad_norm_",
     "M3bError",
     "check_device_errors",
 ]

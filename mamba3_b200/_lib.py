@@ -7,6 +7,7 @@ the library is missing or a tensor is not on a CUDA device the call raises.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import threading
 from pathlib import Path
@@ -136,6 +137,31 @@ class SeqparFoldArgs(C.Structure):
                 ("prev_bx", C.c_void_p)]
 
 
+class GatedFfnArgs(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("x_stride", C.c_int64), ("residual_stride", C.c_int64),
+                ("dout_stride", C.c_int64), ("d_model", C.c_int32), ("d_ff", C.c_int32), ("dtype", C.c_int32),
+                ("residual_scale", C.c_float), ("x", C.c_void_p), ("w_gate", C.c_void_p), ("w_up", C.c_void_p),
+                ("w_down", C.c_void_p), ("b_gate", C.c_void_p), ("b_up", C.c_void_p), ("b_down", C.c_void_p),
+                ("residual", C.c_void_p), ("saved_act", C.c_void_p), ("saved_gu", C.c_void_p), ("out", C.c_void_p),
+                ("dout", C.c_void_p), ("dx", C.c_void_p), ("dw_gate", C.c_void_p), ("dw_up", C.c_void_p),
+                ("dw_down", C.c_void_p), ("db_gate", C.c_void_p), ("db_up", C.c_void_p), ("db_down", C.c_void_p),
+                ("err", C.c_void_p)]
+
+
+class LinearXentArgs(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("hidden_stride", C.c_int64), ("ignore_index", C.c_int64),
+                ("d_model", C.c_int32), ("vocab", C.c_int32), ("dtype", C.c_int32), ("reduction", C.c_int32),
+                ("hidden", C.c_void_p), ("weight", C.c_void_p), ("target", C.c_void_p), ("saved", C.c_void_p),
+                ("loss", C.c_void_p), ("dloss", C.c_void_p), ("dhidden", C.c_void_p), ("dweight", C.c_void_p),
+                ("err", C.c_void_p)]
+
+
+class GradClipArgs(C.Structure):
+    _fields_ = [("n", C.c_int64), ("grads", C.c_void_p), ("outs", C.c_void_p), ("numel", C.c_void_p),
+                ("grad_dtype", C.c_void_p), ("out_dtype", C.c_void_p), ("norm_type", C.c_int32),
+                ("max_norm", C.c_float), ("norm", C.c_void_p)]
+
+
 LAYER_FWD_STAGES = ("prep", "angle_prefix", "chunk_state", "scan", "chunk_out", "last_bx")
 
 
@@ -177,6 +203,19 @@ SIGNATURES = {
     "m3b_swiglu_rows": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_int32, C.c_void_p]),
     "m3b_add_rmsnorm": (C.c_int, [C.c_void_p, C.c_void_p, C.c_float, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64,
                                   C.c_int32, C.c_float, C.c_int32, C.c_void_p]),
+    "m3b_gated_ffn_act_bytes": (C.c_size_t, [C.POINTER(GatedFfnArgs)]),
+    "m3b_gated_ffn_gu_bytes": (C.c_size_t, [C.POINTER(GatedFfnArgs)]),
+    "m3b_gated_ffn_fwd_workspace": (C.c_size_t, [C.POINTER(GatedFfnArgs)]),
+    "m3b_gated_ffn_fwd": (C.c_int, [C.POINTER(GatedFfnArgs), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "m3b_gated_ffn_bwd_workspace": (C.c_size_t, [C.POINTER(GatedFfnArgs)]),
+    "m3b_gated_ffn_bwd": (C.c_int, [C.POINTER(GatedFfnArgs), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "m3b_linear_xent_saved": (C.c_size_t, [C.POINTER(LinearXentArgs)]),
+    "m3b_linear_xent_fwd_workspace": (C.c_size_t, [C.POINTER(LinearXentArgs)]),
+    "m3b_linear_xent_fwd": (C.c_int, [C.POINTER(LinearXentArgs), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "m3b_linear_xent_bwd_workspace": (C.c_size_t, [C.POINTER(LinearXentArgs)]),
+    "m3b_linear_xent_bwd": (C.c_int, [C.POINTER(LinearXentArgs), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "m3b_grad_clip_workspace": (C.c_size_t, [C.POINTER(GradClipArgs)]),
+    "m3b_grad_clip": (C.c_int, [C.POINTER(GradClipArgs), C.c_void_p, C.c_size_t, C.c_void_p]),
     "m3b_selftest_umma": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p]),
     "m3b_selftest_wait": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_int64, C.c_void_p, C.c_void_p]),
 }
@@ -759,3 +798,151 @@ def seqpar_fold(summaries, upto: int, batch: int, H: int, P: int, N: int, h, ang
                        upto, batch, H, P, N, C.c_void_p(h.data_ptr()), C.c_void_p(angle.data_ptr()),
                        C.c_void_p(prev_bx.data_ptr()))
     _check(lib().m3b_seqpar_fold(C.byref(a), _stream(h.device)), "m3b_seqpar_fold")
+
+
+# ---------------------------------------------------------------------------
+# gated feed-forward, linear cross entropy, gradient clipping
+# ---------------------------------------------------------------------------
+def _addr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _on(dev):
+    """The tensors' device as the current one (nothing to do when it already is)."""
+    if dev.index is None or dev.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(dev)
+
+
+def _workspace(nbytes, dev):
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+
+
+def _rows2d(t, d):
+    """t as (rows, d) with unit stride along d and rows at least d elements apart (a copy if it must be)."""
+    t = t.reshape(-1, d)
+    if t.shape[0] and (t.stride(1) != 1 and d > 1 or (t.stride(0) < d and t.shape[0] > 1)):
+        t = t.contiguous()
+    return t
+
+
+def _rows_apart(t, d):
+    return t.stride(0) if t.shape[0] > 1 else d
+
+
+def _ffn_args(x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual, scale):
+    rows, d = x.shape
+    a = GatedFfnArgs(rows, _rows_apart(x, d), 0 if residual is None else _rows_apart(residual, d), 0, d,
+                     w_gate.shape[0], dtype_code(x.dtype), float(scale), _addr(x), _addr(w_gate), _addr(w_up),
+                     _addr(w_down), _addr(b_gate), _addr(b_up), _addr(b_down), _addr(residual))
+    a.err = _addr(device_err_word(x.device))
+    return a
+
+
+def gated_ffn_fwd(x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual, scale, save):
+    """Launch the gated feed-forward; x (rows, d_model), weights and biases contiguous, one dtype.
+    Returns (out, act, gu): act and gu are what the backward reads (gu None unless `save`)."""
+    dev = _cuda(x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual)
+    a = _ffn_args(x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual, scale)
+    L = lib()
+    out = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    act = torch.empty(L.m3b_gated_ffn_act_bytes(C.byref(a)), dtype=torch.uint8, device=dev)
+    gu = torch.empty(L.m3b_gated_ffn_gu_bytes(C.byref(a)), dtype=torch.uint8, device=dev) if save else None
+    a.saved_act, a.saved_gu, a.out = _addr(act), _addr(gu), _addr(out)
+    need = L.m3b_gated_ffn_fwd_workspace(C.byref(a))
+    ws = _workspace(need, dev)
+    with _on(dev):
+        _check(L.m3b_gated_ffn_fwd(C.byref(a), _addr(ws), need, _stream(dev)), "m3b_gated_ffn_fwd")
+    _after_launch(dev)
+    return out, act, gu
+
+
+def gated_ffn_bwd(x, w_gate, w_up, w_down, b_gate, b_up, b_down, scale, act, gu, dout, want):
+    """Gradients of gated_ffn_fwd for (x, w_gate, w_up, w_down, b_gate, b_up, b_down): None where
+    `want` (seven truth values) says so.  dout (rows, d_model), rows at least d_model apart."""
+    dev = _cuda(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act, gu, dout)
+    a = _ffn_args(x, w_gate, w_up, w_down, b_gate, b_up, b_down, None, scale)
+    ins = (x, w_gate, w_up, w_down, b_gate, b_up, b_down)
+    g = [torch.empty(t.shape, dtype=x.dtype, device=dev) if w and t is not None else None for t, w in zip(ins, want)]
+    a.dout_stride, a.dout = _rows_apart(dout, x.shape[1]), _addr(dout)
+    a.saved_act, a.saved_gu = _addr(act), _addr(gu)
+    a.dx, a.dw_gate, a.dw_up, a.dw_down, a.db_gate, a.db_up, a.db_down = [_addr(t) for t in g]
+    L = lib()
+    need = L.m3b_gated_ffn_bwd_workspace(C.byref(a))
+    ws = _workspace(need, dev)
+    with _on(dev):
+        _check(L.m3b_gated_ffn_bwd(C.byref(a), _addr(ws), need, _stream(dev)), "m3b_gated_ffn_bwd")
+    _after_launch(dev)
+    return g
+
+
+REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+
+
+def _xent_args(rows, d, weight, ignore_index, reduction):
+    a = LinearXentArgs(rows, d, ignore_index, d, weight.shape[0], dtype_code(weight.dtype), REDUCTIONS[reduction])
+    a.weight = _addr(weight)
+    a.err = _addr(device_err_word(weight.device))
+    return a
+
+
+def linear_xent_fwd(hidden, weight, target, ignore_index, reduction):
+    """Launch the head's cross entropy; hidden (rows, d_model), weight (vocab, d_model) contiguous of
+    the same dtype, target (rows) int64 contiguous.  Returns (loss fp32, saved)."""
+    dev = _cuda(hidden, weight, target)
+    rows, d = hidden.shape
+    a = _xent_args(rows, d, weight, ignore_index, reduction)
+    a.hidden_stride, a.hidden, a.target = _rows_apart(hidden, d), _addr(hidden), _addr(target)
+    L = lib()
+    loss = torch.empty((rows,) if reduction == "none" else (), dtype=torch.float32, device=dev)
+    saved = torch.empty(max(16, L.m3b_linear_xent_saved(C.byref(a))), dtype=torch.uint8, device=dev)
+    a.saved, a.loss = _addr(saved), _addr(loss)
+    need = L.m3b_linear_xent_fwd_workspace(C.byref(a))
+    ws = _workspace(need, dev)
+    with _on(dev):
+        _check(L.m3b_linear_xent_fwd(C.byref(a), _addr(ws), need, _stream(dev)), "m3b_linear_xent_fwd")
+    _after_launch(dev)
+    return loss, saved
+
+
+def linear_xent_bwd(rows, weight, saved, dloss, ignore_index, reduction, want_hidden, want_weight):
+    """Gradients of linear_xent_fwd: ((rows, d_model) or None, (vocab, d_model) or None)."""
+    dev = _cuda(weight, saved, dloss)
+    d = weight.shape[1]
+    a = _xent_args(rows, d, weight, ignore_index, reduction)
+    dh = torch.empty(rows, d, dtype=weight.dtype, device=dev) if want_hidden else None
+    dw = torch.empty_like(weight) if want_weight else None
+    a.saved, a.dloss, a.dhidden, a.dweight = _addr(saved), _addr(dloss), _addr(dh), _addr(dw)
+    L = lib()
+    need = L.m3b_linear_xent_bwd_workspace(C.byref(a))
+    ws = _workspace(need, dev)
+    with _on(dev):
+        _check(L.m3b_linear_xent_bwd(C.byref(a), _addr(ws), need, _stream(dev)), "m3b_linear_xent_bwd")
+    _after_launch(dev)
+    return dh, dw
+
+
+def grad_clip(grads, outs, max_norm, inf_norm, dev):
+    """Launch the global norm over `grads` (dense tensors on `dev`) and, with `outs` (the same
+    lengths; the same tensors for in place), the clipped values.  Returns the norm (fp32, on `dev`)."""
+    n = len(grads)
+    gp = (C.c_void_p * n)(*[t.data_ptr() for t in grads])
+    num = (C.c_int64 * n)(*[t.numel() for t in grads])
+    gd = (C.c_int32 * n)(*[_DT[t.dtype] for t in grads])
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    a = GradClipArgs(n)
+    a.grads, a.numel, a.grad_dtype = C.addressof(gp), C.addressof(num), C.addressof(gd)
+    if outs is grads:
+        op, od = gp, gd
+    elif outs is not None:
+        op = (C.c_void_p * n)(*[t.data_ptr() for t in outs])
+        od = (C.c_int32 * n)(*[_DT[t.dtype] for t in outs])
+    if outs is not None:
+        a.outs, a.out_dtype = C.addressof(op), C.addressof(od)
+    a.norm_type, a.max_norm, a.norm = (0 if inf_norm else 2), float(max_norm), norm.data_ptr()
+    L = lib()
+    need = L.m3b_grad_clip_workspace(C.byref(a))
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    with _on(dev):
+        _check(L.m3b_grad_clip(C.byref(a), _addr(ws), need, _stream(dev)), "m3b_grad_clip")
+    return norm

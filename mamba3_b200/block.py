@@ -17,6 +17,8 @@ import torch.nn.functional as F
 from torch.utils.checkpoint import checkpoint as grad_checkpoint
 
 from . import ops
+from .ffn import gated_ffn
+from .loss import linear_cross_entropy
 from .mamba3 import KulaMamba, RMSNorm
 
 
@@ -26,10 +28,12 @@ def _residual(x, h, scale):
 
 
 class SwiGLU(nn.Module):
-    """w_down(silu(w_gate x) * w_up x)  (mamba3/block.py:16-26)."""
+    """w_down(silu(w_gate x) * w_up x)  (mamba3/block.py:16-26).  With ``fused`` it runs as the
+    gated_ffn operator, forward and backward, and can take the block's scaled residual along."""
 
-    def __init__(self, d_model: int, d_ff: int | None = None, bias: bool = False):
+    def __init__(self, d_model: int, d_ff: int | None = None, bias: bool = False, *, fused: bool = False):
         super().__init__()
+        self.fused = bool(fused)
         d_ff = d_ff or int(d_model * 8 / 3 / 64 + 1) * 64
         self.w_gate = nn.Linear(d_model, d_ff, bias=bias)
         self.w_up = nn.Linear(d_model, d_ff, bias=bias)
@@ -46,7 +50,13 @@ class SwiGLU(nn.Module):
             self._gu_key = key
         return self._gu_w, self._gu_b
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None, scale: float = 1.0) -> torch.Tensor:
+        """The MLP of x; with `residual`, residual + scale * MLP(x) (in the operator's epilogue when fused)."""
+        if self.fused:
+            return gated_ffn(x, self.w_gate.weight, self.w_up.weight, self.w_down.weight, b_gate=self.w_gate.bias,
+                             b_up=self.w_up.bias, b_down=self.w_down.bias, residual=residual, residual_scale=scale)
+        if residual is not None:
+            return _residual(residual, self.forward(x), scale)
         d_ff = self.w_gate.out_features
         if (ops.kernel_ok(x) and d_ff % 8 == 0
                 and not (torch.is_grad_enabled() and any(p.requires_grad for p in self.parameters()))):
@@ -78,6 +88,7 @@ class KulaMambaBlock(nn.Module):
         gradient_checkpointing: bool = False,
         use_trapezoidal: bool = True,
         use_complex_ssm: bool = True,
+        fused_mlp: bool = False,
     ):
         super().__init__()
         self.residual_scale = residual_scale
@@ -90,12 +101,14 @@ class KulaMambaBlock(nn.Module):
         if use_mlp:
             d_ff = int(d_model * mlp_expand / 64 + 1) * 64
             self.mlp_norm = RMSNorm(d_model, eps=norm_eps)
-            self.mlp = SwiGLU(d_model, d_ff, bias=bias)
+            self.mlp = SwiGLU(d_model, d_ff, bias=bias, fused=fused_mlp)
 
     def _mlp_residual(self, x):
         if self.use_mlp:
             if self.gradient_checkpointing and self.training:
                 m = grad_checkpoint(lambda t: self.mlp(self.mlp_norm(t)), x, use_reentrant=False)
+            elif self.mlp.fused and not torch.is_autocast_enabled("cuda"):  # autocast keeps the stream's dtype
+                return self.mlp(self.mlp_norm(x), x, self.residual_scale)
             else:
                 m = self.mlp(self.mlp_norm(x))
             x = _residual(x, m, self.residual_scale)
@@ -139,7 +152,10 @@ class KulaMambaLM(nn.Module):
         gradient_checkpointing: bool = False,
         use_trapezoidal: bool = True,
         use_complex_ssm: bool = True,
+        fused_mlp: bool = False,
     ):
+        """fused_mlp (extension): every block's MLP runs as the gated_ffn operator, forward and
+        backward; the same parameters, its own rounding."""
         super().__init__()
         self.d_model = d_model
         self.n_layers = n_layers
@@ -149,7 +165,7 @@ class KulaMambaLM(nn.Module):
             KulaMambaBlock(d_model=d_model, d_state=d_state, expand=expand, headdim=headdim, ngroups=ngroups,
                            mimo_rank=mimo_rank, chunk_size=chunk_size, use_mlp=use_mlp, norm_eps=norm_eps, bias=bias,
                            residual_scale=r_scale, gradient_checkpointing=gradient_checkpointing,
-                           use_trapezoidal=use_trapezoidal, use_complex_ssm=use_complex_ssm)
+                           use_trapezoidal=use_trapezoidal, use_complex_ssm=use_complex_ssm, fused_mlp=fused_mlp)
             for _ in range(n_layers)
         ])
         self.norm = RMSNorm(d_model, eps=norm_eps)
@@ -188,15 +204,28 @@ class KulaMambaLM(nn.Module):
                 n = self.norm(_residual(x, h, blk.residual_scale))
         return n
 
-    def forward(self, input_ids, labels=None):
+    def _hidden(self, input_ids):
+        """The final norm's output, which the lm_head reads."""
         x = self.embedding(input_ids)
         if (ops.kernel_ok(x) and x.dtype in (torch.bfloat16, torch.float16) and x.shape[-1] % 8 == 0
                 and x.shape[-1] <= 2048 and not torch.is_grad_enabled()):
-            logits = self.lm_head(self._forward_fused(x))
-        else:
-            for layer in self.layers:
-                x = layer(x)
-            logits = self.lm_head(self.norm(x))
+            return self._forward_fused(x)
+        for layer in self.layers:
+            x = layer(x)
+        return self.norm(x)
+
+    def forward(self, input_ids, labels=None, return_logits=True):
+        """{"logits"} and, with labels, {"loss"}.  return_logits=False (extension) gives the loss
+        alone, by linear_cross_entropy: the (batch, seqlen, vocab) logits are never in memory, in the
+        forward or the backward pass, and labels of -100 cost nothing."""
+        if not return_logits:
+            if labels is None:
+                raise ValueError("return_logits=False needs labels")
+            h = self._hidden(input_ids)
+            # token t predicts label t + 1; the last one predicts nothing
+            targets = F.pad(labels[:, 1:], (0, 1), value=-100)
+            return {"loss": linear_cross_entropy(h, self.lm_head.weight, targets)}
+        logits = self.lm_head(self._hidden(input_ids))
         result = {"logits": logits}
         if labels is not None:
             result["loss"] = F.cross_entropy(logits[:, :-1].reshape(-1, logits.size(-1)), labels[:, 1:].reshape(-1))

@@ -1,0 +1,358 @@
+// Gated feed-forward block, forward and backward (m3b_gated_ffn_fwd / _bwd).
+//
+//   g = x Wg^T + bg, u = x Wu^T + bu, a = silu(g) u, out = residual + s (a Wd^T + bd)
+//   da = s dout Wd;  dg = da u sig(g) (1 + g (1 - sig(g)));  du = da g sig(g)
+//   dx = dg Wg + du Wu;  dWg = dg^T x;  dWu = du^T x;  dWd = s dout^T a
+//   dbg, dbu, dbd = the column sums of dg, du, s dout
+//
+// Forward: one product whose tiles hold gate and up columns side by side, so the activation and the
+// product are its epilogue (g and u never reach memory in inference), then the down product with
+// bias, scale and residual in its epilogue.  Backward: da's product with dg and du as its epilogue;
+// dx as one product over two K segments; the three weight gradients side by side in one launch.
+// 18 rows d_model d_ff operations forward and backward, the least there are: g and u are kept in
+// fp32 (8 bytes a value), because the rounding of a 16-bit copy would reach every gradient.
+#include "gemm.cuh"
+
+namespace m3b {
+
+namespace {
+
+inline int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
+
+struct Carve {
+  uint8_t* base;
+  size_t at = 0;
+  explicit Carve(void* p) : base(static_cast<uint8_t*>(p)) {}
+  void* take(size_t bytes) {
+    void* r = base ? base + at : nullptr;
+    at += (bytes + 255) / 256 * 256;
+    return r;
+  }
+};
+
+struct Dims {
+  int64_t M;
+  int D, F, np;
+  bool f16, f32;
+  explicit Dims(const m3b_gated_ffn_args* a)
+      : M(a->rows), D(a->d_model), F(a->d_ff), np(a->dtype == M3B_F32 ? 3 : 1), f16(a->dtype == M3B_F16),
+        f32(a->dtype == M3B_F32) {}
+};
+
+// A matrix as an operand: in place where the TMA can read it, else packed into the workspace.
+GemmOperand operand(const void* p, int64_t rows, int64_t cols, int64_t ld, const m3b_gated_ffn_args* a, Carve& ws,
+                    bool run, cudaStream_t st, int* rc) {
+  if (a->dtype != M3B_F32 && tma_ok(p, ld)) return GemmOperand{p, rows, cols, ld, 0, 1};
+  const int np = a->dtype == M3B_F32 ? 3 : 1;
+  const int64_t ldp = up(cols, 8), plane = rows * ldp;
+  void* dst = ws.take((size_t)np * plane * 2);
+  if (run && *rc == M3B_OK) *rc = launch_pack(p, a->dtype, rows, cols, ld, dst, ldp, plane, st);
+  return GemmOperand{dst, rows, cols, ldp, plane, np};
+}
+
+GemmOut result(void* p, int64_t ld, int dtype) {
+  GemmOut o{};
+  o.p = p;
+  o.ld = ld;
+  o.kind = dtype == M3B_BF16 ? kOutBf16 : dtype == M3B_F16 ? kOutF16 : kOutF32;
+  o.vec = aligned16(p) && ld % 8 == 0;
+  return o;
+}
+
+GemmOut operand_out(const GemmOperand& o, bool f16) {
+  GemmOut r{};
+  r.p = const_cast<void*>(o.p);
+  r.ld = o.ld;
+  r.plane = o.plane;
+  r.kind = o.planes > 1 ? kOutPlanes : f16 ? kOutF16 : kOutBf16;
+  r.vec = 1;
+  return r;
+}
+
+// Sum over rows of a (rows x cols) matrix times `scale`, in a fixed order: 64 column threads and
+// chunks of rows per block, then the chunks.
+constexpr int kSumRows = 256;
+__global__ void colsum_kernel(const void* __restrict__ x, int dt, int planes, int64_t plane, int64_t ld, int64_t rows,
+                              int cols, float* __restrict__ part) {
+  const int c = blockIdx.x * 64 + threadIdx.x;
+  const int64_t r0 = (int64_t)blockIdx.y * kSumRows, r1 = r0 + kSumRows < rows ? r0 + kSumRows : rows;
+  if (c >= cols) return;
+  float s = 0.f;
+  for (int64_t r = r0; r < r1; ++r)
+    for (int k = planes - 1; k >= 0; --k) s += ldf(x, k * plane + r * ld + c, dt);
+  part[(int64_t)blockIdx.y * cols + c] = s;
+}
+__global__ void colsum_finish_kernel(const float* __restrict__ part, int chunks, int cols, float scale, void* out,
+                                     int dt) {
+  const int c = blockIdx.x * blockDim.x + threadIdx.x;
+  if (c >= cols) return;
+  float s = 0.f;
+  for (int k = 0; k < chunks; ++k) s += part[(int64_t)k * cols + c];
+  stf(out, c, dt, s * scale);
+}
+int colsum(const GemmOperand& o, int dt, float scale, void* out, int out_dt, float* part, cudaStream_t st) {
+  const int chunks = (int)((o.rows + kSumRows - 1) / kSumRows), cols = (int)o.cols;
+  colsum_kernel<<<dim3((cols + 63) / 64, chunks), 64, 0, st>>>(o.p, dt, o.planes, o.plane, o.ld, o.rows, cols, part);
+  colsum_finish_kernel<<<(cols + 255) / 256, 256, 0, st>>>(part, chunks, cols, scale, out, out_dt);
+  return check_launch("colsum_kernel");
+}
+
+int check(const m3b_gated_ffn_args* a, bool bwd) {
+  if (!a) return fail(M3B_ERR_INVALID_ARG, "gated_ffn: null args");
+  if (a->rows < 0 || a->d_model <= 0 || a->d_ff <= 0) return fail(M3B_ERR_INVALID_ARG, "gated_ffn: bad sizes");
+  if (a->rows > (int64_t(1) << 31) - 512 || a->d_model > (1 << 24) || a->d_ff > (1 << 24))
+    return fail(M3B_ERR_INVALID_ARG, "gated_ffn: sizes past the kernels' limits");
+  if (a->dtype != M3B_F32 && a->dtype != M3B_BF16 && a->dtype != M3B_F16)
+    return fail(M3B_ERR_INVALID_ARG, "gated_ffn: dtype");
+  if (!a->w_gate || !a->w_up || !a->w_down || (a->rows && (!a->x || !a->saved_act)))
+    return fail(M3B_ERR_INVALID_ARG, "gated_ffn: null pointer");
+  if ((a->b_gate == nullptr) != (a->b_up == nullptr))
+    return fail(M3B_ERR_INVALID_ARG, "gated_ffn: b_gate and b_up go together");
+  if (a->x_stride < a->d_model || (a->residual && a->residual_stride < a->d_model))
+    return fail(M3B_ERR_INVALID_ARG, "gated_ffn: row strides shorter than the rows");
+  if (!aligned16(a->saved_act) || !aligned16(a->saved_gu))
+    return fail(M3B_ERR_ALIGNMENT, "gated_ffn: saved buffers must be 16-byte aligned");
+  if (bwd) {
+    if (a->rows && (!a->dout || !a->saved_gu)) return fail(M3B_ERR_INVALID_ARG, "gated_ffn_bwd: null pointer");
+    if (a->rows && a->dout_stride < a->d_model) return fail(M3B_ERR_INVALID_ARG, "gated_ffn_bwd: dout stride");
+  } else if (a->rows && !a->out) {
+    return fail(M3B_ERR_INVALID_ARG, "gated_ffn_fwd: null pointer");
+  }
+  return M3B_OK;
+}
+
+bool sizes_ok(const m3b_gated_ffn_args* a) {
+  return a && a->rows >= 0 && a->d_model > 0 && a->d_ff > 0 &&
+         (a->dtype == M3B_F32 || a->dtype == M3B_BF16 || a->dtype == M3B_F16);
+}
+
+GemmOperand act_operand(const m3b_gated_ffn_args* a, void* p) {
+  const Dims d(a);
+  const int64_t ld = up(d.F, 8);
+  return GemmOperand{p, d.M, d.F, ld, d.M * ld, d.np};
+}
+
+#define M3B_TRY(x)                     \
+  do {                                 \
+    const int rc_ = (x);               \
+    if (rc_ != M3B_OK) return rc_;     \
+  } while (0)
+#define M3B_MAP(...) M3B_TRY(gemm_map(__VA_ARGS__))
+
+// run == false only measures the workspace.
+int forward(const m3b_gated_ffn_args* a, void* workspace, size_t* need, bool run, cudaStream_t st) {
+  const Dims d(a);
+  Carve ws(workspace);
+  int rc = M3B_OK;
+  const GemmOperand x = operand(a->x, d.M, d.D, a->x_stride, a, ws, run, st, &rc);
+  const GemmOperand wg = operand(a->w_gate, d.F, d.D, d.D, a, ws, run, st, &rc);
+  const GemmOperand wu = operand(a->w_up, d.F, d.D, d.D, a, ws, run, st, &rc);
+  const GemmOperand wd = operand(a->w_down, d.D, d.F, d.F, a, ws, run, st, &rc);
+  *need = ws.at;
+  if (!run || rc != M3B_OK) return rc;
+  const GemmOperand act = act_operand(a, a->saved_act);
+  const bool pair = d.M > 128;
+  {
+    GemmParams p{};
+    GemmSub& s = p.sub[0];
+    p.nsub = 1;
+    p.bn = pair ? 256 : 64;
+    p.npass = d.f32 ? 6 : 1;
+    p.f16 = d.f16;
+    p.err = a->err;
+    M3B_MAP(&s.a[0], x, false, 128, d.f16);
+    M3B_MAP(&s.b[0], wg, false, gemm_box_b(pair, p.bn, kEpiGlu), d.f16);
+    M3B_MAP(&s.b[1], wu, false, gemm_box_b(pair, p.bn, kEpiGlu), d.f16);
+    s.M = (int)d.M;
+    s.N = d.F;
+    s.nk[0] = (d.D + kGmBK - 1) / kGmBK;
+    s.out = operand_out(act, d.f16);
+    s.bias = a->b_gate;
+    s.bias2 = a->b_up;
+    s.dt = a->dtype;
+    p.gu = static_cast<float*>(a->saved_gu);
+    p.gu_ld4 = up(d.F, 16) / 4;
+    M3B_TRY(launch_gemm(p, kEpiGlu, pair, st));
+  }
+  GemmParams p{};
+  GemmSub& s = p.sub[0];
+  p.nsub = 1;
+  p.bn = pair ? 256 : 32;
+  p.npass = d.f32 ? 6 : 1;
+  p.f16 = d.f16;
+  p.err = a->err;
+  M3B_MAP(&s.a[0], act, false, 128, d.f16);
+  M3B_MAP(&s.b[0], wd, false, gemm_box_b(pair, p.bn, kEpiStore), d.f16);
+  s.M = (int)d.M;
+  s.N = d.D;
+  s.nk[0] = (d.F + kGmBK - 1) / kGmBK;
+  s.out = result(a->out, d.D, a->dtype);
+  s.alpha = a->residual_scale;
+  s.bias = a->b_down;
+  s.residual = a->residual;
+  s.ld_res = a->residual_stride;
+  s.dt = a->dtype;
+  return launch_gemm(p, kEpiStore, pair, st);
+}
+
+int backward(const m3b_gated_ffn_args* a, void* workspace, size_t* need, bool run, cudaStream_t st) {
+  const Dims d(a);
+  Carve ws(workspace);
+  int rc = M3B_OK;
+  const GemmOperand x = operand(a->x, d.M, d.D, a->x_stride, a, ws, run, st, &rc);
+  const GemmOperand wg = operand(a->w_gate, d.F, d.D, d.D, a, ws, run, st, &rc);
+  const GemmOperand wu = operand(a->w_up, d.F, d.D, d.D, a, ws, run, st, &rc);
+  const GemmOperand wd = operand(a->w_down, d.D, d.F, d.F, a, ws, run, st, &rc);
+  const GemmOperand dy = operand(a->dout, d.M, d.D, a->dout_stride, a, ws, run, st, &rc);
+  const size_t one = (size_t)act_operand(a, nullptr).plane * d.np * 2;
+  const GemmOperand dg = act_operand(a, ws.take(one)), du = act_operand(a, ws.take(one));
+  const int64_t chunks = (d.M + kSumRows - 1) / kSumRows;
+  float* part = static_cast<float*>(ws.take((size_t)chunks * (d.F > d.D ? d.F : d.D) * 4));
+  *need = ws.at;
+  if (!run || rc != M3B_OK) return rc;
+  const GemmOperand act = act_operand(a, a->saved_act);
+  const int npass = d.f32 ? 6 : 1;
+  const int bn = 256;
+  {  // da -> dg, du
+    GemmParams p{};
+    GemmSub& s = p.sub[0];
+    p.nsub = 1;
+    p.bn = bn;
+    p.npass = npass;
+    p.f16 = d.f16;
+    p.err = a->err;
+    M3B_MAP(&s.a[0], dy, false, 128, d.f16);
+    M3B_MAP(&s.b[0], wd, true, 0, d.f16);
+    s.b_mn = 1;
+    s.M = (int)d.M;
+    s.N = d.F;
+    s.nk[0] = (d.D + kGmBK - 1) / kGmBK;
+    s.alpha = a->residual_scale;
+    s.out = operand_out(dg, d.f16);
+    s.out2 = operand_out(du, d.f16);
+    p.gu = static_cast<float*>(a->saved_gu);
+    p.gu_ld4 = up(d.F, 16) / 4;
+    M3B_TRY(launch_gemm(p, kEpiDglu, true, st));
+  }
+  if (a->dx) {
+    GemmParams p{};
+    GemmSub& s = p.sub[0];
+    p.nsub = 1;
+    p.bn = bn;
+    p.npass = npass;
+    p.f16 = d.f16;
+    p.err = a->err;
+    M3B_MAP(&s.a[0], dg, false, 128, d.f16);
+    M3B_MAP(&s.a[1], du, false, 128, d.f16);
+    M3B_MAP(&s.b[0], wg, true, 0, d.f16);
+    M3B_MAP(&s.b[1], wu, true, 0, d.f16);
+    s.b_mn = 1;
+    s.M = (int)d.M;
+    s.N = d.D;
+    s.nk[0] = s.nk[1] = (d.F + kGmBK - 1) / kGmBK;
+    s.alpha = 1.f;
+    s.out = result(a->dx, d.D, a->dtype);
+    M3B_TRY(launch_gemm(p, kEpiStore, true, st));
+  }
+  GemmParams p{};
+  p.bn = bn;
+  p.npass = npass;
+  p.f16 = d.f16;
+  p.err = a->err;
+  const struct {
+    void* out;
+    const GemmOperand *l, *r;
+    int M, N;
+    float alpha;
+  } w[3] = {{a->dw_gate, &dg, &x, d.F, d.D, 1.f},
+            {a->dw_up, &du, &x, d.F, d.D, 1.f},
+            {a->dw_down, &dy, &act, d.D, d.F, a->residual_scale}};
+  for (const auto& e : w) {
+    if (!e.out) continue;
+    GemmSub& s = p.sub[p.nsub++];
+    M3B_MAP(&s.a[0], *e.l, true, 0, d.f16);
+    M3B_MAP(&s.b[0], *e.r, true, 0, d.f16);
+    s.a_mn = s.b_mn = 1;
+    s.M = e.M;
+    s.N = e.N;
+    s.nk[0] = (int)((d.M + kGmBK - 1) / kGmBK);
+    s.alpha = e.alpha;
+    s.out = result(e.out, e.N, a->dtype);
+  }
+  if (p.nsub) M3B_TRY(launch_gemm(p, kEpiStore, true, st));
+  const int odt = d.f32 ? M3B_BF16 : a->dtype;  // planes are bf16
+  if (a->db_gate) M3B_TRY(colsum(dg, odt, 1.f, a->db_gate, a->dtype, part, st));
+  if (a->db_up) M3B_TRY(colsum(du, odt, 1.f, a->db_up, a->dtype, part, st));
+  if (a->db_down) M3B_TRY(colsum(dy, odt, a->residual_scale, a->db_down, a->dtype, part, st));
+  return M3B_OK;
+}
+
+int check_workspace(size_t need, const void* ws, size_t bytes) {
+  if (need == 0) return M3B_OK;
+  if (!ws || bytes < need) return fail(M3B_ERR_WORKSPACE, "gated_ffn: workspace of %zu bytes, %zu needed", bytes, need);
+  if (!aligned16(ws)) return fail(M3B_ERR_ALIGNMENT, "gated_ffn: workspace must be 16-byte aligned");
+  return M3B_OK;
+}
+
+}  // namespace
+
+}  // namespace m3b
+
+extern "C" {
+
+size_t m3b_gated_ffn_act_bytes(const m3b_gated_ffn_args* a) {
+  if (!m3b::sizes_ok(a)) return 0;
+  const m3b::GemmOperand o = m3b::act_operand(a, nullptr);
+  return (size_t)o.planes * o.plane * 2;
+}
+
+size_t m3b_gated_ffn_gu_bytes(const m3b_gated_ffn_args* a) {
+  if (!m3b::sizes_ok(a)) return 0;
+  return (size_t)m3b::up(a->rows, 256) * m3b::up(a->d_ff, 16) * 8;
+}
+
+size_t m3b_gated_ffn_fwd_workspace(const m3b_gated_ffn_args* a) {
+  size_t need = 0;
+  if (m3b::sizes_ok(a) && a->rows) m3b::forward(a, nullptr, &need, false, nullptr);
+  return need;
+}
+
+int m3b_gated_ffn_fwd(const m3b_gated_ffn_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+  m3b::clear_error();
+  int rc = m3b::check(a, false);
+  if (rc != M3B_OK || a->rows == 0) return rc;
+  size_t need = 0;
+  m3b::forward(a, nullptr, &need, false, nullptr);
+  rc = m3b::check_workspace(need, workspace, workspace_bytes);
+  return rc != M3B_OK ? rc : m3b::forward(a, workspace, &need, true, static_cast<cudaStream_t>(stream));
+}
+
+size_t m3b_gated_ffn_bwd_workspace(const m3b_gated_ffn_args* a) {
+  size_t need = 0;
+  if (m3b::sizes_ok(a) && a->rows) m3b::backward(a, nullptr, &need, false, nullptr);
+  return need;
+}
+
+int m3b_gated_ffn_bwd(const m3b_gated_ffn_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+  m3b::clear_error();
+  int rc = m3b::check(a, true);
+  if (rc != M3B_OK) return rc;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (a->rows == 0) {  // no rows: every sum is zero
+    const size_t es = a->dtype == M3B_F32 ? 4 : 2, F = (size_t)a->d_ff, D = (size_t)a->d_model;
+    const struct {
+      void* p;
+      size_t n;
+    } z[] = {{a->dw_gate, F * D}, {a->dw_up, F * D}, {a->dw_down, F * D},
+             {a->db_gate, F},     {a->db_up, F},     {a->db_down, D}};
+    for (const auto& e : z)
+      if (e.p && cudaMemsetAsync(e.p, 0, e.n * es, st) != cudaSuccess) return m3b::check_launch("gated_ffn_bwd");
+    return M3B_OK;
+  }
+  size_t need = 0;
+  m3b::backward(a, nullptr, &need, false, nullptr);
+  rc = m3b::check_workspace(need, workspace, workspace_bytes);
+  return rc != M3B_OK ? rc : m3b::backward(a, workspace, &need, true, st);
+}
+
+}  // extern "C"

@@ -1,0 +1,160 @@
+// Host side of the matrix-product kernel (gemm.cuh): tensor maps, launches, and the packing of
+// operands that the TMA cannot read in place.
+#include "gemm.cuh"
+
+#include <mutex>
+
+namespace m3b {
+
+namespace {
+
+// One thread per destination pair of columns: fp32 values become three bf16 planes, 16-bit values
+// are copied; columns past `cols` are zero.  Bound by HBM; rows are short strided runs, so plain
+// 4-byte stores suffice (the copy is a few per cent of the products that read it).
+template <bool F32>
+__global__ void pack_kernel(const void* __restrict__ src, int64_t rows, int64_t cols, int64_t src_ld,
+                            uint16_t* __restrict__ dst, int64_t ld, int64_t plane) {
+  const int64_t half = ld / 2, n = rows * half;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t r = i / half, c = 2 * (i - r * half);
+    uint32_t w[3] = {0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      if (c + e >= cols) break;
+      if constexpr (F32) {
+        uint16_t x[3];
+        split_planes(static_cast<const float*>(src)[r * src_ld + c + e], x);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) w[k] |= (uint32_t)x[k] << (16 * e);
+      } else {
+        w[0] |= (uint32_t) static_cast<const uint16_t*>(src)[r * src_ld + c + e] << (16 * e);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < (F32 ? 3 : 1); ++k) *reinterpret_cast<uint32_t*>(dst + k * plane + r * ld + c) = w[k];
+  }
+}
+
+using KernelFn = void (*)(const GemmParams);
+
+template <int EPI>
+KernelFn pick(bool pair) {
+  return pair ? (KernelFn)gemm_kernel<EPI, true> : (KernelFn)gemm_kernel<EPI, false>;
+}
+
+KernelFn kernel_of(int epi, bool pair) {
+  switch (epi) {
+    case kEpiStore: return pick<kEpiStore>(pair);
+    case kEpiGlu: return pick<kEpiGlu>(pair);
+    case kEpiDglu: return pick<kEpiDglu>(pair);
+    case kEpiLse: return pick<kEpiLse>(pair);
+    default: return pick<kEpiDlogit>(pair);
+  }
+}
+
+cudaLaunchConfig_t config(unsigned grid, bool pair, cudaStream_t st, cudaLaunchAttribute* at) {
+  cudaLaunchConfig_t cfg{};
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = pair ? 2 : 1;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kGmThreads);
+  cfg.dynamicSmemBytes = kGmSmem;
+  cfg.stream = st;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cfg;
+}
+
+// Per device: opt the kernels into their shared memory and count the CTA pairs that can be resident.
+int device_setup(int* pairs) {
+  static std::mutex mu;
+  static int done[64] = {0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64)
+    return fail(M3B_ERR_CUDA, "gemm: no current device");
+  std::lock_guard<std::mutex> lk(mu);
+  if (done[dev]) {
+    *pairs = done[dev];
+    return M3B_OK;
+  }
+  for (int epi = kEpiStore; epi <= kEpiDlogit; ++epi)
+    for (int pr = 0; pr < 2; ++pr) {
+      const cudaError_t e = cudaFuncSetAttribute((const void*)kernel_of(epi, pr != 0),
+                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kGmSmem);
+      if (e != cudaSuccess) return fail(M3B_ERR_CUDA, "gemm: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+    }
+  cudaLaunchAttribute at[1];
+  const cudaLaunchConfig_t cfg = config(2 * (unsigned)(num_sms() / 2), true, nullptr, at);
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, (const void*)kernel_of(kEpiStore, true), &cfg) != cudaSuccess || n <= 0) {
+    cudaGetLastError();
+    return fail(M3B_ERR_UNSUPPORTED, "gemm: no CTA pair can be resident on this device");
+  }
+  done[dev] = n;
+  *pairs = n;
+  return M3B_OK;
+}
+
+}  // namespace
+
+int gemm_map(CUtensorMap* m, const GemmOperand& o, bool mn_major, int box_rows, bool f16) {
+  const EncodeTiledFn enc = encode_tiled();
+  if (!enc) return fail(M3B_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+  const cuuint64_t dims[3] = {(cuuint64_t)o.cols, (cuuint64_t)o.rows, (cuuint64_t)o.planes};
+  const cuuint64_t strides[2] = {(cuuint64_t)o.ld * 2, (cuuint64_t)(o.planes > 1 ? o.plane : o.rows * o.ld) * 2};
+  const cuuint32_t box[3] = {(cuuint32_t)kGmBK, (cuuint32_t)(mn_major ? kGmBK : box_rows), 1};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = CUDA_SUCCESS;
+  for (int attempt = 0; attempt < 2; ++attempt) {
+    r = enc(m, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(o.p),
+            dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_ERROR_INVALID_CONTEXT) break;
+    // a host thread that has made no runtime call yet (autograd's): bind the device's context to it
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) break;
+  }
+  if (r == CUDA_SUCCESS) return M3B_OK;
+  return fail(M3B_ERR_CUDA, "cuTensorMapEncodeTiled refused %p: %lld x %lld, rows %lld apart, %d planes (%d)", o.p,
+              (long long)o.rows, (long long)o.cols, (long long)o.ld, o.planes, (int)r);
+}
+
+int launch_gemm(GemmParams& p, int epi, bool pair, cudaStream_t st) {
+  int pairs = 0;
+  const int rc = device_setup(&pairs);
+  if (rc != M3B_OK) return rc;
+  const int tile_m = gemm_tile_m(pair), tile_n = epi == kEpiGlu ? p.bn / 2 : p.bn;
+  int64_t jobs = 0;
+  for (int i = 0; i < p.nsub; ++i) {
+    GemmSub& s = p.sub[i];
+    s.mt = (s.M + tile_m - 1) / tile_m;
+    s.nt = (s.N + tile_n - 1) / tile_n;
+    jobs += (int64_t)s.mt * s.nt;
+  }
+  if (jobs == 0) return M3B_OK;
+  if (p.wait_ns == 0) p.wait_ns = kWaitLimitNs;
+  const int64_t most = pair ? pairs : num_sms();
+  const unsigned workers = (unsigned)(jobs < most ? jobs : most);
+  cudaLaunchAttribute at[1];
+  const cudaLaunchConfig_t cfg = config(pair ? 2 * workers : workers, pair, st, at);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel_of(epi, pair), p);
+  if (e != cudaSuccess) return fail(M3B_ERR_CUDA, "gemm_kernel: %s", cudaGetErrorString(e));
+  return check_launch("gemm_kernel");
+}
+
+int launch_pack(const void* src, int dtype, int64_t rows, int64_t cols, int64_t src_ld, void* dst, int64_t ld,
+                int64_t plane, cudaStream_t st) {
+  const int64_t n = rows * (ld / 2);
+  if (n == 0) return M3B_OK;
+  const int64_t blocks = (n + 255) / 256, most = (int64_t)num_sms() * 16;
+  const unsigned grid = (unsigned)(blocks < most ? blocks : most);
+  if (dtype == M3B_F32)
+    pack_kernel<true><<<grid, 256, 0, st>>>(src, rows, cols, src_ld, static_cast<uint16_t*>(dst), ld, plane);
+  else
+    pack_kernel<false><<<grid, 256, 0, st>>>(src, rows, cols, src_ld, static_cast<uint16_t*>(dst), ld, plane);
+  return check_launch("pack_kernel");
+}
+
+}  // namespace m3b

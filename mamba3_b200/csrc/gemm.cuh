@@ -1,0 +1,586 @@
+// Persistent tcgen05 matrix-product kernel with operator epilogues (sm_100a), shared by the
+// training and serving operators (ffn.cu, xent.cu).
+//
+//   C (M x N) = sum over segments of A_s (M x K_s) B_s (N x K_s)^T, fp32 accumulate in TMEM
+//
+// * Operands are 16-bit tiles of 64 K values moved by TMA with the 128-byte swizzle.  Either
+//   operand may be stored with K along its rows (K-major) or across them (MN-major, for the
+//   products of the backward passes); the tile then arrives as 64 x 64 boxes and the UMMA
+//   descriptor reads it transposed.
+// * fp32 operands travel as three bf16 planes whose sum is the value exactly (each plane takes
+//   the next 8 significant bits by truncation).  The product runs over the six plane pairs with
+//   2^-16 or more of the leading one's weight, smallest first; the dropped pairs are below 2^-24.
+// * A launch holds up to three products ("subs"), so that products that are too small to fill the
+//   GPU run side by side, and a product has up to two K segments with operands of their own.
+// * Row or K counts may come from device memory (`dyn`): the loss drops ignored tokens without
+//   the host knowing how many remain.
+//
+// Three roles per CTA: warp 0 the TMA producer, warp 1 the MMA issuer, warps 2-9 the epilogue (two
+// warps per 32 TMEM lanes, half of the columns each).  Two TMEM accumulators of 256 columns let a
+// tile's epilogue run under the next tile's MMAs.  PAIR: a cluster of two CTAs computes 256 x bn
+// tiles with cta_group::2, each CTA staging half of the B rows; otherwise single CTAs compute
+// 128 x bn tiles.
+#pragma once
+
+#include "launch.h"
+#include "pair.cuh"
+#include "tmap.h"
+
+namespace m3b {
+
+constexpr int kGmThreads = 320;
+constexpr int kGmBK = 64;
+constexpr int kGmStages = 6;
+constexpr uint32_t kGmStageA = 128 * kGmBK * 2;     // 16 KB
+constexpr uint32_t kGmStage = 2 * kGmStageA;        // + B: at most 128 rows of 64
+constexpr uint32_t kGmRing = kGmStages * kGmStage;  // 192 KB
+constexpr uint32_t kGmBarOff = kGmRing;
+constexpr uint32_t kGmSmem = kGmBarOff + 256 + 1024;
+static_assert(kGmSmem <= 227 * 1024, "shared memory plan");
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+// How a product's result is stored.
+enum GemmOutKind { kOutBf16 = 0, kOutF16 = 1, kOutF32 = 2, kOutPlanes = 3 };
+
+struct GemmOut {
+  void* p;
+  int64_t ld;     // elements between rows
+  int64_t plane;  // elements between planes (kOutPlanes)
+  int kind;
+  int vec;        // rows and columns allow 16-byte stores
+};
+
+enum GemmEpi {
+  kEpiStore = 0,   // out = residual + alpha (acc + bias), or an fp32 running sum over several launches
+  kEpiGlu = 1,     // gate | up accumulators -> silu(g) u, and g, u kept in fp32 for the backward pass
+  kEpiDglu = 2,    // d(silu(g) u) -> dg, du
+  kEpiLse = 3,     // running maximum and sum of each row, and the target's logit
+  kEpiDlogit = 4,  // softmax - one-hot
+};
+
+struct GemmSub {
+  CUtensorMap a[2], b[2];
+  int M, N;        // result rows and columns
+  int nk[2];       // K blocks of each segment
+  int mt, nt;      // tiles
+  int a_mn, b_mn;  // operand stored MN-major
+  int m_dyn, k_dyn;
+  GemmOut out, out2;
+  // kEpiStore
+  float alpha;
+  const float* alpha_num;  // alpha *= alpha_num[0]
+  const int* alpha_den;    // alpha /= alpha_den[0] (0 rows: alpha = 0)
+  const void* bias;        // N values, of `dt`
+  const void* bias2;       // kEpiGlu: the up bias
+  const void* residual;    // (M, N) of `dt`, rows ld_res apart
+  int64_t ld_res;
+  const int* row_index;    // result row r goes to row row_index[r] (negative: nowhere)
+  float* acc;              // running fp32 sum, [row / 32][col / 4][row % 32][4]
+  int acc_mode;            // 0 none, 1 acc = v, 2 acc += v, 3 out = acc + v
+  int dt;                  // dtype code of bias and residual
+};
+
+struct GemmParams {
+  GemmSub sub[3];
+  int nsub;
+  int bn;       // accumulator columns of a tile
+  int npass;    // plane pairs: 1, or 6 for fp32 operands
+  int f16;      // operand type: fp16 instead of bf16
+  const int* dyn;
+  // kEpiGlu / kEpiDglu: g and u in fp32, [row / 32][col / 4][g, u][row % 32][4], ld4 = column quads
+  float* gu;
+  int64_t gu_ld4;
+  // kEpiLse / kEpiDlogit
+  const int* target;       // per row
+  float* target_logit;
+  float2* part;            // (slots, rows): maximum and sum in powers of two
+  int64_t part_ld;
+  const float* lse2;       // log2 of the row's sum of exponentials
+  const float* roww;       // weight per row or null
+  int col0;                // first vocabulary column of this piece
+  int* err;
+  uint64_t wait_ns;
+};
+
+// ---------------------------------------------------------------------------
+// jobs
+// ---------------------------------------------------------------------------
+struct GemmJob {
+  int sub, mt, nt;
+  int kb, ke;  // iterations [kb, ke) of the tile's K blocks times passes
+};
+
+template <bool PAIR>
+struct GemmSched {
+  const GemmParams& p;
+  int dyn;
+  int64_t j, step;
+  static constexpr int kTileM = PAIR ? 256 : 128;
+  __device__ GemmSched(const GemmParams& q, int64_t worker, int64_t nworkers)
+      : p(q), dyn(q.dyn ? *q.dyn : 0), j(worker), step(nworkers) {}
+  __device__ int mtiles(const GemmSub& s) const { return s.m_dyn ? (dyn + kTileM - 1) / kTileM : s.mt; }
+  __device__ int rows(const GemmSub& s) const { return s.m_dyn ? dyn : s.M; }
+  __device__ int nk0(const GemmSub& s) const { return s.k_dyn ? (dyn + kGmBK - 1) / kGmBK : s.nk[0]; }
+  __device__ bool next(GemmJob& o) {
+    int64_t t = j;
+    j += step;
+    for (int i = 0; i < p.nsub; ++i) {
+      const GemmSub& s = p.sub[i];
+      const int mt = mtiles(s);
+      const int64_t n = (int64_t)mt * s.nt;
+      if (t < n) {
+        // bands of 8 row tiles, walked column by column: the tiles in flight share operands in L2
+        const int band = 8 * s.nt;
+        const int g = (int)(t / band), first = g * 8, size = mt - first < 8 ? mt - first : 8;
+        const int r = (int)(t - (int64_t)g * band);
+        o.sub = i;
+        o.mt = first + r % size;
+        o.nt = r / size;
+        o.kb = 0;
+        o.ke = (nk0(s) + s.nk[1]) * p.npass;
+        return true;
+      }
+      t -= n;
+    }
+    return false;
+  }
+};
+
+// ---------------------------------------------------------------------------
+// element helpers
+// ---------------------------------------------------------------------------
+
+// The three bf16 planes of an fp32 value; a value that is not finite lies in the first alone.
+__device__ __forceinline__ void split_planes(float v, uint16_t (&w)[3]) {
+  const uint32_t b = __float_as_uint(v);
+  if ((b & 0x7f800000u) == 0x7f800000u) {
+    w[0] = (b & 0x007fffffu) ? 0x7fff : (uint16_t)(b >> 16);
+    w[1] = w[2] = 0;
+    return;
+  }
+  const float hi = __uint_as_float(b & 0xffff0000u), r = v - hi;
+  const uint32_t m = __float_as_uint(r) & 0xffff0000u;
+  w[0] = (uint16_t)(b >> 16);
+  w[1] = (uint16_t)(m >> 16);
+  w[2] = (uint16_t)(__float_as_uint(r - __uint_as_float(m)) >> 16);
+}
+
+__device__ __forceinline__ uint32_t pack16(float a, float b, bool f16) {
+  if (f16) {
+    __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&h);
+  }
+  return pack_bf16x2(a, b);
+}
+
+// 16 columns of one row from column `col` on (those below N).
+__device__ __forceinline__ void store16(const GemmOut& o, int64_t row, int col, int N, const float (&v)[16]) {
+  if (col >= N) return;
+  const int64_t at = row * o.ld + col;
+  const bool full = o.vec && col + 16 <= N;
+  if (o.kind == kOutF32) {
+    float* q = static_cast<float*>(o.p) + at;
+    if (full) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        reinterpret_cast<float4*>(q)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (col + i < N) q[i] = v[i];
+    }
+    return;
+  }
+  uint16_t* q = static_cast<uint16_t*>(o.p) + at;
+  const int np = o.kind == kOutPlanes ? 3 : 1;
+  for (int pl = 0; pl < np; ++pl, q += o.plane) {
+    uint32_t w[8];
+    if (o.kind == kOutPlanes) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        uint16_t a[3], b[3];
+        split_planes(v[2 * i], a);
+        split_planes(v[2 * i + 1], b);
+        const uint32_t x = pl == 0 ? a[0] : pl == 1 ? a[1] : a[2], y = pl == 0 ? b[0] : pl == 1 ? b[1] : b[2];
+        w[i] = x | (y << 16);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = pack16(v[2 * i], v[2 * i + 1], o.kind == kOutF16);
+    }
+    if (full) {
+      reinterpret_cast<uint4*>(q)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+      reinterpret_cast<uint4*>(q)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (col + i < N) q[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// the kernel
+// ---------------------------------------------------------------------------
+template <int EPI, bool PAIR>
+__global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_constant__ GemmParams p) {
+  constexpr int kTileM = PAIR ? 256 : 128;
+  extern __shared__ uint8_t smraw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smraw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + kGmBarOff);
+  uint64_t* full = bars;                  // [kGmStages]: the stage's copies landed
+  uint64_t* empty = bars + kGmStages;     // [kGmStages]: the MMAs reading the stage completed
+  uint64_t* accf = bars + 2 * kGmStages;  // [2]: accumulator finished
+  uint64_t* acce = accf + 2;              // [2]: accumulator read
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(acce + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tslot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kGmStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&accf[i], 1);
+      mbar_init(&acce[i], PAIR ? 16 : 8);  // one arrival per epilogue warp (of both CTAs)
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0) pair_tmem_alloc<PAIR>(tslot, 512);
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (PAIR) cluster_sync();  // both CTAs' barriers are initialised before any remote use
+  tc_fence_after();
+  const uint32_t tbase = *tslot;
+  const uint32_t rank = PAIR ? cluster_rank() : 0u;
+  const int64_t worker = PAIR ? blockIdx.x / 2 : blockIdx.x, nworkers = PAIR ? gridDim.x / 2 : gridDim.x;
+  const int bn = p.bn;
+  const int brows = PAIR ? bn / 2 : bn;  // B rows staged by this CTA
+  GemmSched<PAIR> sched(p, worker, nworkers);
+  auto give_up = [&]() {
+    *abort_flag = 1;
+    record_error(p.err, M3B_ERR_TIMEOUT);
+  };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      const uint32_t bytes = kGmStageA + (uint32_t)brows * 128u;
+      uint32_t it = 0;
+      GemmJob job;
+      while (!*abort_flag && sched.next(job)) {
+        const GemmSub& s = p.sub[job.sub];
+        const int nk0 = sched.nk0(s), nks = nk0 + s.nk[1];
+        const int arow = job.mt * kTileM + (int)rank * 128;
+        // B rows of this CTA; the gated product stages bn / 2 gate and bn / 2 up rows (paired: the
+        // first CTA holds the gate's, the second the up's)
+        const int brow = EPI == kEpiGlu ? job.nt * (bn / 2) : job.nt * bn + (int)rank * brows;
+        int pass = job.kb / (nks > 0 ? nks : 1), r = job.kb - pass * nks;
+        for (int i = job.kb; i < job.ke; ++i, ++it) {
+          const int st = (int)(it % kGmStages);
+          if (!mbar_wait(&empty[st], ((it / kGmStages) & 1) ^ 1, p.wait_ns)) {
+            give_up();
+            break;
+          }
+          const int seg = r >= nk0 ? 1 : 0, k = (seg ? r - nk0 : r) * kGmBK;
+          // plane pairs, smallest first: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0)
+          const int pp = (pass + 6 - p.npass) * 4;
+          const int pa = (0x001102 >> pp) & 3, pb = (0x010120 >> pp) & 3;
+          uint8_t* dA = sm + st * kGmStage;
+          uint8_t* dB = dA + kGmStageA;
+          uint32_t fb = smem_u32(&full[st]);
+          if constexpr (PAIR) {
+            if (rank == 0) mbar_arrive_expect_tx(&full[st], 2 * bytes);
+            fb = mapa_shared(fb, 0);
+          } else {
+            mbar_arrive_expect_tx(&full[st], bytes);
+          }
+          auto load = [&](void* dst, const CUtensorMap* m, int c0, int c1, int c2) {
+            if constexpr (PAIR) tma_load_3d_pair(dst, m, c0, c1, c2, fb);
+            else tma_load_3d(dst, m, c0, c1, c2, &full[st]);
+          };
+          if (s.a_mn) {
+            load(dA, &s.a[seg], arow, k, pa);
+            load(dA + 8192, &s.a[seg], arow + 64, k, pa);
+          } else {
+            load(dA, &s.a[seg], k, arow, pa);
+          }
+          if constexpr (EPI == kEpiGlu) {
+            if constexpr (PAIR) {
+              load(dB, &s.b[rank], k, brow, pb);
+            } else {
+              load(dB, &s.b[0], k, brow, pb);
+              load(dB + (bn / 2) * 128, &s.b[1], k, brow, pb);
+            }
+          } else if (s.b_mn) {
+            for (int c = 0; c < brows; c += 64) load(dB + c * 128, &s.b[seg], brow + c, k, pb);
+          } else {
+            load(dB, &s.b[seg], k, brow, pb);
+          }
+          if (++r == nks) {
+            r = 0;
+            ++pass;
+          }
+        }
+      }
+      // an aborted run leaves once the copies in flight have landed
+      if (*abort_flag && rank == 0)
+        for (uint32_t b = it > kGmStages ? it - kGmStages : 0; b < it; ++b)
+          mbar_wait(&full[b % kGmStages], (b / kGmStages) & 1, 10000000ull);
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      auto commit_both = [&](uint64_t* bar) {
+        if constexpr (PAIR) {
+          umma_commit_pair(smem_u32(bar));
+          umma_commit_pair(mapa_shared(smem_u32(bar), 1));
+        } else {
+          umma_commit(bar);
+        }
+      };
+      uint32_t it = 0, sc = 0;
+      GemmJob job;
+      for (; !*abort_flag && sched.next(job); ++sc) {
+        const GemmSub& s = p.sub[job.sub];
+        const int acc = (int)(sc & 1);
+        const bool drained = PAIR ? mbar_wait_cluster(&acce[acc], ((sc >> 1) & 1) ^ 1, p.wait_ns)
+                                  : mbar_wait(&acce[acc], ((sc >> 1) & 1) ^ 1, p.wait_ns);
+        if (!drained) {
+          give_up();
+          break;
+        }
+        tc_fence_after();
+        uint32_t idesc = idesc_bf16(kTileM, bn, s.a_mn != 0, s.b_mn != 0);
+        if (p.f16) idesc &= ~((1u << 7) | (1u << 10));
+        const uint32_t dt = tbase + (uint32_t)(acc * 256);
+        // descriptor step per 16 K values, in its 16-byte units: 32 bytes along a swizzled row, or
+        // two 8-row groups of an MN-major tile
+        const uint64_t sa = s.a_mn ? 128 : 2, sb = s.b_mn ? 128 : 2;
+        const uint32_t la = s.a_mn ? 8192 : 16, lb = s.b_mn ? 8192 : 16;
+        for (int i = job.kb; i < job.ke; ++i, ++it) {
+          const int st = (int)(it % kGmStages);
+          if (!mbar_wait(&full[st], (it / kGmStages) & 1, p.wait_ns)) {
+            give_up();
+            break;
+          }
+          tc_fence_after();
+          const uint32_t base = smem_u32(sm + st * kGmStage);
+          const uint64_t da = sdesc_sw128(base, la, 1024), db = sdesc_sw128(base + kGmStageA, lb, 1024);
+#pragma unroll
+          for (int kk = 0; kk < kGmBK / 16; ++kk) {
+            const uint32_t on = (i != job.kb || kk != 0) ? 1u : 0u;
+            if constexpr (PAIR) umma_bf16_pair(dt, da + kk * sa, db + kk * sb, idesc, on);
+            else umma_bf16(dt, da + kk * sa, db + kk * sb, idesc, on);
+          }
+          commit_both(&empty[st]);
+        }
+        if (*abort_flag) break;
+        commit_both(&accf[acc]);
+      }
+    }
+  } else {
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    const uint32_t tl = tbase + ((uint32_t)(q * 32) << 16);
+    uint32_t sc = 0;
+    GemmJob job;
+    for (; !__any_sync(0xffffffffu, *abort_flag) && sched.next(job); ++sc) {
+      const GemmSub& s = p.sub[job.sub];
+      const int acc = (int)(sc & 1);
+      const int64_t grow = (int64_t)job.mt * kTileM + (int64_t)rank * 128 + q * 32 + lane;
+      const int M = sched.rows(s);
+      const bool rok = grow < M;
+      const bool none = job.ke == job.kb;  // no K at all: the sum is zero
+      if (!__all_sync(0xffffffffu, mbar_wait(&accf[acc], (sc >> 1) & 1, p.wait_ns))) {
+        give_up();
+        break;
+      }
+      tc_fence_after();
+      const uint32_t tc = tl + (uint32_t)(acc * 256);
+      auto release = [&]() {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (PAIR) mbar_arrive_cluster(mapa_shared(smem_u32(&acce[acc]), 0));
+          else mbar_arrive(&acce[acc]);
+        }
+      };
+      auto ld16 = [&](int c, float (&v)[16]) {
+        uint32_t r[16];
+        __syncwarp();
+        tmem_ld16_async(tc + c, r);
+        tmem_wait_ld(r);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = none ? 0.f : __uint_as_float(r[i]);
+      };
+      if constexpr (EPI == kEpiStore) {
+        const int c1 = (half + 1) * (bn / 2);
+        float alpha = s.alpha;
+        if (s.alpha_num) alpha *= *s.alpha_num;
+        if (s.alpha_den) alpha = *s.alpha_den > 0 ? alpha / (float)*s.alpha_den : 0.f;
+        int64_t orow = grow;
+        if (s.row_index) orow = rok ? s.row_index[grow] : -1;
+        const int nq = s.nt * bn / 4;
+        for (int c = half * (bn / 2); c < c1; c += 16) {
+          const int col = job.nt * bn + c;
+          float v[16];
+          ld16(c, v);
+          if (col >= s.N) continue;
+          if (s.acc_mode != 0) {
+            float4* ap = reinterpret_cast<float4*>(s.acc) + ((grow >> 5) * nq + (col >> 2)) * 32 + lane;
+#pragma unroll
+            for (int i = 0; i < 4; ++i, ap += 32) {
+              if (s.acc_mode != 1) {
+                const float4 o = *ap;
+                v[4 * i] += o.x, v[4 * i + 1] += o.y, v[4 * i + 2] += o.z, v[4 * i + 3] += o.w;
+              }
+              if (s.acc_mode != 3) *ap = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+            }
+            if (s.acc_mode != 3) continue;
+          }
+          if (!rok || orow < 0) continue;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            if (s.bias && col + i < s.N) v[i] += ldf(s.bias, col + i, s.dt);
+            v[i] *= alpha;
+            if (s.residual && col + i < s.N) v[i] += ldf(s.residual, grow * s.ld_res + col + i, s.dt);
+          }
+          store16(s.out, orow, col, s.N, v);
+        }
+      } else if constexpr (EPI == kEpiGlu) {
+        const int hb = bn / 2, c1 = (half + 1) * (hb / 2);
+        for (int c = half * (hb / 2); c < c1; c += 16) {
+          const int col = job.nt * hb + c;
+          float g[16], u[16];
+          ld16(c, g);
+          ld16(hb + c, u);
+          if (col >= s.N) continue;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            if (s.bias && col + i < s.N) g[i] += ldf(s.bias, col + i, s.dt);
+            if (s.bias2 && col + i < s.N) u[i] += ldf(s.bias2, col + i, s.dt);
+          }
+          if (p.gu) {
+            float4* gp = reinterpret_cast<float4*>(p.gu) + ((grow >> 5) * p.gu_ld4 + (col >> 2)) * 64 + lane;
+#pragma unroll
+            for (int i = 0; i < 4; ++i, gp += 64) {
+              gp[0] = make_float4(g[4 * i], g[4 * i + 1], g[4 * i + 2], g[4 * i + 3]);
+              gp[32] = make_float4(u[4 * i], u[4 * i + 1], u[4 * i + 2], u[4 * i + 3]);
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) g[i] = g[i] * sigmoid_fast(g[i]) * u[i];
+          if (rok) store16(s.out, grow, col, s.N, g);
+        }
+      } else if constexpr (EPI == kEpiDglu) {
+        const int c1 = (half + 1) * (bn / 2);
+        for (int c = half * (bn / 2); c < c1; c += 16) {
+          const int col = job.nt * bn + c;
+          float d[16], g[16], u[16];
+          ld16(c, d);
+          if (col >= s.N || !rok) continue;
+          const float4* gp = reinterpret_cast<const float4*>(p.gu) + ((grow >> 5) * p.gu_ld4 + (col >> 2)) * 64 + lane;
+#pragma unroll
+          for (int i = 0; i < 4; ++i, gp += 64) {
+            const float4 a = gp[0], b = gp[32];
+            g[4 * i] = a.x, g[4 * i + 1] = a.y, g[4 * i + 2] = a.z, g[4 * i + 3] = a.w;
+            u[4 * i] = b.x, u[4 * i + 1] = b.y, u[4 * i + 2] = b.z, u[4 * i + 3] = b.w;
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float sg = sigmoid_fast(g[i]), da = d[i] * s.alpha, ds = da * sg;
+            d[i] = ds * u[i] * fmaf(g[i], 1.f - sg, 1.f);
+            u[i] = ds * g[i];
+          }
+          store16(s.out, grow, col, s.N, d);
+          store16(s.out2, grow, col, s.N, u);
+        }
+      } else if constexpr (EPI == kEpiLse) {
+        const int c1 = (half + 1) * (bn / 2);
+        const int tgt = rok ? p.target[grow] : -1;
+        float m = -1e30f, sum = 0.f;
+        for (int c = half * (bn / 2); c < c1; c += 16) {
+          const int col = job.nt * bn + c;
+          float v[16];
+          ld16(c, v);
+          if (col >= s.N) continue;
+          const int to = tgt - col;
+          if (to >= 0 && to < 16) {
+            float x = v[0];
+#pragma unroll
+            for (int i = 1; i < 16; ++i) x = to == i ? v[i] : x;
+            p.target_logit[grow] = x;
+          }
+          float top = m;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            v[i] = col + i < s.N ? v[i] * kLog2e : -INFINITY;
+            top = fmaxf(top, v[i]);
+          }
+          sum *= ex2_fast(m - top);
+          m = top;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sum += ex2_fast(v[i] - top);
+        }
+        if (rok) p.part[(int64_t)(job.nt * 2 + half) * p.part_ld + grow] = make_float2(m, sum);
+      } else {
+        const int c1 = (half + 1) * (bn / 2);
+        const int tgt = rok ? p.target[grow] - p.col0 : -1;
+        const float l2 = rok ? p.lse2[grow] : 0.f, w = rok && p.roww ? p.roww[grow] : 1.f;
+        for (int c = half * (bn / 2); c < c1; c += 16) {
+          const int col = job.nt * bn + c;
+          float v[16];
+          ld16(c, v);
+          if (col >= s.N) continue;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float e = ex2_fast(fmaf(v[i], kLog2e, -l2));
+            // rows behind the last kept token are K values of the next products: zero
+            v[i] = rok ? w * (col + i == tgt ? e - 1.f : e) : 0.f;
+          }
+          store16(s.out, grow, col, s.N, v);
+        }
+      }
+      release();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (PAIR) cluster_sync();  // no remote arrivals or MMAs into this CTA remain
+  if (warp == 0) {
+    tc_fence_after();
+    pair_tmem_dealloc<PAIR>(tbase, 512);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host side (gemm.cu)
+// ---------------------------------------------------------------------------
+
+// A 16-bit operand in memory: `planes` matrices of rows x cols, rows ld elements apart.
+struct GemmOperand {
+  const void* p;
+  int64_t rows, cols, ld, plane;
+  int planes;
+};
+// A matrix as the TMA can read it in place: 16-byte aligned rows.
+inline bool tma_ok(const void* p, int64_t ld_elems) { return aligned16(p) && ld_elems % 8 == 0; }
+
+// Tensor map of an operand; box_rows counts the other dimension's box when K is along the rows
+// (K-major), MN-major maps always use 64 x 64 boxes.
+int gemm_map(CUtensorMap* m, const GemmOperand& o, bool mn_major, int box_rows, bool f16);
+// Launch on `st`; fills mt / nt from M, N and bn.
+int launch_gemm(GemmParams& p, int epi, bool pair, cudaStream_t st);
+inline int gemm_tile_m(bool pair) { return pair ? 256 : 128; }
+// Rows of B per tensor-map box for `bn` accumulator columns.
+inline int gemm_box_b(bool pair, int bn, int epi) { return epi == kEpiGlu || pair ? bn / 2 : bn; }
+
+// dst planes (rows x cols, rows ld apart, zero up to ld_pad columns and rows_pad rows) of src
+// (dtype, rows src_ld apart, column stride src_cs): the operand form of a matrix the TMA cannot read
+// in place, or of an fp32 one (three bf16 planes).
+int launch_pack(const void* src, int dtype, int64_t rows, int64_t cols, int64_t src_ld, void* dst, int64_t ld,
+                int64_t plane, cudaStream_t st);
+
+}  // namespace m3b

@@ -29,6 +29,7 @@
 
 #include "common.cuh"
 #include "launch.h"
+#include "pair.cuh"
 #include "tmap.h"
 
 namespace m3b {
@@ -71,88 +72,6 @@ __device__ __forceinline__ void ip_fail(const IpParams& a, volatile int* abort_f
   record_error(a.err, M3B_ERR_TIMEOUT);
 }
 
-// ---- CTA-pair forms (PAIR) next to the single-CTA ones ----
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-// The shared::cluster address of the same offset in CTA `rank` of this cluster.
-__device__ __forceinline__ uint32_t mapa_shared(uint32_t addr, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-template <bool PAIR>
-__device__ __forceinline__ void ip_tmem_alloc(uint32_t* dst, uint32_t ncols) {
-  if constexpr (PAIR) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst)), "r"(ncols)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-  } else {
-    tmem_alloc(dst, ncols);
-    tmem_relinquish();
-  }
-}
-template <bool PAIR>
-__device__ __forceinline__ void ip_tmem_dealloc(uint32_t taddr, uint32_t ncols) {
-  if constexpr (PAIR)
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
-  else
-    tmem_dealloc(taddr, ncols);
-}
-// D (+)= A B^T over the pair: A rows [0, 128) from the first CTA's shared memory, [128, 256) from
-// the second's (same offset), B rows likewise split in halves; D rows in each CTA's TMEM.
-__device__ __forceinline__ void umma_bf16_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                               uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-// Arrive once on the mbarrier at shared::cluster address `bar` (this CTA's or its peer's) when the
-// pair MMAs issued so far by this thread have completed.
-__device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
-// TMA load into this CTA's shared memory whose completion counts on the mbarrier at shared::cluster
-// address `bar`, which may be the peer CTA's (no multicast: every CTA fetches its own box).
-__device__ __forceinline__ void tma_load_2d_pair(void* dst, const void* tmap, int c0, int c1, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
-      "[%4];" ::"r"(smem_u32(dst)),
-      "l"(tmap), "r"(c0), "r"(c1), "r"(bar)
-      : "memory");
-}
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-// mbar_wait with cluster-scope acquire (the phase completes by arrivals from the peer CTA too).
-__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, uint64_t limit_ns) {
-  auto try_wait = [&]() {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(smem_u32(bar)), "r"(parity), "r"(100000u)
-        : "memory");
-    return done != 0;
-  };
-  if (try_wait()) return true;
-  const uint64_t t0 = globaltimer_ns();
-  while (true) {
-    if (try_wait()) return true;
-    if (globaltimer_ns() - t0 > limit_ns) return false;
-  }
-}
-
 template <bool PAIR>
 __global__ void __launch_bounds__(kIpThreads, 1)
     in_proj_kernel(const __grid_constant__ IpParams a, const __grid_constant__ CUtensorMap tm_x,
@@ -184,7 +103,7 @@ __global__ void __launch_bounds__(kIpThreads, 1)
     *abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == 0) ip_tmem_alloc<PAIR>(tslot, 512);
+  if (warp == 0) pair_tmem_alloc<PAIR>(tslot, 512);
   if (warp == 1 && lane == 0) {
     prefetch_tensormap(&tm_x);
     prefetch_tensormap(&tm_w);
@@ -391,7 +310,7 @@ __global__ void __launch_bounds__(kIpThreads, 1)
   if constexpr (PAIR) cluster_sync();  // no remote arrivals or MMAs into this CTA remain
   if (warp == 0) {
     tc_fence_after();
-    ip_tmem_dealloc<PAIR>(tbase, 512);
+    pair_tmem_dealloc<PAIR>(tbase, 512);
   }
 }
 

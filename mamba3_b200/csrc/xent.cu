@@ -1,0 +1,478 @@
+// Cross entropy of the language-model head from the hidden states (m3b_linear_xent_fwd / _bwd).
+//
+//   z = h W^T;  lse_i = log sum_v exp(z_iv);  loss_i = lse_i - z_i[t_i]
+//   dz_iv = w_i (exp(z_iv - lse_i) - [v = t_i]);  dh = dz W;  dW = dz^T h
+// with w_i = dloss / kept rows (mean), dloss (sum) or dloss_i.
+//
+// The kept rows are first gathered into a dense operand, so ignored tokens cost nothing in any
+// product (and what they hold, NaN included, reaches no sum); how many remain is read on the device.
+// Forward: one product over all vocabulary tiles whose epilogue keeps each row's running maximum
+// and sum (in powers of two) and the target's logit; the logits never leave the SM.  A small kernel
+// joins the tiles' statistics.  Backward: a piece of the vocabulary at a time, the logits once more
+// with the softmax as their epilogue, and the piece's share of both gradients; dh is summed over the
+// pieces in fp32.  8 rows d_model vocab operations forward and backward, 2 more than with the
+// logits kept.
+#include "gemm.cuh"
+
+namespace m3b {
+
+namespace {
+
+constexpr size_t kPieceBytes = size_t(256) << 20;  // of softmax - onehot in memory at once
+constexpr int kPieceLeast = 2048;                   // columns of a piece at least
+
+inline int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
+
+struct Saved {
+  uint16_t* h;     // [planes][Tp][Dp] kept rows
+  int* row;        // [Tp] where they come from
+  int* target;     // [Tp]; -1 behind the last, -2 out of range
+  float* lse2;     // [Tp]
+  int* count;      // kept rows
+  size_t bytes;
+};
+
+struct Dims {
+  int64_t T, Tp, Dp;
+  int D, V, np;
+  bool f16, f32;
+  explicit Dims(const m3b_linear_xent_args* a)
+      : T(a->rows), Tp(up(a->rows, 256)), Dp(up(a->d_model, 8)), D(a->d_model), V(a->vocab),
+        np(a->dtype == M3B_F32 ? 3 : 1), f16(a->dtype == M3B_F16), f32(a->dtype == M3B_F32) {}
+};
+
+struct Carve {
+  uint8_t* base;
+  size_t at = 0;
+  explicit Carve(void* p) : base(static_cast<uint8_t*>(p)) {}
+  void* take(size_t bytes) {
+    void* r = base ? base + at : nullptr;
+    at += (bytes + 255) / 256 * 256;
+    return r;
+  }
+};
+
+Saved saved_of(const m3b_linear_xent_args* a, void* p) {
+  const Dims d(a);
+  Carve c(p);
+  Saved s{};
+  s.h = static_cast<uint16_t*>(c.take((size_t)d.np * d.Tp * d.Dp * 2));
+  s.row = static_cast<int*>(c.take((size_t)d.Tp * 4));
+  s.target = static_cast<int*>(c.take((size_t)d.Tp * 4));
+  s.lse2 = static_cast<float*>(c.take((size_t)d.Tp * 4));
+  s.count = static_cast<int*>(c.take(4));
+  s.bytes = c.at;
+  return s;
+}
+
+// One block: the kept rows' numbers and targets in order.  Each thread takes a run of rows, so one
+// scan over the threads' counts orders them.
+__global__ void __launch_bounds__(1024) keep_kernel(const int64_t* __restrict__ target, int64_t ignore, int64_t T,
+                                                    int64_t Tp, int V, Saved s, int* err) {
+  __shared__ int sums[32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t run = (T + 1023) / 1024, r0 = tid * run < T ? tid * run : T, r1 = r0 + run < T ? r0 + run : T;
+  int n = 0;
+#pragma unroll 4
+  for (int64_t r = r0; r < r1; ++r) n += target[r] != ignore;
+  int x = n;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  if (lane == 31) sums[warp] = x;
+  __syncthreads();
+  if (warp == 0) {
+    int w = sums[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, w, o);
+      if (lane >= o) w += y;
+    }
+    sums[lane] = w;
+  }
+  __syncthreads();
+  int at = x - n + (warp ? sums[warp - 1] : 0);
+  const int total = sums[31];
+#pragma unroll 4
+  for (int64_t r = r0; r < r1; ++r) {
+    const int64_t t = target[r];
+    if (t == ignore) continue;
+    const bool ok = t >= 0 && t < V;
+    if (!ok) record_error(err, M3B_ERR_INVALID_ARG);
+    s.row[at] = (int)r;
+    s.target[at] = ok ? (int)t : -2;
+    ++at;
+  }
+  for (int64_t i = total + tid; i < Tp; i += 1024) {
+    s.row[i] = -1;
+    s.target[i] = -1;
+  }
+  if (tid == 0) *s.count = total;
+}
+
+// One warp per row of the dense operand; rows behind the last kept one are zero up to the tile's end.
+__global__ void __launch_bounds__(256) gather_kernel(const void* __restrict__ h, int dt, int64_t ld, int D, int64_t Tp,
+                                                     int64_t Dp, int vec, Saved s) {
+  const int lane = threadIdx.x & 31;
+  const int64_t n = *s.count, end = (n + 255) / 256 * 256 < Tp ? (n + 255) / 256 * 256 : Tp;
+  const int64_t step = (int64_t)gridDim.x * 8, plane = Tp * Dp;
+  for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < end; i += step) {
+    const int64_t r = s.row[i];
+    uint16_t* dst = s.h + i * Dp;
+    if (dt != M3B_F32) {
+      const uint16_t* src = static_cast<const uint16_t*>(h) + r * ld;
+      if (vec) {
+        for (int c = lane; c < D / 8; c += 32)
+          reinterpret_cast<uint4*>(dst)[c] =
+              r >= 0 ? __ldg(reinterpret_cast<const uint4*>(src) + c) : make_uint4(0, 0, 0, 0);
+      } else {
+        for (int c = lane; c < Dp; c += 32) dst[c] = r >= 0 && c < D ? src[c] : 0;
+      }
+    } else {
+      const float* src = static_cast<const float*>(h) + r * ld;
+      for (int c = lane; c < Dp; c += 32) {
+        uint16_t w[3];
+        split_planes(r >= 0 && c < D ? src[c] : 0.f, w);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) dst[k * plane + c] = w[k];
+      }
+    }
+  }
+}
+
+// Join the tiles' statistics: 32 rows per block, eight threads per row.
+__global__ void __launch_bounds__(256) join_kernel(const float2* __restrict__ part, int slots, int64_t Tp,
+                                                   const float* __restrict__ target_logit, Saved s,
+                                                   float* __restrict__ row_loss) {
+  __shared__ float2 sm[8][32];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int n = *s.count;
+  const int64_t row = (int64_t)blockIdx.x * 32 + lane;
+  if ((int64_t)blockIdx.x * 32 >= n) return;
+  float m = -1e30f, sum = 0.f;
+  if (row < n) {
+#pragma unroll 4
+    for (int k = w; k < slots; k += 8) {
+      const float2 v = part[(int64_t)k * Tp + row];
+      const float top = fmaxf(m, v.x);
+      sum = sum * exp2f(m - top) + v.y * exp2f(v.x - top);
+      m = top;
+    }
+  }
+  sm[w][lane] = make_float2(m, sum);
+  __syncthreads();
+  if (w != 0 || row >= n) return;
+#pragma unroll
+  for (int k = 1; k < 8; ++k) {
+    const float2 v = sm[k][lane];
+    const float top = fmaxf(m, v.x);
+    sum = sum * exp2f(m - top) + v.y * exp2f(v.x - top);
+    m = top;
+  }
+  const bool ok = s.target[row] >= 0;
+  const float l2 = ok ? m + log2f(sum) : __int_as_float(0x7fffffff);
+  s.lse2[row] = l2;
+  row_loss[row] = l2 * kLn2 - (ok ? target_logit[row] : 0.f);
+}
+
+// The loss from the rows' losses: summed in a fixed order in fp64, or put at the rows' places.
+__global__ void __launch_bounds__(1024) loss_kernel(const float* __restrict__ row_loss, Saved s, int reduction,
+                                                    float* __restrict__ loss) {
+  const int n = *s.count;
+  if (reduction == 0) {
+    for (int i = threadIdx.x; i < n; i += 1024) loss[s.row[i]] = row_loss[i];
+    return;
+  }
+  __shared__ double sm[32];
+  double x = 0.0;
+  for (int i = threadIdx.x; i < n; i += 1024) x += (double)row_loss[i];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = x;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    x = sm[threadIdx.x];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    if (threadIdx.x == 0) *loss = (float)(reduction == 1 ? x / (double)n : x);
+  }
+}
+
+__global__ void roww_kernel(const float* __restrict__ dloss, Saved s, float* __restrict__ roww) {
+  const int n = *s.count;
+  for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < n; i += gridDim.x * blockDim.x) roww[i] = dloss[s.row[i]];
+}
+
+bool sizes_ok(const m3b_linear_xent_args* a) {
+  return a && a->rows >= 0 && a->d_model > 0 && a->vocab > 0 &&
+         (a->dtype == M3B_F32 || a->dtype == M3B_BF16 || a->dtype == M3B_F16);
+}
+
+int check(const m3b_linear_xent_args* a, bool bwd) {
+  if (!a) return fail(M3B_ERR_INVALID_ARG, "linear_xent: null args");
+  if (!sizes_ok(a)) return fail(M3B_ERR_INVALID_ARG, "linear_xent: bad sizes or dtype");
+  if (a->rows > (int64_t(1) << 31) - 512 || a->d_model > (1 << 24) || a->vocab > (1 << 30))
+    return fail(M3B_ERR_INVALID_ARG, "linear_xent: sizes past the kernels' limits");
+  if (a->reduction < 0 || a->reduction > 2) return fail(M3B_ERR_INVALID_ARG, "linear_xent: reduction");
+  if (!a->weight || !a->saved) return fail(M3B_ERR_INVALID_ARG, "linear_xent: null pointer");
+  if (!aligned16(a->saved)) return fail(M3B_ERR_ALIGNMENT, "linear_xent: saved must be 16-byte aligned");
+  if (bwd) {
+    if (!a->dloss) return fail(M3B_ERR_INVALID_ARG, "linear_xent_bwd: null pointer");
+  } else {
+    if ((a->rows && (!a->hidden || !a->target)) || (!a->loss && (a->rows || a->reduction)))
+      return fail(M3B_ERR_INVALID_ARG, "linear_xent_fwd: null pointer");
+    if (a->rows && a->hidden_stride < a->d_model)
+      return fail(M3B_ERR_INVALID_ARG, "linear_xent_fwd: row stride shorter than the rows");
+  }
+  return M3B_OK;
+}
+
+// The weight as an operand: in place, or packed (fp32, or rows that the TMA cannot read).
+GemmOperand weight_of(const m3b_linear_xent_args* a, Carve& ws, bool run, cudaStream_t st, int* rc) {
+  const Dims d(a);
+  if (!d.f32 && tma_ok(a->weight, d.D)) return GemmOperand{a->weight, d.V, d.D, d.D, 0, 1};
+  const int64_t plane = (int64_t)d.V * d.Dp;
+  void* p = ws.take((size_t)d.np * plane * 2);
+  if (run && *rc == M3B_OK) *rc = launch_pack(a->weight, a->dtype, d.V, d.D, d.D, p, d.Dp, plane, st);
+  return GemmOperand{p, d.V, d.D, d.Dp, plane, d.np};
+}
+
+GemmOperand piece_of(const GemmOperand& w, int64_t c0, int64_t cols) {
+  GemmOperand o = w;
+  o.p = static_cast<const uint16_t*>(w.p) + c0 * w.ld;
+  o.rows = cols;
+  if (o.planes == 1) o.plane = 0;
+  return o;
+}
+
+#define M3B_TRY(x)                     \
+  do {                                 \
+    const int rc_ = (x);               \
+    if (rc_ != M3B_OK) return rc_;     \
+  } while (0)
+#define M3B_MAP(...) M3B_TRY(gemm_map(__VA_ARGS__))
+
+int forward(const m3b_linear_xent_args* a, void* workspace, size_t* need, bool run, cudaStream_t st) {
+  const Dims d(a);
+  Carve ws(workspace);
+  const bool pair = d.T > 128;
+  const int bn = pair ? 256 : 128;
+  const int nt = (d.V + bn - 1) / bn;
+  float* target_logit = static_cast<float*>(ws.take((size_t)d.Tp * 4));
+  float* row_loss = static_cast<float*>(ws.take((size_t)d.Tp * 4));
+  float2* part = static_cast<float2*>(ws.take((size_t)nt * 2 * d.Tp * 8));
+  const Saved s = saved_of(a, a->saved);
+  int rc = M3B_OK;
+  if (run) {
+    keep_kernel<<<1, 1024, 0, st>>>(a->target, a->ignore_index, d.T, d.Tp, d.V, s, a->err);
+    const int64_t blocks = d.Tp / 8, most = (int64_t)num_sms() * 8;
+    const int vec = !d.f32 && d.D % 8 == 0 && a->hidden_stride % 8 == 0 && aligned16(a->hidden);
+    gather_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, st>>>(a->hidden, a->dtype, a->hidden_stride, d.D,
+                                                                            d.Tp, d.Dp, vec, s);
+    M3B_TRY(check_launch("linear_xent gather"));
+  }
+  const GemmOperand w = weight_of(a, ws, run, st, &rc);
+  *need = ws.at;
+  if (!run || rc != M3B_OK) return rc;
+  GemmParams p{};
+  GemmSub& g = p.sub[0];
+  p.nsub = 1;
+  p.bn = bn;
+  p.npass = d.f32 ? 6 : 1;
+  p.f16 = d.f16;
+  p.dyn = s.count;
+  p.err = a->err;
+  const GemmOperand h{s.h, d.Tp, d.D, d.Dp, d.Tp * d.Dp, d.np};
+  M3B_MAP(&g.a[0], h, false, 128, d.f16);
+  M3B_MAP(&g.b[0], w, false, gemm_box_b(pair, bn, kEpiLse), d.f16);
+  g.M = (int)d.T;
+  g.m_dyn = 1;
+  g.N = d.V;
+  g.nk[0] = (d.D + kGmBK - 1) / kGmBK;
+  p.target = s.target;
+  p.target_logit = target_logit;
+  p.part = part;
+  p.part_ld = d.Tp;
+  M3B_TRY(launch_gemm(p, kEpiLse, pair, st));
+  join_kernel<<<(unsigned)(d.Tp / 32), 256, 0, st>>>(part, nt * 2, d.Tp, target_logit, s, row_loss);
+  if (a->reduction == 0 && cudaMemsetAsync(a->loss, 0, (size_t)d.T * 4, st) != cudaSuccess)
+    return check_launch("linear_xent loss");
+  loss_kernel<<<1, 1024, 0, st>>>(row_loss, s, a->reduction, a->loss);
+  return check_launch("linear_xent loss");
+}
+
+// Columns of a piece of the vocabulary.
+int64_t piece_cols(const Dims& d) {
+  int64_t c = (int64_t)(kPieceBytes / ((size_t)d.np * 2 * d.Tp)) / 256 * 256;
+  if (c < kPieceLeast) c = kPieceLeast;
+  return c < d.V ? c : d.V;
+}
+
+int backward(const m3b_linear_xent_args* a, void* workspace, size_t* need, bool run, cudaStream_t st) {
+  const Dims d(a);
+  Carve ws(workspace);
+  const int64_t cols = piece_cols(d), ldz = up(cols, 8);
+  const int bn = 256;
+  int rc = M3B_OK;
+  uint16_t* dz = static_cast<uint16_t*>(ws.take((size_t)d.np * d.Tp * ldz * 2));
+  float* acc = nullptr;
+  if (a->dhidden && cols < d.V) acc = static_cast<float*>(ws.take((size_t)d.Tp * up(d.D, bn) * 4));
+  float* roww = nullptr;
+  if (a->reduction == 0) roww = static_cast<float*>(ws.take((size_t)d.Tp * 4));
+  const GemmOperand w = weight_of(a, ws, run, st, &rc);
+  *need = ws.at;
+  if (!run || rc != M3B_OK) return rc;
+  const Saved s = saved_of(a, a->saved);
+  const size_t es = d.f32 ? 4 : 2;
+  if (a->dhidden && cudaMemsetAsync(a->dhidden, 0, (size_t)d.T * d.D * es, st) != cudaSuccess)
+    return check_launch("linear_xent_bwd");
+  if (roww) {
+    roww_kernel<<<64, 256, 0, st>>>(a->dloss, s, roww);
+    M3B_TRY(check_launch("linear_xent roww"));
+  }
+  const GemmOperand h{s.h, d.Tp, d.D, d.Dp, d.Tp * d.Dp, d.np};
+  const int okind = d.f32 ? kOutF32 : d.f16 ? kOutF16 : kOutBf16;
+  for (int64_t c0 = 0; c0 < d.V; c0 += cols) {
+    const int64_t n = d.V - c0 < cols ? d.V - c0 : cols;
+    const GemmOperand wp = piece_of(w, c0, n);
+    const GemmOperand z{dz, d.Tp, n, ldz, d.Tp * ldz, d.np};
+    GemmParams base{};
+    base.bn = bn;
+    base.nsub = 1;
+    base.npass = d.f32 ? 6 : 1;
+    base.f16 = d.f16;
+    base.dyn = s.count;
+    base.err = a->err;
+    {  // softmax - onehot of the piece
+      GemmParams p = base;
+      GemmSub& g = p.sub[0];
+      M3B_MAP(&g.a[0], h, false, 128, d.f16);
+      M3B_MAP(&g.b[0], wp, false, gemm_box_b(true, bn, kEpiDlogit), d.f16);
+      g.M = (int)d.T;
+      g.m_dyn = 1;
+      g.N = (int)n;
+      g.nk[0] = (d.D + kGmBK - 1) / kGmBK;
+      g.out.p = dz;
+      g.out.ld = ldz;
+      g.out.plane = z.plane;
+      g.out.kind = d.f32 ? kOutPlanes : okind;
+      g.out.vec = 1;
+      p.target = s.target;
+      p.lse2 = s.lse2;
+      p.roww = roww;
+      p.col0 = (int)c0;
+      M3B_TRY(launch_gemm(p, kEpiDlogit, true, st));
+    }
+    auto scaled = [&](GemmSub& g) {
+      g.alpha = 1.f;
+      if (a->reduction != 0) g.alpha_num = a->dloss;
+      if (a->reduction == 1) g.alpha_den = s.count;
+      g.out.kind = okind;
+      g.out.ld = d.D;
+    };
+    if (a->dhidden) {
+      GemmParams p = base;
+      GemmSub& g = p.sub[0];
+      M3B_MAP(&g.a[0], z, false, 128, d.f16);
+      M3B_MAP(&g.b[0], wp, true, 0, d.f16);
+      g.b_mn = 1;
+      g.M = (int)d.T;
+      g.m_dyn = 1;
+      g.N = d.D;
+      g.nk[0] = (int)((n + kGmBK - 1) / kGmBK);
+      scaled(g);
+      g.out.p = a->dhidden;
+      g.out.vec = aligned16(a->dhidden) && d.D % 8 == 0;
+      g.row_index = s.row;
+      g.acc = acc;
+      g.acc_mode = !acc ? 0 : c0 == 0 ? 1 : c0 + cols < d.V ? 2 : 3;
+      M3B_TRY(launch_gemm(p, kEpiStore, true, st));
+    }
+    if (a->dweight) {
+      GemmParams p = base;
+      GemmSub& g = p.sub[0];
+      M3B_MAP(&g.a[0], z, true, 0, d.f16);
+      M3B_MAP(&g.b[0], h, true, 0, d.f16);
+      g.a_mn = g.b_mn = 1;
+      g.M = (int)n;
+      g.N = d.D;
+      g.nk[0] = 1;
+      g.k_dyn = 1;
+      scaled(g);
+      g.out.p = static_cast<uint8_t*>(a->dweight) + (size_t)c0 * d.D * es;
+      g.out.vec = aligned16(g.out.p) && d.D % 8 == 0;
+      M3B_TRY(launch_gemm(p, kEpiStore, true, st));
+    }
+  }
+  return M3B_OK;
+}
+
+int check_workspace(size_t need, const void* ws, size_t bytes) {
+  if (!ws || bytes < need) return fail(M3B_ERR_WORKSPACE, "linear_xent: workspace of %zu bytes, %zu needed", bytes, need);
+  if (!aligned16(ws)) return fail(M3B_ERR_ALIGNMENT, "linear_xent: workspace must be 16-byte aligned");
+  return M3B_OK;
+}
+
+// No rows: the sum is 0, the mean 0 / 0.
+__global__ void empty_loss_kernel(float* loss, int reduction) {
+  *loss = reduction == 1 ? __int_as_float(0x7fffffff) : 0.f;
+}
+
+}  // namespace
+
+}  // namespace m3b
+
+extern "C" {
+
+size_t m3b_linear_xent_saved(const m3b_linear_xent_args* a) {
+  return m3b::sizes_ok(a) ? m3b::saved_of(a, nullptr).bytes : 0;
+}
+
+size_t m3b_linear_xent_fwd_workspace(const m3b_linear_xent_args* a) {
+  size_t need = 0;
+  if (m3b::sizes_ok(a) && a->rows) m3b::forward(a, nullptr, &need, false, nullptr);
+  return need;
+}
+
+int m3b_linear_xent_fwd(const m3b_linear_xent_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+  m3b::clear_error();
+  int rc = m3b::check(a, false);
+  if (rc != M3B_OK) return rc;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (a->rows == 0) {
+    if (a->reduction == 0) return M3B_OK;
+    m3b::empty_loss_kernel<<<1, 1, 0, st>>>(a->loss, a->reduction);
+    return m3b::check_launch("linear_xent_fwd");
+  }
+  size_t need = 0;
+  m3b::forward(a, nullptr, &need, false, nullptr);
+  rc = m3b::check_workspace(need, workspace, workspace_bytes);
+  return rc != M3B_OK ? rc : m3b::forward(a, workspace, &need, true, st);
+}
+
+size_t m3b_linear_xent_bwd_workspace(const m3b_linear_xent_args* a) {
+  size_t need = 0;
+  if (m3b::sizes_ok(a) && a->rows) m3b::backward(a, nullptr, &need, false, nullptr);
+  return need;
+}
+
+int m3b_linear_xent_bwd(const m3b_linear_xent_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+  m3b::clear_error();
+  int rc = m3b::check(a, true);
+  if (rc != M3B_OK) return rc;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (a->rows == 0) {
+    const size_t es = a->dtype == M3B_F32 ? 4 : 2;
+    if (a->dweight && cudaMemsetAsync(a->dweight, 0, (size_t)a->vocab * a->d_model * es, st) != cudaSuccess)
+      return m3b::check_launch("linear_xent_bwd");
+    return M3B_OK;
+  }
+  size_t need = 0;
+  m3b::backward(a, nullptr, &need, false, nullptr);
+  rc = m3b::check_workspace(need, workspace, workspace_bytes);
+  return rc != M3B_OK ? rc : m3b::backward(a, workspace, &need, true, st);
+}
+
+}  // extern "C"

@@ -1,0 +1,85 @@
+"""The gated feed-forward block as one operator, forward and backward (``gated_ffn``).
+
+    out = residual + residual_scale * (silu(x Wg^T + bg) * (x Wu^T + bu)) Wd^T + bd scaled alike
+
+It is the blocks' SwiGLU (mamba3/block.py:16-26) with the scaled residual that follows it
+(mamba3/block.py:79-107): both projections, the activation and the product are one kernel, the down
+projection with bias and residual another; single tokens, decode batches and long prompts run the
+same call.  ``SwiGLU(..., fused=True)``, ``KulaMambaBlock`` / ``KulaMambaLM(..., fused_mlp=True)``
+run their MLP through it.
+"""
+
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib, ops
+
+
+class _GatedFfn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual, scale):
+        out, act, gu = ops.gated_ffn_fwd(x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual, scale, True)
+        ctx.save_for_backward(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act, gu)
+        ctx.scale = scale
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        x, w_gate, w_up, w_down, b_gate, b_up, b_down, act, gu = ctx.saved_tensors
+        want = ctx.needs_input_grad
+        grads = [None] * 7
+        if any(want[:7]):
+            grads = ops.gated_ffn_bwd(x, w_gate, w_up, w_down, b_gate, b_up, b_down, ctx.scale, act, gu,
+                                      _lib._rows2d(dout, x.shape[1]), list(want[:7]))
+        return (*grads, dout if want[7] else None, None)
+
+
+def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, *,
+              b_gate: torch.Tensor | None = None, b_up: torch.Tensor | None = None,
+              b_down: torch.Tensor | None = None, residual: torch.Tensor | None = None,
+              residual_scale: float = 1.0) -> torch.Tensor:
+    """residual + residual_scale * (act w_down^T + b_down), act = silu(x w_gate^T + b_gate) * (x w_up^T + b_up).
+
+    x (..., d_model); w_gate, w_up (d_ff, d_model); w_down (d_model, d_ff), as nn.Linear stores them;
+    b_gate and b_up (d_ff) come together, b_down (d_model) on its own; residual has x's shape.  All of
+    one dtype (fp32, bf16 or fp16) on one CUDA device; under autocast every argument is cast to the
+    autocast dtype first.  Any sizes and strides: operands that the copies cannot read in place
+    (widths that are no multiple of 8, a last dimension with a stride, fp32) are laid out once per
+    call.  Differentiable in every tensor argument; sums in fp32, and the activation (forward) and its
+    two factors' gradients (backward) rounded to a 16-bit dtype once."""
+    ts = [x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual]
+    if x.is_cuda and torch.is_autocast_enabled("cuda"):
+        dt = torch.get_autocast_dtype("cuda")
+        ts = [t if t is None or t.dtype == dt else t.to(dt) for t in ts]
+        x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual = ts
+    _lib._cuda(*ts)
+    if any(t is not None and t.dtype != x.dtype for t in ts):
+        raise _lib.M3bError(f"gated_ffn: one dtype expected, got {[t.dtype for t in ts if t is not None]}")
+    _lib.dtype_code(x.dtype)
+    if x.dim() < 1 or w_gate.dim() != 2:
+        raise ValueError("gated_ffn: x (..., d_model) and w_gate (d_ff, d_model) expected")
+    f, d = w_gate.shape
+    if x.shape[-1] != d or w_up.shape != (f, d) or w_down.shape != (d, f):
+        raise ValueError(f"gated_ffn: x (..., {d}), w_up ({f}, {d}) and w_down ({d}, {f}) expected, got "
+                         f"{tuple(x.shape)}, {tuple(w_up.shape)} and {tuple(w_down.shape)}")
+    if d == 0 or f == 0:
+        raise ValueError("gated_ffn: d_model and d_ff must be positive")
+    if (b_gate is None) != (b_up is None):
+        raise ValueError("gated_ffn: b_gate and b_up go together")
+    for name, b, n in (("b_gate", b_gate, f), ("b_up", b_up, f), ("b_down", b_down, d)):
+        if b is not None and b.shape != (n,):
+            raise ValueError(f"gated_ffn: {name} ({n},) expected, got {tuple(b.shape)}")
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError(f"gated_ffn: residual must have x's shape {tuple(x.shape)}, got {tuple(residual.shape)}")
+    x2 = _lib._rows2d(x, d)
+    r2 = None if residual is None else _lib._rows2d(residual, d)
+    ws = [None if t is None else t.contiguous() for t in (w_gate, w_up, w_down, b_gate, b_up, b_down)]
+    scale = float(residual_scale)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+        y = _GatedFfn.apply(x2, *ws, r2, scale)
+    else:
+        y = ops.gated_ffn_fwd(x2, *ws, r2, scale, False)[0]
+    return y.view(x.shape)

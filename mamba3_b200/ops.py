@@ -458,3 +458,103 @@ def layer_state_compact(proj, prm_tensors, dims, state=None):
                    h_final=out["h"], angle_final=out["angle"], prev_b_final=out["prev_B"],
                    prev_x_final=out["prev_x"], stage_events=current_stage_events(), algo=_LAYER_ALGO)
     return y, out
+
+
+# ---------------------------------------------------------------------------
+# gated feed-forward and the head's cross entropy.  The custom ops make them opaque nodes
+# under torch.compile; eager calls go straight to the library (a custom op costs tens of
+# microseconds of host time, more than a single-token call takes on the device).
+# ---------------------------------------------------------------------------
+def _opt(t, dev, dt=torch.uint8):
+    return torch.empty(0, dtype=dt, device=dev) if t is None else t
+
+
+@torch.library.custom_op("mamba3_b200::gated_ffn_fwd", mutates_args=())
+def _gated_ffn_fwd_op(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
+                      b_gate: Optional[torch.Tensor], b_up: Optional[torch.Tensor], b_down: Optional[torch.Tensor],
+                      residual: Optional[torch.Tensor], scale: float,
+                      save: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    out, act, gu = _lib.gated_ffn_fwd(x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual, scale, save)
+    return out, act, _opt(gu, x.device)
+
+
+def _ffn_saved_bytes(x, f):
+    rows, planes = x.shape[0], 3 if x.dtype == torch.float32 else 1
+    return planes * rows * ((f + 7) // 8 * 8) * 2, ((rows + 255) // 256 * 256) * ((f + 15) // 16 * 16) * 8
+
+
+@_gated_ffn_fwd_op.register_fake
+def _(x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual, scale, save):
+    act, gu = _ffn_saved_bytes(x, w_gate.shape[0])
+    u8 = dict(dtype=torch.uint8, device=x.device)
+    return x.new_empty(x.shape), torch.empty(act, **u8), torch.empty(gu if save else 0, **u8)
+
+
+@torch.library.custom_op("mamba3_b200::gated_ffn_bwd", mutates_args=())
+def _gated_ffn_bwd_op(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
+                      b_gate: Optional[torch.Tensor], b_up: Optional[torch.Tensor], b_down: Optional[torch.Tensor],
+                      scale: float, act: torch.Tensor, gu: torch.Tensor, dout: torch.Tensor,
+                      want: list[bool]) -> list[torch.Tensor]:
+    g = _lib.gated_ffn_bwd(x, w_gate, w_up, w_down, b_gate, b_up, b_down, scale, act, gu, dout, want)
+    return [_opt(t, x.device, x.dtype) for t in g]
+
+
+@_gated_ffn_bwd_op.register_fake
+def _(x, w_gate, w_up, w_down, b_gate, b_up, b_down, scale, act, gu, dout, want):
+    ins = (x, w_gate, w_up, w_down, b_gate, b_up, b_down)
+    return [x.new_empty(t.shape if w and t is not None else (0,)) for t, w in zip(ins, want)]
+
+
+def gated_ffn_fwd(x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual, scale, save):
+    f = _gated_ffn_fwd_op if torch.compiler.is_compiling() else _lib.gated_ffn_fwd
+    return f(x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual, scale, save)
+
+
+def gated_ffn_bwd(x, w_gate, w_up, w_down, b_gate, b_up, b_down, scale, act, gu, dout, want):
+    if not torch.compiler.is_compiling():
+        return _lib.gated_ffn_bwd(x, w_gate, w_up, w_down, b_gate, b_up, b_down, scale, act, gu, dout, want)
+    ins = (x, w_gate, w_up, w_down, b_gate, b_up, b_down)
+    g = _gated_ffn_bwd_op(x, w_gate, w_up, w_down, b_gate, b_up, b_down, scale, act, gu, dout, want)
+    return [r if w and t is not None else None for r, w, t in zip(g, want, ins)]
+
+
+@torch.library.custom_op("mamba3_b200::linear_xent_fwd", mutates_args=())
+def _linear_xent_fwd_op(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, ignore_index: int,
+                        reduction: str) -> tuple[torch.Tensor, torch.Tensor]:
+    return _lib.linear_xent_fwd(hidden, weight, target, ignore_index, reduction)
+
+
+@_linear_xent_fwd_op.register_fake
+def _(hidden, weight, target, ignore_index, reduction):
+    rows, d = hidden.shape
+    tp, planes = (rows + 255) // 256 * 256, 3 if hidden.dtype == torch.float32 else 1
+    up = lambda n: (n + 255) // 256 * 256  # noqa: E731
+    saved = up(planes * tp * ((d + 7) // 8 * 8) * 2) + 3 * up(tp * 4) + 256
+    return (torch.empty((rows,) if reduction == "none" else (), dtype=torch.float32, device=hidden.device),
+            torch.empty(saved, dtype=torch.uint8, device=hidden.device))
+
+
+@torch.library.custom_op("mamba3_b200::linear_xent_bwd", mutates_args=())
+def _linear_xent_bwd_op(rows: int, weight: torch.Tensor, saved: torch.Tensor, dloss: torch.Tensor, ignore_index: int,
+                        reduction: str, want_hidden: bool,
+                        want_weight: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    dh, dw = _lib.linear_xent_bwd(rows, weight, saved, dloss, ignore_index, reduction, want_hidden, want_weight)
+    return _opt(dh, weight.device, weight.dtype), _opt(dw, weight.device, weight.dtype)
+
+
+@_linear_xent_bwd_op.register_fake
+def _(rows, weight, saved, dloss, ignore_index, reduction, want_hidden, want_weight):
+    return (weight.new_empty((rows, weight.shape[1]) if want_hidden else (0,)),
+            weight.new_empty(weight.shape if want_weight else (0,)))
+
+
+def linear_xent_fwd(hidden, weight, target, ignore_index, reduction):
+    f = _linear_xent_fwd_op if torch.compiler.is_compiling() else _lib.linear_xent_fwd
+    return f(hidden, weight, target, ignore_index, reduction)
+
+
+def linear_xent_bwd(rows, weight, saved, dloss, ignore_index, reduction, want_hidden, want_weight):
+    if not torch.compiler.is_compiling():
+        return _lib.linear_xent_bwd(rows, weight, saved, dloss, ignore_index, reduction, want_hidden, want_weight)
+    dh, dw = _linear_xent_bwd_op(rows, weight, saved, dloss, ignore_index, reduction, want_hidden, want_weight)
+    return dh if want_hidden else None, dw if want_weight else None
