@@ -156,7 +156,7 @@ int forward(const m3b_gated_ffn_args* a, void* workspace, size_t* need, bool run
     GemmParams p{};
     GemmSub& s = p.sub[0];
     p.nsub = 1;
-    p.bn = pair ? 256 : 64;
+    p.bn = pair ? 256 : 128;
     p.npass = d.f32 ? 6 : 1;
     p.f16 = d.f16;
     p.err = a->err;
@@ -171,13 +171,13 @@ int forward(const m3b_gated_ffn_args* a, void* workspace, size_t* need, bool run
     s.bias2 = a->b_up;
     s.dt = a->dtype;
     p.gu = static_cast<float*>(a->saved_gu);
-    p.gu_ld4 = up(d.F, 16) / 4;
+    p.gu_ld4 = up(d.F, 32) / 4;
     M3B_TRY(launch_gemm(p, kEpiGlu, pair, st));
   }
   GemmParams p{};
   GemmSub& s = p.sub[0];
   p.nsub = 1;
-  p.bn = pair ? 256 : 32;
+  p.bn = pair ? 256 : 64;
   p.npass = d.f32 ? 6 : 1;
   p.f16 = d.f16;
   p.err = a->err;
@@ -191,6 +191,7 @@ int forward(const m3b_gated_ffn_args* a, void* workspace, size_t* need, bool run
   s.bias = a->b_down;
   s.residual = a->residual;
   s.ld_res = a->residual_stride;
+  s.res_vec = aligned16(a->residual) && a->residual_stride % 4 == 0;
   s.dt = a->dtype;
   return launch_gemm(p, kEpiStore, pair, st);
 }
@@ -231,7 +232,7 @@ int backward(const m3b_gated_ffn_args* a, void* workspace, size_t* need, bool ru
     s.out = operand_out(dg, d.f16);
     s.out2 = operand_out(du, d.f16);
     p.gu = static_cast<float*>(a->saved_gu);
-    p.gu_ld4 = up(d.F, 16) / 4;
+    p.gu_ld4 = up(d.F, 32) / 4;
     M3B_TRY(launch_gemm(p, kEpiDglu, true, st));
   }
   if (a->dx) {
@@ -308,7 +309,7 @@ size_t m3b_gated_ffn_act_bytes(const m3b_gated_ffn_args* a) {
 
 size_t m3b_gated_ffn_gu_bytes(const m3b_gated_ffn_args* a) {
   if (!m3b::sizes_ok(a)) return 0;
-  return (size_t)m3b::up(a->rows, 256) * m3b::up(a->d_ff, 16) * 8;
+  return (size_t)m3b::up(a->rows, 256) * m3b::up(a->d_ff, 32) * 8;
 }
 
 size_t m3b_gated_ffn_fwd_workspace(const m3b_gated_ffn_args* a) {

@@ -34,7 +34,9 @@ constexpr int kGmStages = 6;
 constexpr uint32_t kGmStageA = 128 * kGmBK * 2;     // 16 KB
 constexpr uint32_t kGmStage = 2 * kGmStageA;        // + B: at most 128 rows of 64
 constexpr uint32_t kGmRing = kGmStages * kGmStage;  // 192 KB
-constexpr uint32_t kGmBarOff = kGmRing;
+constexpr uint32_t kGmBox = 32 * 128;               // staging of an epilogue warp: 32 rows x 32 fp32
+constexpr uint32_t kGmBoxOff = kGmRing;
+constexpr uint32_t kGmBarOff = kGmBoxOff + 8 * kGmBox;
 constexpr uint32_t kGmSmem = kGmBarOff + 256 + 1024;
 static_assert(kGmSmem <= 227 * 1024, "shared memory plan");
 
@@ -79,7 +81,7 @@ struct GemmSub {
   const int* row_index;    // result row r goes to row row_index[r] (negative: nowhere)
   float* acc;              // running fp32 sum, [row / 32][col / 4][row % 32][4]
   int acc_mode;            // 0 none, 1 acc = v, 2 acc += v, 3 out = acc + v
-  int dt;                  // dtype code of bias and residual
+  int dt, res_vec;         // dtype code of bias and residual; the residual's rows allow vector loads
 };
 
 struct GemmParams {
@@ -89,7 +91,8 @@ struct GemmParams {
   int npass;    // plane pairs: 1, or 6 for fp32 operands
   int f16;      // operand type: fp16 instead of bf16
   const int* dyn;
-  // kEpiGlu / kEpiDglu: g and u in fp32, [row / 32][col / 4][g, u][row % 32][4], ld4 = column quads
+  // kEpiGlu / kEpiDglu: g and u in fp32, [row / 32][col / 4][g, u][row % 32][4], ld4 = column quads (of
+  // whole runs of 32 columns)
   float* gu;
   int64_t gu_ld4;
   // kEpiLse / kEpiDlogit
@@ -175,49 +178,157 @@ __device__ __forceinline__ uint32_t pack16(float a, float b, bool f16) {
   return pack_bf16x2(a, b);
 }
 
-// 16 columns of one row from column `col` on (those below N).
-__device__ __forceinline__ void store16(const GemmOut& o, int64_t row, int col, int N, const float (&v)[16]) {
-  if (col >= N) return;
-  const int64_t at = row * o.ld + col;
-  const bool full = o.vec && col + 16 <= N;
-  if (o.kind == kOutF32) {
-    float* q = static_cast<float*>(o.p) + at;
-    if (full) {
+// Results leave through a staging box per epilogue warp: a thread owns one row of the accumulator,
+// but a warp's stores should cover whole 32-byte sectors of few rows.  Each thread writes its 32
+// columns into the box (16-byte chunks swizzled by the row, so neither side has bank conflicts) and
+// the warp reads the box back row by row.
+struct GemmRows {
+  int64_t row0;          // first of the warp's 32 rows
+  int M;                 // rows of the result
+  const int* row_index;  // or null
+  __device__ __forceinline__ int64_t out_row(int r) const {
+    const int64_t row = row0 + r;
+    if (row >= M) return -1;
+    return row_index ? (int64_t)row_index[row] : row;
+  }
+};
+
+// 32 columns from `col` on of 16-bit values, packed in pairs.
+__device__ __forceinline__ void put16(uint8_t* box, const GemmOut& o, uint16_t* base, const GemmRows& rows, int col, int N,
+                                      const uint32_t (&w)[16]) {
+  const int lane = threadIdx.x & 31;
+  __syncwarp();  // the box has been read
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        reinterpret_cast<float4*>(q)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+  for (int k = 0; k < 4; ++k)
+    *reinterpret_cast<uint4*>(box + lane * 64 + ((k ^ ((lane >> 1) & 3)) << 4)) =
+        make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+  __syncwarp();
+  const int k = lane & 3, c = col + 8 * k;
+#pragma unroll
+  for (int it = 0; it < 4; ++it) {
+    const int r = it * 8 + (lane >> 2);
+    const uint4 v = *reinterpret_cast<const uint4*>(box + r * 64 + ((k ^ ((r >> 1) & 3)) << 4));
+    const int64_t orow = rows.out_row(r);
+    if (orow < 0 || c >= N) continue;
+    uint16_t* q = base + orow * o.ld + c;
+    if (o.vec && c + 8 <= N) {
+      *reinterpret_cast<uint4*>(q) = v;
     } else {
+      const uint32_t x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (col + i < N) q[i] = v[i];
+      for (int e = 0; e < 8; ++e)
+        if (c + e < N) q[e] = (uint16_t)(x[e >> 1] >> (16 * (e & 1)));
     }
+  }
+}
+
+// The same of fp32 values, stored as a 16-bit type or as planes.
+__device__ __forceinline__ void put_operand(uint8_t* box, const GemmOut& o, const GemmRows& rows, int col, int N,
+                                            const float (&v)[32]) {
+  uint16_t* base = static_cast<uint16_t*>(o.p);
+  if (o.kind != kOutPlanes) {
+    uint32_t w[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w[i] = pack16(v[2 * i], v[2 * i + 1], o.kind == kOutF16);
+    put16(box, o, base, rows, col, N, w);
     return;
   }
-  uint16_t* q = static_cast<uint16_t*>(o.p) + at;
-  const int np = o.kind == kOutPlanes ? 3 : 1;
-  for (int pl = 0; pl < np; ++pl, q += o.plane) {
-    uint32_t w[8];
-    if (o.kind == kOutPlanes) {
+#pragma unroll 1
+  for (int pl = 0; pl < 3; ++pl, base += o.plane) {
+    uint32_t w[16];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        uint16_t a[3], b[3];
-        split_planes(v[2 * i], a);
-        split_planes(v[2 * i + 1], b);
-        const uint32_t x = pl == 0 ? a[0] : pl == 1 ? a[1] : a[2], y = pl == 0 ? b[0] : pl == 1 ? b[1] : b[2];
-        w[i] = x | (y << 16);
+    for (int i = 0; i < 16; ++i) {
+      uint16_t a[3], b[3];
+      split_planes(v[2 * i], a);
+      split_planes(v[2 * i + 1], b);
+      w[i] = (pl == 0 ? a[0] : pl == 1 ? a[1] : a[2]) | (uint32_t)(pl == 0 ? b[0] : pl == 1 ? b[1] : b[2]) << 16;
+    }
+    put16(box, o, base, rows, col, N, w);
+  }
+}
+
+// Four values of one row (those below N) as a final result: (v + bias) alpha + residual.
+struct GemmFinal {
+  float alpha;
+  const void* residual;
+  int64_t ld_res;
+  int dt, res_vec;
+};
+__device__ __forceinline__ void put4(const GemmOut& o, const GemmFinal& f, int64_t row, int64_t orow, int c, int N, float4 b,
+                                     float4 v) {
+  float x[4] = {(v.x + b.x) * f.alpha, (v.y + b.y) * f.alpha, (v.z + b.z) * f.alpha, (v.w + b.w) * f.alpha};
+  if (f.residual) {
+    const int64_t at = row * f.ld_res + c;
+    if (f.res_vec && c + 4 <= N) {
+      if (f.dt == M3B_F32) {
+        const float4 r = *reinterpret_cast<const float4*>(static_cast<const float*>(f.residual) + at);
+        x[0] += r.x, x[1] += r.y, x[2] += r.z, x[3] += r.w;
+      } else {
+        const uint2 r = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(f.residual) + at);
+        float2 p, q;
+        if (f.dt == M3B_BF16) {
+          p = bf2_to_f2(r.x), q = bf2_to_f2(r.y);
+        } else {
+          p = __half22float2(*reinterpret_cast<const __half2*>(&r.x));
+          q = __half22float2(*reinterpret_cast<const __half2*>(&r.y));
+        }
+        x[0] += p.x, x[1] += p.y, x[2] += q.x, x[3] += q.y;
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = pack16(v[2 * i], v[2 * i + 1], o.kind == kOutF16);
+      for (int e = 0; e < 4; ++e)
+        if (c + e < N) x[e] += ldf(f.residual, at + e, f.dt);
     }
-    if (full) {
-      reinterpret_cast<uint4*>(q)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-      reinterpret_cast<uint4*>(q)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  }
+  const int64_t at = orow * o.ld + c;
+  if (o.kind == kOutF32) {
+    float* q = static_cast<float*>(o.p) + at;
+    if (o.vec && c + 4 <= N) {
+      *reinterpret_cast<float4*>(q) = make_float4(x[0], x[1], x[2], x[3]);
     } else {
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (col + i < N) q[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+      for (int e = 0; e < 4; ++e)
+        if (c + e < N) q[e] = x[e];
     }
+  } else {
+    uint16_t* q = static_cast<uint16_t*>(o.p) + at;
+    const uint2 w = make_uint2(pack16(x[0], x[1], o.kind == kOutF16), pack16(x[2], x[3], o.kind == kOutF16));
+    if (o.vec && c + 4 <= N) {
+      *reinterpret_cast<uint2*>(q) = w;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (c + e < N) q[e] = (uint16_t)((e < 2 ? w.x : w.y) >> (16 * (e & 1)));
+    }
+  }
+}
+__device__ __forceinline__ float4 bias4(const void* bias, int dt, int c, int N) {
+  float b[4] = {0.f, 0.f, 0.f, 0.f};
+  if (bias)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (c + e < N) b[e] = ldf(bias, c + e, dt);
+  return make_float4(b[0], b[1], b[2], b[3]);
+}
+
+// 32 columns as final results with bias and residual (fp32 until the one rounding).
+__device__ __forceinline__ void put_final(uint8_t* box, const GemmOut& o, const GemmFinal& f, const void* bias,
+                                          const GemmRows& rows, int col, int N, const float (&v)[32]) {
+  const int lane = threadIdx.x & 31;
+  __syncwarp();
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    *reinterpret_cast<float4*>(box + lane * 128 + ((k ^ (lane & 7)) << 4)) =
+        make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+  __syncwarp();
+  const int k = lane & 7, c = col + 4 * k;
+  const float4 b = bias4(bias, f.dt, c, N);
+#pragma unroll
+  for (int it = 0; it < 8; ++it) {
+    const int r = it * 4 + (lane >> 3);
+    const float4 x = *reinterpret_cast<const float4*>(box + r * 128 + ((k ^ (r & 7)) << 4));
+    const int64_t orow = rows.out_row(r);
+    if (orow >= 0 && c < N) put4(o, f, rows.row0 + r, orow, c, N, b, x);
   }
 }
 
@@ -391,7 +502,7 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
       const int acc = (int)(sc & 1);
       const int64_t grow = (int64_t)job.mt * kTileM + (int64_t)rank * 128 + q * 32 + lane;
       const int M = sched.rows(s);
-      const bool rok = grow < M;
+      const bool rok = grow < M;  // grow is the row of this thread
       const bool none = job.ke == job.kb;  // no K at all: the sum is zero
       if (!__all_sync(0xffffffffu, mbar_wait(&accf[acc], (sc >> 1) & 1, p.wait_ns))) {
         give_up();
@@ -407,141 +518,158 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
           else mbar_arrive(&acce[acc]);
         }
       };
-      auto ld16 = [&](int c, float (&v)[16]) {
-        uint32_t r[16];
-        __syncwarp();
-        tmem_ld16_async(tc + c, r);
-        tmem_wait_ld(r);
+      uint8_t* box = sm + kGmBoxOff + (uint32_t)(warp - 2) * kGmBox;
+      GemmRows rows{(int64_t)job.mt * kTileM + (int64_t)rank * 128 + q * 32, M, nullptr};
+      // Columns [c0, c1) of this warp, 32 at a time.  The load is waited for at once: a register that
+      // an asynchronous load still writes must not be moved or spilled, and the second warp of the
+      // same lanes covers the wait.
+      auto columns = [&](int c0, int c1, auto&& f) {
+        for (int c = c0; c < c1; c += 32) {
+          uint32_t ra[32];
+          __syncwarp();
+          tmem_ld32_async(tc + c, ra);
+          tmem_wait_ld(ra);
+          float v[32];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = none ? 0.f : __uint_as_float(r[i]);
+          for (int i = 0; i < 32; ++i) v[i] = none ? 0.f : __uint_as_float(ra[i]);
+          f(c, v);
+        }
       };
       if constexpr (EPI == kEpiStore) {
-        const int c1 = (half + 1) * (bn / 2);
-        float alpha = s.alpha;
-        if (s.alpha_num) alpha *= *s.alpha_num;
-        if (s.alpha_den) alpha = *s.alpha_den > 0 ? alpha / (float)*s.alpha_den : 0.f;
-        int64_t orow = grow;
-        if (s.row_index) orow = rok ? s.row_index[grow] : -1;
+        GemmFinal fin{s.alpha, s.residual, s.ld_res, s.dt, s.res_vec};
+        if (s.alpha_num) fin.alpha *= *s.alpha_num;
+        if (s.alpha_den) fin.alpha = *s.alpha_den > 0 ? fin.alpha / (float)*s.alpha_den : 0.f;
+        rows.row_index = s.row_index;
         const int nq = s.nt * bn / 4;
-        for (int c = half * (bn / 2); c < c1; c += 16) {
+        const bool plain = s.out.kind != kOutF32 && !s.residual && !s.bias;
+        columns(half * (bn / 2), (half + 1) * (bn / 2), [&](int c, float (&v)[32]) {
           const int col = job.nt * bn + c;
-          float v[16];
-          ld16(c, v);
-          if (col >= s.N) continue;
+          if (col >= s.N) return;
           if (s.acc_mode != 0) {
             float4* ap = reinterpret_cast<float4*>(s.acc) + ((grow >> 5) * nq + (col >> 2)) * 32 + lane;
 #pragma unroll
-            for (int i = 0; i < 4; ++i, ap += 32) {
+            for (int i = 0; i < 8; ++i, ap += 32) {
               if (s.acc_mode != 1) {
                 const float4 o = *ap;
                 v[4 * i] += o.x, v[4 * i + 1] += o.y, v[4 * i + 2] += o.z, v[4 * i + 3] += o.w;
               }
               if (s.acc_mode != 3) *ap = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
             }
-            if (s.acc_mode != 3) continue;
+            if (s.acc_mode != 3) return;
           }
-          if (!rok || orow < 0) continue;
+          if (plain) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            if (s.bias && col + i < s.N) v[i] += ldf(s.bias, col + i, s.dt);
-            v[i] *= alpha;
-            if (s.residual && col + i < s.N) v[i] += ldf(s.residual, grow * s.ld_res + col + i, s.dt);
+            for (int i = 0; i < 32; ++i) v[i] *= fin.alpha;
+            put_operand(box, s.out, rows, col, s.N, v);
+          } else {
+            put_final(box, s.out, fin, s.bias, rows, col, s.N, v);
           }
-          store16(s.out, orow, col, s.N, v);
-        }
+        });
       } else if constexpr (EPI == kEpiGlu) {
-        const int hb = bn / 2, c1 = (half + 1) * (hb / 2);
-        for (int c = half * (hb / 2); c < c1; c += 16) {
+        const int hb = bn / 2;
+        for (int c = half * (hb / 2); c < (half + 1) * (hb / 2); c += 32) {
           const int col = job.nt * hb + c;
-          float g[16], u[16];
-          ld16(c, g);
-          ld16(hb + c, u);
+          uint32_t rg[32], ru[32];
+          __syncwarp();
+          tmem_ld32_async(tc + c, rg);
+          tmem_ld32_async(tc + hb + c, ru);
+          tmem_wait_ld(rg, ru);
           if (col >= s.N) continue;
+          float g[32], u[32];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            if (s.bias && col + i < s.N) g[i] += ldf(s.bias, col + i, s.dt);
-            if (s.bias2 && col + i < s.N) u[i] += ldf(s.bias2, col + i, s.dt);
+          for (int i = 0; i < 32; ++i) g[i] = __uint_as_float(rg[i]), u[i] = __uint_as_float(ru[i]);
+          if (s.bias) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const float4 a = bias4(s.bias, s.dt, col + 4 * k, s.N), b = bias4(s.bias2, s.dt, col + 4 * k, s.N);
+              g[4 * k] += a.x, g[4 * k + 1] += a.y, g[4 * k + 2] += a.z, g[4 * k + 3] += a.w;
+              u[4 * k] += b.x, u[4 * k + 1] += b.y, u[4 * k + 2] += b.z, u[4 * k + 3] += b.w;
+            }
           }
           if (p.gu) {
             float4* gp = reinterpret_cast<float4*>(p.gu) + ((grow >> 5) * p.gu_ld4 + (col >> 2)) * 64 + lane;
 #pragma unroll
-            for (int i = 0; i < 4; ++i, gp += 64) {
+            for (int i = 0; i < 8; ++i, gp += 64) {
               gp[0] = make_float4(g[4 * i], g[4 * i + 1], g[4 * i + 2], g[4 * i + 3]);
               gp[32] = make_float4(u[4 * i], u[4 * i + 1], u[4 * i + 2], u[4 * i + 3]);
             }
           }
 #pragma unroll
-          for (int i = 0; i < 16; ++i) g[i] = g[i] * sigmoid_fast(g[i]) * u[i];
-          if (rok) store16(s.out, grow, col, s.N, g);
+          for (int i = 0; i < 32; ++i) g[i] = g[i] * sigmoid_fast(g[i]) * u[i];
+          put_operand(box, s.out, rows, col, s.N, g);
         }
       } else if constexpr (EPI == kEpiDglu) {
-        const int c1 = (half + 1) * (bn / 2);
-        for (int c = half * (bn / 2); c < c1; c += 16) {
+        columns(half * (bn / 2), (half + 1) * (bn / 2), [&](int c, float (&d)[32]) {
           const int col = job.nt * bn + c;
-          float d[16], g[16], u[16];
-          ld16(c, d);
-          if (col >= s.N || !rok) continue;
+          if (col >= s.N) return;
           const float4* gp = reinterpret_cast<const float4*>(p.gu) + ((grow >> 5) * p.gu_ld4 + (col >> 2)) * 64 + lane;
+          float u[32];
 #pragma unroll
-          for (int i = 0; i < 4; ++i, gp += 64) {
+          for (int i = 0; i < 8; ++i, gp += 64) {
             const float4 a = gp[0], b = gp[32];
-            g[4 * i] = a.x, g[4 * i + 1] = a.y, g[4 * i + 2] = a.z, g[4 * i + 3] = a.w;
-            u[4 * i] = b.x, u[4 * i + 1] = b.y, u[4 * i + 2] = b.z, u[4 * i + 3] = b.w;
-          }
+            const float g4[4] = {a.x, a.y, a.z, a.w}, u4[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float sg = sigmoid_fast(g[i]), da = d[i] * s.alpha, ds = da * sg;
-            d[i] = ds * u[i] * fmaf(g[i], 1.f - sg, 1.f);
-            u[i] = ds * g[i];
+            for (int e = 0; e < 4; ++e) {
+              const float g = g4[e], sg = sigmoid_fast(g), ds = d[4 * i + e] * s.alpha * sg;
+              d[4 * i + e] = ds * u4[e] * fmaf(g, 1.f - sg, 1.f);
+              u[4 * i + e] = ds * g;
+            }
           }
-          store16(s.out, grow, col, s.N, d);
-          store16(s.out2, grow, col, s.N, u);
-        }
+          put_operand(box, s.out, rows, col, s.N, d);
+          put_operand(box, s.out2, rows, col, s.N, u);
+        });
       } else if constexpr (EPI == kEpiLse) {
-        const int c1 = (half + 1) * (bn / 2);
         const int tgt = rok ? p.target[grow] : -1;
-        float m = -1e30f, sum = 0.f;
-        for (int c = half * (bn / 2); c < c1; c += 16) {
+        float m = -1e30f, sum = 0.f;  // m in powers of two
+        columns(half * (bn / 2), (half + 1) * (bn / 2), [&](int c, float (&v)[32]) {
           const int col = job.nt * bn + c;
-          float v[16];
-          ld16(c, v);
-          if (col >= s.N) continue;
+          if (col >= s.N) return;
           const int to = tgt - col;
-          if (to >= 0 && to < 16) {
+          if (to >= 0 && to < 32) {
             float x = v[0];
 #pragma unroll
-            for (int i = 1; i < 16; ++i) x = to == i ? v[i] : x;
+            for (int i = 1; i < 32; ++i) x = to == i ? v[i] : x;
             p.target_logit[grow] = x;
           }
-          float top = m;
+          if (col + 32 > s.N) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            v[i] = col + i < s.N ? v[i] * kLog2e : -INFINITY;
-            top = fmaxf(top, v[i]);
+            for (int i = 0; i < 32; ++i) v[i] = col + i < s.N ? v[i] : -INFINITY;
           }
-          sum *= ex2_fast(m - top);
+          float t[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+          for (int i = 4; i < 32; ++i) t[i & 3] = fmaxf(t[i & 3], v[i]);
+          const float top = fmaxf(m, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * kLog2e);
+          float e[4] = {sum * ex2_fast(m - top), 0.f, 0.f, 0.f};
           m = top;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) sum += ex2_fast(v[i] - top);
-        }
+          for (int i = 0; i < 32; ++i) e[i & 3] += ex2_fast(fmaf(v[i], kLog2e, -top));
+          sum = (e[0] + e[1]) + (e[2] + e[3]);
+        });
         if (rok) p.part[(int64_t)(job.nt * 2 + half) * p.part_ld + grow] = make_float2(m, sum);
       } else {
-        const int c1 = (half + 1) * (bn / 2);
         const int tgt = rok ? p.target[grow] - p.col0 : -1;
         const float l2 = rok ? p.lse2[grow] : 0.f, w = rok && p.roww ? p.roww[grow] : 1.f;
-        for (int c = half * (bn / 2); c < c1; c += 16) {
+        rows.M = 0x7fffffff;  // rows behind the last kept token are K values of the next products: zero
+        columns(half * (bn / 2), (half + 1) * (bn / 2), [&](int c, float (&v)[32]) {
           const int col = job.nt * bn + c;
-          float v[16];
-          ld16(c, v);
-          if (col >= s.N) continue;
+          if (col >= s.N) return;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float e = ex2_fast(fmaf(v[i], kLog2e, -l2));
-            // rows behind the last kept token are K values of the next products: zero
-            v[i] = rok ? w * (col + i == tgt ? e - 1.f : e) : 0.f;
+          for (int i = 0; i < 32; ++i) v[i] = ex2_fast(fmaf(v[i], kLog2e, -l2));
+          const int to = tgt - col;
+          if (to >= 0 && to < 32) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = to == i ? v[i] - 1.f : v[i];
           }
-          store16(s.out, grow, col, s.N, v);
-        }
+          if (p.roww) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] *= w;
+          }
+          if (!rok) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = 0.f;
+          }
+          put_operand(box, s.out, rows, col, s.N, v);
+        });
       }
       release();
     }

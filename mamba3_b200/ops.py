@@ -480,7 +480,7 @@ def _gated_ffn_fwd_op(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
 
 def _ffn_saved_bytes(x, f):
     rows, planes = x.shape[0], 3 if x.dtype == torch.float32 else 1
-    return planes * rows * ((f + 7) // 8 * 8) * 2, ((rows + 255) // 256 * 256) * ((f + 15) // 16 * 16) * 8
+    return planes * rows * ((f + 7) // 8 * 8) * 2, ((rows + 255) // 256 * 256) * ((f + 31) // 32 * 32) * 8
 
 
 @_gated_ffn_fwd_op.register_fake
