@@ -332,6 +332,76 @@ __device__ __forceinline__ void put_final(uint8_t* box, const GemmOut& o, const 
   }
 }
 
+// Waits of the producer and the MMA issuer: the plain test in a loop (the sleeping form of mbar_wait
+// wakes too late for a stage that lasts a third of a microsecond); the clock is read only rarely.
+template <bool CLUSTER>
+__device__ __forceinline__ bool gm_wait(uint64_t* bar, uint32_t parity, uint64_t limit_ns) {
+  auto test = [&]() {
+    uint32_t done;
+    if constexpr (CLUSTER)
+      asm volatile(
+          "{\n\t.reg .pred p;\n\t"
+          "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+          "selp.u32 %0, 1, 0, p;\n\t}"
+          : "=r"(done)
+          : "r"(smem_u32(bar)), "r"(parity)
+          : "memory");
+    else
+      done = mbar_try_wait(bar, parity);
+    return done != 0;
+  };
+  if (test()) return true;
+  uint64_t t0 = 0;
+  while (true) {
+#pragma unroll 1
+    for (int i = 0; i < 256; ++i)
+      if (test()) return true;
+    const uint64_t t = globaltimer_ns();
+    if (t0 == 0) t0 = t;
+    else if (t - t0 > limit_ns) return false;
+  }
+}
+
+// One thread of the (converged) warp, the same at every call.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+  return p != 0;
+}
+// TMA load of one box to shared address `dst`, completing on the barrier at shared::cluster address `bar`.
+template <bool PAIR>
+__device__ __forceinline__ void gm_load(uint32_t dst, const CUtensorMap* m, int c0, int c1, int c2, uint32_t bar) {
+  if constexpr (PAIR)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, "
+        "%4}], [%5];" ::"r"(dst),
+        "l"(m), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+        "[%5];" ::"r"(dst),
+        "l"(m), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+        : "memory");
+}
+// Arrive on the barrier, paired: on both CTAs', when the MMAs issued so far have completed.
+template <bool PAIR>
+__device__ __forceinline__ void gm_commit(uint64_t* bar) {
+  if constexpr (PAIR)
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_u32(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+  else
+    umma_commit(bar);
+}
+__device__ __forceinline__ uint64_t gm_desc(uint32_t lo, uint32_t hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
+  return d;
+}
+
 // ---------------------------------------------------------------------------
 // the kernel
 // ---------------------------------------------------------------------------
@@ -377,120 +447,114 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
     record_error(p.err, M3B_ERR_TIMEOUT);
   };
 
+  // The producer's and the issuer's loops run warp-uniform, with one elected thread for the copies,
+  // the MMAs and the commits: their addresses and descriptors then live in uniform registers.  As
+  // single-thread loops they took 360 ns a stage whatever the stage held (MMAs: 305 ns).
   if (warp == 0) {
-    if (lane == 0) {
-      const uint32_t bytes = kGmStageA + (uint32_t)brows * 128u;
-      uint32_t it = 0;
-      GemmJob job;
-      while (!*abort_flag && sched.next(job)) {
-        const GemmSub& s = p.sub[job.sub];
-        const int nk0 = sched.nk0(s), nks = nk0 + s.nk[1];
-        const int arow = job.mt * kTileM + (int)rank * 128;
-        // B rows of this CTA; the gated product stages bn / 2 gate and bn / 2 up rows (paired: the
-        // first CTA holds the gate's, the second the up's)
-        const int brow = EPI == kEpiGlu ? job.nt * (bn / 2) : job.nt * bn + (int)rank * brows;
-        int pass = job.kb / (nks > 0 ? nks : 1), r = job.kb - pass * nks;
-        for (int i = job.kb; i < job.ke; ++i, ++it) {
-          const int st = (int)(it % kGmStages);
-          if (!mbar_wait(&empty[st], ((it / kGmStages) & 1) ^ 1, p.wait_ns)) {
-            give_up();
-            break;
-          }
-          const int seg = r >= nk0 ? 1 : 0, k = (seg ? r - nk0 : r) * kGmBK;
-          // plane pairs, smallest first: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0)
-          const int pp = (pass + 6 - p.npass) * 4;
-          const int pa = (0x001102 >> pp) & 3, pb = (0x010120 >> pp) & 3;
-          uint8_t* dA = sm + st * kGmStage;
-          uint8_t* dB = dA + kGmStageA;
-          uint32_t fb = smem_u32(&full[st]);
-          if constexpr (PAIR) {
-            if (rank == 0) mbar_arrive_expect_tx(&full[st], 2 * bytes);
-            fb = mapa_shared(fb, 0);
-          } else {
-            mbar_arrive_expect_tx(&full[st], bytes);
-          }
-          auto load = [&](void* dst, const CUtensorMap* m, int c0, int c1, int c2) {
-            if constexpr (PAIR) tma_load_3d_pair(dst, m, c0, c1, c2, fb);
-            else tma_load_3d(dst, m, c0, c1, c2, &full[st]);
-          };
+    const bool leader = elect_one();
+    const uint32_t bytes = (PAIR ? 2u : 1u) * (kGmStageA + (uint32_t)brows * 128u);
+    const uint32_t ring = smem_u32(sm);
+    // the copies of both CTAs complete on the first CTA's barriers
+    const uint32_t full0 = PAIR ? mapa_shared(smem_u32(full), 0) : smem_u32(full);
+    uint32_t st = 0, ph = 1, it = 0;
+    GemmJob job;
+    bool ok = true;
+    while (ok && sched.next(job)) {
+      const GemmSub& s = p.sub[job.sub];
+      const int nk0 = sched.nk0(s), nks = nk0 + s.nk[1];
+      const int arow = job.mt * kTileM + (int)rank * 128;
+      // B rows of this CTA; the gated product stages bn / 2 gate and bn / 2 up rows (paired: the
+      // first CTA holds the gate's, the second the up's)
+      const int brow = EPI == kEpiGlu ? job.nt * (bn / 2) : job.nt * bn + (int)rank * brows;
+      int pass = job.kb / (nks > 0 ? nks : 1), r = job.kb - pass * nks;
+      for (int i = job.kb; i < job.ke; ++i, ++it) {
+        ok = __all_sync(0xffffffffu, gm_wait<PAIR>(&empty[st], ph, p.wait_ns));
+        if (!ok) break;
+        const int seg = r >= nk0 ? 1 : 0, k = (seg ? r - nk0 : r) * kGmBK;
+        // plane pairs, smallest first: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0)
+        const int pp = (pass + 6 - p.npass) * 4;
+        const int pa = (0x001102 >> pp) & 3, pb = (0x010120 >> pp) & 3;
+        const uint32_t dA = ring + st * kGmStage, dB = dA + kGmStageA, fb = full0 + st * 8;
+        const CUtensorMap *ma = &s.a[seg], *mb = &s.b[EPI == kEpiGlu ? (PAIR ? (int)rank : 0) : seg];
+        if (leader) {
+          if (rank == 0) mbar_arrive_expect_tx(&full[st], bytes);
           if (s.a_mn) {
-            load(dA, &s.a[seg], arow, k, pa);
-            load(dA + 8192, &s.a[seg], arow + 64, k, pa);
+            gm_load<PAIR>(dA, ma, arow, k, pa, fb);
+            gm_load<PAIR>(dA + 8192, ma, arow + 64, k, pa, fb);
           } else {
-            load(dA, &s.a[seg], k, arow, pa);
+            gm_load<PAIR>(dA, ma, k, arow, pa, fb);
           }
-          if constexpr (EPI == kEpiGlu) {
-            if constexpr (PAIR) {
-              load(dB, &s.b[rank], k, brow, pb);
-            } else {
-              load(dB, &s.b[0], k, brow, pb);
-              load(dB + (bn / 2) * 128, &s.b[1], k, brow, pb);
-            }
-          } else if (s.b_mn) {
-            for (int c = 0; c < brows; c += 64) load(dB + c * 128, &s.b[seg], brow + c, k, pb);
+          if (EPI != kEpiGlu && s.b_mn) {
+            gm_load<PAIR>(dB, mb, brow, k, pb, fb);
+            if (brows > 64) gm_load<PAIR>(dB + 8192, mb, brow + 64, k, pb, fb);
           } else {
-            load(dB, &s.b[seg], k, brow, pb);
+            gm_load<PAIR>(dB, mb, k, brow, pb, fb);
+            if constexpr (EPI == kEpiGlu && !PAIR) gm_load<PAIR>(dB + (uint32_t)(bn / 2) * 128u, &s.b[1], k, brow, pb, fb);
           }
-          if (++r == nks) {
-            r = 0;
-            ++pass;
-          }
+        }
+        if (++r == nks) {
+          r = 0;
+          ++pass;
+        }
+        if (++st == kGmStages) {
+          st = 0;
+          ph ^= 1;
         }
       }
+    }
+    if (!ok) {
+      give_up();
       // an aborted run leaves once the copies in flight have landed
-      if (*abort_flag && rank == 0)
-        for (uint32_t b = it > kGmStages ? it - kGmStages : 0; b < it; ++b)
-          mbar_wait(&full[b % kGmStages], (b / kGmStages) & 1, 10000000ull);
+      if (rank == 0)
+        for (uint32_t n = it > kGmStages ? it - kGmStages : 0; n < it; ++n)
+          mbar_wait(&full[n % kGmStages], (n / kGmStages) & 1, 10000000ull);
     }
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
-      auto commit_both = [&](uint64_t* bar) {
-        if constexpr (PAIR) {
-          umma_commit_pair(smem_u32(bar));
-          umma_commit_pair(mapa_shared(smem_u32(bar), 1));
-        } else {
-          umma_commit(bar);
-        }
-      };
-      uint32_t it = 0, sc = 0;
+    if (rank == 0) {
+      const bool leader = elect_one();
+      const uint32_t ring = smem_u32(sm) >> 4;
+      uint32_t st = 0, ph = 0, sc = 0;
       GemmJob job;
-      for (; !*abort_flag && sched.next(job); ++sc) {
+      bool ok = true;
+      for (; ok && sched.next(job); ++sc) {
         const GemmSub& s = p.sub[job.sub];
-        const int acc = (int)(sc & 1);
-        const bool drained = PAIR ? mbar_wait_cluster(&acce[acc], ((sc >> 1) & 1) ^ 1, p.wait_ns)
-                                  : mbar_wait(&acce[acc], ((sc >> 1) & 1) ^ 1, p.wait_ns);
-        if (!drained) {
-          give_up();
-          break;
-        }
+        const uint32_t acc = sc & 1;
+        ok = __all_sync(0xffffffffu, gm_wait<PAIR>(&acce[acc], ((sc >> 1) & 1) ^ 1, p.wait_ns));
+        if (!ok) break;
         tc_fence_after();
         uint32_t idesc = idesc_bf16(kTileM, bn, s.a_mn != 0, s.b_mn != 0);
         if (p.f16) idesc &= ~((1u << 7) | (1u << 10));
-        const uint32_t dt = tbase + (uint32_t)(acc * 256);
-        // descriptor step per 16 K values, in its 16-byte units: 32 bytes along a swizzled row, or
+        const uint32_t dt = tbase + acc * 256;
+        // descriptors: the address in 16-byte units in the low bits, then the leading offset (MN-major:
+        // 8192 bytes between 64-column blocks); a step of 16 K values is 32 bytes along a swizzled row, or
         // two 8-row groups of an MN-major tile
-        const uint64_t sa = s.a_mn ? 128 : 2, sb = s.b_mn ? 128 : 2;
-        const uint32_t la = s.a_mn ? 8192 : 16, lb = s.b_mn ? 8192 : 16;
-        for (int i = job.kb; i < job.ke; ++i, ++it) {
-          const int st = (int)(it % kGmStages);
-          if (!mbar_wait(&full[st], (it / kGmStages) & 1, p.wait_ns)) {
-            give_up();
-            break;
-          }
+        const uint32_t sa = s.a_mn ? 128 : 2, sb = s.b_mn ? 128 : 2;
+        const uint32_t la = (s.a_mn ? 8192u >> 4 : 1u) << 16, lb = (s.b_mn ? 8192u >> 4 : 1u) << 16;
+        const uint32_t hi = (1024u >> 4) | (1u << 14) | (2u << 29);
+        uint32_t on = 0;
+        for (int i = job.kb; i < job.ke; ++i) {
+          ok = __all_sync(0xffffffffu, gm_wait<PAIR>(&full[st], ph, p.wait_ns));
+          if (!ok) break;
           tc_fence_after();
-          const uint32_t base = smem_u32(sm + st * kGmStage);
-          const uint64_t da = sdesc_sw128(base, la, 1024), db = sdesc_sw128(base + kGmStageA, lb, 1024);
+          const uint32_t a0 = (ring + st * (kGmStage >> 4)) | la, b0 = (ring + st * (kGmStage >> 4) + (kGmStageA >> 4)) | lb;
+          if (leader) {
 #pragma unroll
-          for (int kk = 0; kk < kGmBK / 16; ++kk) {
-            const uint32_t on = (i != job.kb || kk != 0) ? 1u : 0u;
-            if constexpr (PAIR) umma_bf16_pair(dt, da + kk * sa, db + kk * sb, idesc, on);
-            else umma_bf16(dt, da + kk * sa, db + kk * sb, idesc, on);
+            for (uint32_t kk = 0; kk < kGmBK / 16; ++kk) {
+              const uint64_t da = gm_desc(a0 + kk * sa, hi), db = gm_desc(b0 + kk * sb, hi);
+              if constexpr (PAIR) umma_bf16_pair(dt, da, db, idesc, kk == 0 ? on : 1u);
+              else umma_bf16(dt, da, db, idesc, kk == 0 ? on : 1u);
+            }
+            gm_commit<PAIR>(&empty[st]);  // the stage is free, in both CTAs, once these MMAs have read it
           }
-          commit_both(&empty[st]);
+          on = 1;
+          if (++st == kGmStages) {
+            st = 0;
+            ph ^= 1;
+          }
         }
-        if (*abort_flag) break;
-        commit_both(&accf[acc]);
+        if (ok && leader) gm_commit<PAIR>(&accf[acc]);
       }
+      if (!ok) give_up();
     }
   } else {
     const int q = warp & 3, half = (warp - 2) >> 2;
@@ -504,7 +568,7 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
       const int M = sched.rows(s);
       const bool rok = grow < M;  // grow is the row of this thread
       const bool none = job.ke == job.kb;  // no K at all: the sum is zero
-      if (!__all_sync(0xffffffffu, mbar_wait(&accf[acc], (sc >> 1) & 1, p.wait_ns))) {
+      if (!__all_sync(0xffffffffu, gm_wait<PAIR>(&accf[acc], (sc >> 1) & 1, p.wait_ns))) {
         give_up();
         break;
       }
