@@ -7,6 +7,7 @@ the library is missing or a tensor is not on a CUDA device the call raises.
 
 from __future__ import annotations
 
+import array
 import contextlib
 import ctypes as C
 import threading
@@ -922,24 +923,20 @@ def linear_xent_bwd(rows, weight, saved, dloss, ignore_index, reduction, want_hi
     return dh, dw
 
 
-def grad_clip(grads, outs, max_norm, inf_norm, dev):
-    """Launch the global norm over `grads` (dense tensors on `dev`) and, with `outs` (the same
-    lengths; the same tensors for in place), the clipped values.  Returns the norm (fp32, on `dev`)."""
-    n = len(grads)
-    gp = (C.c_void_p * n)(*[t.data_ptr() for t in grads])
-    num = (C.c_int64 * n)(*[t.numel() for t in grads])
-    gd = (C.c_int32 * n)(*[_DT[t.dtype] for t in grads])
+def grad_clip(ptrs, numel, dtypes, out_ptrs, out_dtypes, max_norm, inf_norm, dev):
+    """Launch the global norm over tensors on `dev`, given as lists of addresses, lengths and dtypes, and,
+    with out_ptrs (the same list for in place), the clipped values.  Returns the norm (fp32, on `dev`)."""
+    code = _DT.__getitem__
+    gp, num = array.array("Q", ptrs), array.array("q", numel)
+    gd = array.array("i", map(code, dtypes))
+    op, od = gp, gd
     norm = torch.empty((), dtype=torch.float32, device=dev)
-    a = GradClipArgs(n)
-    a.grads, a.numel, a.grad_dtype = C.addressof(gp), C.addressof(num), C.addressof(gd)
-    if outs is grads:
-        op, od = gp, gd
-    elif outs is not None:
-        op = (C.c_void_p * n)(*[t.data_ptr() for t in outs])
-        od = (C.c_int32 * n)(*[_DT[t.dtype] for t in outs])
-    if outs is not None:
-        a.outs, a.out_dtype = C.addressof(op), C.addressof(od)
-    a.norm_type, a.max_norm, a.norm = (0 if inf_norm else 2), float(max_norm), norm.data_ptr()
+    a = GradClipArgs(len(ptrs))
+    a.grads, a.numel, a.grad_dtype = gp.buffer_info()[0], num.buffer_info()[0], gd.buffer_info()[0]
+    if out_ptrs is not ptrs:
+        op, od = array.array("Q", out_ptrs), array.array("i", map(code, out_dtypes))
+    a.outs, a.out_dtype = op.buffer_info()[0], od.buffer_info()[0]
+    a.norm_type, a.max_norm, a.norm = (0 if inf_norm else 2), max_norm, norm.data_ptr()
     L = lib()
     need = L.m3b_grad_clip_workspace(C.byref(a))
     ws = torch.empty(need, dtype=torch.uint8, device=dev)

@@ -15,6 +15,10 @@ import torch
 
 from . import _lib
 
+# The methods themselves, for map(): with hundreds of tensors the host's time is in these calls.
+_get_device, _data_ptr, _numel = torch.Tensor.get_device, torch.Tensor.data_ptr, torch.Tensor.numel
+_is_contiguous, _dtype = torch.Tensor.is_contiguous, torch.Tensor.dtype.__get__
+
 
 def _dense(t):
     """True when t's elements fill one run of memory in some order."""
@@ -35,7 +39,7 @@ def clip_grads(grads: Iterable[torch.Tensor], max_norm: float, norm_type: float 
 
     grads: dense tensors (fp32, bf16 or fp16, mixed as they come) on one CUDA device, no two of which
     share memory.  Without `out` they are clipped in place, and left unwritten when the norm is within
-    max_norm.  With `out` (one tensor for each, of its shape and memory order; the dtypes may
+    max_norm.  With `out` (one tensor for each, of its length and memory order; the dtypes may
     differ: the fp32 main gradients of a bf16 model, say) the clipped values go there.  max_norm may
     be math.inf (copies, or only the norm).  norm_type 2 or inf.  A norm that is not finite
     spreads as torch's rule has it: NaN makes every value NaN, infinity makes them 0 (inf itself NaN)."""
@@ -50,24 +54,35 @@ def clip_grads(grads: Iterable[torch.Tensor], max_norm: float, norm_type: float 
         raise ValueError(f"clip_grads: {len(gs)} gradients and {len(os)} outputs")
     if not gs:
         return torch.zeros(())
-    dev = gs[0].device
-    for t in gs if out is None else gs + os:
-        if t.device != dev or not t.is_cuda:
-            raise _lib.M3bError(f"clip_grads: tensors on one CUDA device expected, got {dev} and {t.device}")
-        if t.dtype not in _lib._DT:
-            raise _lib.M3bError(f"unsupported dtype {t.dtype}")
-        if not _dense(t):
-            raise ValueError(f"clip_grads: dense tensors expected, got strides {t.stride()} of shape {tuple(t.shape)}")
-    if out is not None:
+    every = gs if os is gs else gs + os
+    places = set(map(_get_device, every))
+    if len(places) != 1 or -1 in places:
+        raise _lib.M3bError(f"clip_grads: tensors on one CUDA device expected, got {sorted({str(t.device) for t in every})}")
+    dtypes = list(map(_dtype, gs))
+    out_dtypes = dtypes if os is gs else list(map(_dtype, os))
+    for dt in {*dtypes, *out_dtypes}:
+        _lib.dtype_code(dt)
+    numel = list(map(_numel, gs))
+    if not all(map(_is_contiguous, every)):
+        for t in every:
+            if not _dense(t):
+                raise ValueError(f"clip_grads: dense tensors expected, got strides {t.stride()} of shape {tuple(t.shape)}")
         for g, o in zip(gs, os):
-            if g.shape != o.shape or (g.stride() != o.stride() and not (g.is_contiguous() and o.is_contiguous())):
+            if not (g.is_contiguous() and o.is_contiguous()) and (g.shape != o.shape or g.stride() != o.stride()):
                 raise ValueError("clip_grads: each output needs its gradient's shape and memory order")
-            if g.numel() and g.data_ptr() == o.data_ptr() and g.dtype != o.dtype:
-                raise ValueError("clip_grads: an output in its gradient's place needs its dtype")
-    ptrs = [t.data_ptr() for t in os if t.numel()]
-    if len(set(ptrs)) != len(ptrs):
+    ptrs = list(map(_data_ptr, gs))
+    out_ptrs = ptrs
+    if os is not gs:
+        if numel != list(map(_numel, os)):
+            raise ValueError("clip_grads: each output needs its gradient's length")
+        out_ptrs = list(map(_data_ptr, os))
+        if dtypes != out_dtypes and any(n and p == q and a != b
+                                        for n, p, q, a, b in zip(numel, ptrs, out_ptrs, dtypes, out_dtypes)):
+            raise ValueError("clip_grads: an output in its gradient's place needs its dtype")
+    used = [p for p, n in zip(out_ptrs, numel) if n]
+    if len(set(used)) != len(used):
         raise ValueError("clip_grads: the same tensor twice")
-    return _lib.grad_clip(gs, os, max_norm, norm_type == math.inf, dev)
+    return _lib.grad_clip(ptrs, numel, dtypes, out_ptrs, out_dtypes, max_norm, norm_type == math.inf, gs[0].device)
 
 
 def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0,

@@ -111,7 +111,8 @@ def test_loss_refuses():
         m.linear_cross_entropy(h, fake(20, 8, dtype=torch.float16), t)
 
 
-def test_clip_refuses():
+def test_clip_refuses(monkeypatch):
+    monkeypatch.setattr("mamba3_b200.clip._get_device", lambda t: 0 if t.is_cuda else -1)
     g = torch.zeros(10)
     for call in (lambda: m.clip_grads([_Cuda(g)], -1.0), lambda: m.clip_grads([_Cuda(g)], math.nan),
                  lambda: m.clip_grads([_Cuda(g)], 1.0, 1.0), lambda: m.clip_grads([_Cuda(g), _Cuda(g)], 1.0),
