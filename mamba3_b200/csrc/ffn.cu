@@ -182,7 +182,7 @@ int forward(const m3b_gated_ffn_args* a, void* workspace, size_t* need, bool run
   p.f16 = d.f16;
   p.err = a->err;
   M3B_MAP(&s.a[0], act, false, 128, d.f16);
-  M3B_MAP(&s.b[0], wd, false, gemm_box_b(pair, p.bn, kEpiStore), d.f16);
+  M3B_MAP(&s.b[0], wd, false, gemm_box_b(pair, p.bn, kEpiFinal), d.f16);
   s.M = (int)d.M;
   s.N = d.D;
   s.nk[0] = (d.F + kGmBK - 1) / kGmBK;
@@ -193,7 +193,7 @@ int forward(const m3b_gated_ffn_args* a, void* workspace, size_t* need, bool run
   s.ld_res = a->residual_stride;
   s.res_vec = aligned16(a->residual) && a->residual_stride % 4 == 0;
   s.dt = a->dtype;
-  return launch_gemm(p, kEpiStore, pair, st);
+  return launch_gemm(p, kEpiFinal, pair, st);
 }
 
 int backward(const m3b_gated_ffn_args* a, void* workspace, size_t* need, bool run, cudaStream_t st) {

@@ -38,17 +38,23 @@ __global__ void pack_kernel(const void* __restrict__ src, int64_t rows, int64_t 
 using KernelFn = void (*)(const GemmParams);
 
 template <int EPI>
-KernelFn pick(bool pair) {
-  return pair ? (KernelFn)gemm_kernel<EPI, true> : (KernelFn)gemm_kernel<EPI, false>;
+KernelFn pick(bool pair, bool planes) {
+  // results of these leave as operands of a following product
+  constexpr bool kOperand = EPI == kEpiGlu || EPI == kEpiDglu || EPI == kEpiDlogit;
+  if constexpr (kOperand)
+    if (planes) return pair ? (KernelFn)gemm_kernel<EPI, true, true> : (KernelFn)gemm_kernel<EPI, false, true>;
+  return pair ? (KernelFn)gemm_kernel<EPI, true, false> : (KernelFn)gemm_kernel<EPI, false, false>;
 }
 
-KernelFn kernel_of(int epi, bool pair) {
+KernelFn kernel_of(int epi, bool pair, bool planes) {
   switch (epi) {
-    case kEpiStore: return pick<kEpiStore>(pair);
-    case kEpiGlu: return pick<kEpiGlu>(pair);
-    case kEpiDglu: return pick<kEpiDglu>(pair);
-    case kEpiLse: return pick<kEpiLse>(pair);
-    default: return pick<kEpiDlogit>(pair);
+    case kEpiStore: return pick<kEpiStore>(pair, planes);
+    case kEpiFinal: return pick<kEpiFinal>(pair, planes);
+    case kEpiAcc: return pick<kEpiAcc>(pair, planes);
+    case kEpiGlu: return pick<kEpiGlu>(pair, planes);
+    case kEpiDglu: return pick<kEpiDglu>(pair, planes);
+    case kEpiLse: return pick<kEpiLse>(pair, planes);
+    default: return pick<kEpiDlogit>(pair, planes);
   }
 }
 
@@ -79,16 +85,16 @@ int device_setup(int* pairs) {
     *pairs = done[dev];
     return M3B_OK;
   }
-  for (int epi = kEpiStore; epi <= kEpiDlogit; ++epi)
-    for (int pr = 0; pr < 2; ++pr) {
-      const cudaError_t e = cudaFuncSetAttribute((const void*)kernel_of(epi, pr != 0),
+  for (int epi = 0; epi < kEpiCount; ++epi)
+    for (int k = 0; k < 4; ++k) {
+      const cudaError_t e = cudaFuncSetAttribute((const void*)kernel_of(epi, (k & 1) != 0, k >= 2),
                                                  cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kGmSmem);
       if (e != cudaSuccess) return fail(M3B_ERR_CUDA, "gemm: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
     }
   cudaLaunchAttribute at[1];
   const cudaLaunchConfig_t cfg = config(2 * (unsigned)(num_sms() / 2), true, nullptr, at);
   int n = 0;
-  if (cudaOccupancyMaxActiveClusters(&n, (const void*)kernel_of(kEpiStore, true), &cfg) != cudaSuccess || n <= 0) {
+  if (cudaOccupancyMaxActiveClusters(&n, (const void*)kernel_of(kEpiStore, true, false), &cfg) != cudaSuccess || n <= 0) {
     cudaGetLastError();
     return fail(M3B_ERR_UNSUPPORTED, "gemm: no CTA pair can be resident on this device");
   }
@@ -139,7 +145,7 @@ int launch_gemm(GemmParams& p, int epi, bool pair, cudaStream_t st) {
   const unsigned workers = (unsigned)(jobs < most ? jobs : most);
   cudaLaunchAttribute at[1];
   const cudaLaunchConfig_t cfg = config(pair ? 2 * workers : workers, pair, st, at);
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel_of(epi, pair), p);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel_of(epi, pair, p.npass > 1), p);
   if (e != cudaSuccess) return fail(M3B_ERR_CUDA, "gemm_kernel: %s", cudaGetErrorString(e));
   return check_launch("gemm_kernel");
 }

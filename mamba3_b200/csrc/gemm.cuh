@@ -54,13 +54,18 @@ struct GemmOut {
   int vec;        // rows and columns allow 16-byte stores
 };
 
+// (Forms of their own rather than flags: a spilled register costs an L2 round trip here, because the
+// stage ring leaves the L1 cache almost nothing.)
 enum GemmEpi {
-  kEpiStore = 0,   // out = residual + alpha (acc + bias), or an fp32 running sum over several launches
-  kEpiGlu = 1,     // gate | up accumulators -> silu(g) u, and g, u kept in fp32 for the backward pass
-  kEpiDglu = 2,    // d(silu(g) u) -> dg, du
-  kEpiLse = 3,     // running maximum and sum of each row, and the target's logit
-  kEpiDlogit = 4,  // softmax - one-hot
+  kEpiStore = 0,   // out = alpha acc
+  kEpiFinal = 1,   // out = residual + alpha (acc + bias)
+  kEpiAcc = 2,     // out row_index[r] = alpha (sum of several launches' accumulators)
+  kEpiGlu = 3,     // gate | up accumulators -> silu(g) u, and g, u kept in fp32 for the backward pass
+  kEpiDglu = 4,    // d(silu(g) u) -> dg, du
+  kEpiLse = 5,     // running maximum and sum of each row, and the target's logit
+  kEpiDlogit = 6,  // softmax - one-hot
 };
+constexpr int kEpiCount = 7;
 
 struct GemmSub {
   CUtensorMap a[2], b[2];
@@ -70,7 +75,7 @@ struct GemmSub {
   int a_mn, b_mn;  // operand stored MN-major
   int m_dyn, k_dyn;
   GemmOut out, out2;
-  // kEpiStore
+  // kEpiStore, kEpiFinal, kEpiAcc
   float alpha;
   const float* alpha_num;  // alpha *= alpha_num[0]
   const int* alpha_den;    // alpha /= alpha_den[0] (0 rows: alpha = 0)
@@ -207,113 +212,22 @@ __device__ __forceinline__ void put16(uint8_t* box, const GemmOut& o, uint16_t* 
 #pragma unroll
   for (int it = 0; it < 4; ++it) {
     const int r = it * 8 + (lane >> 2);
-    const uint4 v = *reinterpret_cast<const uint4*>(box + r * 64 + ((k ^ ((r >> 1) & 3)) << 4));
+    const uint8_t* src = box + r * 64 + ((k ^ ((r >> 1) & 3)) << 4);
     const int64_t orow = rows.out_row(r);
     if (orow < 0 || c >= N) continue;
     uint16_t* q = base + orow * o.ld + c;
     if (o.vec && c + 8 <= N) {
-      *reinterpret_cast<uint4*>(q) = v;
+      *reinterpret_cast<uint4*>(q) = *reinterpret_cast<const uint4*>(src);
     } else {
-      const uint32_t x[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (c + e < N) q[e] = (uint16_t)(x[e >> 1] >> (16 * (e & 1)));
-    }
-  }
-}
-
-// The same of fp32 values, stored as a 16-bit type or as planes.
-__device__ __forceinline__ void put_operand(uint8_t* box, const GemmOut& o, const GemmRows& rows, int col, int N,
-                                            const float (&v)[32]) {
-  uint16_t* base = static_cast<uint16_t*>(o.p);
-  if (o.kind != kOutPlanes) {
-    uint32_t w[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) w[i] = pack16(v[2 * i], v[2 * i + 1], o.kind == kOutF16);
-    put16(box, o, base, rows, col, N, w);
-    return;
-  }
 #pragma unroll 1
-  for (int pl = 0; pl < 3; ++pl, base += o.plane) {
-    uint32_t w[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      uint16_t a[3], b[3];
-      split_planes(v[2 * i], a);
-      split_planes(v[2 * i + 1], b);
-      w[i] = (pl == 0 ? a[0] : pl == 1 ? a[1] : a[2]) | (uint32_t)(pl == 0 ? b[0] : pl == 1 ? b[1] : b[2]) << 16;
+      for (int e = 0; e < 8 && c + e < N; ++e) q[e] = reinterpret_cast<const uint16_t*>(src)[e];
     }
-    put16(box, o, base, rows, col, N, w);
   }
 }
 
-// Four values of one row (those below N) as a final result: (v + bias) alpha + residual.
-struct GemmFinal {
-  float alpha;
-  const void* residual;
-  int64_t ld_res;
-  int dt, res_vec;
-};
-__device__ __forceinline__ void put4(const GemmOut& o, const GemmFinal& f, int64_t row, int64_t orow, int c, int N, float4 b,
-                                     float4 v) {
-  float x[4] = {(v.x + b.x) * f.alpha, (v.y + b.y) * f.alpha, (v.z + b.z) * f.alpha, (v.w + b.w) * f.alpha};
-  if (f.residual) {
-    const int64_t at = row * f.ld_res + c;
-    if (f.res_vec && c + 4 <= N) {
-      if (f.dt == M3B_F32) {
-        const float4 r = *reinterpret_cast<const float4*>(static_cast<const float*>(f.residual) + at);
-        x[0] += r.x, x[1] += r.y, x[2] += r.z, x[3] += r.w;
-      } else {
-        const uint2 r = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(f.residual) + at);
-        float2 p, q;
-        if (f.dt == M3B_BF16) {
-          p = bf2_to_f2(r.x), q = bf2_to_f2(r.y);
-        } else {
-          p = __half22float2(*reinterpret_cast<const __half2*>(&r.x));
-          q = __half22float2(*reinterpret_cast<const __half2*>(&r.y));
-        }
-        x[0] += p.x, x[1] += p.y, x[2] += q.x, x[3] += q.y;
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (c + e < N) x[e] += ldf(f.residual, at + e, f.dt);
-    }
-  }
-  const int64_t at = orow * o.ld + c;
-  if (o.kind == kOutF32) {
-    float* q = static_cast<float*>(o.p) + at;
-    if (o.vec && c + 4 <= N) {
-      *reinterpret_cast<float4*>(q) = make_float4(x[0], x[1], x[2], x[3]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (c + e < N) q[e] = x[e];
-    }
-  } else {
-    uint16_t* q = static_cast<uint16_t*>(o.p) + at;
-    const uint2 w = make_uint2(pack16(x[0], x[1], o.kind == kOutF16), pack16(x[2], x[3], o.kind == kOutF16));
-    if (o.vec && c + 4 <= N) {
-      *reinterpret_cast<uint2*>(q) = w;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (c + e < N) q[e] = (uint16_t)((e < 2 ? w.x : w.y) >> (16 * (e & 1)));
-    }
-  }
-}
-__device__ __forceinline__ float4 bias4(const void* bias, int dt, int c, int N) {
-  float b[4] = {0.f, 0.f, 0.f, 0.f};
-  if (bias)
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (c + e < N) b[e] = ldf(bias, c + e, dt);
-  return make_float4(b[0], b[1], b[2], b[3]);
-}
-
-// 32 columns as final results with bias and residual (fp32 until the one rounding).
-__device__ __forceinline__ void put_final(uint8_t* box, const GemmOut& o, const GemmFinal& f, const void* bias,
-                                          const GemmRows& rows, int col, int N, const float (&v)[32]) {
+// 32 columns of fp32 results.
+__device__ __forceinline__ void put32(uint8_t* box, const GemmOut& o, const GemmRows& rows, int col, int N,
+                                      const float (&v)[32]) {
   const int lane = threadIdx.x & 31;
   __syncwarp();
 #pragma unroll
@@ -322,13 +236,121 @@ __device__ __forceinline__ void put_final(uint8_t* box, const GemmOut& o, const 
         make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
   __syncwarp();
   const int k = lane & 7, c = col + 4 * k;
-  const float4 b = bias4(bias, f.dt, c, N);
+#pragma unroll 4
+  for (int it = 0; it < 8; ++it) {
+    const int r = it * 4 + (lane >> 3);
+    const uint8_t* src = box + r * 128 + ((k ^ (r & 7)) << 4);
+    const int64_t orow = rows.out_row(r);
+    if (orow < 0 || c >= N) continue;
+    float* q = static_cast<float*>(o.p) + orow * o.ld + c;
+    if (o.vec && c + 4 <= N) {
+      *reinterpret_cast<float4*>(q) = *reinterpret_cast<const float4*>(src);
+    } else {
+#pragma unroll 1
+      for (int e = 0; e < 4 && c + e < N; ++e) q[e] = reinterpret_cast<const float*>(src)[e];
+    }
+  }
+}
+
+// 32 columns of a following product's operand: a 16-bit type, or the planes of fp32 values.
+template <bool PLANES>
+__device__ __forceinline__ void put_operand(uint8_t* box, const GemmOut& o, const GemmRows& rows, int col, int N,
+                                            const float (&v)[32]) {
+  uint16_t* base = static_cast<uint16_t*>(o.p);
+  uint32_t w[16];
+  if constexpr (!PLANES) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w[i] = pack16(v[2 * i], v[2 * i + 1], o.kind == kOutF16);
+    put16(box, o, base, rows, col, N, w);
+  } else {
+#pragma unroll 1
+    for (int pl = 0; pl < 3; ++pl, base += o.plane) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        uint16_t a[3], b[3];
+        split_planes(v[2 * i], a);
+        split_planes(v[2 * i + 1], b);
+        w[i] = (pl == 0 ? a[0] : pl == 1 ? a[1] : a[2]) | (uint32_t)(pl == 0 ? b[0] : pl == 1 ? b[1] : b[2]) << 16;
+      }
+      put16(box, o, base, rows, col, N, w);
+    }
+  }
+}
+
+// 32 columns as final results, (v + bias) alpha + residual, fp32 until the one rounding.
+struct GemmFinal {
+  float alpha;
+  const void *bias, *residual;
+  int64_t ld_res;
+  int dt, res_vec;
+};
+__device__ __forceinline__ float4 final4(const GemmOut& o, const GemmFinal& f, float4 b, float4 t, float4 r) {
+  return make_float4(fmaf(t.x + b.x, f.alpha, r.x), fmaf(t.y + b.y, f.alpha, r.y), fmaf(t.z + b.z, f.alpha, r.z),
+                     fmaf(t.w + b.w, f.alpha, r.w));
+}
+__device__ __forceinline__ float4 bias4(const void* bias, int dt, int c, int N) {
+  float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (bias) {
+    if (c < N) b.x = ldf(bias, c, dt);
+    if (c + 1 < N) b.y = ldf(bias, c + 1, dt);
+    if (c + 2 < N) b.z = ldf(bias, c + 2, dt);
+    if (c + 3 < N) b.w = ldf(bias, c + 3, dt);
+  }
+  return b;
+}
+// Four residual values of 16 bits, as they lie in memory.
+__device__ __forceinline__ float4 wide4(uint2 r, int dt) {
+  float2 p, q;
+  if (dt == M3B_BF16) {
+    p = bf2_to_f2(r.x), q = bf2_to_f2(r.y);
+  } else {
+    p = __half22float2(*reinterpret_cast<const __half2*>(&r.x));
+    q = __half22float2(*reinterpret_cast<const __half2*>(&r.y));
+  }
+  return make_float4(p.x, p.y, q.x, q.y);
+}
+__device__ __forceinline__ void put_final(uint8_t* box, const GemmOut& o, const GemmFinal& f, const GemmRows& rows, int col,
+                                          int N, const float (&v)[32]) {
+  const int lane = threadIdx.x & 31, k = lane & 7, c = col + 4 * k;
+  const bool whole = o.vec && c + 4 <= N && o.kind != kOutF32 && (!f.residual || f.res_vec);
+  // the residual's loads of all rows are in flight while the box fills: one by one between the stores
+  // each cost its whole latency
+  uint2 raw[8];
+#pragma unroll
+  for (int it = 0; it < 8; ++it) {
+    const int64_t row = rows.row0 + it * 4 + (lane >> 3);
+    raw[it] = make_uint2(0u, 0u);
+    if (whole && f.residual && row < rows.M)
+      raw[it] = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(f.residual) + row * f.ld_res + c));
+  }
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    *reinterpret_cast<float4*>(box + lane * 128 + ((i ^ (lane & 7)) << 4)) =
+        make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+  __syncwarp();
+  const float4 b = bias4(f.bias, f.dt, c, N);
 #pragma unroll
   for (int it = 0; it < 8; ++it) {
     const int r = it * 4 + (lane >> 3);
-    const float4 x = *reinterpret_cast<const float4*>(box + r * 128 + ((k ^ (r & 7)) << 4));
-    const int64_t orow = rows.out_row(r);
-    if (orow >= 0 && c < N) put4(o, f, rows.row0 + r, orow, c, N, b, x);
+    const int64_t row = rows.row0 + r;
+    if (row >= rows.M || c >= N) continue;
+    const float4 t = *reinterpret_cast<const float4*>(box + r * 128 + ((k ^ (r & 7)) << 4));
+    if (whole) {
+      const float4 x = final4(o, f, b, t, wide4(raw[it], f.dt));
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(o.p) + row * o.ld + c) =
+          make_uint2(pack16(x.x, x.y, o.kind == kOutF16), pack16(x.z, x.w, o.kind == kOutF16));
+    } else {
+      const float* src = reinterpret_cast<const float*>(box + r * 128 + ((k ^ (r & 7)) << 4));
+#pragma unroll 1
+      for (int e = 0; e < 4 && c + e < N; ++e) {
+        float x = src[e];
+        if (f.bias) x += ldf(f.bias, c + e, f.dt);
+        x *= f.alpha;
+        if (f.residual) x += ldf(f.residual, row * f.ld_res + c + e, f.dt);
+        stf(o.p, row * o.ld + c + e, o.kind == kOutF32 ? M3B_F32 : o.kind == kOutF16 ? M3B_F16 : M3B_BF16, x);
+      }
+    }
   }
 }
 
@@ -405,7 +427,7 @@ __device__ __forceinline__ uint64_t gm_desc(uint32_t lo, uint32_t hi) {
 // ---------------------------------------------------------------------------
 // the kernel
 // ---------------------------------------------------------------------------
-template <int EPI, bool PAIR>
+template <int EPI, bool PAIR, bool PLANES>
 __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_constant__ GemmParams p) {
   constexpr int kTileM = PAIR ? 256 : 128;
   extern __shared__ uint8_t smraw[];
@@ -466,6 +488,14 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
       // B rows of this CTA; the gated product stages bn / 2 gate and bn / 2 up rows (paired: the
       // first CTA holds the gate's, the second the up's)
       const int brow = EPI == kEpiGlu ? job.nt * (bn / 2) : job.nt * bn + (int)rank * brows;
+      if constexpr (EPI == kEpiDglu) {
+        // the tile's g and u on their way into L2 while its products run
+        const int64_t q0 = (int64_t)job.nt * (bn / 4), quads = p.gu_ld4 - q0 < bn / 4 ? p.gu_ld4 - q0 : bn / 4;
+        if (lane < 4 && arow + 32 * lane < s.M)
+          prefetch_l2(reinterpret_cast<const float4*>(p.gu) + ((int64_t)(arow / 32 + lane) * p.gu_ld4 + q0) * 64,
+                      (uint32_t)quads * 1024u);
+        __syncwarp();
+      }
       int pass = job.kb / (nks > 0 ? nks : 1), r = job.kb - pass * nks;
       for (int i = job.kb; i < job.ke; ++i, ++it) {
         ok = __all_sync(0xffffffffu, gm_wait<PAIR>(&empty[st], ph, p.wait_ns));
@@ -599,35 +629,55 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
           f(c, v);
         }
       };
+      const int cfirst = half * (bn / 2), clast = cfirst + bn / 2;
+      auto scale_of = [&]() {
+        float alpha = s.alpha;
+        if (s.alpha_num) alpha *= *s.alpha_num;
+        if (s.alpha_den) alpha = *s.alpha_den > 0 ? alpha / (float)*s.alpha_den : 0.f;
+        return alpha;
+      };
+      auto put_scaled = [&](int col, float (&v)[32], float alpha) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] *= alpha;
+        if (s.out.kind == kOutF32) put32(box, s.out, rows, col, s.N, v);
+        else put_operand<false>(box, s.out, rows, col, s.N, v);
+      };
       if constexpr (EPI == kEpiStore) {
-        GemmFinal fin{s.alpha, s.residual, s.ld_res, s.dt, s.res_vec};
-        if (s.alpha_num) fin.alpha *= *s.alpha_num;
-        if (s.alpha_den) fin.alpha = *s.alpha_den > 0 ? fin.alpha / (float)*s.alpha_den : 0.f;
+        const float alpha = scale_of();
+        columns(cfirst, clast, [&](int c, float (&v)[32]) {
+          const int col = job.nt * bn + c;
+          if (col < s.N) put_scaled(col, v, alpha);
+        });
+      } else if constexpr (EPI == kEpiFinal) {
+        const GemmFinal fin{s.alpha, s.bias, s.residual, s.ld_res, s.dt, s.res_vec};
+        columns(cfirst, clast, [&](int c, float (&v)[32]) {
+          const int col = job.nt * bn + c;
+          if (col < s.N) put_final(box, s.out, fin, rows, col, s.N, v);
+        });
+      } else if constexpr (EPI == kEpiAcc) {
+        const float alpha = scale_of();
         rows.row_index = s.row_index;
         const int nq = s.nt * bn / 4;
-        const bool plain = s.out.kind != kOutF32 && !s.residual && !s.bias;
-        columns(half * (bn / 2), (half + 1) * (bn / 2), [&](int c, float (&v)[32]) {
+        columns(cfirst, clast, [&](int c, float (&v)[32]) {
           const int col = job.nt * bn + c;
           if (col >= s.N) return;
           if (s.acc_mode != 0) {
             float4* ap = reinterpret_cast<float4*>(s.acc) + ((grow >> 5) * nq + (col >> 2)) * 32 + lane;
+            if (s.acc_mode != 1) {
+              float4 o[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i, ap += 32) {
-              if (s.acc_mode != 1) {
-                const float4 o = *ap;
-                v[4 * i] += o.x, v[4 * i + 1] += o.y, v[4 * i + 2] += o.z, v[4 * i + 3] += o.w;
-              }
-              if (s.acc_mode != 3) *ap = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+              for (int i = 0; i < 8; ++i) o[i] = ap[i * 32];
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                v[4 * i] += o[i].x, v[4 * i + 1] += o[i].y, v[4 * i + 2] += o[i].z, v[4 * i + 3] += o[i].w;
             }
-            if (s.acc_mode != 3) return;
-          }
-          if (plain) {
+            if (s.acc_mode != 3) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] *= fin.alpha;
-            put_operand(box, s.out, rows, col, s.N, v);
-          } else {
-            put_final(box, s.out, fin, s.bias, rows, col, s.N, v);
+              for (int i = 0; i < 8; ++i) ap[i * 32] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+              return;
+            }
           }
+          put_scaled(col, v, alpha);
         });
       } else if constexpr (EPI == kEpiGlu) {
         const int hb = bn / 2;
@@ -660,32 +710,38 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
           }
 #pragma unroll
           for (int i = 0; i < 32; ++i) g[i] = g[i] * sigmoid_fast(g[i]) * u[i];
-          put_operand(box, s.out, rows, col, s.N, g);
+          put_operand<PLANES>(box, s.out, rows, col, s.N, g);
         }
       } else if constexpr (EPI == kEpiDglu) {
-        columns(half * (bn / 2), (half + 1) * (bn / 2), [&](int c, float (&d)[32]) {
+        columns(cfirst, clast, [&](int c, float (&d)[32]) {
           const int col = job.nt * bn + c;
           if (col >= s.N) return;
           const float4* gp = reinterpret_cast<const float4*>(p.gu) + ((grow >> 5) * p.gu_ld4 + (col >> 2)) * 64 + lane;
           float u[32];
 #pragma unroll
-          for (int i = 0; i < 8; ++i, gp += 64) {
-            const float4 a = gp[0], b = gp[32];
-            const float g4[4] = {a.x, a.y, a.z, a.w}, u4[4] = {b.x, b.y, b.z, b.w};
+          for (int h = 0; h < 8; h += 4) {
+            float4 a[4], b[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float g = g4[e], sg = sigmoid_fast(g), ds = d[4 * i + e] * s.alpha * sg;
-              d[4 * i + e] = ds * u4[e] * fmaf(g, 1.f - sg, 1.f);
-              u[4 * i + e] = ds * g;
+            for (int i = 0; i < 4; ++i) a[i] = __ldg(gp + (h + i) * 64), b[i] = __ldg(gp + (h + i) * 64 + 32);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float g4[4] = {a[i].x, a[i].y, a[i].z, a[i].w}, u4[4] = {b[i].x, b[i].y, b[i].z, b[i].w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int j = 4 * (h + i) + e;
+                const float sg = sigmoid_fast(g4[e]), ds = d[j] * s.alpha * sg;
+                d[j] = ds * u4[e] * fmaf(g4[e], 1.f - sg, 1.f);
+                u[j] = ds * g4[e];
+              }
             }
           }
-          put_operand(box, s.out, rows, col, s.N, d);
-          put_operand(box, s.out2, rows, col, s.N, u);
+          put_operand<PLANES>(box, s.out, rows, col, s.N, d);
+          put_operand<PLANES>(box, s.out2, rows, col, s.N, u);
         });
       } else if constexpr (EPI == kEpiLse) {
         const int tgt = rok ? p.target[grow] : -1;
         float m = -1e30f, sum = 0.f;  // m in powers of two
-        columns(half * (bn / 2), (half + 1) * (bn / 2), [&](int c, float (&v)[32]) {
+        columns(cfirst, clast, [&](int c, float (&v)[32]) {
           const int col = job.nt * bn + c;
           if (col >= s.N) return;
           const int to = tgt - col;
@@ -714,7 +770,7 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
         const int tgt = rok ? p.target[grow] - p.col0 : -1;
         const float l2 = rok ? p.lse2[grow] : 0.f, w = rok && p.roww ? p.roww[grow] : 1.f;
         rows.M = 0x7fffffff;  // rows behind the last kept token are K values of the next products: zero
-        columns(half * (bn / 2), (half + 1) * (bn / 2), [&](int c, float (&v)[32]) {
+        columns(cfirst, clast, [&](int c, float (&v)[32]) {
           const int col = job.nt * bn + c;
           if (col >= s.N) return;
 #pragma unroll
@@ -732,7 +788,7 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = 0.f;
           }
-          put_operand(box, s.out, rows, col, s.N, v);
+          put_operand<PLANES>(box, s.out, rows, col, s.N, v);
         });
       }
       release();

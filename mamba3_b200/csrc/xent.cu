@@ -388,7 +388,7 @@ int backward(const m3b_linear_xent_args* a, void* workspace, size_t* need, bool 
       g.row_index = s.row;
       g.acc = acc;
       g.acc_mode = !acc ? 0 : c0 == 0 ? 1 : c0 + cols < d.V ? 2 : 3;
-      M3B_TRY(launch_gemm(p, kEpiStore, true, st));
+      M3B_TRY(launch_gemm(p, kEpiAcc, true, st));
     }
     if (a->dweight) {
       GemmParams p = base;
