@@ -8,7 +8,7 @@
 // Forward: one product whose tiles hold gate and up columns side by side, so the activation and the
 // product are its epilogue (g and u never reach memory in inference), then the down product with
 // bias, scale and residual in its epilogue.  Backward: da's product with dg and du as its epilogue;
-// dx as one product over two K segments; the three weight gradients side by side in one launch.
+// dx (one product over two K segments) and the three weight gradients side by side in one launch.
 // 18 rows d_model d_ff operations forward and backward, the least there are: g and u are kept in
 // fp32 (8 bytes a value), because the rounding of a 16-bit copy would reach every gradient.
 #include "gemm.cuh"
@@ -69,31 +69,57 @@ GemmOut operand_out(const GemmOperand& o, bool f16) {
   return r;
 }
 
-// Sum over rows of a (rows x cols) matrix times `scale`, in a fixed order: 64 column threads and
-// chunks of rows per block, then the chunks.
-constexpr int kSumRows = 256;
-__global__ void colsum_kernel(const void* __restrict__ x, int dt, int planes, int64_t plane, int64_t ld, int64_t rows,
-                              int cols, float* __restrict__ part) {
-  const int c = blockIdx.x * 64 + threadIdx.x;
+// Sum over the rows of an operand times `scale`, in a fixed order.  A block takes 64 columns (two a
+// lane) and kSumRows rows, its warps every eighth row, and leaves one partial; the chunks' partials
+// are added by a second kernel.
+constexpr int kSumRows = 128;
+__global__ void __launch_bounds__(256) colsum_kernel(const uint16_t* __restrict__ x, int f16, int planes, int64_t plane,
+                                                     int64_t ld, int64_t rows, int cols, float* __restrict__ part) {
+  __shared__ float2 sm[8][32];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = blockIdx.x * 64 + 2 * lane;
   const int64_t r0 = (int64_t)blockIdx.y * kSumRows, r1 = r0 + kSumRows < rows ? r0 + kSumRows : rows;
-  if (c >= cols) return;
-  float s = 0.f;
-  for (int64_t r = r0; r < r1; ++r)
-    for (int k = planes - 1; k >= 0; --k) s += ldf(x, k * plane + r * ld + c, dt);
-  part[(int64_t)blockIdx.y * cols + c] = s;
+  float2 s = make_float2(0.f, 0.f);
+  if (c < cols) {
+#pragma unroll 8
+    for (int64_t r = r0 + w; r < r1; r += 8) {
+      for (int k = planes - 1; k >= 0; --k) {
+        const uint16_t* p = x + k * plane + r * ld + c;
+        const uint32_t v = c + 1 < cols ? *reinterpret_cast<const uint32_t*>(p) : (uint32_t)*p;
+        const float2 f = f16 ? __half22float2(*reinterpret_cast<const __half2*>(&v)) : bf2_to_f2(v);
+        s.x += f.x;
+        s.y += f.y;
+      }
+    }
+  }
+  sm[w][lane] = s;
+  __syncthreads();
+  if (w != 0 || c >= cols) return;
+  for (int k = 1; k < 8; ++k) s.x += sm[k][lane].x, s.y += sm[k][lane].y;
+  float* o = part + (int64_t)blockIdx.y * cols + c;
+  o[0] = s.x;
+  if (c + 1 < cols) o[1] = s.y;
 }
-__global__ void colsum_finish_kernel(const float* __restrict__ part, int chunks, int cols, float scale, void* out,
-                                     int dt) {
-  const int c = blockIdx.x * blockDim.x + threadIdx.x;
-  if (c >= cols) return;
+__global__ void __launch_bounds__(256) colsum_finish_kernel(const float* __restrict__ part, int chunks, int cols, float scale,
+                                                            void* out, int dt) {
+  __shared__ float sm[8][32];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
   float s = 0.f;
-  for (int k = 0; k < chunks; ++k) s += part[(int64_t)k * cols + c];
+  if (c < cols) {
+#pragma unroll 4
+    for (int k = w; k < chunks; k += 8) s += part[(int64_t)k * cols + c];
+  }
+  sm[w][lane] = s;
+  __syncthreads();
+  if (w != 0 || c >= cols) return;
+  for (int k = 1; k < 8; ++k) s += sm[k][lane];
   stf(out, c, dt, s * scale);
 }
-int colsum(const GemmOperand& o, int dt, float scale, void* out, int out_dt, float* part, cudaStream_t st) {
+int colsum(const GemmOperand& o, bool f16, float scale, void* out, int out_dt, float* part, cudaStream_t st) {
   const int chunks = (int)((o.rows + kSumRows - 1) / kSumRows), cols = (int)o.cols;
-  colsum_kernel<<<dim3((cols + 63) / 64, chunks), 64, 0, st>>>(o.p, dt, o.planes, o.plane, o.ld, o.rows, cols, part);
-  colsum_finish_kernel<<<(cols + 255) / 256, 256, 0, st>>>(part, chunks, cols, scale, out, out_dt);
+  if (chunks > 65535) return fail(M3B_ERR_UNSUPPORTED, "gated_ffn_bwd: bias gradients over more than 8,388,480 rows");
+  colsum_kernel<<<dim3((cols + 63) / 64, chunks), 256, 0, st>>>(static_cast<const uint16_t*>(o.p), f16, o.planes, o.plane,
+                                                               o.ld, o.rows, cols, part);
+  colsum_finish_kernel<<<(cols + 31) / 32, 256, 0, st>>>(part, chunks, cols, scale, out, out_dt);
   return check_launch("colsum_kernel");
 }
 
@@ -139,6 +165,16 @@ GemmOperand act_operand(const m3b_gated_ffn_args* a, void* p) {
   } while (0)
 #define M3B_MAP(...) M3B_TRY(gemm_map(__VA_ARGS__))
 
+GemmParams params(const Dims& d, const m3b_gated_ffn_args* a, int bn) {
+  GemmParams p{};
+  p.bn = bn;
+  p.npass = d.f32 ? 6 : 1;
+  p.f16 = d.f16;
+  p.err = a->err;
+  return p;
+}
+int blocks_of(int64_t k) { return (int)((k + kGmBK - 1) / kGmBK); }
+
 // run == false only measures the workspace.
 int forward(const m3b_gated_ffn_args* a, void* workspace, size_t* need, bool run, cudaStream_t st) {
   const Dims d(a);
@@ -148,52 +184,47 @@ int forward(const m3b_gated_ffn_args* a, void* workspace, size_t* need, bool run
   const GemmOperand wg = operand(a->w_gate, d.F, d.D, d.D, a, ws, run, st, &rc);
   const GemmOperand wu = operand(a->w_up, d.F, d.D, d.D, a, ws, run, st, &rc);
   const GemmOperand wd = operand(a->w_down, d.D, d.F, d.F, a, ws, run, st, &rc);
-  *need = ws.at;
-  if (!run || rc != M3B_OK) return rc;
   const GemmOperand act = act_operand(a, a->saved_act);
   const bool pair = d.M > 128;
-  {
-    GemmParams p{};
-    GemmSub& s = p.sub[0];
-    p.nsub = 1;
-    p.bn = pair ? 256 : 128;
-    p.npass = d.f32 ? 6 : 1;
-    p.f16 = d.f16;
-    p.err = a->err;
-    M3B_MAP(&s.a[0], x, false, 128, d.f16);
-    M3B_MAP(&s.b[0], wg, false, gemm_box_b(pair, p.bn, kEpiGlu), d.f16);
-    M3B_MAP(&s.b[1], wu, false, gemm_box_b(pair, p.bn, kEpiGlu), d.f16);
-    s.M = (int)d.M;
-    s.N = d.F;
-    s.nk[0] = (d.D + kGmBK - 1) / kGmBK;
-    s.out = operand_out(act, d.f16);
-    s.bias = a->b_gate;
-    s.bias2 = a->b_up;
-    s.dt = a->dtype;
-    p.gu = static_cast<float*>(a->saved_gu);
-    p.gu_ld4 = up(d.F, 32) / 4;
-    M3B_TRY(launch_gemm(p, kEpiGlu, pair, st));
-  }
-  GemmParams p{};
+
+  GemmParams p = params(d, a, pair ? 256 : 128);
   GemmSub& s = p.sub[0];
   p.nsub = 1;
-  p.bn = pair ? 256 : 64;
-  p.npass = d.f32 ? 6 : 1;
-  p.f16 = d.f16;
-  p.err = a->err;
-  M3B_MAP(&s.a[0], act, false, 128, d.f16);
-  M3B_MAP(&s.b[0], wd, false, gemm_box_b(pair, p.bn, kEpiFinal), d.f16);
   s.M = (int)d.M;
-  s.N = d.D;
-  s.nk[0] = (d.F + kGmBK - 1) / kGmBK;
-  s.out = result(a->out, d.D, a->dtype);
-  s.alpha = a->residual_scale;
-  s.bias = a->b_down;
-  s.residual = a->residual;
-  s.ld_res = a->residual_stride;
-  s.res_vec = aligned16(a->residual) && a->residual_stride % 4 == 0;
+  s.N = d.F;
+  s.nk[0] = blocks_of(d.D);
+  s.out = operand_out(act, d.f16);
+  s.bias = a->b_gate;
+  s.bias2 = a->b_up;
   s.dt = a->dtype;
-  return launch_gemm(p, kEpiFinal, pair, st);
+  p.gu = static_cast<float*>(a->saved_gu);
+  p.gu_ld4 = up(d.F, 32) / 4;
+  plan_gemm(p, kEpiGlu, pair);
+
+  GemmParams q = params(d, a, pair ? 256 : 64);
+  GemmSub& t = q.sub[0];
+  q.nsub = 1;
+  t.M = (int)d.M;
+  t.N = d.D;
+  t.nk[0] = blocks_of(d.F);
+  t.out = result(a->out, d.D, a->dtype);
+  t.alpha = a->residual_scale;
+  t.bias = a->b_down;
+  t.residual = a->residual;
+  t.ld_res = a->residual_stride;
+  t.res_vec = aligned16(a->residual) && a->residual_stride % 4 == 0;
+  t.dt = a->dtype;
+  void* parts = ws.take(plan_gemm(q, kEpiFinal, pair));
+  *need = ws.at;
+  if (!run || rc != M3B_OK) return rc;
+
+  M3B_MAP(&s.a[0], x, false, 128, d.f16);
+  M3B_MAP(&s.b[0], wg, false, gemm_box_b(pair, p.bn, kEpiGlu), d.f16);
+  M3B_MAP(&s.b[1], wu, false, gemm_box_b(pair, p.bn, kEpiGlu), d.f16);
+  M3B_TRY(launch_gemm(p, kEpiGlu, pair, nullptr, st));
+  M3B_MAP(&t.a[0], act, false, 128, d.f16);
+  M3B_MAP(&t.b[0], wd, false, gemm_box_b(pair, q.bn, kEpiFinal), d.f16);
+  return launch_gemm(q, kEpiFinal, pair, parts, st);
 }
 
 int backward(const m3b_gated_ffn_args* a, void* workspace, size_t* need, bool run, cudaStream_t st) {
@@ -207,84 +238,68 @@ int backward(const m3b_gated_ffn_args* a, void* workspace, size_t* need, bool ru
   const GemmOperand dy = operand(a->dout, d.M, d.D, a->dout_stride, a, ws, run, st, &rc);
   const size_t one = (size_t)act_operand(a, nullptr).plane * d.np * 2;
   const GemmOperand dg = act_operand(a, ws.take(one)), du = act_operand(a, ws.take(one));
+  const GemmOperand act = act_operand(a, a->saved_act);
   const int64_t chunks = (d.M + kSumRows - 1) / kSumRows;
   float* part = static_cast<float*>(ws.take((size_t)chunks * (d.F > d.D ? d.F : d.D) * 4));
+  int* ticket = static_cast<int*>(ws.take(4));
+
+  // dx and the three weight gradients, side by side
+  GemmParams q = params(d, a, 256);
+  q.ticket = ticket;
+  struct Product {
+    void* out;
+    const GemmOperand *a[2], *b[2];
+    bool a_mn;
+    int64_t M, N, K;
+    float alpha;
+  };
+  const Product all[4] = {{a->dx, {&dg, &du}, {&wg, &wu}, false, d.M, d.D, d.F, 1.f},
+                          {a->dw_gate, {&dg, nullptr}, {&x, nullptr}, true, d.F, d.D, d.M, 1.f},
+                          {a->dw_up, {&du, nullptr}, {&x, nullptr}, true, d.F, d.D, d.M, 1.f},
+                          {a->dw_down, {&dy, nullptr}, {&act, nullptr}, true, d.D, d.F, d.M, a->residual_scale}};
+  for (const Product& e : all) {
+    if (!e.out) continue;
+    GemmSub& s = q.sub[q.nsub++];
+    for (int k = 0; k < 2 && e.a[k]; ++k) {
+      if (run) {
+        M3B_MAP(&s.a[k], *e.a[k], e.a_mn, 128, d.f16);
+        M3B_MAP(&s.b[k], *e.b[k], true, 0, d.f16);
+      }
+      s.nk[k] = blocks_of(e.K);
+    }
+    s.a_mn = e.a_mn;
+    s.b_mn = 1;
+    s.M = (int)e.M;
+    s.N = (int)e.N;
+    s.alpha = e.alpha;
+    s.out = result(e.out, e.N, a->dtype);
+  }
+  void* parts = ws.take(plan_gemm(q, kEpiStore, true));
   *need = ws.at;
   if (!run || rc != M3B_OK) return rc;
-  const GemmOperand act = act_operand(a, a->saved_act);
-  const int npass = d.f32 ? 6 : 1;
-  const int bn = 256;
+  if (cudaMemsetAsync(ticket, 0, 4, st) != cudaSuccess) return check_launch("gated_ffn_bwd");
   {  // da -> dg, du
-    GemmParams p{};
+    GemmParams p = params(d, a, 256);
     GemmSub& s = p.sub[0];
     p.nsub = 1;
-    p.bn = bn;
-    p.npass = npass;
-    p.f16 = d.f16;
-    p.err = a->err;
     M3B_MAP(&s.a[0], dy, false, 128, d.f16);
     M3B_MAP(&s.b[0], wd, true, 0, d.f16);
     s.b_mn = 1;
     s.M = (int)d.M;
     s.N = d.F;
-    s.nk[0] = (d.D + kGmBK - 1) / kGmBK;
+    s.nk[0] = blocks_of(d.D);
     s.alpha = a->residual_scale;
     s.out = operand_out(dg, d.f16);
     s.out2 = operand_out(du, d.f16);
     p.gu = static_cast<float*>(a->saved_gu);
     p.gu_ld4 = up(d.F, 32) / 4;
-    M3B_TRY(launch_gemm(p, kEpiDglu, true, st));
+    plan_gemm(p, kEpiDglu, true);
+    M3B_TRY(launch_gemm(p, kEpiDglu, true, nullptr, st));
   }
-  if (a->dx) {
-    GemmParams p{};
-    GemmSub& s = p.sub[0];
-    p.nsub = 1;
-    p.bn = bn;
-    p.npass = npass;
-    p.f16 = d.f16;
-    p.err = a->err;
-    M3B_MAP(&s.a[0], dg, false, 128, d.f16);
-    M3B_MAP(&s.a[1], du, false, 128, d.f16);
-    M3B_MAP(&s.b[0], wg, true, 0, d.f16);
-    M3B_MAP(&s.b[1], wu, true, 0, d.f16);
-    s.b_mn = 1;
-    s.M = (int)d.M;
-    s.N = d.D;
-    s.nk[0] = s.nk[1] = (d.F + kGmBK - 1) / kGmBK;
-    s.alpha = 1.f;
-    s.out = result(a->dx, d.D, a->dtype);
-    M3B_TRY(launch_gemm(p, kEpiStore, true, st));
-  }
-  GemmParams p{};
-  p.bn = bn;
-  p.npass = npass;
-  p.f16 = d.f16;
-  p.err = a->err;
-  const struct {
-    void* out;
-    const GemmOperand *l, *r;
-    int M, N;
-    float alpha;
-  } w[3] = {{a->dw_gate, &dg, &x, d.F, d.D, 1.f},
-            {a->dw_up, &du, &x, d.F, d.D, 1.f},
-            {a->dw_down, &dy, &act, d.D, d.F, a->residual_scale}};
-  for (const auto& e : w) {
-    if (!e.out) continue;
-    GemmSub& s = p.sub[p.nsub++];
-    M3B_MAP(&s.a[0], *e.l, true, 0, d.f16);
-    M3B_MAP(&s.b[0], *e.r, true, 0, d.f16);
-    s.a_mn = s.b_mn = 1;
-    s.M = e.M;
-    s.N = e.N;
-    s.nk[0] = (int)((d.M + kGmBK - 1) / kGmBK);
-    s.alpha = e.alpha;
-    s.out = result(e.out, e.N, a->dtype);
-  }
-  if (p.nsub) M3B_TRY(launch_gemm(p, kEpiStore, true, st));
-  const int odt = d.f32 ? M3B_BF16 : a->dtype;  // planes are bf16
-  if (a->db_gate) M3B_TRY(colsum(dg, odt, 1.f, a->db_gate, a->dtype, part, st));
-  if (a->db_up) M3B_TRY(colsum(du, odt, 1.f, a->db_up, a->dtype, part, st));
-  if (a->db_down) M3B_TRY(colsum(dy, odt, a->residual_scale, a->db_down, a->dtype, part, st));
+  if (q.nsub) M3B_TRY(launch_gemm(q, kEpiStore, true, parts, st));
+  if (a->db_gate) M3B_TRY(colsum(dg, d.f16, 1.f, a->db_gate, a->dtype, part, st));
+  if (a->db_up) M3B_TRY(colsum(du, d.f16, 1.f, a->db_up, a->dtype, part, st));
+  if (a->db_down) M3B_TRY(colsum(dy, d.f16, a->residual_scale, a->db_down, a->dtype, part, st));
   return M3B_OK;
 }
 

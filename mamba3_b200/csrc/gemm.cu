@@ -127,26 +127,96 @@ int gemm_map(CUtensorMap* m, const GemmOperand& o, bool mn_major, int box_rows, 
               (long long)o.rows, (long long)o.cols, (long long)o.ld, o.planes, (int)r);
 }
 
-int launch_gemm(GemmParams& p, int epi, bool pair, cudaStream_t st) {
-  int pairs = 0;
-  const int rc = device_setup(&pairs);
-  if (rc != M3B_OK) return rc;
+size_t plan_gemm(GemmParams& p, int epi, bool pair) {
   const int tile_m = gemm_tile_m(pair), tile_n = epi == kEpiGlu ? p.bn / 2 : p.bn;
-  int64_t jobs = 0;
+  const double workers = pair ? num_sms() / 2 : num_sms();
+  auto length = [&](const GemmSub& s) { return (double)(s.nk[0] + s.nk[1]) * p.npass; };
+  double longest = 0.0, work = 0.0;
   for (int i = 0; i < p.nsub; ++i) {
     GemmSub& s = p.sub[i];
     s.mt = (s.M + tile_m - 1) / tile_m;
     s.nt = (s.N + tile_n - 1) / tile_n;
-    jobs += (int64_t)s.mt * s.nt;
+    s.split = 1;
+    work += length(s) * s.mt * s.nt;
+    longest = length(s) > longest ? length(s) : longest;
+  }
+  auto part_bytes = [&](const GemmSub& s, int split) { return (double)split * s.mt * tile_m * s.nt * p.bn * 4.0; };
+  if (epi == kEpiStore || epi == kEpiFinal || epi == kEpiAcc) {
+    // How finely to split K: the length no job may pass, from none to many small ones, by an estimate in
+    // K blocks (0.36 us each).  Equal jobs finish in whole rounds; drawn ones leave half the longest
+    // idle.  A split costs the parts' way out and in (3 TB/s measured: 1.1 MB a block) and a launch.
+    // 16384 x 768 x 2112: 50 us whole, 94 us in two; 4096 tokens x 768 into 768 x 32000 (30 tiles of 500
+    // blocks beside 375 of 39): 240 us whole, 160 us in four.
+    double best = 0.0, limit = longest;
+    for (double most = longest; most >= 4.0; most *= 0.8) {
+      double jobs = 0.0, sum = 0.0, top = 0.0, extra = 0.0, one = 0.0;
+      for (int i = 0; i < p.nsub; ++i) {
+        const GemmSub& s = p.sub[i];
+        const int split = (int)((length(s) + most - 1.0) / most);
+        const double len = (length(s) + split - 1.0) / split + 4.0, n = (double)s.mt * s.nt * split;
+        jobs += n;
+        sum += n * len;
+        top = len > top ? len : top;
+        one = len;
+        if (split > 1) extra += part_bytes(s, split + 1) / 1.1e6;
+      }
+      if (extra > 0.0) extra += 8.0;
+      double t = sum / workers + top / 2.0 > top ? sum / workers + top / 2.0 : top;
+      if (p.nsub == 1) t = (double)(int64_t)((jobs + workers - 1.0) / workers) * one;
+      if (best == 0.0 || t + extra < best * 0.98) {
+        best = t + extra;
+        limit = most;
+      }
+    }
+    for (int i = 0; i < p.nsub; ++i) p.sub[i].split = (int)((length(p.sub[i]) + limit - 1.0) / limit);
+  }
+  size_t bytes = 0;
+  for (int i = 0; i < p.nsub; ++i) {
+    if (p.sub[i].split < 1) p.sub[i].split = 1;
+    if (p.sub[i].split > 1) bytes += (size_t)part_bytes(p.sub[i], p.sub[i].split);
+  }
+  for (int i = 1; i < p.nsub; ++i)  // longest jobs first
+    for (int k = i; k > 0 && length(p.sub[k]) / p.sub[k].split > length(p.sub[k - 1]) / p.sub[k - 1].split; --k) {
+      const GemmSub t = p.sub[k];
+      p.sub[k] = p.sub[k - 1];
+      p.sub[k - 1] = t;
+    }
+  return bytes;
+}
+
+int launch_gemm(GemmParams& p, int epi, bool pair, void* parts, cudaStream_t st) {
+  int pairs = 0;
+  const int rc = device_setup(&pairs);
+  if (rc != M3B_OK) return rc;
+  const int tile_m = gemm_tile_m(pair);
+  int64_t jobs = 0, pieces = 0;
+  float* at = static_cast<float*>(parts);
+  for (int i = 0; i < p.nsub; ++i) {
+    GemmSub& s = p.sub[i];
+    jobs += (int64_t)s.mt * s.nt * s.split;
+    if (s.split > 1) {
+      s.part = at;
+      at += (size_t)s.split * s.mt * tile_m * s.nt * p.bn;
+      pieces += (int64_t)((s.M + 31) / 32) * ((s.N + 31) / 32);
+    }
   }
   if (jobs == 0) return M3B_OK;
+  if (jobs > (int64_t(1) << 30)) return fail(M3B_ERR_UNSUPPORTED, "gemm: too many tiles");
   if (p.wait_ns == 0) p.wait_ns = kWaitLimitNs;
   const int64_t most = pair ? pairs : num_sms();
   const unsigned workers = (unsigned)(jobs < most ? jobs : most);
-  cudaLaunchAttribute at[1];
-  const cudaLaunchConfig_t cfg = config(pair ? 2 * workers : workers, pair, st, at);
+  cudaLaunchAttribute attr[1];
+  const cudaLaunchConfig_t cfg = config(pair ? 2 * workers : workers, pair, st, attr);
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel_of(epi, pair, p.npass > 1), p);
   if (e != cudaSuccess) return fail(M3B_ERR_CUDA, "gemm_kernel: %s", cudaGetErrorString(e));
+  if (pieces) {
+    int split = 1, warps = 1;  // warps to a piece
+    for (int i = 0; i < p.nsub; ++i) split = p.sub[i].split > split ? p.sub[i].split : split;
+    while (warps < 8 && warps * 2 < split) warps *= 2;
+    const unsigned grid = (unsigned)((pieces + 8 / warps - 1) / (8 / warps));
+    if (epi == kEpiFinal) gemm_join_kernel<kEpiFinal><<<grid, 256, 0, st>>>(p, tile_m, warps);
+    else gemm_join_kernel<kEpiAcc><<<grid, 256, 0, st>>>(p, tile_m, warps);
+  }
   return check_launch("gemm_kernel");
 }
 

@@ -10,14 +10,20 @@
 // * fp32 operands travel as three bf16 planes whose sum is the value exactly (each plane takes
 //   the next 8 significant bits by truncation).  The product runs over the six plane pairs with
 //   2^-16 or more of the leading one's weight, smallest first; the dropped pairs are below 2^-24.
-// * A launch holds up to three products ("subs"), so that products that are too small to fill the
+// * A launch holds up to four products ("subs"), so that products that are too small to fill the
 //   GPU run side by side, and a product has up to two K segments with operands of their own.
 // * Row or K counts may come from device memory (`dyn`): the loss drops ignored tokens without
 //   the host knowing how many remain.
 //
 // Three roles per CTA: warp 0 the TMA producer, warp 1 the MMA issuer, warps 2-9 the epilogue (two
 // warps per 32 TMEM lanes, half of the columns each).  Two TMEM accumulators of 256 columns let a
-// tile's epilogue run under the next tile's MMAs.  PAIR: a cluster of two CTAs computes 256 x bn
+// tile's epilogue run under the next tile's MMAs.  Jobs of one length are dealt in turn; jobs of
+// several lengths (several products, or one whose long K is split) are listed longest first and drawn
+// from a counter in device memory by whoever is nearly free (the first CTA's producer, a dozen K blocks
+// before it has none left; it passes the job on to the other roles through a small queue), which leaves
+// idle at most the last job's length.
+// A split product's parts go to the workspace in fp32 and a join kernel adds them in order, so the
+// result does not depend on who took which job.  PAIR: a cluster of two CTAs computes 256 x bn
 // tiles with cta_group::2, each CTA staging half of the B rows; otherwise single CTAs compute
 // 128 x bn tiles.
 #pragma once
@@ -29,6 +35,8 @@
 namespace m3b {
 
 constexpr int kGmThreads = 320;
+constexpr int kGmSubs = 4;      // products of a launch at most
+constexpr int kGmQueue = 4;     // drawn jobs that the producer may be ahead of the epilogue
 constexpr int kGmBK = 64;
 constexpr int kGmStages = 6;
 constexpr uint32_t kGmStageA = 128 * kGmBK * 2;     // 16 KB
@@ -37,7 +45,7 @@ constexpr uint32_t kGmRing = kGmStages * kGmStage;  // 192 KB
 constexpr uint32_t kGmBox = 32 * 128;               // staging of an epilogue warp: 32 rows x 32 fp32
 constexpr uint32_t kGmBoxOff = kGmRing;
 constexpr uint32_t kGmBarOff = kGmBoxOff + 8 * kGmBox;
-constexpr uint32_t kGmSmem = kGmBarOff + 256 + 1024;
+constexpr uint32_t kGmSmem = kGmBarOff + 384 + 1024;  // barriers, job queue, TMEM slot; alignment
 static_assert(kGmSmem <= 227 * 1024, "shared memory plan");
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -74,6 +82,8 @@ struct GemmSub {
   int mt, nt;      // tiles
   int a_mn, b_mn;  // operand stored MN-major
   int m_dyn, k_dyn;
+  int split;       // jobs along K of each tile
+  float* part;     // [split][row / 32][col / 4][row % 32][4] fp32 when split > 1
   GemmOut out, out2;
   // kEpiStore, kEpiFinal, kEpiAcc
   float alpha;
@@ -90,12 +100,13 @@ struct GemmSub {
 };
 
 struct GemmParams {
-  GemmSub sub[3];
+  GemmSub sub[kGmSubs];
   int nsub;
   int bn;       // accumulator columns of a tile
   int npass;    // plane pairs: 1, or 6 for fp32 operands
   int f16;      // operand type: fp16 instead of bf16
   const int* dyn;
+  int* ticket;  // zeroed counter that jobs are drawn from, or null: dealt in turn
   // kEpiGlu / kEpiDglu: g and u in fp32, [row / 32][col / 4][g, u][row % 32][4], ld4 = column quads (of
   // whole runs of 32 columns)
   float* gu;
@@ -112,11 +123,14 @@ struct GemmParams {
   uint64_t wait_ns;
 };
 
+static_assert(sizeof(GemmParams) <= 4096, "kernel parameters");
+
 // ---------------------------------------------------------------------------
 // jobs
 // ---------------------------------------------------------------------------
 struct GemmJob {
   int sub, mt, nt;
+  int ks;      // part of K
   int kb, ke;  // iterations [kb, ke) of the tile's K blocks times passes
 };
 
@@ -124,35 +138,46 @@ template <bool PAIR>
 struct GemmSched {
   const GemmParams& p;
   int dyn;
-  int64_t j, step;
   static constexpr int kTileM = PAIR ? 256 : 128;
-  __device__ GemmSched(const GemmParams& q, int64_t worker, int64_t nworkers)
-      : p(q), dyn(q.dyn ? *q.dyn : 0), j(worker), step(nworkers) {}
+  __device__ explicit GemmSched(const GemmParams& q) : p(q), dyn(q.dyn ? *q.dyn : 0) {}
   __device__ int mtiles(const GemmSub& s) const { return s.m_dyn ? (dyn + kTileM - 1) / kTileM : s.mt; }
   __device__ int rows(const GemmSub& s) const { return s.m_dyn ? dyn : s.M; }
   __device__ int nk0(const GemmSub& s) const { return s.k_dyn ? (dyn + kGmBK - 1) / kGmBK : s.nk[0]; }
-  __device__ bool next(GemmJob& o) {
-    int64_t t = j;
-    j += step;
+  __device__ int jobs() const {
+    int n = 0;
+    for (int i = 0; i < p.nsub; ++i) n += mtiles(p.sub[i]) * p.sub[i].nt * p.sub[i].split;
+    return n;
+  }
+  __device__ GemmJob job(int t) const {
+    GemmJob o{};
     for (int i = 0; i < p.nsub; ++i) {
       const GemmSub& s = p.sub[i];
-      const int mt = mtiles(s);
-      const int64_t n = (int64_t)mt * s.nt;
-      if (t < n) {
-        // bands of 8 row tiles, walked column by column: the tiles in flight share operands in L2
-        const int band = 8 * s.nt;
-        const int g = (int)(t / band), first = g * 8, size = mt - first < 8 ? mt - first : 8;
-        const int r = (int)(t - (int64_t)g * band);
-        o.sub = i;
-        o.mt = first + r % size;
-        o.nt = r / size;
-        o.kb = 0;
-        o.ke = (nk0(s) + s.nk[1]) * p.npass;
-        return true;
+      const int mt = mtiles(s), tiles = mt * s.nt, n = tiles * s.split;
+      if (t >= n) {
+        t -= n;
+        continue;
       }
-      t -= n;
+      // the tiles of one part of K together: what is in flight then shares operands in L2
+      if (s.split > 1) {
+        o.ks = t / tiles;
+        t -= o.ks * tiles;
+      }
+      // bands of 8 row tiles, walked column by column, for the same reason
+      const int band = 8 * s.nt;
+      const int g = t / band, first = g * 8, size = mt - first < 8 ? mt - first : 8, r = t - g * band;
+      o.sub = i;
+      o.mt = first + r % size;
+      o.nt = r / size;
+      const int all = (nk0(s) + s.nk[1]) * p.npass;
+      o.ke = all;
+      if (s.split > 1) {
+        const int len = (all + s.split - 1) / s.split;
+        o.kb = o.ks * len < all ? o.ks * len : all;
+        o.ke = o.kb + len < all ? o.kb + len : all;
+      }
+      break;
     }
-    return false;
+    return o;
   }
 };
 
@@ -313,15 +338,16 @@ __device__ __forceinline__ void put_final(uint8_t* box, const GemmOut& o, const 
                                           int N, const float (&v)[32]) {
   const int lane = threadIdx.x & 31, k = lane & 7, c = col + 4 * k;
   const bool whole = o.vec && c + 4 <= N && o.kind != kOutF32 && (!f.residual || f.res_vec);
+  const int64_t first = rows.row0 + (lane >> 3);
+  const int live = rows.M - first > 32 ? 8 : rows.M <= first ? 0 : (int)((rows.M - first + 3) / 4);  // of this lane's rows
   // the residual's loads of all rows are in flight while the box fills: one by one between the stores
   // each cost its whole latency
   uint2 raw[8];
+  {
+    const uint16_t* rp = static_cast<const uint16_t*>(f.residual) + first * f.ld_res + c;
 #pragma unroll
-  for (int it = 0; it < 8; ++it) {
-    const int64_t row = rows.row0 + it * 4 + (lane >> 3);
-    raw[it] = make_uint2(0u, 0u);
-    if (whole && f.residual && row < rows.M)
-      raw[it] = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(f.residual) + row * f.ld_res + c));
+    for (int it = 0; it < 8; ++it, rp += 4 * f.ld_res)
+      raw[it] = whole && f.residual && it < live ? __ldg(reinterpret_cast<const uint2*>(rp)) : make_uint2(0u, 0u);
   }
   __syncwarp();
 #pragma unroll
@@ -329,59 +355,58 @@ __device__ __forceinline__ void put_final(uint8_t* box, const GemmOut& o, const 
     *reinterpret_cast<float4*>(box + lane * 128 + ((i ^ (lane & 7)) << 4)) =
         make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
   __syncwarp();
-  const float4 b = bias4(f.bias, f.dt, c, N);
+  if (c >= N) return;
+  if (whole) {
+    const float4 b = bias4(f.bias, f.dt, c, N);
+    uint16_t* op = static_cast<uint16_t*>(o.p) + first * o.ld + c;
 #pragma unroll
-  for (int it = 0; it < 8; ++it) {
+    for (int it = 0; it < 8; ++it, op += 4 * o.ld) {
+      const int r = it * 4 + (lane >> 3);
+      const float4 x = final4(o, f, b, *reinterpret_cast<const float4*>(box + r * 128 + ((k ^ (r & 7)) << 4)), wide4(raw[it], f.dt));
+      if (it < live)
+        *reinterpret_cast<uint2*>(op) = make_uint2(pack16(x.x, x.y, o.kind == kOutF16), pack16(x.z, x.w, o.kind == kOutF16));
+    }
+    return;
+  }
+#pragma unroll 1
+  for (int it = 0; it < live; ++it) {
     const int r = it * 4 + (lane >> 3);
     const int64_t row = rows.row0 + r;
-    if (row >= rows.M || c >= N) continue;
-    const float4 t = *reinterpret_cast<const float4*>(box + r * 128 + ((k ^ (r & 7)) << 4));
-    if (whole) {
-      const float4 x = final4(o, f, b, t, wide4(raw[it], f.dt));
-      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(o.p) + row * o.ld + c) =
-          make_uint2(pack16(x.x, x.y, o.kind == kOutF16), pack16(x.z, x.w, o.kind == kOutF16));
-    } else {
-      const float* src = reinterpret_cast<const float*>(box + r * 128 + ((k ^ (r & 7)) << 4));
+    const float* src = reinterpret_cast<const float*>(box + r * 128 + ((k ^ (r & 7)) << 4));
 #pragma unroll 1
-      for (int e = 0; e < 4 && c + e < N; ++e) {
-        float x = src[e];
-        if (f.bias) x += ldf(f.bias, c + e, f.dt);
-        x *= f.alpha;
-        if (f.residual) x += ldf(f.residual, row * f.ld_res + c + e, f.dt);
-        stf(o.p, row * o.ld + c + e, o.kind == kOutF32 ? M3B_F32 : o.kind == kOutF16 ? M3B_F16 : M3B_BF16, x);
-      }
+    for (int e = 0; e < 4 && c + e < N; ++e) {
+      float x = src[e];
+      if (f.bias) x += ldf(f.bias, c + e, f.dt);
+      x *= f.alpha;
+      if (f.residual) x += ldf(f.residual, row * f.ld_res + c + e, f.dt);
+      stf(o.p, row * o.ld + c + e, o.kind == kOutF32 ? M3B_F32 : o.kind == kOutF16 ? M3B_F16 : M3B_BF16, x);
     }
   }
 }
 
-// Waits of the producer and the MMA issuer: the plain test in a loop (the sleeping form of mbar_wait
-// wakes too late for a stage that lasts a third of a microsecond); the clock is read only rarely.
-template <bool CLUSTER>
+// Waits of all roles: the plain test in a loop (the sleeping form of mbar_wait may wake late for a
+// stage that lasts a third of a microsecond); the clock is read only rarely.
 __device__ __forceinline__ bool gm_wait(uint64_t* bar, uint32_t parity, uint64_t limit_ns) {
-  auto test = [&]() {
-    uint32_t done;
-    if constexpr (CLUSTER)
-      asm volatile(
-          "{\n\t.reg .pred p;\n\t"
-          "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-          "selp.u32 %0, 1, 0, p;\n\t}"
-          : "=r"(done)
-          : "r"(smem_u32(bar)), "r"(parity)
-          : "memory");
-    else
-      done = mbar_try_wait(bar, parity);
-    return done != 0;
-  };
-  if (test()) return true;
+  if (mbar_try_wait(bar, parity)) return true;
   uint64_t t0 = 0;
   while (true) {
 #pragma unroll 1
     for (int i = 0; i < 256; ++i)
-      if (test()) return true;
+      if (mbar_try_wait(bar, parity)) return true;
     const uint64_t t = globaltimer_ns();
     if (t0 == 0) t0 = t;
     else if (t - t0 > limit_ns) return false;
   }
+}
+// Arrive on the first CTA's barrier from either CTA.  What it signals is that reads have ended (their
+// values are in registers), so it orders no memory across the cluster: with .release.cluster it waited
+// for the warp's outstanding stores.
+template <bool PAIR>
+__device__ __forceinline__ void gm_arrive_first(uint64_t* bar) {
+  if constexpr (PAIR)
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(mapa_shared(smem_u32(bar), 0)) : "memory");
+  else
+    mbar_arrive(bar);
 }
 
 // One thread of the (converged) warp, the same at every call.
@@ -430,6 +455,7 @@ __device__ __forceinline__ uint64_t gm_desc(uint32_t lo, uint32_t hi) {
 template <int EPI, bool PAIR, bool PLANES>
 __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_constant__ GemmParams p) {
   constexpr int kTileM = PAIR ? 256 : 128;
+  constexpr bool kDraws = EPI == kEpiStore || EPI == kEpiAcc;  // forms with several products a launch
   extern __shared__ uint8_t smraw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smraw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + kGmBarOff);
@@ -437,8 +463,10 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
   uint64_t* empty = bars + kGmStages;     // [kGmStages]: the MMAs reading the stage completed
   uint64_t* accf = bars + 2 * kGmStages;  // [2]: accumulator finished
   uint64_t* acce = accf + 2;              // [2]: accumulator read
-  uint32_t* tslot = reinterpret_cast<uint32_t*>(acce + 2);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tslot + 1);
+  uint64_t* jfull = acce + 2;             // [kGmQueue]: a job number is in jq
+  uint64_t* jempty = jfull + kGmQueue;    // [kGmQueue]: every role of the cluster has read it (first CTA)
+  int4* jq = reinterpret_cast<int4*>(jempty + kGmQueue);  // [kGmQueue][2]: the jobs, ready to use
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(jq + 2 * kGmQueue);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -450,7 +478,10 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
       mbar_init(&accf[i], 1);
       mbar_init(&acce[i], PAIR ? 16 : 8);  // one arrival per epilogue warp (of both CTAs)
     }
-    *abort_flag = 0;
+    for (int i = 0; i < kGmQueue; ++i) {
+      mbar_init(&jfull[i], 1);
+      mbar_init(&jempty[i], PAIR ? 18 : 9);  // issuer, second producer, epilogue warps
+    }
     fence_mbar_init();
   }
   if (warp == 0) pair_tmem_alloc<PAIR>(tslot, 512);
@@ -460,15 +491,55 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
   tc_fence_after();
   const uint32_t tbase = *tslot;
   const uint32_t rank = PAIR ? cluster_rank() : 0u;
-  const int64_t worker = PAIR ? blockIdx.x / 2 : blockIdx.x, nworkers = PAIR ? gridDim.x / 2 : gridDim.x;
+  const int worker = PAIR ? blockIdx.x / 2 : blockIdx.x, nworkers = PAIR ? gridDim.x / 2 : gridDim.x;
   const int bn = p.bn;
   const int brows = PAIR ? bn / 2 : bn;  // B rows staged by this CTA
-  GemmSched<PAIR> sched(p, worker, nworkers);
-  auto give_up = [&]() {
-    *abort_flag = 1;
-    record_error(p.err, M3B_ERR_TIMEOUT);
+  const GemmSched<PAIR> sched(p);
+  auto give_up = [&]() { record_error(p.err, M3B_ERR_TIMEOUT); };
+  // The n-th job, for a whole warp; sub < 0 when there is none left (-1) or the wait ran out (-2).  Jobs
+  // that are dealt in turn, and every worker's first, each role works out for itself; drawn ones come
+  // through the queue.
+  const int total = sched.jobs();
+  auto job_of = [&](int t) {
+    GemmJob o{};
+    o.sub = -1;
+    if (t < total) o = sched.job(t);
+    return o;
   };
-
+  auto next_job = [&](uint32_t n) {
+    if (n == 0 || !kDraws || !p.ticket) return job_of(worker + (int)n * nworkers);
+    const uint32_t slot = (n - 1) % kGmQueue;
+    GemmJob o{};
+    o.sub = -2;
+    if (!__all_sync(0xffffffffu, gm_wait(&jfull[slot], ((n - 1) / kGmQueue) & 1, p.wait_ns))) return o;
+    const int4 x = jq[2 * slot], y = jq[2 * slot + 1];
+    // broadcasts, so that the compiler knows the fields to be the same in all lanes and keeps the loops'
+    // addresses in uniform registers
+    auto uni = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
+    o.sub = uni(x.x), o.mt = uni(x.y), o.nt = uni(x.z), o.ks = uni(x.w), o.kb = uni(y.x), o.ke = uni(y.y);
+    if (lane == 0) gm_arrive_first<PAIR>(&jempty[slot]);
+    return o;
+  };
+  // The first CTA's producer, one thread: job n into both CTAs' queues.
+  auto pass_on = [&](uint32_t n, const GemmJob& j) {
+    const uint32_t slot = (n - 1) % kGmQueue;
+    if (!gm_wait(&jempty[slot], (((n - 1) / kGmQueue) & 1) ^ 1, p.wait_ns)) return false;
+    jq[2 * slot] = make_int4(j.sub, j.mt, j.nt, j.ks);
+    jq[2 * slot + 1] = make_int4(j.kb, j.ke, 0, 0);
+    mbar_arrive(&jfull[slot]);
+    if constexpr (PAIR) {
+      // the second CTA's copy completes on its own barrier
+      const uint32_t fb = mapa_shared(smem_u32(&jfull[slot]), 1), q0 = mapa_shared(smem_u32(&jq[2 * slot]), 1);
+      asm volatile("mbarrier.arrive.expect_tx.release.cluster.shared::cluster.b64 _, [%0], 24;" ::"r"(fb) : "memory");
+      asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(q0),
+                   "r"(j.sub), "r"(j.mt), "r"(j.nt), "r"(j.ks), "r"(fb)
+                   : "memory");
+      asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.b32 [%0], {%1, %2}, [%3];" ::"r"(q0 + 16),
+                   "r"(j.kb), "r"(j.ke), "r"(fb)
+                   : "memory");
+    }
+    return true;
+  };
   // The producer's and the issuer's loops run warp-uniform, with one elected thread for the copies,
   // the MMAs and the commits: their addresses and descriptors then live in uniform registers.  As
   // single-thread loops they took 360 ns a stage whatever the stage held (MMAs: 305 ns).
@@ -478,10 +549,15 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
     const uint32_t ring = smem_u32(sm);
     // the copies of both CTAs complete on the first CTA's barriers
     const uint32_t full0 = PAIR ? mapa_shared(smem_u32(full), 0) : smem_u32(full);
-    uint32_t st = 0, ph = 1, it = 0;
-    GemmJob job;
+    uint32_t st = 0, ph = 1, it = 0, jn = 1;
     bool ok = true;
-    while (ok && sched.next(job)) {
+    const bool draws = kDraws && p.ticket && rank == 0;
+    const int lead = __ffs(__ballot_sync(0xffffffffu, leader)) - 1;
+    GemmJob job = next_job(0);
+    for (; ok && job.sub >= 0; ++jn) {
+      const int draw_at = job.ke - 12 > job.kb ? job.ke - 12 : job.kb;
+      int drawn = 0;
+      if (draws && job.ke == job.kb && leader) drawn = atomicAdd(p.ticket, 1);
       const GemmSub& s = p.sub[job.sub];
       const int nk0 = sched.nk0(s), nks = nk0 + s.nk[1];
       const int arow = job.mt * kTileM + (int)rank * 128;
@@ -498,7 +574,7 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
       }
       int pass = job.kb / (nks > 0 ? nks : 1), r = job.kb - pass * nks;
       for (int i = job.kb; i < job.ke; ++i, ++it) {
-        ok = __all_sync(0xffffffffu, gm_wait<PAIR>(&empty[st], ph, p.wait_ns));
+        ok = __all_sync(0xffffffffu, gm_wait(&empty[st], ph, p.wait_ns));
         if (!ok) break;
         const int seg = r >= nk0 ? 1 : 0, k = (seg ? r - nk0 : r) * kGmBK;
         // plane pairs, smallest first: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0)
@@ -507,6 +583,7 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
         const uint32_t dA = ring + st * kGmStage, dB = dA + kGmStageA, fb = full0 + st * 8;
         const CUtensorMap *ma = &s.a[seg], *mb = &s.b[EPI == kEpiGlu ? (PAIR ? (int)rank : 0) : seg];
         if (leader) {
+          if (draws && i == draw_at) drawn = atomicAdd(p.ticket, 1);  // its latency passes under the copies
           if (rank == 0) mbar_arrive_expect_tx(&full[st], bytes);
           if (s.a_mn) {
             gm_load<PAIR>(dA, ma, arow, k, pa, fb);
@@ -531,7 +608,17 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
           ph ^= 1;
         }
       }
+      if (!ok) break;
+      if (draws) {
+        job = job_of(nworkers + __shfl_sync(0xffffffffu, drawn, lead));
+        bool passed = true;
+        if (leader) passed = pass_on(jn, job);
+        ok = __all_sync(0xffffffffu, passed);
+      } else {
+        job = next_job(jn);
+      }
     }
+    if (job.sub == -2) ok = false;
     if (!ok) {
       give_up();
       // an aborted run leaves once the copies in flight have landed
@@ -544,12 +631,12 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
       const bool leader = elect_one();
       const uint32_t ring = smem_u32(sm) >> 4;
       uint32_t st = 0, ph = 0, sc = 0;
-      GemmJob job;
       bool ok = true;
-      for (; ok && sched.next(job); ++sc) {
+      GemmJob job = next_job(0);
+      for (; ok && job.sub >= 0; ++sc, job = next_job(sc)) {
         const GemmSub& s = p.sub[job.sub];
         const uint32_t acc = sc & 1;
-        ok = __all_sync(0xffffffffu, gm_wait<PAIR>(&acce[acc], ((sc >> 1) & 1) ^ 1, p.wait_ns));
+        ok = __all_sync(0xffffffffu, gm_wait(&acce[acc], ((sc >> 1) & 1) ^ 1, p.wait_ns));
         if (!ok) break;
         tc_fence_after();
         uint32_t idesc = idesc_bf16(kTileM, bn, s.a_mn != 0, s.b_mn != 0);
@@ -563,7 +650,7 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
         const uint32_t hi = (1024u >> 4) | (1u << 14) | (2u << 29);
         uint32_t on = 0;
         for (int i = job.kb; i < job.ke; ++i) {
-          ok = __all_sync(0xffffffffu, gm_wait<PAIR>(&full[st], ph, p.wait_ns));
+          ok = __all_sync(0xffffffffu, gm_wait(&full[st], ph, p.wait_ns));
           if (!ok) break;
           tc_fence_after();
           const uint32_t a0 = (ring + st * (kGmStage >> 4)) | la, b0 = (ring + st * (kGmStage >> 4) + (kGmStageA >> 4)) | lb;
@@ -584,21 +671,21 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
         }
         if (ok && leader) gm_commit<PAIR>(&accf[acc]);
       }
-      if (!ok) give_up();
+      if (!ok || job.sub == -2) give_up();
     }
   } else {
     const int q = warp & 3, half = (warp - 2) >> 2;
     const uint32_t tl = tbase + ((uint32_t)(q * 32) << 16);
     uint32_t sc = 0;
-    GemmJob job;
-    for (; !__any_sync(0xffffffffu, *abort_flag) && sched.next(job); ++sc) {
+    GemmJob job = next_job(0);
+    for (; job.sub >= 0; ++sc, job = next_job(sc)) {
       const GemmSub& s = p.sub[job.sub];
       const int acc = (int)(sc & 1);
       const int64_t grow = (int64_t)job.mt * kTileM + (int64_t)rank * 128 + q * 32 + lane;
       const int M = sched.rows(s);
       const bool rok = grow < M;  // grow is the row of this thread
       const bool none = job.ke == job.kb;  // no K at all: the sum is zero
-      if (!__all_sync(0xffffffffu, gm_wait<PAIR>(&accf[acc], (sc >> 1) & 1, p.wait_ns))) {
+      if (!__all_sync(0xffffffffu, gm_wait(&accf[acc], (sc >> 1) & 1, p.wait_ns))) {
         give_up();
         break;
       }
@@ -607,10 +694,7 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
       auto release = [&]() {
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) {
-          if constexpr (PAIR) mbar_arrive_cluster(mapa_shared(smem_u32(&acce[acc]), 0));
-          else mbar_arrive(&acce[acc]);
-        }
+        if (lane == 0) gm_arrive_first<PAIR>(&acce[acc]);
       };
       uint8_t* box = sm + kGmBoxOff + (uint32_t)(warp - 2) * kGmBox;
       GemmRows rows{(int64_t)job.mt * kTileM + (int64_t)rank * 128 + q * 32, M, nullptr};
@@ -642,17 +726,28 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
         if (s.out.kind == kOutF32) put32(box, s.out, rows, col, s.N, v);
         else put_operand<false>(box, s.out, rows, col, s.N, v);
       };
+      // a part of a split product, as it is
+      auto put_part = [&](int col, const float (&v)[32]) {
+        const int64_t nq = (int64_t)s.nt * bn / 4, size = (int64_t)s.mt * kTileM / 32 * nq * 32;
+        float4* ap = reinterpret_cast<float4*>(s.part) + job.ks * size + ((grow >> 5) * nq + (col >> 2)) * 32 + lane;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ap[i * 32] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+      };
       if constexpr (EPI == kEpiStore) {
         const float alpha = scale_of();
         columns(cfirst, clast, [&](int c, float (&v)[32]) {
           const int col = job.nt * bn + c;
-          if (col < s.N) put_scaled(col, v, alpha);
+          if (col >= s.N) return;
+          if (s.split > 1) put_part(col, v);
+          else put_scaled(col, v, alpha);
         });
       } else if constexpr (EPI == kEpiFinal) {
         const GemmFinal fin{s.alpha, s.bias, s.residual, s.ld_res, s.dt, s.res_vec};
         columns(cfirst, clast, [&](int c, float (&v)[32]) {
           const int col = job.nt * bn + c;
-          if (col < s.N) put_final(box, s.out, fin, rows, col, s.N, v);
+          if (col >= s.N) return;
+          if (s.split > 1) put_part(col, v);
+          else put_final(box, s.out, fin, rows, col, s.N, v);
         });
       } else if constexpr (EPI == kEpiAcc) {
         const float alpha = scale_of();
@@ -661,6 +756,10 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
         columns(cfirst, clast, [&](int c, float (&v)[32]) {
           const int col = job.nt * bn + c;
           if (col >= s.N) return;
+          if (s.split > 1) {
+            put_part(col, v);
+            return;
+          }
           if (s.acc_mode != 0) {
             float4* ap = reinterpret_cast<float4*>(s.acc) + ((grow >> 5) * nq + (col >> 2)) * 32 + lane;
             if (s.acc_mode != 1) {
@@ -793,6 +892,7 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
       }
       release();
     }
+    if (job.sub == -2) give_up();
   }
   tc_fence_before();
   __syncthreads();
@@ -800,6 +900,91 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
   if (warp == 0) {
     tc_fence_after();
     pair_tmem_dealloc<PAIR>(tbase, 512);
+  }
+}
+
+// The split products of a launch: add the parts in order and store as the kernel's epilogue would.
+// `warps` (a power of two) warps per 32 x 32 piece, lane = row, each with a run of the parts; bound by
+// L2 (the parts were just written) and, with few pieces, by the latency of one load after the other.
+template <int EPI>
+__global__ void __launch_bounds__(256) gemm_join_kernel(const __grid_constant__ GemmParams p, int tile_m, int warps) {
+  __shared__ __align__(1024) uint8_t boxes[8 * kGmBox];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, w = warp & (warps - 1);
+  uint8_t* box = boxes + warp * kGmBox;
+  const int dyn = p.dyn ? *p.dyn : 0;
+  int64_t u = (int64_t)blockIdx.x * (8 / warps) + warp / warps;
+  int i = 0;
+  for (; i < p.nsub; ++i) {
+    const GemmSub& s = p.sub[i];
+    if (s.split <= 1) continue;
+    const int64_t n = (int64_t)(((s.m_dyn ? dyn : s.M) + 31) / 32) * ((s.N + 31) / 32);
+    if (u < n) break;
+    u -= n;
+  }
+  const bool live = i < p.nsub;
+  const GemmSub& s = p.sub[live ? i : 0];
+  const int M = s.m_dyn ? dyn : s.M, cb = (s.N + 31) / 32;
+  const int row0 = live ? (int)(u / cb) * 32 : 0, col = live ? (int)(u % cb) * 32 : 0;
+  float v[32];
+#pragma unroll
+  for (int k = 0; k < 32; ++k) v[k] = 0.f;
+  if (live) {
+    const int64_t nq = (int64_t)s.nt * p.bn / 4, size = (int64_t)s.mt * tile_m / 32 * nq * 32;
+    const int each = (s.split + warps - 1) / warps, k0 = w * each, k1 = k0 + each < s.split ? k0 + each : s.split;
+    const float4* ap = reinterpret_cast<const float4*>(s.part) + k0 * size + ((row0 >> 5) * nq + (col >> 2)) * 32 + lane;
+    for (int ks = k0; ks < k1; ++ks, ap += size) {
+      float4 o[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) o[k] = ap[k * 32];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[4 * k] += o[k].x, v[4 * k + 1] += o[k].y, v[4 * k + 2] += o[k].z, v[4 * k + 3] += o[k].w;
+    }
+  }
+  if (warps > 1) {  // the runs' sums in order
+    float4* mine = reinterpret_cast<float4*>(box);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) mine[k * 32 + lane] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+    __syncthreads();
+    if (w != 0) return;
+    for (int k2 = 1; k2 < warps; ++k2) {
+      const float4* other = reinterpret_cast<const float4*>(box + k2 * kGmBox);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float4 o = other[k * 32 + lane];
+        v[4 * k] += o.x, v[4 * k + 1] += o.y, v[4 * k + 2] += o.z, v[4 * k + 3] += o.w;
+      }
+    }
+  }
+  if (live) {
+    const GemmRows rows{row0, M, s.row_index};
+    if constexpr (EPI == kEpiFinal) {
+      const GemmFinal fin{s.alpha, s.bias, s.residual, s.ld_res, s.dt, s.res_vec};
+      put_final(box, s.out, fin, rows, col, s.N, v);
+    } else {
+      if (s.acc_mode != 0) {
+        const int64_t nqa = (int64_t)s.nt * p.bn / 4;
+        float4* acc = reinterpret_cast<float4*>(s.acc) + ((row0 >> 5) * nqa + (col >> 2)) * 32 + lane;
+        if (s.acc_mode != 1) {
+          float4 o[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) o[k] = acc[k * 32];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[4 * k] += o[k].x, v[4 * k + 1] += o[k].y, v[4 * k + 2] += o[k].z, v[4 * k + 3] += o[k].w;
+        }
+        if (s.acc_mode != 3) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) acc[k * 32] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+          return;
+        }
+      }
+      float alpha = s.alpha;
+      if (s.alpha_num) alpha *= *s.alpha_num;
+      if (s.alpha_den) alpha = *s.alpha_den > 0 ? alpha / (float)*s.alpha_den : 0.f;
+#pragma unroll
+      for (int k = 0; k < 32; ++k) v[k] *= alpha;
+      if (s.out.kind == kOutF32) put32(box, s.out, rows, col, s.N, v);
+      else put_operand<false>(box, s.out, rows, col, s.N, v);
+    }
   }
 }
 
@@ -819,8 +1004,12 @@ inline bool tma_ok(const void* p, int64_t ld_elems) { return aligned16(p) && ld_
 // Tensor map of an operand; box_rows counts the other dimension's box when K is along the rows
 // (K-major), MN-major maps always use 64 x 64 boxes.
 int gemm_map(CUtensorMap* m, const GemmOperand& o, bool mn_major, int box_rows, bool f16);
-// Launch on `st`; fills mt / nt from M, N and bn.
-int launch_gemm(GemmParams& p, int epi, bool pair, cudaStream_t st);
+// Fills mt, nt and split from M, N, nk, npass and bn, and orders the products longest job first;
+// returns the bytes of fp32 parts the split ones need (to be carved and given to launch_gemm).
+size_t plan_gemm(GemmParams& p, int epi, bool pair);
+// Launch a planned set of products on `st`; `parts`: plan_gemm's bytes; a launch with jobs of several
+// lengths draws them from p.ticket (a zeroed int; null deals them in turn).
+int launch_gemm(GemmParams& p, int epi, bool pair, void* parts, cudaStream_t st);
 inline int gemm_tile_m(bool pair) { return pair ? 256 : 128; }
 // Rows of B per tensor-map box for `bn` accumulator columns.
 inline int gemm_box_b(bool pair, int bn, int epi) { return epi == kEpiGlu || pair ? bn / 2 : bn; }

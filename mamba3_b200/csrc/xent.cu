@@ -65,45 +65,46 @@ Saved saved_of(const m3b_linear_xent_args* a, void* p) {
   return s;
 }
 
-// One block: the kept rows' numbers and targets in order.  Each thread takes a run of rows, so one
-// scan over the threads' counts orders them.
+// One block: the kept rows' numbers and targets in order, four targets a thread at a time.  (One long
+// run per thread, its loads a line each: 52 us for 16384 targets; this 8 us.)
 __global__ void __launch_bounds__(1024) keep_kernel(const int64_t* __restrict__ target, int64_t ignore, int64_t T,
                                                     int64_t Tp, int V, Saved s, int* err) {
-  __shared__ int sums[32];
+  __shared__ int sums[2][32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int64_t run = (T + 1023) / 1024, r0 = tid * run < T ? tid * run : T, r1 = r0 + run < T ? r0 + run : T;
-  int n = 0;
-#pragma unroll 4
-  for (int64_t r = r0; r < r1; ++r) n += target[r] != ignore;
-  int x = n;
+  int total = 0, side = 0;
+  for (int64_t base = 0; base < T; base += 4096, side ^= 1) {
+    const int64_t r0 = base + tid * 4;
+    int64_t t[4];
+    int n = 0;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
-  }
-  if (lane == 31) sums[warp] = x;
-  __syncthreads();
-  if (warp == 0) {
-    int w = sums[lane];
+    for (int k = 0; k < 4; ++k) t[k] = r0 + k < T ? target[r0 + k] : ignore;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) n += t[k] != ignore;
+    int x = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) sums[side][warp] = x;
+    __syncthreads();  // the other side is written next, so one barrier a turn is enough
+    int w = sums[side][lane];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int y = __shfl_up_sync(0xffffffffu, w, o);
       if (lane >= o) w += y;
     }
-    sums[lane] = w;
-  }
-  __syncthreads();
-  int at = x - n + (warp ? sums[warp - 1] : 0);
-  const int total = sums[31];
-#pragma unroll 4
-  for (int64_t r = r0; r < r1; ++r) {
-    const int64_t t = target[r];
-    if (t == ignore) continue;
-    const bool ok = t >= 0 && t < V;
-    if (!ok) record_error(err, M3B_ERR_INVALID_ARG);
-    s.row[at] = (int)r;
-    s.target[at] = ok ? (int)t : -2;
-    ++at;
+    int at = total + x - n + (warp ? __shfl_sync(0xffffffffu, w, warp - 1) : 0);
+    total += __shfl_sync(0xffffffffu, w, 31);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (t[k] == ignore) continue;
+      const bool ok = t[k] >= 0 && t[k] < V;
+      if (!ok) record_error(err, M3B_ERR_INVALID_ARG);
+      s.row[at] = (int)(r0 + k);
+      s.target[at] = ok ? (int)t[k] : -2;
+      ++at;
+    }
   }
   for (int64_t i = total + tid; i < Tp; i += 1024) {
     s.row[i] = -1;
@@ -142,37 +143,42 @@ __global__ void __launch_bounds__(256) gather_kernel(const void* __restrict__ h,
   }
 }
 
-// Join the tiles' statistics: 32 rows per block, eight threads per row.
-__global__ void __launch_bounds__(256) join_kernel(const float2* __restrict__ part, int slots, int64_t Tp,
+// Join the tiles' statistics: 32 rows per block, sixteen threads per row, each with four pairs in
+// flight (one after the other, their latencies and exponentials made 30 us of 16384 rows x 394 pairs).
+__device__ __forceinline__ void join2(float& m, float& sum, float2 v) {
+  const float top = fmaxf(m, v.x);
+  sum = sum * ex2_fast(m - top) + v.y * ex2_fast(v.x - top);
+  m = top;
+}
+__global__ void __launch_bounds__(512) join_kernel(const float2* __restrict__ part, int slots, int64_t Tp,
                                                    const float* __restrict__ target_logit, Saved s,
                                                    float* __restrict__ row_loss) {
-  __shared__ float2 sm[8][32];
+  __shared__ float2 sm[16][32];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int n = *s.count;
   const int64_t row = (int64_t)blockIdx.x * 32 + lane;
   if ((int64_t)blockIdx.x * 32 >= n) return;
-  float m = -1e30f, sum = 0.f;
+  float m[4] = {-1e30f, -1e30f, -1e30f, -1e30f}, sum[4] = {0.f, 0.f, 0.f, 0.f};
   if (row < n) {
-#pragma unroll 4
-    for (int k = w; k < slots; k += 8) {
-      const float2 v = part[(int64_t)k * Tp + row];
-      const float top = fmaxf(m, v.x);
-      sum = sum * exp2f(m - top) + v.y * exp2f(v.x - top);
-      m = top;
+    int k = w;
+    for (; k + 48 < slots; k += 64) {
+      float2 v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = part[(int64_t)(k + 16 * i) * Tp + row];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) join2(m[i], sum[i], v[i]);
     }
+    for (; k < slots; k += 16) join2(m[0], sum[0], part[(int64_t)k * Tp + row]);
+#pragma unroll
+    for (int i = 1; i < 4; ++i) join2(m[0], sum[0], make_float2(m[i], sum[i]));
   }
-  sm[w][lane] = make_float2(m, sum);
+  sm[w][lane] = make_float2(m[0], sum[0]);
   __syncthreads();
   if (w != 0 || row >= n) return;
 #pragma unroll
-  for (int k = 1; k < 8; ++k) {
-    const float2 v = sm[k][lane];
-    const float top = fmaxf(m, v.x);
-    sum = sum * exp2f(m - top) + v.y * exp2f(v.x - top);
-    m = top;
-  }
+  for (int k = 1; k < 16; ++k) join2(m[0], sum[0], sm[k][lane]);
   const bool ok = s.target[row] >= 0;
-  const float l2 = ok ? m + log2f(sum) : __int_as_float(0x7fffffff);
+  const float l2 = ok ? m[0] + log2f(sum[0]) : __int_as_float(0x7fffffff);
   s.lse2[row] = l2;
   row_loss[row] = l2 * kLn2 - (ok ? target_logit[row] : 0.f);
 }
@@ -295,8 +301,9 @@ int forward(const m3b_linear_xent_args* a, void* workspace, size_t* need, bool r
   p.target_logit = target_logit;
   p.part = part;
   p.part_ld = d.Tp;
-  M3B_TRY(launch_gemm(p, kEpiLse, pair, st));
-  join_kernel<<<(unsigned)(d.Tp / 32), 256, 0, st>>>(part, nt * 2, d.Tp, target_logit, s, row_loss);
+  plan_gemm(p, kEpiLse, pair);
+  M3B_TRY(launch_gemm(p, kEpiLse, pair, nullptr, st));
+  join_kernel<<<(unsigned)(d.Tp / 32), 512, 0, st>>>(part, nt * 2, d.Tp, target_logit, s, row_loss);
   if (a->reduction == 0 && cudaMemsetAsync(a->loss, 0, (size_t)d.T * 4, st) != cudaSuccess)
     return check_launch("linear_xent loss");
   loss_kernel<<<1, 1024, 0, st>>>(row_loss, s, a->reduction, a->loss);
@@ -314,40 +321,90 @@ int backward(const m3b_linear_xent_args* a, void* workspace, size_t* need, bool 
   const Dims d(a);
   Carve ws(workspace);
   const int64_t cols = piece_cols(d), ldz = up(cols, 8);
-  const int bn = 256;
+  const int bn = 256, pieces = (int)((d.V + cols - 1) / cols);
   int rc = M3B_OK;
   uint16_t* dz = static_cast<uint16_t*>(ws.take((size_t)d.np * d.Tp * ldz * 2));
   float* acc = nullptr;
-  if (a->dhidden && cols < d.V) acc = static_cast<float*>(ws.take((size_t)d.Tp * up(d.D, bn) * 4));
+  if (a->dhidden && pieces > 1) acc = static_cast<float*>(ws.take((size_t)d.Tp * up(d.D, bn) * 4));
   float* roww = nullptr;
   if (a->reduction == 0) roww = static_cast<float*>(ws.take((size_t)d.Tp * 4));
+  int* ticket = static_cast<int*>(ws.take((size_t)pieces * 4));
   const GemmOperand w = weight_of(a, ws, run, st, &rc);
+  const Saved s = saved_of(a, a->saved);
+  const GemmOperand h{s.h, d.Tp, d.D, d.Dp, d.Tp * d.Dp, d.np};
+  const size_t es = d.f32 ? 4 : 2;
+  const int okind = d.f32 ? kOutF32 : d.f16 ? kOutF16 : kOutBf16;
+  GemmParams base{};
+  base.bn = bn;
+  base.npass = d.f32 ? 6 : 1;
+  base.f16 = d.f16;
+  base.dyn = s.count;
+  base.err = a->err;
+
+  // the two gradients' shares of the piece of n columns from c0 on, side by side
+  auto gradients = [&](GemmParams& p, int64_t c0, int64_t n, const GemmOperand* z, const GemmOperand* wp) {
+    auto sub = [&](void* out, int M, int K) -> GemmSub& {
+      GemmSub& g = p.sub[p.nsub++];
+      g.M = M;
+      g.N = d.D;
+      g.nk[0] = K;
+      g.b_mn = 1;
+      g.alpha = 1.f;
+      if (a->reduction != 0) g.alpha_num = a->dloss;
+      if (a->reduction == 1) g.alpha_den = s.count;
+      g.out.kind = okind;
+      g.out.ld = d.D;
+      g.out.p = out;
+      g.out.vec = aligned16(out) && d.D % 8 == 0;
+      return g;
+    };
+    if (a->dhidden) {
+      GemmSub& g = sub(a->dhidden, (int)d.T, (int)((n + kGmBK - 1) / kGmBK));
+      g.m_dyn = 1;
+      g.row_index = s.row;
+      g.acc = acc;
+      g.acc_mode = !acc ? 0 : c0 == 0 ? 1 : c0 + cols < d.V ? 2 : 3;
+      if (z) {
+        M3B_TRY(gemm_map(&g.a[0], *z, false, 128, d.f16));
+        M3B_TRY(gemm_map(&g.b[0], *wp, true, 0, d.f16));
+      }
+    }
+    if (a->dweight) {
+      GemmSub& g = sub(static_cast<uint8_t*>(a->dweight) + (size_t)c0 * d.D * es, (int)n, (int)(d.Tp / kGmBK));
+      g.k_dyn = 1;
+      g.a_mn = 1;
+      if (z) {
+        M3B_TRY(gemm_map(&g.a[0], *z, true, 0, d.f16));
+        M3B_TRY(gemm_map(&g.b[0], h, true, 0, d.f16));
+      }
+    }
+    return (int)M3B_OK;
+  };
+  size_t parts_bytes = 0;
+  for (int64_t c0 = 0; c0 < d.V; c0 += cols) {  // the last piece is shorter: its plan may be another one
+    GemmParams p = base;
+    gradients(p, c0, d.V - c0 < cols ? d.V - c0 : cols, nullptr, nullptr);
+    const size_t b = plan_gemm(p, kEpiAcc, true);
+    if (b > parts_bytes) parts_bytes = b;
+  }
+  void* parts = ws.take(parts_bytes);
   *need = ws.at;
   if (!run || rc != M3B_OK) return rc;
-  const Saved s = saved_of(a, a->saved);
-  const size_t es = d.f32 ? 4 : 2;
   if (a->dhidden && cudaMemsetAsync(a->dhidden, 0, (size_t)d.T * d.D * es, st) != cudaSuccess)
     return check_launch("linear_xent_bwd");
+  if (cudaMemsetAsync(ticket, 0, (size_t)pieces * 4, st) != cudaSuccess) return check_launch("linear_xent_bwd");
   if (roww) {
     roww_kernel<<<64, 256, 0, st>>>(a->dloss, s, roww);
     M3B_TRY(check_launch("linear_xent roww"));
   }
-  const GemmOperand h{s.h, d.Tp, d.D, d.Dp, d.Tp * d.Dp, d.np};
-  const int okind = d.f32 ? kOutF32 : d.f16 ? kOutF16 : kOutBf16;
   for (int64_t c0 = 0; c0 < d.V; c0 += cols) {
     const int64_t n = d.V - c0 < cols ? d.V - c0 : cols;
     const GemmOperand wp = piece_of(w, c0, n);
     const GemmOperand z{dz, d.Tp, n, ldz, d.Tp * ldz, d.np};
-    GemmParams base{};
-    base.bn = bn;
-    base.nsub = 1;
-    base.npass = d.f32 ? 6 : 1;
-    base.f16 = d.f16;
-    base.dyn = s.count;
-    base.err = a->err;
     {  // softmax - onehot of the piece
       GemmParams p = base;
       GemmSub& g = p.sub[0];
+      p.nsub = 1;
       M3B_MAP(&g.a[0], h, false, 128, d.f16);
       M3B_MAP(&g.b[0], wp, false, gemm_box_b(true, bn, kEpiDlogit), d.f16);
       g.M = (int)d.T;
@@ -363,48 +420,14 @@ int backward(const m3b_linear_xent_args* a, void* workspace, size_t* need, bool 
       p.lse2 = s.lse2;
       p.roww = roww;
       p.col0 = (int)c0;
-      M3B_TRY(launch_gemm(p, kEpiDlogit, true, st));
+      plan_gemm(p, kEpiDlogit, true);
+      M3B_TRY(launch_gemm(p, kEpiDlogit, true, nullptr, st));
     }
-    auto scaled = [&](GemmSub& g) {
-      g.alpha = 1.f;
-      if (a->reduction != 0) g.alpha_num = a->dloss;
-      if (a->reduction == 1) g.alpha_den = s.count;
-      g.out.kind = okind;
-      g.out.ld = d.D;
-    };
-    if (a->dhidden) {
-      GemmParams p = base;
-      GemmSub& g = p.sub[0];
-      M3B_MAP(&g.a[0], z, false, 128, d.f16);
-      M3B_MAP(&g.b[0], wp, true, 0, d.f16);
-      g.b_mn = 1;
-      g.M = (int)d.T;
-      g.m_dyn = 1;
-      g.N = d.D;
-      g.nk[0] = (int)((n + kGmBK - 1) / kGmBK);
-      scaled(g);
-      g.out.p = a->dhidden;
-      g.out.vec = aligned16(a->dhidden) && d.D % 8 == 0;
-      g.row_index = s.row;
-      g.acc = acc;
-      g.acc_mode = !acc ? 0 : c0 == 0 ? 1 : c0 + cols < d.V ? 2 : 3;
-      M3B_TRY(launch_gemm(p, kEpiAcc, true, st));
-    }
-    if (a->dweight) {
-      GemmParams p = base;
-      GemmSub& g = p.sub[0];
-      M3B_MAP(&g.a[0], z, true, 0, d.f16);
-      M3B_MAP(&g.b[0], h, true, 0, d.f16);
-      g.a_mn = g.b_mn = 1;
-      g.M = (int)n;
-      g.N = d.D;
-      g.nk[0] = 1;
-      g.k_dyn = 1;
-      scaled(g);
-      g.out.p = static_cast<uint8_t*>(a->dweight) + (size_t)c0 * d.D * es;
-      g.out.vec = aligned16(g.out.p) && d.D % 8 == 0;
-      M3B_TRY(launch_gemm(p, kEpiStore, true, st));
-    }
+    GemmParams p = base;
+    M3B_TRY(gradients(p, c0, n, &z, &wp));
+    plan_gemm(p, kEpiAcc, true);
+    p.ticket = ticket + c0 / cols;
+    if (p.nsub) M3B_TRY(launch_gemm(p, kEpiAcc, true, parts, st));
   }
   return M3B_OK;
 }
