@@ -38,14 +38,13 @@ constexpr int kGmThreads = 320;
 constexpr int kGmSubs = 4;      // products of a launch at most
 constexpr int kGmQueue = 4;     // drawn jobs that the producer may be ahead of the epilogue
 constexpr int kGmBK = 64;
-constexpr int kGmStages = 6;
 constexpr uint32_t kGmStageA = 128 * kGmBK * 2;     // 16 KB
 constexpr uint32_t kGmStage = 2 * kGmStageA;        // + B: at most 128 rows of 64
-constexpr uint32_t kGmRing = kGmStages * kGmStage;  // 192 KB
 constexpr uint32_t kGmBox = 32 * 128;               // staging of an epilogue warp: 32 rows x 32 fp32
-constexpr uint32_t kGmBoxOff = kGmRing;
-constexpr uint32_t kGmBarOff = kGmBoxOff + 8 * kGmBox;
-constexpr uint32_t kGmSmem = kGmBarOff + 384 + 1024;  // barriers, job queue, TMEM slot; alignment
+constexpr int kGuSlots = 4;                         // kEpiDglu: runs of 8 columns of g and u per epilogue warp
+constexpr uint32_t kGuRun = 8 * 2 * 32 * 4;         // 2 KB
+constexpr uint32_t kGmBarOff = 6 * kGmStage + 8 * kGmBox;
+constexpr uint32_t kGmSmem = kGmBarOff + 768 + 1024;  // barriers, job queue, TMEM slot; alignment
 static_assert(kGmSmem <= 227 * 1024, "shared memory plan");
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -455,6 +454,10 @@ __device__ __forceinline__ uint64_t gm_desc(uint32_t lo, uint32_t hi) {
 template <int EPI, bool PAIR, bool PLANES>
 __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_constant__ GemmParams p) {
   constexpr int kTileM = PAIR ? 256 : 128;
+  // six stages; kEpiDglu gives two of them to the runs of g and u
+  constexpr int kGmStages = EPI == kEpiDglu ? 4 : 6;
+  constexpr uint32_t kGmBoxOff = kGmStages * kGmStage, kGuOff = kGmBoxOff + 8 * kGmBox;
+  static_assert(kGuOff + (EPI == kEpiDglu ? 8 * kGuSlots * kGuRun : 0) <= kGmBarOff, "shared memory plan");
   constexpr bool kDraws = EPI == kEpiStore || EPI == kEpiAcc;  // forms with several products a launch
   extern __shared__ uint8_t smraw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smraw) + 1023) & ~uintptr_t(1023));
@@ -465,7 +468,8 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
   uint64_t* acce = accf + 2;              // [2]: accumulator read
   uint64_t* jfull = acce + 2;             // [kGmQueue]: a job number is in jq
   uint64_t* jempty = jfull + kGmQueue;    // [kGmQueue]: every role of the cluster has read it (first CTA)
-  int4* jq = reinterpret_cast<int4*>(jempty + kGmQueue);  // [kGmQueue][2]: the jobs, ready to use
+  uint64_t* gufull = jempty + kGmQueue;   // [8][kGuSlots]: the run landed (kEpiDglu)
+  int4* jq = reinterpret_cast<int4*>(gufull + 8 * kGuSlots);  // [kGmQueue][2]: the jobs, ready to use
   uint32_t* tslot = reinterpret_cast<uint32_t*>(jq + 2 * kGmQueue);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -478,6 +482,7 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
       mbar_init(&accf[i], 1);
       mbar_init(&acce[i], PAIR ? 16 : 8);  // one arrival per epilogue warp (of both CTAs)
     }
+    for (int i = 0; i < 8 * kGuSlots; ++i) mbar_init(&gufull[i], 1);
     for (int i = 0; i < kGmQueue; ++i) {
       mbar_init(&jfull[i], 1);
       mbar_init(&jempty[i], PAIR ? 18 : 9);  // issuer, second producer, epilogue warps
@@ -513,9 +518,9 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
     o.sub = -2;
     if (!__all_sync(0xffffffffu, gm_wait(&jfull[slot], ((n - 1) / kGmQueue) & 1, p.wait_ns))) return o;
     const int4 x = jq[2 * slot], y = jq[2 * slot + 1];
-    // broadcasts, so that the compiler knows the fields to be the same in all lanes and keeps the loops'
+    // reductions, so that the compiler knows the fields to be the same in all lanes and keeps the loops'
     // addresses in uniform registers
-    auto uni = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
+    auto uni = [](int v) { return (int)__reduce_or_sync(0xffffffffu, (unsigned)v); };
     o.sub = uni(x.x), o.mt = uni(x.y), o.nt = uni(x.z), o.ks = uni(x.w), o.kb = uni(y.x), o.ke = uni(y.y);
     if (lane == 0) gm_arrive_first<PAIR>(&jempty[slot]);
     return o;
@@ -564,14 +569,6 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
       // B rows of this CTA; the gated product stages bn / 2 gate and bn / 2 up rows (paired: the
       // first CTA holds the gate's, the second the up's)
       const int brow = EPI == kEpiGlu ? job.nt * (bn / 2) : job.nt * bn + (int)rank * brows;
-      if constexpr (EPI == kEpiDglu) {
-        // the tile's g and u on their way into L2 while its products run
-        const int64_t q0 = (int64_t)job.nt * (bn / 4), quads = p.gu_ld4 - q0 < bn / 4 ? p.gu_ld4 - q0 : bn / 4;
-        if (lane < 4 && arow + 32 * lane < s.M)
-          prefetch_l2(reinterpret_cast<const float4*>(p.gu) + ((int64_t)(arow / 32 + lane) * p.gu_ld4 + q0) * 64,
-                      (uint32_t)quads * 1024u);
-        __syncwarp();
-      }
       int pass = job.kb / (nks > 0 ? nks : 1), r = job.kb - pass * nks;
       for (int i = job.kb; i < job.ke; ++i, ++it) {
         ok = __all_sync(0xffffffffu, gm_wait(&empty[st], ph, p.wait_ns));
@@ -677,6 +674,41 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
     const int q = warp & 3, half = (warp - 2) >> 2;
     const uint32_t tl = tbase + ((uint32_t)(q * 32) << 16);
     uint32_t sc = 0;
+    // kEpiDglu: this warp's runs of g and u, in the order it will use them (the jobs are dealt, so the
+    // next tile's are known), kGuSlots of them on their way or in shared memory
+    uint64_t* gub = gufull + (warp - 2) * kGuSlots;
+    const uint8_t* gus = sm + kGuOff + (uint32_t)(warp - 2) * kGuSlots * kGuRun;
+    uint32_t gu_used = 0, gu_sent = 0, gu_tile = 0;
+    int gu_run = 0, gu_runs = 0;
+    const float4* gu_at = nullptr;
+    auto gu_enter = [&](const GemmJob& j) {  // the runs of tile j
+      const int64_t row = (int64_t)j.mt * kTileM + (int64_t)rank * 128 + q * 32;
+      const int col = j.nt * bn + half * (bn / 2), n = p.sub[0].N - col < bn / 2 ? p.sub[0].N - col : bn / 2;
+      gu_run = 0;
+      gu_runs = n > 0 ? (n + 31) / 32 * 4 : 0;
+      gu_at = reinterpret_cast<const float4*>(p.gu) + ((row >> 5) * p.gu_ld4 + (col >> 2)) * 64;
+    };
+    auto gu_send = [&]() {
+      while (gu_run >= gu_runs) {
+        const GemmJob j = next_job(gu_tile++);
+        if (j.sub < 0) {
+          --gu_tile;
+          return;
+        }
+        gu_enter(j);
+      }
+      const uint32_t slot = gu_sent++ % kGuSlots;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&gub[slot], kGuRun);
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                         smem_u32(gus + slot * kGuRun)),
+                     "l"(gu_at + (int64_t)gu_run * 128), "r"(kGuRun), "r"(smem_u32(&gub[slot]))
+                     : "memory");
+      }
+      ++gu_run;
+    };
+    if constexpr (EPI == kEpiDglu)
+      for (int i = 0; i < kGuSlots; ++i) gu_send();
     GemmJob job = next_job(0);
     for (; job.sub >= 0; ++sc, job = next_job(sc)) {
       const GemmSub& s = p.sub[job.sub];
@@ -685,6 +717,7 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
       const int M = sched.rows(s);
       const bool rok = grow < M;  // grow is the row of this thread
       const bool none = job.ke == job.kb;  // no K at all: the sum is zero
+      const int cfirst = half * (bn / 2), clast = cfirst + bn / 2;
       if (!__all_sync(0xffffffffu, gm_wait(&accf[acc], (sc >> 1) & 1, p.wait_ns))) {
         give_up();
         break;
@@ -713,7 +746,6 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
           f(c, v);
         }
       };
-      const int cfirst = half * (bn / 2), clast = cfirst + bn / 2;
       auto scale_of = [&]() {
         float alpha = s.alpha;
         if (s.alpha_num) alpha *= *s.alpha_num;
@@ -815,27 +847,42 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
         columns(cfirst, clast, [&](int c, float (&d)[32]) {
           const int col = job.nt * bn + c;
           if (col >= s.N) return;
-          const float4* gp = reinterpret_cast<const float4*>(p.gu) + ((grow >> 5) * p.gu_ld4 + (col >> 2)) * 64 + lane;
-          float u[32];
+          // 16-bit results are packed as they come: two packed arrays instead of two of 32
+          float dg[PLANES ? 32 : 8], du[PLANES ? 32 : 8];
+          uint32_t wg[16], wu[16];
 #pragma unroll
-          for (int h = 0; h < 8; h += 4) {
-            float4 a[4], b[4];
+          for (int h = 0; h < 4; ++h, ++gu_used) {
+            const uint32_t slot = gu_used % kGuSlots;
+            if (!__all_sync(0xffffffffu, gm_wait(&gub[slot], (gu_used / kGuSlots) & 1, p.wait_ns))) give_up();
+            const float4* run = reinterpret_cast<const float4*>(gus + slot * kGuRun) + lane;
+            const float4 g2[2] = {run[0], run[64]}, u2[2] = {run[32], run[96]};
+            __syncwarp();
+            gu_send();
 #pragma unroll
-            for (int i = 0; i < 4; ++i) a[i] = __ldg(gp + (h + i) * 64), b[i] = __ldg(gp + (h + i) * 64 + 32);
+            for (int i = 0; i < 8; ++i) {
+              const float4 gq = g2[i >> 2], uq = u2[i >> 2];
+              const float g = (i & 3) == 0 ? gq.x : (i & 3) == 1 ? gq.y : (i & 3) == 2 ? gq.z : gq.w;
+              const float u = (i & 3) == 0 ? uq.x : (i & 3) == 1 ? uq.y : (i & 3) == 2 ? uq.z : uq.w;
+              const float sg = sigmoid_fast(g), ds = d[8 * h + i] * s.alpha * sg;
+              const int k = PLANES ? 8 * h + i : i;
+              dg[k] = ds * u * fmaf(g, 1.f - sg, 1.f);
+              du[k] = ds * g;
+            }
+            if constexpr (!PLANES) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float g4[4] = {a[i].x, a[i].y, a[i].z, a[i].w}, u4[4] = {b[i].x, b[i].y, b[i].z, b[i].w};
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int j = 4 * (h + i) + e;
-                const float sg = sigmoid_fast(g4[e]), ds = d[j] * s.alpha * sg;
-                d[j] = ds * u4[e] * fmaf(g4[e], 1.f - sg, 1.f);
-                u[j] = ds * g4[e];
+              for (int i = 0; i < 4; ++i) {
+                wg[4 * h + i] = pack16(dg[2 * i], dg[2 * i + 1], s.out.kind == kOutF16);
+                wu[4 * h + i] = pack16(du[2 * i], du[2 * i + 1], s.out.kind == kOutF16);
               }
             }
           }
-          put_operand<PLANES>(box, s.out, rows, col, s.N, d);
-          put_operand<PLANES>(box, s.out2, rows, col, s.N, u);
+          if constexpr (PLANES) {
+            put_operand<true>(box, s.out, rows, col, s.N, dg);
+            put_operand<true>(box, s.out2, rows, col, s.N, du);
+          } else {
+            put16(box, s.out, static_cast<uint16_t*>(s.out.p), rows, col, s.N, wg);
+            put16(box, s.out2, static_cast<uint16_t*>(s.out2.p), rows, col, s.N, wu);
+          }
         });
       } else if constexpr (EPI == kEpiLse) {
         const int tgt = rok ? p.target[grow] : -1;
@@ -893,6 +940,8 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
       release();
     }
     if (job.sub == -2) give_up();
+    if constexpr (EPI == kEpiDglu)  // an aborted run leaves once its copies have landed
+      for (; gu_used < gu_sent; ++gu_used) mbar_wait(&gub[gu_used % kGuSlots], (gu_used / kGuSlots) & 1, 10000000ull);
   }
   tc_fence_before();
   __syncthreads();
