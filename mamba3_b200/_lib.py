@@ -8,7 +8,6 @@ the library is missing or a tensor is not on a CUDA device the call raises.
 from __future__ import annotations
 
 import array
-import contextlib
 import ctypes as C
 import threading
 from pathlib import Path
@@ -808,21 +807,41 @@ def _addr(t):
     return None if t is None else t.data_ptr()
 
 
-def _on(dev):
-    """The tensors' device as the current one (nothing to do when it already is)."""
-    if dev.index is None or dev.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(dev)
+def _same_gpu(name, ts):
+    """The CUDA device every tensor of `ts` (None skipped) is on."""
+    dev = -1
+    for t in ts:
+        if t is not None:
+            if not t.is_cuda:
+                raise M3bError("mamba3_b200 kernels need CUDA tensors (there is no CPU path)")
+            if dev < 0:
+                dev = t.get_device()
+            elif t.get_device() != dev:
+                raise M3bError(f"{name}: tensors on different devices: cuda:{dev} vs {t.device}")
+    return dev
 
 
-def _workspace(nbytes, dev):
-    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+def _call(fn, what, index, *args):
+    """fn(*args, workspace bytes.., stream) on GPU `index` and its current stream."""
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    _check(rc, what)
+    if _SYNC_CHECK:
+        check_device_errors(torch.device("cuda", index))
+
+
+def _bytes(n, index):
+    return torch.empty(n, dtype=torch.uint8, device=torch.device("cuda", index))
 
 
 def _rows2d(t, d):
     """t as (rows, d) with unit stride along d and rows at least d elements apart (a copy if it must be)."""
-    t = t.reshape(-1, d)
-    if t.shape[0] and (t.stride(1) != 1 and d > 1 or (t.stride(0) < d and t.shape[0] > 1)):
+    if t.dim() != 2:
+        t = t.reshape(-1, d)
+    if not t.is_contiguous() and (t.stride(1) != 1 and d > 1 or (t.stride(0) < d and t.shape[0] > 1)):
         t = t.contiguous()
     return t
 
@@ -831,49 +850,59 @@ def _rows_apart(t, d):
     return t.stride(0) if t.shape[0] > 1 else d
 
 
+def _err_addr(index):
+    w = _err_words.get(index)
+    if w is None:
+        w = device_err_word(torch.device("cuda", index))
+    return None if w is None else w.data_ptr()
+
+
 def _ffn_args(x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual, scale):
     rows, d = x.shape
     a = GatedFfnArgs(rows, _rows_apart(x, d), 0 if residual is None else _rows_apart(residual, d), 0, d,
-                     w_gate.shape[0], dtype_code(x.dtype), float(scale), _addr(x), _addr(w_gate), _addr(w_up),
-                     _addr(w_down), _addr(b_gate), _addr(b_up), _addr(b_down), _addr(residual))
-    a.err = _addr(device_err_word(x.device))
+                     w_gate.shape[0], _DT[x.dtype], scale, x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(),
+                     w_down.data_ptr(), _addr(b_gate), _addr(b_up), _addr(b_down), _addr(residual))
+    a.err = _err_addr(x.get_device())
     return a
 
 
 def gated_ffn_fwd(x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual, scale, save):
     """Launch the gated feed-forward; x (rows, d_model), weights and biases contiguous, one dtype.
     Returns (out, act, gu): act and gu are what the backward reads (gu None unless `save`)."""
-    dev = _cuda(x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual)
+    index = x.get_device()
     a = _ffn_args(x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual, scale)
+    p = C.byref(a)
     L = lib()
-    out = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    act = torch.empty(L.m3b_gated_ffn_act_bytes(C.byref(a)), dtype=torch.uint8, device=dev)
-    gu = torch.empty(L.m3b_gated_ffn_gu_bytes(C.byref(a)), dtype=torch.uint8, device=dev) if save else None
-    a.saved_act, a.saved_gu, a.out = _addr(act), _addr(gu), _addr(out)
-    need = L.m3b_gated_ffn_fwd_workspace(C.byref(a))
-    ws = _workspace(need, dev)
-    with _on(dev):
-        _check(L.m3b_gated_ffn_fwd(C.byref(a), _addr(ws), need, _stream(dev)), "m3b_gated_ffn_fwd")
-    _after_launch(dev)
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    n = L.m3b_gated_ffn_act_bytes(p)
+    gu = _bytes(L.m3b_gated_ffn_gu_bytes(p), index) if save else None
+    a.saved_gu = _addr(gu)
+    need = L.m3b_gated_ffn_fwd_workspace(p)
+    # act and the workspace in one allocation where act is not kept
+    room = -(-n // 256) * 256
+    act = _bytes(n if save else room + need, index)
+    ws = (_bytes(need, index).data_ptr() if need else None) if save else act.data_ptr() + room
+    a.saved_act, a.out = act.data_ptr(), out.data_ptr()
+    _call(L.m3b_gated_ffn_fwd, "m3b_gated_ffn_fwd", index, p, ws, need)
     return out, act, gu
 
 
 def gated_ffn_bwd(x, w_gate, w_up, w_down, b_gate, b_up, b_down, scale, act, gu, dout, want):
     """Gradients of gated_ffn_fwd for (x, w_gate, w_up, w_down, b_gate, b_up, b_down): None where
     `want` (seven truth values) says so.  dout (rows, d_model), rows at least d_model apart."""
-    dev = _cuda(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act, gu, dout)
+    index = _same_gpu("gated_ffn_bwd", (x, act, dout))
     a = _ffn_args(x, w_gate, w_up, w_down, b_gate, b_up, b_down, None, scale)
     ins = (x, w_gate, w_up, w_down, b_gate, b_up, b_down)
-    g = [torch.empty(t.shape, dtype=x.dtype, device=dev) if w and t is not None else None for t, w in zip(ins, want)]
-    a.dout_stride, a.dout = _rows_apart(dout, x.shape[1]), _addr(dout)
-    a.saved_act, a.saved_gu = _addr(act), _addr(gu)
+    g = [torch.empty(t.shape, dtype=x.dtype, device=x.device) if w and t is not None else None
+         for t, w in zip(ins, want)]
+    a.dout_stride, a.dout = _rows_apart(dout, x.shape[1]), dout.data_ptr()
+    a.saved_act, a.saved_gu = act.data_ptr(), gu.data_ptr()
     a.dx, a.dw_gate, a.dw_up, a.dw_down, a.db_gate, a.db_up, a.db_down = [_addr(t) for t in g]
+    p = C.byref(a)
     L = lib()
-    need = L.m3b_gated_ffn_bwd_workspace(C.byref(a))
-    ws = _workspace(need, dev)
-    with _on(dev):
-        _check(L.m3b_gated_ffn_bwd(C.byref(a), _addr(ws), need, _stream(dev)), "m3b_gated_ffn_bwd")
-    _after_launch(dev)
+    need = L.m3b_gated_ffn_bwd_workspace(p)
+    ws = _bytes(need, index)
+    _call(L.m3b_gated_ffn_bwd, "m3b_gated_ffn_bwd", index, p, ws.data_ptr(), need)
     return g
 
 
@@ -881,45 +910,43 @@ REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
 
 def _xent_args(rows, d, weight, ignore_index, reduction):
-    a = LinearXentArgs(rows, d, ignore_index, d, weight.shape[0], dtype_code(weight.dtype), REDUCTIONS[reduction])
-    a.weight = _addr(weight)
-    a.err = _addr(device_err_word(weight.device))
+    a = LinearXentArgs(rows, d, ignore_index, d, weight.shape[0], _DT[weight.dtype], REDUCTIONS[reduction])
+    a.weight = weight.data_ptr()
+    a.err = _err_addr(weight.get_device())
     return a
 
 
 def linear_xent_fwd(hidden, weight, target, ignore_index, reduction):
     """Launch the head's cross entropy; hidden (rows, d_model), weight (vocab, d_model) contiguous of
     the same dtype, target (rows) int64 contiguous.  Returns (loss fp32, saved)."""
-    dev = _cuda(hidden, weight, target)
+    index = hidden.get_device()
     rows, d = hidden.shape
     a = _xent_args(rows, d, weight, ignore_index, reduction)
-    a.hidden_stride, a.hidden, a.target = _rows_apart(hidden, d), _addr(hidden), _addr(target)
+    a.hidden_stride, a.hidden, a.target = _rows_apart(hidden, d), hidden.data_ptr(), target.data_ptr()
+    p = C.byref(a)
     L = lib()
-    loss = torch.empty((rows,) if reduction == "none" else (), dtype=torch.float32, device=dev)
-    saved = torch.empty(max(16, L.m3b_linear_xent_saved(C.byref(a))), dtype=torch.uint8, device=dev)
-    a.saved, a.loss = _addr(saved), _addr(loss)
-    need = L.m3b_linear_xent_fwd_workspace(C.byref(a))
-    ws = _workspace(need, dev)
-    with _on(dev):
-        _check(L.m3b_linear_xent_fwd(C.byref(a), _addr(ws), need, _stream(dev)), "m3b_linear_xent_fwd")
-    _after_launch(dev)
+    loss = torch.empty((rows,) if reduction == "none" else (), dtype=torch.float32, device=hidden.device)
+    saved = _bytes(max(16, L.m3b_linear_xent_saved(p)), index)
+    a.saved, a.loss = saved.data_ptr(), loss.data_ptr()
+    need = L.m3b_linear_xent_fwd_workspace(p)
+    ws = _bytes(need, index)
+    _call(L.m3b_linear_xent_fwd, "m3b_linear_xent_fwd", index, p, ws.data_ptr(), need)
     return loss, saved
 
 
 def linear_xent_bwd(rows, weight, saved, dloss, ignore_index, reduction, want_hidden, want_weight):
     """Gradients of linear_xent_fwd: ((rows, d_model) or None, (vocab, d_model) or None)."""
-    dev = _cuda(weight, saved, dloss)
+    index = _same_gpu("linear_xent_bwd", (weight, saved, dloss))
     d = weight.shape[1]
     a = _xent_args(rows, d, weight, ignore_index, reduction)
-    dh = torch.empty(rows, d, dtype=weight.dtype, device=dev) if want_hidden else None
+    dh = torch.empty(rows, d, dtype=weight.dtype, device=weight.device) if want_hidden else None
     dw = torch.empty_like(weight) if want_weight else None
-    a.saved, a.dloss, a.dhidden, a.dweight = _addr(saved), _addr(dloss), _addr(dh), _addr(dw)
+    a.saved, a.dloss, a.dhidden, a.dweight = saved.data_ptr(), dloss.data_ptr(), _addr(dh), _addr(dw)
+    p = C.byref(a)
     L = lib()
-    need = L.m3b_linear_xent_bwd_workspace(C.byref(a))
-    ws = _workspace(need, dev)
-    with _on(dev):
-        _check(L.m3b_linear_xent_bwd(C.byref(a), _addr(ws), need, _stream(dev)), "m3b_linear_xent_bwd")
-    _after_launch(dev)
+    need = L.m3b_linear_xent_bwd_workspace(p)
+    ws = _bytes(need, index)
+    _call(L.m3b_linear_xent_bwd, "m3b_linear_xent_bwd", index, p, ws.data_ptr(), need)
     return dh, dw
 
 
@@ -939,7 +966,6 @@ def grad_clip(ptrs, numel, dtypes, out_ptrs, out_dtypes, max_norm, inf_norm, dev
     a.norm_type, a.max_norm, a.norm = (0 if inf_norm else 2), max_norm, norm.data_ptr()
     L = lib()
     need = L.m3b_grad_clip_workspace(C.byref(a))
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    with _on(dev):
-        _check(L.m3b_grad_clip(C.byref(a), _addr(ws), need, _stream(dev)), "m3b_grad_clip")
+    ws = _bytes(need, dev.index)
+    _call(L.m3b_grad_clip, "m3b_grad_clip", dev.index, C.byref(a), ws.data_ptr(), need)
     return norm

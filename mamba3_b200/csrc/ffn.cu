@@ -9,8 +9,10 @@
 // product are its epilogue (g and u never reach memory in inference), then the down product with
 // bias, scale and residual in its epilogue.  Backward: da's product with dg and du as its epilogue;
 // dx (one product over two K segments) and the three weight gradients side by side in one launch.
+// Inference on at most kSmallRows rows (a decoding step) runs the matrix-vector form of ffn_small.cu.
 // 18 rows d_model d_ff operations forward and backward, the least there are: g and u are kept in
 // fp32 (8 bytes a value), because the rounding of a 16-bit copy would reach every gradient.
+#include "ffn_small.h"
 #include "gemm.cuh"
 
 namespace m3b {
@@ -178,6 +180,23 @@ int blocks_of(int64_t k) { return (int)((k + kGmBK - 1) / kGmBK); }
 // run == false only measures the workspace.
 int forward(const m3b_gated_ffn_args* a, void* workspace, size_t* need, bool run, cudaStream_t st) {
   const Dims d(a);
+  // Few rows and nothing to save: 1 row of 768 x 2112 took 18 us of three tensor-core launches.
+  if (d.M <= kSmallRows && !a->saved_gu) {
+    *need = 0;
+    if (!run) return M3B_OK;
+    SmallFfn p{};
+    p.M = (int)d.M, p.D = d.D, p.F = d.F;
+    p.x_stride = a->x_stride, p.res_stride = a->residual_stride;
+    p.ld_act = up(d.F, 8);
+    p.x = a->x, p.w_gate = a->w_gate, p.w_up = a->w_up, p.w_down = a->w_down;
+    p.b_gate = a->b_gate, p.b_up = a->b_up, p.b_down = a->b_down, p.residual = a->residual;
+    p.act = a->saved_act, p.out = a->out;
+    p.scale = a->residual_scale;
+    const int v = d.f32 ? 4 : 8;
+    p.vec = aligned16(a->x) && aligned16(a->w_gate) && aligned16(a->w_up) && aligned16(a->w_down) && d.D % v == 0 &&
+            d.F % v == 0 && a->x_stride % v == 0;
+    return launch_small_ffn(p, a->dtype, st);
+  }
   Carve ws(workspace);
   int rc = M3B_OK;
   const GemmOperand x = operand(a->x, d.M, d.D, a->x_stride, a, ws, run, st, &rc);

@@ -50,15 +50,18 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     (widths that are no multiple of 8, a last dimension with a stride, fp32) are laid out once per
     call.  Differentiable in every tensor argument; sums in fp32, and the activation (forward) and its
     two factors' gradients (backward) rounded to a 16-bit dtype once."""
-    ts = [x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual]
     if x.is_cuda and torch.is_autocast_enabled("cuda"):
         dt = torch.get_autocast_dtype("cuda")
-        ts = [t if t is None or t.dtype == dt else t.to(dt) for t in ts]
-        x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual = ts
-    _lib._cuda(*ts)
-    if any(t is not None and t.dtype != x.dtype for t in ts):
-        raise _lib.M3bError(f"gated_ffn: one dtype expected, got {[t.dtype for t in ts if t is not None]}")
-    _lib.dtype_code(x.dtype)
+        x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual = [
+            t if t is None or t.dtype == dt else t.to(dt)
+            for t in (x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual)]
+    ts = [t for t in (x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual) if t is not None]
+    _lib._same_gpu("gated_ffn", ts)
+    dt = x.dtype
+    for t in ts:
+        if t.dtype != dt:
+            raise _lib.M3bError(f"gated_ffn: one dtype expected, got {[t.dtype for t in ts]}")
+    _lib.dtype_code(dt)
     if x.dim() < 1 or w_gate.dim() != 2:
         raise ValueError("gated_ffn: x (..., d_model) and w_gate (d_ff, d_model) expected")
     f, d = w_gate.shape
@@ -69,17 +72,20 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
         raise ValueError("gated_ffn: d_model and d_ff must be positive")
     if (b_gate is None) != (b_up is None):
         raise ValueError("gated_ffn: b_gate and b_up go together")
-    for name, b, n in (("b_gate", b_gate, f), ("b_up", b_up, f), ("b_down", b_down, d)):
-        if b is not None and b.shape != (n,):
-            raise ValueError(f"gated_ffn: {name} ({n},) expected, got {tuple(b.shape)}")
-    if residual is not None and residual.shape != x.shape:
-        raise ValueError(f"gated_ffn: residual must have x's shape {tuple(x.shape)}, got {tuple(residual.shape)}")
+    if len(ts) > 4:
+        for name, b, n in (("b_gate", b_gate, f), ("b_up", b_up, f), ("b_down", b_down, d)):
+            if b is not None:
+                if b.shape != (n,):
+                    raise ValueError(f"gated_ffn: {name} ({n},) expected, got {tuple(b.shape)}")
+        b_gate, b_up, b_down = [b if b is None else b.contiguous() for b in (b_gate, b_up, b_down)]
+        if residual is not None and residual.shape != x.shape:
+            raise ValueError(f"gated_ffn: residual must have x's shape {tuple(x.shape)}, got {tuple(residual.shape)}")
     x2 = _lib._rows2d(x, d)
     r2 = None if residual is None else _lib._rows2d(residual, d)
-    ws = [None if t is None else t.contiguous() for t in (w_gate, w_up, w_down, b_gate, b_up, b_down)]
+    w_gate, w_up, w_down = w_gate.contiguous(), w_up.contiguous(), w_down.contiguous()
     scale = float(residual_scale)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
-        y = _GatedFfn.apply(x2, *ws, r2, scale)
+    if torch.is_grad_enabled() and any([t.requires_grad for t in ts]):
+        y = _GatedFfn.apply(x2, w_gate, w_up, w_down, b_gate, b_up, b_down, r2, scale)
     else:
-        y = ops.gated_ffn_fwd(x2, *ws, r2, scale, False)[0]
-    return y.view(x.shape)
+        y = ops.gated_ffn_fwd(x2, w_gate, w_up, w_down, b_gate, b_up, b_down, r2, scale, False)[0]
+    return y if y.dim() == x.dim() else y.view(x.shape)

@@ -46,7 +46,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     if hidden.is_cuda and torch.is_autocast_enabled("cuda"):
         dt = torch.get_autocast_dtype("cuda")
         hidden, weight = hidden.to(dt), weight.to(dt)
-    _lib._cuda(hidden, weight, targets)
+    _lib._same_gpu("linear_cross_entropy", (hidden, weight, targets))
     if hidden.dtype != weight.dtype:
         raise _lib.M3bError(f"linear_cross_entropy: one dtype expected, got {hidden.dtype} and {weight.dtype}")
     _lib.dtype_code(hidden.dtype)
@@ -62,7 +62,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     if targets.dtype not in (torch.int64, torch.int32, torch.int16, torch.uint8, torch.int8):
         raise ValueError(f"linear_cross_entropy: integer targets expected, got {targets.dtype}")
     h2 = _lib._rows2d(hidden, weight.shape[1])
-    t1 = targets.reshape(-1).to(torch.int64).contiguous()
+    t1 = (targets if targets.dim() == 1 else targets.reshape(-1)).to(torch.int64).contiguous()
     w = weight.contiguous()
     if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
         loss = _LinearXent.apply(h2, w, t1, int(ignore_index), reduction)

@@ -36,9 +36,9 @@ def test_short_workspace_is_refused():
     L = _lib.lib()
     buf = ctypes.create_string_buffer(1 << 16)
     p = (ctypes.addressof(buf) + 255) // 256 * 256
-    a = _lib.GatedFfnArgs(4, 63, 0, 63, 63, 128, 1, 1.0, p, p, p, p, None, None, None, None, p, None, p)
+    a = _lib.GatedFfnArgs(40, 63, 0, 63, 63, 128, 1, 1.0, p, p, p, p, None, None, None, None, p, None, p)
     need = L.m3b_gated_ffn_fwd_workspace(ctypes.byref(a))
-    assert need >= 4 * 64 * 2 + 2 * 128 * 64 * 2  # x, w_gate and w_up laid out with rows of 64
+    assert need >= 40 * 64 * 2 + 2 * 128 * 64 * 2  # x, w_gate and w_up laid out with rows of 64
     assert L.m3b_gated_ffn_fwd(ctypes.byref(a), p, need - 1, None) == 6
     assert L.m3b_gated_ffn_fwd(ctypes.byref(a), p + 4, need, None) == 4
     a.saved_act = p + 2
