@@ -41,14 +41,14 @@ struct Dims {
         f32(a->dtype == M3B_F32) {}
 };
 
-// A matrix as an operand: in place where the TMA can read it, else packed into the workspace.
+// A matrix as an operand: in place where the TMA can read it, else listed for packing into the workspace.
 GemmOperand operand(const void* p, int64_t rows, int64_t cols, int64_t ld, const m3b_gated_ffn_args* a, Carve& ws,
-                    bool run, cudaStream_t st, int* rc) {
+                    PackList& packs) {
   if (a->dtype != M3B_F32 && tma_ok(p, ld)) return GemmOperand{p, rows, cols, ld, 0, 1};
   const int np = a->dtype == M3B_F32 ? 3 : 1;
   const int64_t ldp = up(cols, 8), plane = rows * ldp;
   void* dst = ws.take((size_t)np * plane * 2);
-  if (run && *rc == M3B_OK) *rc = launch_pack(p, a->dtype, rows, cols, ld, dst, ldp, plane, st);
+  packs.add(p, rows, cols, ld, dst, ldp, plane);
   return GemmOperand{dst, rows, cols, ldp, plane, np};
 }
 
@@ -71,23 +71,37 @@ GemmOut operand_out(const GemmOperand& o, bool f16) {
   return r;
 }
 
-// Sum over the rows of an operand times `scale`, in a fixed order.  A block takes 64 columns (two a
+// Sums over the rows of up to three operands, times `scale`, in a fixed order.  A block takes 64 columns (two a
 // lane) and kSumRows rows, its warps every eighth row, and leaves one partial; the chunks' partials
 // are added by a second kernel.
 constexpr int kSumRows = 128;
-__global__ void __launch_bounds__(256) colsum_kernel(const uint16_t* __restrict__ x, int f16, int planes, int64_t plane,
-                                                     int64_t ld, int64_t rows, int cols, float* __restrict__ part) {
+struct Sums {
+  struct {
+    const uint16_t* x;
+    int64_t plane, ld;
+    int cols;
+    float scale;
+    void* out;
+    float* part;
+  } s[3];
+  int n, f16, planes, dt, chunks;
+  int64_t rows;
+};
+__global__ void __launch_bounds__(256) colsum_kernel(const __grid_constant__ Sums a) {
   __shared__ float2 sm[8][32];
+  pdl_wait_primary();
+  pdl_launch_dependents();
+  const auto& m = a.s[blockIdx.z];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = blockIdx.x * 64 + 2 * lane;
-  const int64_t r0 = (int64_t)blockIdx.y * kSumRows, r1 = r0 + kSumRows < rows ? r0 + kSumRows : rows;
+  const int64_t r0 = (int64_t)blockIdx.y * kSumRows, r1 = r0 + kSumRows < a.rows ? r0 + kSumRows : a.rows;
   float2 s = make_float2(0.f, 0.f);
-  if (c < cols) {
+  if (c < m.cols) {
 #pragma unroll 8
     for (int64_t r = r0 + w; r < r1; r += 8) {
-      for (int k = planes - 1; k >= 0; --k) {
-        const uint16_t* p = x + k * plane + r * ld + c;
-        const uint32_t v = c + 1 < cols ? *reinterpret_cast<const uint32_t*>(p) : (uint32_t)*p;
-        const float2 f = f16 ? __half22float2(*reinterpret_cast<const __half2*>(&v)) : bf2_to_f2(v);
+      for (int k = a.planes - 1; k >= 0; --k) {
+        const uint16_t* p = m.x + k * m.plane + r * m.ld + c;
+        const uint32_t v = c + 1 < m.cols ? *reinterpret_cast<const uint32_t*>(p) : (uint32_t)*p;
+        const float2 f = a.f16 ? __half22float2(*reinterpret_cast<const __half2*>(&v)) : bf2_to_f2(v);
         s.x += f.x;
         s.y += f.y;
       }
@@ -95,34 +109,35 @@ __global__ void __launch_bounds__(256) colsum_kernel(const uint16_t* __restrict_
   }
   sm[w][lane] = s;
   __syncthreads();
-  if (w != 0 || c >= cols) return;
+  if (w != 0 || c >= m.cols) return;
   for (int k = 1; k < 8; ++k) s.x += sm[k][lane].x, s.y += sm[k][lane].y;
-  float* o = part + (int64_t)blockIdx.y * cols + c;
+  float* o = m.part + (int64_t)blockIdx.y * m.cols + c;
   o[0] = s.x;
-  if (c + 1 < cols) o[1] = s.y;
+  if (c + 1 < m.cols) o[1] = s.y;
 }
-__global__ void __launch_bounds__(256) colsum_finish_kernel(const float* __restrict__ part, int chunks, int cols, float scale,
-                                                            void* out, int dt) {
+__global__ void __launch_bounds__(256) colsum_finish_kernel(const __grid_constant__ Sums a) {
   __shared__ float sm[8][32];
+  pdl_wait_primary();
+  const auto& m = a.s[blockIdx.y];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
   float s = 0.f;
-  if (c < cols) {
+  if (c < m.cols) {
 #pragma unroll 4
-    for (int k = w; k < chunks; k += 8) s += part[(int64_t)k * cols + c];
+    for (int k = w; k < a.chunks; k += 8) s += m.part[(int64_t)k * m.cols + c];
   }
   sm[w][lane] = s;
   __syncthreads();
-  if (w != 0 || c >= cols) return;
+  if (w != 0 || c >= m.cols) return;
   for (int k = 1; k < 8; ++k) s += sm[k][lane];
-  stf(out, c, dt, s * scale);
+  stf(m.out, c, a.dt, s * m.scale);
 }
-int colsum(const GemmOperand& o, bool f16, float scale, void* out, int out_dt, float* part, cudaStream_t st) {
-  const int chunks = (int)((o.rows + kSumRows - 1) / kSumRows), cols = (int)o.cols;
-  if (chunks > 65535) return fail(M3B_ERR_UNSUPPORTED, "gated_ffn_bwd: bias gradients over more than 8,388,480 rows");
-  colsum_kernel<<<dim3((cols + 63) / 64, chunks), 256, 0, st>>>(static_cast<const uint16_t*>(o.p), f16, o.planes, o.plane,
-                                                               o.ld, o.rows, cols, part);
-  colsum_finish_kernel<<<(cols + 31) / 32, 256, 0, st>>>(part, chunks, cols, scale, out, out_dt);
-  return check_launch("colsum_kernel");
+int colsums(const Sums& a, cudaStream_t st) {
+  if (a.n == 0) return M3B_OK;
+  if (a.chunks > 65535) return fail(M3B_ERR_UNSUPPORTED, "gated_ffn_bwd: bias gradients over more than 8,388,480 rows");
+  int cols = 0;
+  for (int i = 0; i < a.n; ++i) cols = a.s[i].cols > cols ? a.s[i].cols : cols;
+  const int rc = launch_dependent(colsum_kernel, dim3((cols + 63) / 64, a.chunks, a.n), 256, st, a);
+  return rc != M3B_OK ? rc : launch_dependent(colsum_finish_kernel, dim3((cols + 31) / 32, a.n), 256, st, a);
 }
 
 int check(const m3b_gated_ffn_args* a, bool bwd) {
@@ -198,11 +213,11 @@ int forward(const m3b_gated_ffn_args* a, void* workspace, size_t* need, bool run
     return launch_small_ffn(p, a->dtype, st);
   }
   Carve ws(workspace);
-  int rc = M3B_OK;
-  const GemmOperand x = operand(a->x, d.M, d.D, a->x_stride, a, ws, run, st, &rc);
-  const GemmOperand wg = operand(a->w_gate, d.F, d.D, d.D, a, ws, run, st, &rc);
-  const GemmOperand wu = operand(a->w_up, d.F, d.D, d.D, a, ws, run, st, &rc);
-  const GemmOperand wd = operand(a->w_down, d.D, d.F, d.F, a, ws, run, st, &rc);
+  PackList packs;
+  const GemmOperand x = operand(a->x, d.M, d.D, a->x_stride, a, ws, packs);
+  const GemmOperand wg = operand(a->w_gate, d.F, d.D, d.D, a, ws, packs);
+  const GemmOperand wu = operand(a->w_up, d.F, d.D, d.D, a, ws, packs);
+  const GemmOperand wd = operand(a->w_down, d.D, d.F, d.F, a, ws, packs);
   const GemmOperand act = act_operand(a, a->saved_act);
   const bool pair = d.M > 128;
 
@@ -235,7 +250,8 @@ int forward(const m3b_gated_ffn_args* a, void* workspace, size_t* need, bool run
   t.dt = a->dtype;
   void* parts = ws.take(plan_gemm(q, kEpiFinal, pair));
   *need = ws.at;
-  if (!run || rc != M3B_OK) return rc;
+  if (!run) return M3B_OK;
+  M3B_TRY(launch_pack(packs, a->dtype, st));
 
   M3B_MAP(&s.a[0], x, false, 128, d.f16);
   M3B_MAP(&s.b[0], wg, false, gemm_box_b(pair, p.bn, kEpiGlu), d.f16);
@@ -249,17 +265,26 @@ int forward(const m3b_gated_ffn_args* a, void* workspace, size_t* need, bool run
 int backward(const m3b_gated_ffn_args* a, void* workspace, size_t* need, bool run, cudaStream_t st) {
   const Dims d(a);
   Carve ws(workspace);
-  int rc = M3B_OK;
-  const GemmOperand x = operand(a->x, d.M, d.D, a->x_stride, a, ws, run, st, &rc);
-  const GemmOperand wg = operand(a->w_gate, d.F, d.D, d.D, a, ws, run, st, &rc);
-  const GemmOperand wu = operand(a->w_up, d.F, d.D, d.D, a, ws, run, st, &rc);
-  const GemmOperand wd = operand(a->w_down, d.D, d.F, d.F, a, ws, run, st, &rc);
-  const GemmOperand dy = operand(a->dout, d.M, d.D, a->dout_stride, a, ws, run, st, &rc);
+  PackList packs;
+  const GemmOperand x = operand(a->x, d.M, d.D, a->x_stride, a, ws, packs);
+  const GemmOperand wg = operand(a->w_gate, d.F, d.D, d.D, a, ws, packs);
+  const GemmOperand wu = operand(a->w_up, d.F, d.D, d.D, a, ws, packs);
+  const GemmOperand wd = operand(a->w_down, d.D, d.F, d.F, a, ws, packs);
+  const GemmOperand dy = operand(a->dout, d.M, d.D, a->dout_stride, a, ws, packs);
   const size_t one = (size_t)act_operand(a, nullptr).plane * d.np * 2;
   const GemmOperand dg = act_operand(a, ws.take(one)), du = act_operand(a, ws.take(one));
   const GemmOperand act = act_operand(a, a->saved_act);
-  const int64_t chunks = (d.M + kSumRows - 1) / kSumRows;
-  float* part = static_cast<float*>(ws.take((size_t)chunks * (d.F > d.D ? d.F : d.D) * 4));
+  Sums sums{};
+  sums.f16 = d.f16, sums.planes = d.np, sums.dt = a->dtype, sums.rows = d.M;
+  sums.chunks = (int)((d.M + kSumRows - 1) / kSumRows);
+  auto sum = [&](const GemmOperand& o, float scale, void* out) {
+    if (!out) return;
+    float* part = static_cast<float*>(ws.take((size_t)sums.chunks * o.cols * 4));
+    sums.s[sums.n++] = {static_cast<const uint16_t*>(o.p), o.plane, o.ld, (int)o.cols, scale, out, part};
+  };
+  sum(dg, 1.f, a->db_gate);
+  sum(du, 1.f, a->db_up);
+  sum(dy, a->residual_scale, a->db_down);
   int* ticket = static_cast<int*>(ws.take(4));
 
   // dx and the three weight gradients, side by side
@@ -295,8 +320,8 @@ int backward(const m3b_gated_ffn_args* a, void* workspace, size_t* need, bool ru
   }
   void* parts = ws.take(plan_gemm(q, kEpiStore, true));
   *need = ws.at;
-  if (!run || rc != M3B_OK) return rc;
-  if (cudaMemsetAsync(ticket, 0, 4, st) != cudaSuccess) return check_launch("gated_ffn_bwd");
+  if (!run) return M3B_OK;
+  M3B_TRY(launch_pack(packs, a->dtype, st));
   {  // da -> dg, du
     GemmParams p = params(d, a, 256);
     GemmSub& s = p.sub[0];
@@ -312,14 +337,12 @@ int backward(const m3b_gated_ffn_args* a, void* workspace, size_t* need, bool ru
     s.out2 = operand_out(du, d.f16);
     p.gu = static_cast<float*>(a->saved_gu);
     p.gu_ld4 = up(d.F, 32) / 4;
+    p.clear = ticket;
     plan_gemm(p, kEpiDglu, true);
     M3B_TRY(launch_gemm(p, kEpiDglu, true, nullptr, st));
   }
   if (q.nsub) M3B_TRY(launch_gemm(q, kEpiStore, true, parts, st));
-  if (a->db_gate) M3B_TRY(colsum(dg, d.f16, 1.f, a->db_gate, a->dtype, part, st));
-  if (a->db_up) M3B_TRY(colsum(du, d.f16, 1.f, a->db_up, a->dtype, part, st));
-  if (a->db_down) M3B_TRY(colsum(dy, d.f16, a->residual_scale, a->db_down, a->dtype, part, st));
-  return M3B_OK;
+  return colsums(sums, st);
 }
 
 int check_workspace(size_t need, const void* ws, size_t bytes) {

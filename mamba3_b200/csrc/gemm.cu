@@ -8,30 +8,33 @@ namespace m3b {
 
 namespace {
 
-// One thread per destination pair of columns: fp32 values become three bf16 planes, 16-bit values
-// are copied; columns past `cols` are zero.  Bound by HBM; rows are short strided runs, so plain
-// 4-byte stores suffice (the copy is a few per cent of the products that read it).
+// One thread per destination pair of columns, one row of blocks per matrix: fp32 values become three
+// bf16 planes, 16-bit values are copied; columns past `cols` are zero.  Bound by HBM; rows are short
+// strided runs, so plain 4-byte stores suffice (the copy is a few per cent of the products that read it).
 template <bool F32>
-__global__ void pack_kernel(const void* __restrict__ src, int64_t rows, int64_t cols, int64_t src_ld,
-                            uint16_t* __restrict__ dst, int64_t ld, int64_t plane) {
-  const int64_t half = ld / 2, n = rows * half;
+__global__ void pack_kernel(const __grid_constant__ PackList l) {
+  pdl_wait_primary();
+  pdl_launch_dependents();
+  const auto& m = l.m[blockIdx.y];
+  const int64_t half = m.ld / 2, n = m.rows * half;
+  uint16_t* dst = static_cast<uint16_t*>(m.dst);
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
     const int64_t r = i / half, c = 2 * (i - r * half);
     uint32_t w[3] = {0, 0, 0};
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      if (c + e >= cols) break;
+      if (c + e >= m.cols) break;
       if constexpr (F32) {
         uint16_t x[3];
-        split_planes(static_cast<const float*>(src)[r * src_ld + c + e], x);
+        split_planes(static_cast<const float*>(m.src)[r * m.src_ld + c + e], x);
 #pragma unroll
         for (int k = 0; k < 3; ++k) w[k] |= (uint32_t)x[k] << (16 * e);
       } else {
-        w[0] |= (uint32_t) static_cast<const uint16_t*>(src)[r * src_ld + c + e] << (16 * e);
+        w[0] |= (uint32_t) static_cast<const uint16_t*>(m.src)[r * m.src_ld + c + e] << (16 * e);
       }
     }
 #pragma unroll
-    for (int k = 0; k < (F32 ? 3 : 1); ++k) *reinterpret_cast<uint32_t*>(dst + k * plane + r * ld + c) = w[k];
+    for (int k = 0; k < (F32 ? 3 : 1); ++k) *reinterpret_cast<uint32_t*>(dst + k * m.plane + r * m.ld + c) = w[k];
   }
 }
 
@@ -64,12 +67,14 @@ cudaLaunchConfig_t config(unsigned grid, bool pair, cudaStream_t st, cudaLaunchA
   at[0].val.clusterDim.x = pair ? 2 : 1;
   at[0].val.clusterDim.y = 1;
   at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(kGmThreads);
   cfg.dynamicSmemBytes = kGmSmem;
   cfg.stream = st;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   return cfg;
 }
 
@@ -91,8 +96,9 @@ int device_setup(int* pairs) {
                                                  cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kGmSmem);
       if (e != cudaSuccess) return fail(M3B_ERR_CUDA, "gemm: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
     }
-  cudaLaunchAttribute at[1];
-  const cudaLaunchConfig_t cfg = config(2 * (unsigned)(num_sms() / 2), true, nullptr, at);
+  cudaLaunchAttribute at[2];
+  cudaLaunchConfig_t cfg = config(2 * (unsigned)(num_sms() / 2), true, nullptr, at);
+  cfg.numAttrs = 1;
   int n = 0;
   if (cudaOccupancyMaxActiveClusters(&n, (const void*)kernel_of(kEpiStore, true, false), &cfg) != cudaSuccess || n <= 0) {
     cudaGetLastError();
@@ -205,7 +211,7 @@ int launch_gemm(GemmParams& p, int epi, bool pair, void* parts, cudaStream_t st)
   if (p.wait_ns == 0) p.wait_ns = kWaitLimitNs;
   const int64_t most = pair ? pairs : num_sms();
   const unsigned workers = (unsigned)(jobs < most ? jobs : most);
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   const cudaLaunchConfig_t cfg = config(pair ? 2 * workers : workers, pair, st, attr);
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel_of(epi, pair, p.npass > 1), p);
   if (e != cudaSuccess) return fail(M3B_ERR_CUDA, "gemm_kernel: %s", cudaGetErrorString(e));
@@ -214,23 +220,20 @@ int launch_gemm(GemmParams& p, int epi, bool pair, void* parts, cudaStream_t st)
     for (int i = 0; i < p.nsub; ++i) split = p.sub[i].split > split ? p.sub[i].split : split;
     while (warps < 8 && warps * 2 < split) warps *= 2;
     const unsigned grid = (unsigned)((pieces + 8 / warps - 1) / (8 / warps));
-    if (epi == kEpiFinal) gemm_join_kernel<kEpiFinal><<<grid, 256, 0, st>>>(p, tile_m, warps);
-    else gemm_join_kernel<kEpiAcc><<<grid, 256, 0, st>>>(p, tile_m, warps);
+    const int rj = launch_dependent(epi == kEpiFinal ? gemm_join_kernel<kEpiFinal> : gemm_join_kernel<kEpiAcc>,
+                                    dim3(grid), 256, st, p, tile_m, warps);
+    if (rj != M3B_OK) return rj;
   }
   return check_launch("gemm_kernel");
 }
 
-int launch_pack(const void* src, int dtype, int64_t rows, int64_t cols, int64_t src_ld, void* dst, int64_t ld,
-                int64_t plane, cudaStream_t st) {
-  const int64_t n = rows * (ld / 2);
+int launch_pack(const PackList& l, int dtype, cudaStream_t st) {
+  int64_t n = 0;
+  for (int i = 0; i < l.n; ++i) n = l.m[i].rows * (l.m[i].ld / 2) > n ? l.m[i].rows * (l.m[i].ld / 2) : n;
   if (n == 0) return M3B_OK;
   const int64_t blocks = (n + 255) / 256, most = (int64_t)num_sms() * 16;
-  const unsigned grid = (unsigned)(blocks < most ? blocks : most);
-  if (dtype == M3B_F32)
-    pack_kernel<true><<<grid, 256, 0, st>>>(src, rows, cols, src_ld, static_cast<uint16_t*>(dst), ld, plane);
-  else
-    pack_kernel<false><<<grid, 256, 0, st>>>(src, rows, cols, src_ld, static_cast<uint16_t*>(dst), ld, plane);
-  return check_launch("pack_kernel");
+  const dim3 grid((unsigned)(blocks < most ? blocks : most), l.n);
+  return launch_dependent(dtype == M3B_F32 ? pack_kernel<true> : pack_kernel<false>, grid, 256, st, l);
 }
 
 }  // namespace m3b

@@ -106,6 +106,7 @@ struct GemmParams {
   int f16;      // operand type: fp16 instead of bf16
   const int* dyn;
   int* ticket;  // zeroed counter that jobs are drawn from, or null: dealt in turn
+  int* clear;   // a counter to zero for the launch that follows
   // kEpiGlu / kEpiDglu: g and u in fp32, [row / 32][col / 4][g, u][row % 32][4], ld4 = column quads (of
   // whole runs of 32 columns)
   float* gu;
@@ -494,6 +495,11 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
   __syncthreads();
   if constexpr (PAIR) cluster_sync();  // both CTAs' barriers are initialised before any remote use
   tc_fence_after();
+  // so far nothing was read that another kernel writes: launched as a programmatic dependent, this part
+  // ran under the end of the kernel before
+  pdl_wait_primary();
+  pdl_launch_dependents();
+  if (p.clear && blockIdx.x == 0 && threadIdx.x == 0) *p.clear = 0;
   const uint32_t tbase = *tslot;
   const uint32_t rank = PAIR ? cluster_rank() : 0u;
   const int worker = PAIR ? blockIdx.x / 2 : blockIdx.x, nworkers = PAIR ? gridDim.x / 2 : gridDim.x;
@@ -958,6 +964,8 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
 template <int EPI>
 __global__ void __launch_bounds__(256) gemm_join_kernel(const __grid_constant__ GemmParams p, int tile_m, int warps) {
   __shared__ __align__(1024) uint8_t boxes[8 * kGmBox];
+  pdl_wait_primary();
+  pdl_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, w = warp & (warps - 1);
   uint8_t* box = boxes + warp * kGmBox;
   const int dyn = p.dyn ? *p.dyn : 0;
@@ -1063,10 +1071,19 @@ inline int gemm_tile_m(bool pair) { return pair ? 256 : 128; }
 // Rows of B per tensor-map box for `bn` accumulator columns.
 inline int gemm_box_b(bool pair, int bn, int epi) { return epi == kEpiGlu || pair ? bn / 2 : bn; }
 
-// dst planes (rows x cols, rows ld apart, zero up to ld_pad columns and rows_pad rows) of src
-// (dtype, rows src_ld apart, column stride src_cs): the operand form of a matrix the TMA cannot read
-// in place, or of an fp32 one (three bf16 planes).
-int launch_pack(const void* src, int dtype, int64_t rows, int64_t cols, int64_t src_ld, void* dst, int64_t ld,
-                int64_t plane, cudaStream_t st);
+// dst planes (rows ld apart, zero from cols to ld) of src (rows src_ld apart): the operand form of a
+// matrix the TMA cannot read in place, or of an fp32 one (three bf16 planes).
+struct PackList {
+  struct {
+    const void* src;
+    void* dst;
+    int64_t rows, cols, src_ld, ld, plane;
+  } m[5];
+  int n = 0;
+  void add(const void* src, int64_t rows, int64_t cols, int64_t src_ld, void* dst, int64_t ld, int64_t plane) {
+    m[n++] = {src, dst, rows, cols, src_ld, ld, plane};
+  }
+};
+int launch_pack(const PackList& l, int dtype, cudaStream_t st);
 
 }  // namespace m3b

@@ -17,6 +17,23 @@ int check_launch(const char* what);
 // Number of SMs of the current device (cached per device).
 int num_sms();
 
+// Launch as a programmatic dependent of the kernel before it on the stream: `kernel` waits for that one
+// (pdl_wait_primary) before it touches memory that another kernel writes or reads.
+template <typename K, typename... A>
+int launch_dependent(K kernel, dim3 grid, int threads, cudaStream_t st, const A&... args) {
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.stream = st;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  return e == cudaSuccess ? M3B_OK : fail(M3B_ERR_CUDA, "launch: %s", cudaGetErrorString(e));
+}
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 struct ScanLaunch {

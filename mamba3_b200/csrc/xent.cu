@@ -70,6 +70,7 @@ Saved saved_of(const m3b_linear_xent_args* a, void* p) {
 __global__ void __launch_bounds__(1024) keep_kernel(const int64_t* __restrict__ target, int64_t ignore, int64_t T,
                                                     int64_t Tp, int V, Saved s, int* err) {
   __shared__ int sums[2][32];
+  pdl_launch_dependents();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int total = 0, side = 0;
   for (int64_t base = 0; base < T; base += 4096, side ^= 1) {
@@ -116,6 +117,8 @@ __global__ void __launch_bounds__(1024) keep_kernel(const int64_t* __restrict__ 
 // One warp per row of the dense operand; rows behind the last kept one are zero up to the tile's end.
 __global__ void __launch_bounds__(256) gather_kernel(const void* __restrict__ h, int dt, int64_t ld, int D, int64_t Tp,
                                                      int64_t Dp, int vec, Saved s) {
+  pdl_wait_primary();
+  pdl_launch_dependents();
   const int lane = threadIdx.x & 31;
   const int64_t n = *s.count, end = (n + 255) / 256 * 256 < Tp ? (n + 255) / 256 * 256 : Tp;
   const int64_t step = (int64_t)gridDim.x * 8, plane = Tp * Dp;
@@ -154,6 +157,8 @@ __global__ void __launch_bounds__(512) join_kernel(const float2* __restrict__ pa
                                                    const float* __restrict__ target_logit, Saved s,
                                                    float* __restrict__ row_loss) {
   __shared__ float2 sm[16][32];
+  pdl_wait_primary();
+  pdl_launch_dependents();
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int n = *s.count;
   const int64_t row = (int64_t)blockIdx.x * 32 + lane;
@@ -186,6 +191,7 @@ __global__ void __launch_bounds__(512) join_kernel(const float2* __restrict__ pa
 // The loss from the rows' losses: summed in a fixed order in fp64, or put at the rows' places.
 __global__ void __launch_bounds__(1024) loss_kernel(const float* __restrict__ row_loss, Saved s, int reduction,
                                                     float* __restrict__ loss) {
+  pdl_wait_primary();
   const int n = *s.count;
   if (reduction == 0) {
     for (int i = threadIdx.x; i < n; i += 1024) loss[s.row[i]] = row_loss[i];
@@ -241,7 +247,11 @@ GemmOperand weight_of(const m3b_linear_xent_args* a, Carve& ws, bool run, cudaSt
   if (!d.f32 && tma_ok(a->weight, d.D)) return GemmOperand{a->weight, d.V, d.D, d.D, 0, 1};
   const int64_t plane = (int64_t)d.V * d.Dp;
   void* p = ws.take((size_t)d.np * plane * 2);
-  if (run && *rc == M3B_OK) *rc = launch_pack(a->weight, a->dtype, d.V, d.D, d.D, p, d.Dp, plane, st);
+  if (run && *rc == M3B_OK) {
+    PackList packs;
+    packs.add(a->weight, d.V, d.D, d.D, p, d.Dp, plane);
+    *rc = launch_pack(packs, a->dtype, st);
+  }
   return GemmOperand{p, d.V, d.D, d.Dp, plane, d.np};
 }
 
@@ -275,9 +285,9 @@ int forward(const m3b_linear_xent_args* a, void* workspace, size_t* need, bool r
     keep_kernel<<<1, 1024, 0, st>>>(a->target, a->ignore_index, d.T, d.Tp, d.V, s, a->err);
     const int64_t blocks = d.Tp / 8, most = (int64_t)num_sms() * 8;
     const int vec = !d.f32 && d.D % 8 == 0 && a->hidden_stride % 8 == 0 && aligned16(a->hidden);
-    gather_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, st>>>(a->hidden, a->dtype, a->hidden_stride, d.D,
-                                                                            d.Tp, d.Dp, vec, s);
-    M3B_TRY(check_launch("linear_xent gather"));
+    M3B_TRY(check_launch("linear_xent keep"));
+    M3B_TRY(launch_dependent(gather_kernel, dim3((unsigned)(blocks < most ? blocks : most)), 256, st, a->hidden,
+                             (int)a->dtype, a->hidden_stride, d.D, d.Tp, d.Dp, vec, s));
   }
   const GemmOperand w = weight_of(a, ws, run, st, &rc);
   *need = ws.at;
@@ -303,11 +313,11 @@ int forward(const m3b_linear_xent_args* a, void* workspace, size_t* need, bool r
   p.part_ld = d.Tp;
   plan_gemm(p, kEpiLse, pair);
   M3B_TRY(launch_gemm(p, kEpiLse, pair, nullptr, st));
-  join_kernel<<<(unsigned)(d.Tp / 32), 512, 0, st>>>(part, nt * 2, d.Tp, target_logit, s, row_loss);
   if (a->reduction == 0 && cudaMemsetAsync(a->loss, 0, (size_t)d.T * 4, st) != cudaSuccess)
     return check_launch("linear_xent loss");
-  loss_kernel<<<1, 1024, 0, st>>>(row_loss, s, a->reduction, a->loss);
-  return check_launch("linear_xent loss");
+  M3B_TRY(launch_dependent(join_kernel, dim3((unsigned)(d.Tp / 32)), 512, st, (const float2*)part, nt * 2, d.Tp,
+                           (const float*)target_logit, s, row_loss));
+  return launch_dependent(loss_kernel, dim3(1), 1024, st, (const float*)row_loss, s, (int)a->reduction, a->loss);
 }
 
 // Columns of a piece of the vocabulary.
@@ -328,7 +338,7 @@ int backward(const m3b_linear_xent_args* a, void* workspace, size_t* need, bool 
   if (a->dhidden && pieces > 1) acc = static_cast<float*>(ws.take((size_t)d.Tp * up(d.D, bn) * 4));
   float* roww = nullptr;
   if (a->reduction == 0) roww = static_cast<float*>(ws.take((size_t)d.Tp * 4));
-  int* ticket = static_cast<int*>(ws.take((size_t)pieces * 4));
+  int* ticket = static_cast<int*>(ws.take(4));
   const GemmOperand w = weight_of(a, ws, run, st, &rc);
   const Saved s = saved_of(a, a->saved);
   const GemmOperand h{s.h, d.Tp, d.D, d.Dp, d.Tp * d.Dp, d.np};
@@ -392,7 +402,6 @@ int backward(const m3b_linear_xent_args* a, void* workspace, size_t* need, bool 
   if (!run || rc != M3B_OK) return rc;
   if (a->dhidden && cudaMemsetAsync(a->dhidden, 0, (size_t)d.T * d.D * es, st) != cudaSuccess)
     return check_launch("linear_xent_bwd");
-  if (cudaMemsetAsync(ticket, 0, (size_t)pieces * 4, st) != cudaSuccess) return check_launch("linear_xent_bwd");
   if (roww) {
     roww_kernel<<<64, 256, 0, st>>>(a->dloss, s, roww);
     M3B_TRY(check_launch("linear_xent roww"));
@@ -420,13 +429,14 @@ int backward(const m3b_linear_xent_args* a, void* workspace, size_t* need, bool 
       p.lse2 = s.lse2;
       p.roww = roww;
       p.col0 = (int)c0;
+      p.clear = ticket;
       plan_gemm(p, kEpiDlogit, true);
       M3B_TRY(launch_gemm(p, kEpiDlogit, true, nullptr, st));
     }
     GemmParams p = base;
     M3B_TRY(gradients(p, c0, n, &z, &wp));
     plan_gemm(p, kEpiAcc, true);
-    p.ticket = ticket + c0 / cols;
+    p.ticket = ticket;
     if (p.nsub) M3B_TRY(launch_gemm(p, kEpiAcc, true, parts, st));
   }
   return M3B_OK;
