@@ -32,7 +32,6 @@ def _dense(t):
     return True
 
 
-@torch.no_grad()
 def clip_grads(grads: Iterable[torch.Tensor], max_norm: float, norm_type: float = 2.0,
                out: Optional[Iterable[torch.Tensor]] = None) -> torch.Tensor:
     """Clip `grads` by their global norm; returns the norm before clipping (fp32, on their device).

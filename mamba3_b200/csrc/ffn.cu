@@ -221,7 +221,7 @@ int forward(const m3b_gated_ffn_args* a, void* workspace, size_t* need, bool run
   const GemmOperand act = act_operand(a, a->saved_act);
   const bool pair = d.M > 128;
 
-  GemmParams p = params(d, a, pair ? 256 : 128);
+  GemmParams p = params(d, a, pair ? gemm_columns(d.M, 2 * (int64_t)d.F) : 128);
   GemmSub& s = p.sub[0];
   p.nsub = 1;
   s.M = (int)d.M;
@@ -323,7 +323,7 @@ int backward(const m3b_gated_ffn_args* a, void* workspace, size_t* need, bool ru
   if (!run) return M3B_OK;
   M3B_TRY(launch_pack(packs, a->dtype, st));
   {  // da -> dg, du
-    GemmParams p = params(d, a, 256);
+    GemmParams p = params(d, a, gemm_columns(d.M, d.F));
     GemmSub& s = p.sub[0];
     p.nsub = 1;
     M3B_MAP(&s.a[0], dy, false, 128, d.f16);

@@ -133,6 +133,10 @@ int gemm_map(CUtensorMap* m, const GemmOperand& o, bool mn_major, int box_rows, 
               (long long)o.rows, (long long)o.cols, (long long)o.ld, o.planes, (int)r);
 }
 
+int gemm_columns(int64_t M, int64_t N) {
+  return ((M + 255) / 256) * ((N + 127) / 128) <= num_sms() / 2 ? 128 : 256;
+}
+
 size_t plan_gemm(GemmParams& p, int epi, bool pair) {
   const int tile_m = gemm_tile_m(pair), tile_n = epi == kEpiGlu ? p.bn / 2 : p.bn;
   const double workers = pair ? num_sms() / 2 : num_sms();

@@ -277,25 +277,29 @@ __device__ __forceinline__ void put32(uint8_t* box, const GemmOut& o, const Gemm
   }
 }
 
-// 32 columns of a following product's operand: a 16-bit type, or the planes of fp32 values.
+// 32 columns of a following product's operand: a 16-bit type, or the planes of fp32 values (each plane
+// takes the upper halves and leaves the remainders; a value that is not finite lies in the first alone).
 template <bool PLANES>
 __device__ __forceinline__ void put_operand(uint8_t* box, const GemmOut& o, const GemmRows& rows, int col, int N,
-                                            const float (&v)[32]) {
+                                            float (&v)[32]) {
   uint16_t* base = static_cast<uint16_t*>(o.p);
-  uint32_t w[16];
   if constexpr (!PLANES) {
+    uint32_t w[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) w[i] = pack16(v[2 * i], v[2 * i + 1], o.kind == kOutF16);
     put16(box, o, base, rows, col, N, w);
   } else {
 #pragma unroll 1
     for (int pl = 0; pl < 3; ++pl, base += o.plane) {
+      uint32_t w[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        uint16_t a[3], b[3];
-        split_planes(v[2 * i], a);
-        split_planes(v[2 * i + 1], b);
-        w[i] = (pl == 0 ? a[0] : pl == 1 ? a[1] : a[2]) | (uint32_t)(pl == 0 ? b[0] : pl == 1 ? b[1] : b[2]) << 16;
+      for (int i = 0; i < 32; ++i) {
+        const uint32_t b = __float_as_uint(v[i]);
+        const bool fin = (b & 0x7f800000u) != 0x7f800000u;
+        const uint32_t top = v[i] != v[i] ? 0x7fffu : b >> 16;  // a NaN whose set bits are all below stays one
+        v[i] = fin ? v[i] - __uint_as_float(b & 0xffff0000u) : 0.f;
+        if (i & 1) w[i >> 1] |= top << 16;
+        else w[i >> 1] = top;
       }
       put16(box, o, base, rows, col, N, w);
     }
@@ -854,7 +858,7 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
           const int col = job.nt * bn + c;
           if (col >= s.N) return;
           // 16-bit results are packed as they come: two packed arrays instead of two of 32
-          float dg[PLANES ? 32 : 8], du[PLANES ? 32 : 8];
+          float dg[8], du[PLANES ? 32 : 8];
           uint32_t wg[16], wu[16];
 #pragma unroll
           for (int h = 0; h < 4; ++h, ++gu_used) {
@@ -870,9 +874,10 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
               const float g = (i & 3) == 0 ? gq.x : (i & 3) == 1 ? gq.y : (i & 3) == 2 ? gq.z : gq.w;
               const float u = (i & 3) == 0 ? uq.x : (i & 3) == 1 ? uq.y : (i & 3) == 2 ? uq.z : uq.w;
               const float sg = sigmoid_fast(g), ds = d[8 * h + i] * s.alpha * sg;
-              const int k = PLANES ? 8 * h + i : i;
-              dg[k] = ds * u * fmaf(g, 1.f - sg, 1.f);
-              du[k] = ds * g;
+              du[PLANES ? 8 * h + i : i] = ds * g;
+              const float x = ds * u * fmaf(g, 1.f - sg, 1.f);
+              if constexpr (PLANES) d[8 * h + i] = x;
+              else dg[i] = x;
             }
             if constexpr (!PLANES) {
 #pragma unroll
@@ -883,7 +888,7 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
             }
           }
           if constexpr (PLANES) {
-            put_operand<true>(box, s.out, rows, col, s.N, dg);
+            put_operand<true>(box, s.out, rows, col, s.N, d);
             put_operand<true>(box, s.out2, rows, col, s.N, du);
           } else {
             put16(box, s.out, static_cast<uint16_t*>(s.out.p), rows, col, s.N, wg);
@@ -1068,6 +1073,10 @@ size_t plan_gemm(GemmParams& p, int epi, bool pair);
 // lengths draws them from p.ticket (a zeroed int; null deals them in turn).
 int launch_gemm(GemmParams& p, int epi, bool pair, void* parts, cudaStream_t st);
 inline int gemm_tile_m(bool pair) { return pair ? 256 : 128; }
+// Accumulator columns of a CTA pair's tiles for M x N columns (GLU: both halves): 256, or 128 where that
+// still leaves every tile a pair of its own.  A tile of 128 takes as long over K (0.34 us a block against
+// 0.36) but half as long on its way out (777 x 897 fp32: dg and du 60 us with 16 tiles, 38 us with 32).
+int gemm_columns(int64_t M, int64_t N);
 // Rows of B per tensor-map box for `bn` accumulator columns.
 inline int gemm_box_b(bool pair, int bn, int epi) { return epi == kEpiGlu || pair ? bn / 2 : bn; }
 

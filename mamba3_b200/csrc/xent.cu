@@ -274,7 +274,7 @@ int forward(const m3b_linear_xent_args* a, void* workspace, size_t* need, bool r
   const Dims d(a);
   Carve ws(workspace);
   const bool pair = d.T > 128;
-  const int bn = pair ? 256 : 128;
+  const int bn = pair ? gemm_columns(d.T, d.V) : 128;
   const int nt = (d.V + bn - 1) / bn;
   float* target_logit = static_cast<float*>(ws.take((size_t)d.Tp * 4));
   float* row_loss = static_cast<float*>(ws.take((size_t)d.Tp * 4));
@@ -414,8 +414,9 @@ int backward(const m3b_linear_xent_args* a, void* workspace, size_t* need, bool 
       GemmParams p = base;
       GemmSub& g = p.sub[0];
       p.nsub = 1;
+      p.bn = gemm_columns(d.T, n);
       M3B_MAP(&g.a[0], h, false, 128, d.f16);
-      M3B_MAP(&g.b[0], wp, false, gemm_box_b(true, bn, kEpiDlogit), d.f16);
+      M3B_MAP(&g.b[0], wp, false, gemm_box_b(true, p.bn, kEpiDlogit), d.f16);
       g.M = (int)d.T;
       g.m_dyn = 1;
       g.N = (int)n;
