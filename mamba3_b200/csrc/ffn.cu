@@ -221,7 +221,7 @@ int forward(const m3b_gated_ffn_args* a, void* workspace, size_t* need, bool run
   const GemmOperand act = act_operand(a, a->saved_act);
   const bool pair = d.M > 128;
 
-  GemmParams p = params(d, a, pair ? gemm_columns(d.M, 2 * (int64_t)d.F) : 128);
+  GemmParams p = params(d, a, pair ? gemm_columns(d.M, 2 * (int64_t)d.F, d.f32) : 128);
   GemmSub& s = p.sub[0];
   p.nsub = 1;
   s.M = (int)d.M;
@@ -235,7 +235,7 @@ int forward(const m3b_gated_ffn_args* a, void* workspace, size_t* need, bool run
   p.gu_ld4 = up(d.F, 32) / 4;
   plan_gemm(p, kEpiGlu, pair);
 
-  GemmParams q = params(d, a, pair ? 256 : 64);
+  GemmParams q = params(d, a, pair ? (d.f32 ? 128 : 256) : 64);
   GemmSub& t = q.sub[0];
   q.nsub = 1;
   t.M = (int)d.M;
@@ -288,7 +288,7 @@ int backward(const m3b_gated_ffn_args* a, void* workspace, size_t* need, bool ru
   int* ticket = static_cast<int*>(ws.take(4));
 
   // dx and the three weight gradients, side by side
-  GemmParams q = params(d, a, 256);
+  GemmParams q = params(d, a, d.f32 ? 128 : 256);
   q.ticket = ticket;
   struct Product {
     void* out;
@@ -323,7 +323,7 @@ int backward(const m3b_gated_ffn_args* a, void* workspace, size_t* need, bool ru
   if (!run) return M3B_OK;
   M3B_TRY(launch_pack(packs, a->dtype, st));
   {  // da -> dg, du
-    GemmParams p = params(d, a, gemm_columns(d.M, d.F));
+    GemmParams p = params(d, a, gemm_columns(d.M, d.F, d.f32));
     GemmSub& s = p.sub[0];
     p.nsub = 1;
     M3B_MAP(&s.a[0], dy, false, 128, d.f16);

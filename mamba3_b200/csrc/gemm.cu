@@ -42,10 +42,7 @@ using KernelFn = void (*)(const GemmParams);
 
 template <int EPI>
 KernelFn pick(bool pair, bool planes) {
-  // results of these leave as operands of a following product
-  constexpr bool kOperand = EPI == kEpiGlu || EPI == kEpiDglu || EPI == kEpiDlogit;
-  if constexpr (kOperand)
-    if (planes) return pair ? (KernelFn)gemm_kernel<EPI, true, true> : (KernelFn)gemm_kernel<EPI, false, true>;
+  if (planes) return pair ? (KernelFn)gemm_kernel<EPI, true, true> : (KernelFn)gemm_kernel<EPI, false, true>;
   return pair ? (KernelFn)gemm_kernel<EPI, true, false> : (KernelFn)gemm_kernel<EPI, false, false>;
 }
 
@@ -133,8 +130,8 @@ int gemm_map(CUtensorMap* m, const GemmOperand& o, bool mn_major, int box_rows, 
               (long long)o.rows, (long long)o.cols, (long long)o.ld, o.planes, (int)r);
 }
 
-int gemm_columns(int64_t M, int64_t N) {
-  return ((M + 255) / 256) * ((N + 127) / 128) <= num_sms() / 2 ? 128 : 256;
+int gemm_columns(int64_t M, int64_t N, bool planes) {
+  return planes || ((M + 255) / 256) * ((N + 127) / 128) <= num_sms() / 2 ? 128 : 256;
 }
 
 size_t plan_gemm(GemmParams& p, int epi, bool pair) {

@@ -9,7 +9,10 @@
 //   descriptor reads it transposed.
 // * fp32 operands travel as three bf16 planes whose sum is the value exactly (each plane takes
 //   the next 8 significant bits by truncation).  The product runs over the six plane pairs with
-//   2^-16 or more of the leading one's weight, smallest first; the dropped pairs are below 2^-24.
+//   2^-16 or more of the leading one's weight, smallest first; the dropped pairs are below 2^-24.  The
+//   tensor core cuts its sums off instead of rounding them, a bias of half a step per addition that
+//   fp32 results would show (3e-6 of a 323 x 897 product): so every kGmGroup K blocks are a sum of
+//   their own, and the epilogue adds them, rounded, in registers (8e-7).
 // * A launch holds up to four products ("subs"), so that products that are too small to fill the
 //   GPU run side by side, and a product has up to two K segments with operands of their own.
 // * Row or K counts may come from device memory (`dyn`): the loss drops ignored tokens without
@@ -38,6 +41,7 @@ constexpr int kGmThreads = 320;
 constexpr int kGmSubs = 4;      // products of a launch at most
 constexpr int kGmQueue = 4;     // drawn jobs that the producer may be ahead of the epilogue
 constexpr int kGmBK = 64;
+constexpr int kGmGroup = 4;     // K blocks of fp32 operands summed in one accumulator
 constexpr uint32_t kGmStageA = 128 * kGmBK * 2;     // 16 KB
 constexpr uint32_t kGmStage = 2 * kGmStageA;        // + B: at most 128 rows of 64
 constexpr uint32_t kGmBox = 32 * 128;               // staging of an epilogue warp: 32 rows x 32 fp32
@@ -535,6 +539,10 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
     if (lane == 0) gm_arrive_first<PAIR>(&jempty[slot]);
     return o;
   };
+  auto group_end = [](const GemmJob& j, int i) {
+    const int e = (i / (6 * kGmGroup) + 1) * 6 * kGmGroup;
+    return e < j.ke ? e : j.ke;
+  };
   // The first CTA's producer, one thread: job n into both CTAs' queues.
   auto pass_on = [&](uint32_t n, const GemmJob& j) {
     const uint32_t slot = (n - 1) % kGmQueue;
@@ -579,14 +587,23 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
       // B rows of this CTA; the gated product stages bn / 2 gate and bn / 2 up rows (paired: the
       // first CTA holds the gate's, the second the up's)
       const int brow = EPI == kEpiGlu ? job.nt * (bn / 2) : job.nt * bn + (int)rank * brows;
-      int pass = job.kb / (nks > 0 ? nks : 1), r = job.kb - pass * nks;
+      // K block r; with planes, the pairs of a group of blocks from g0 on one after the other
+      int r = job.kb, pass = 5, g0 = 0, gn = 1;
+      if constexpr (PLANES) {
+        if (job.kb < job.ke) {
+          const int g = job.kb / (6 * kGmGroup), in = job.kb - g * 6 * kGmGroup;
+          g0 = g * kGmGroup;
+          gn = nks - g0 < kGmGroup ? nks - g0 : kGmGroup;
+          pass = in / gn;
+          r = g0 + in - pass * gn;
+        }
+      }
       for (int i = job.kb; i < job.ke; ++i, ++it) {
         ok = __all_sync(0xffffffffu, gm_wait(&empty[st], ph, p.wait_ns));
         if (!ok) break;
         const int seg = r >= nk0 ? 1 : 0, k = (seg ? r - nk0 : r) * kGmBK;
         // plane pairs, smallest first: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0)
-        const int pp = (pass + 6 - p.npass) * 4;
-        const int pa = (0x001102 >> pp) & 3, pb = (0x010120 >> pp) & 3;
+        const int pa = PLANES ? (0x001102 >> (4 * pass)) & 3 : 0, pb = PLANES ? (0x010120 >> (4 * pass)) & 3 : 0;
         const uint32_t dA = ring + st * kGmStage, dB = dA + kGmStageA, fb = full0 + st * 8;
         const CUtensorMap *ma = &s.a[seg], *mb = &s.b[EPI == kEpiGlu ? (PAIR ? (int)rank : 0) : seg];
         if (leader) {
@@ -606,9 +623,16 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
             if constexpr (EPI == kEpiGlu && !PAIR) gm_load<PAIR>(dB + (uint32_t)(bn / 2) * 128u, &s.b[1], k, brow, pb, fb);
           }
         }
-        if (++r == nks) {
-          r = 0;
-          ++pass;
+        ++r;
+        if constexpr (PLANES) {
+          if (r == g0 + gn) {
+            if (++pass == 6) {
+              pass = 0;
+              g0 += kGmGroup;
+              gn = nks - g0 < kGmGroup ? nks - g0 : kGmGroup;
+            }
+            r = g0;
+          }
         }
         if (++st == kGmStages) {
           st = 0;
@@ -637,46 +661,53 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
     if (rank == 0) {
       const bool leader = elect_one();
       const uint32_t ring = smem_u32(sm) >> 4;
-      uint32_t st = 0, ph = 0, sc = 0;
+      uint32_t st = 0, ph = 0, sc = 0, jn = 0;
       bool ok = true;
       GemmJob job = next_job(0);
-      for (; ok && job.sub >= 0; ++sc, job = next_job(sc)) {
+      for (; ok && job.sub >= 0; job = next_job(++jn)) {
         const GemmSub& s = p.sub[job.sub];
-        const uint32_t acc = sc & 1;
-        ok = __all_sync(0xffffffffu, gm_wait(&acce[acc], ((sc >> 1) & 1) ^ 1, p.wait_ns));
-        if (!ok) break;
-        tc_fence_after();
         uint32_t idesc = idesc_bf16(kTileM, bn, s.a_mn != 0, s.b_mn != 0);
         if (p.f16) idesc &= ~((1u << 7) | (1u << 10));
-        const uint32_t dt = tbase + acc * 256;
         // descriptors: the address in 16-byte units in the low bits, then the leading offset (MN-major:
         // 8192 bytes between 64-column blocks); a step of 16 K values is 32 bytes along a swizzled row, or
         // two 8-row groups of an MN-major tile
         const uint32_t sa = s.a_mn ? 128 : 2, sb = s.b_mn ? 128 : 2;
         const uint32_t la = (s.a_mn ? 8192u >> 4 : 1u) << 16, lb = (s.b_mn ? 8192u >> 4 : 1u) << 16;
         const uint32_t hi = (1024u >> 4) | (1u << 14) | (2u << 29);
-        uint32_t on = 0;
-        for (int i = job.kb; i < job.ke; ++i) {
-          ok = __all_sync(0xffffffffu, gm_wait(&full[st], ph, p.wait_ns));
+        int i = job.kb;
+        do {  // one accumulator a job, with planes one a group of K blocks
+          const int e = PLANES ? group_end(job, i) : job.ke;
+          if (PLANES && i == e) break;
+          const uint32_t acc = sc & 1;
+          ok = __all_sync(0xffffffffu, gm_wait(&acce[acc], ((sc >> 1) & 1) ^ 1, p.wait_ns));
           if (!ok) break;
           tc_fence_after();
-          const uint32_t a0 = (ring + st * (kGmStage >> 4)) | la, b0 = (ring + st * (kGmStage >> 4) + (kGmStageA >> 4)) | lb;
-          if (leader) {
+          const uint32_t dt = tbase + acc * 256;
+          uint32_t on = 0;
+          for (; i < e; ++i) {
+            ok = __all_sync(0xffffffffu, gm_wait(&full[st], ph, p.wait_ns));
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t a0 = (ring + st * (kGmStage >> 4)) | la;
+            const uint32_t b0 = (ring + st * (kGmStage >> 4) + (kGmStageA >> 4)) | lb;
+            if (leader) {
 #pragma unroll
-            for (uint32_t kk = 0; kk < kGmBK / 16; ++kk) {
-              const uint64_t da = gm_desc(a0 + kk * sa, hi), db = gm_desc(b0 + kk * sb, hi);
-              if constexpr (PAIR) umma_bf16_pair(dt, da, db, idesc, kk == 0 ? on : 1u);
-              else umma_bf16(dt, da, db, idesc, kk == 0 ? on : 1u);
+              for (uint32_t kk = 0; kk < kGmBK / 16; ++kk) {
+                const uint64_t da = gm_desc(a0 + kk * sa, hi), db = gm_desc(b0 + kk * sb, hi);
+                if constexpr (PAIR) umma_bf16_pair(dt, da, db, idesc, kk == 0 ? on : 1u);
+                else umma_bf16(dt, da, db, idesc, kk == 0 ? on : 1u);
+              }
+              gm_commit<PAIR>(&empty[st]);  // the stage is free, in both CTAs, once these MMAs have read it
             }
-            gm_commit<PAIR>(&empty[st]);  // the stage is free, in both CTAs, once these MMAs have read it
+            on = 1;
+            if (++st == kGmStages) {
+              st = 0;
+              ph ^= 1;
+            }
           }
-          on = 1;
-          if (++st == kGmStages) {
-            st = 0;
-            ph ^= 1;
-          }
-        }
-        if (ok && leader) gm_commit<PAIR>(&accf[acc]);
+          if (ok && leader) gm_commit<PAIR>(&accf[acc]);
+          ++sc;
+        } while (PLANES && ok && i < job.ke);
       }
       if (!ok || job.sub == -2) give_up();
     }
@@ -719,32 +750,72 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
     };
     if constexpr (EPI == kEpiDglu)
       for (int i = 0; i < kGuSlots; ++i) gu_send();
+    uint32_t jn = 0;
     GemmJob job = next_job(0);
-    for (; job.sub >= 0; ++sc, job = next_job(sc)) {
+    for (; job.sub >= 0; job = next_job(++jn)) {
       const GemmSub& s = p.sub[job.sub];
-      const int acc = (int)(sc & 1);
       const int64_t grow = (int64_t)job.mt * kTileM + (int64_t)rank * 128 + q * 32 + lane;
       const int M = sched.rows(s);
       const bool rok = grow < M;  // grow is the row of this thread
       const bool none = job.ke == job.kb;  // no K at all: the sum is zero
       const int cfirst = half * (bn / 2), clast = cfirst + bn / 2;
-      if (!__all_sync(0xffffffffu, gm_wait(&accf[acc], (sc >> 1) & 1, p.wait_ns))) {
-        give_up();
-        break;
-      }
-      tc_fence_after();
-      const uint32_t tc = tl + (uint32_t)(acc * 256);
+      // waits for the next accumulator; tc: its columns of this warp's lanes
+      uint32_t tc = 0;
+      auto await = [&]() {
+        const uint32_t acc = sc & 1;
+        if (!__all_sync(0xffffffffu, gm_wait(&accf[acc], (sc >> 1) & 1, p.wait_ns))) return false;
+        tc_fence_after();
+        tc = tl + acc * 256;
+        return true;
+      };
       auto release = [&]() {
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) gm_arrive_first<PAIR>(&acce[acc]);
+        if (lane == 0) gm_arrive_first<PAIR>(&acce[sc & 1]);
+        ++sc;
       };
+      float part[2][32];  // with planes: 64 columns (GLU: 32 of either half), summed over the groups
+      if constexpr (PLANES) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) part[k][i] = 0.f;
+        bool fine = true;
+        for (int i = job.kb; i < job.ke; i = group_end(job, i)) {
+          fine = await();
+          if (!fine) break;
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            if (k == 1 && EPI != kEpiGlu && bn < 128) break;
+            uint32_t ra[32];
+            __syncwarp();
+            tmem_ld32_async(tc + (EPI == kEpiGlu ? half * (bn / 4) + k * (bn / 2) : cfirst + 32 * k), ra);
+            tmem_wait_ld(ra);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) part[k][e] += __uint_as_float(ra[e]);
+          }
+          release();
+        }
+        if (!fine) {
+          give_up();
+          break;
+        }
+      } else if (!await()) {
+        give_up();
+        break;
+      }
       uint8_t* box = sm + kGmBoxOff + (uint32_t)(warp - 2) * kGmBox;
       GemmRows rows{(int64_t)job.mt * kTileM + (int64_t)rank * 128 + q * 32, M, nullptr};
       // Columns [c0, c1) of this warp, 32 at a time.  The load is waited for at once: a register that
       // an asynchronous load still writes must not be moved or spilled, and the second warp of the
       // same lanes covers the wait.
       auto columns = [&](int c0, int c1, auto&& f) {
+        if constexpr (PLANES) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            if (c0 + 32 * k < c1) f(c0 + 32 * k, part[k]);
+          return;
+        }
         for (int c = c0; c < c1; c += 32) {
           uint32_t ra[32];
           __syncwarp();
@@ -824,15 +895,20 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
         const int hb = bn / 2;
         for (int c = half * (hb / 2); c < (half + 1) * (hb / 2); c += 32) {
           const int col = job.nt * hb + c;
-          uint32_t rg[32], ru[32];
-          __syncwarp();
-          tmem_ld32_async(tc + c, rg);
-          tmem_ld32_async(tc + hb + c, ru);
-          tmem_wait_ld(rg, ru);
-          if (col >= s.N) continue;
           float g[32], u[32];
+          if constexpr (PLANES) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) g[i] = __uint_as_float(rg[i]), u[i] = __uint_as_float(ru[i]);
+            for (int i = 0; i < 32; ++i) g[i] = part[0][i], u[i] = part[1][i];
+          } else {
+            uint32_t rg[32], ru[32];
+            __syncwarp();
+            tmem_ld32_async(tc + c, rg);
+            tmem_ld32_async(tc + hb + c, ru);
+            tmem_wait_ld(rg, ru);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) g[i] = __uint_as_float(rg[i]), u[i] = __uint_as_float(ru[i]);
+          }
+          if (col >= s.N) continue;
           if (s.bias) {
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
@@ -948,7 +1024,7 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
           put_operand<PLANES>(box, s.out, rows, col, s.N, v);
         });
       }
-      release();
+      if constexpr (!PLANES) release();
     }
     if (job.sub == -2) give_up();
     if constexpr (EPI == kEpiDglu)  // an aborted run leaves once its copies have landed
@@ -1076,7 +1152,8 @@ inline int gemm_tile_m(bool pair) { return pair ? 256 : 128; }
 // Accumulator columns of a CTA pair's tiles for M x N columns (GLU: both halves): 256, or 128 where that
 // still leaves every tile a pair of its own.  A tile of 128 takes as long over K (0.34 us a block against
 // 0.36) but half as long on its way out (777 x 897 fp32: dg and du 60 us with 16 tiles, 38 us with 32).
-int gemm_columns(int64_t M, int64_t N);
+// Planes: 128, whose 64 columns a thread can sum in registers.
+int gemm_columns(int64_t M, int64_t N, bool planes);
 // Rows of B per tensor-map box for `bn` accumulator columns.
 inline int gemm_box_b(bool pair, int bn, int epi) { return epi == kEpiGlu || pair ? bn / 2 : bn; }
 

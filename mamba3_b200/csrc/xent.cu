@@ -274,7 +274,7 @@ int forward(const m3b_linear_xent_args* a, void* workspace, size_t* need, bool r
   const Dims d(a);
   Carve ws(workspace);
   const bool pair = d.T > 128;
-  const int bn = pair ? gemm_columns(d.T, d.V) : 128;
+  const int bn = pair ? gemm_columns(d.T, d.V, d.f32) : d.f32 ? 64 : 128;
   const int nt = (d.V + bn - 1) / bn;
   float* target_logit = static_cast<float*>(ws.take((size_t)d.Tp * 4));
   float* row_loss = static_cast<float*>(ws.take((size_t)d.Tp * 4));
@@ -331,7 +331,7 @@ int backward(const m3b_linear_xent_args* a, void* workspace, size_t* need, bool 
   const Dims d(a);
   Carve ws(workspace);
   const int64_t cols = piece_cols(d), ldz = up(cols, 8);
-  const int bn = 256, pieces = (int)((d.V + cols - 1) / cols);
+  const int bn = d.f32 ? 128 : 256, pieces = (int)((d.V + cols - 1) / cols);
   int rc = M3B_OK;
   uint16_t* dz = static_cast<uint16_t*>(ws.take((size_t)d.np * d.Tp * ldz * 2));
   float* acc = nullptr;
@@ -414,7 +414,7 @@ int backward(const m3b_linear_xent_args* a, void* workspace, size_t* need, bool 
       GemmParams p = base;
       GemmSub& g = p.sub[0];
       p.nsub = 1;
-      p.bn = gemm_columns(d.T, n);
+      p.bn = gemm_columns(d.T, n, d.f32);
       M3B_MAP(&g.a[0], h, false, 128, d.f16);
       M3B_MAP(&g.b[0], wp, false, gemm_box_b(true, p.bn, kEpiDlogit), d.f16);
       g.M = (int)d.T;
