@@ -19,6 +19,8 @@ namespace m3b {
 
 namespace {
 
+constexpr int kMaxWidth = (1 << 22) - 64;  // column blocks of the bias gradients' grid
+
 inline int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 
 struct Carve {
@@ -92,8 +94,8 @@ __global__ void __launch_bounds__(256) colsum_kernel(const __grid_constant__ Sum
   pdl_wait_primary();
   pdl_launch_dependents();
   const auto& m = a.s[blockIdx.z];
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = blockIdx.x * 64 + 2 * lane;
-  const int64_t r0 = (int64_t)blockIdx.y * kSumRows, r1 = r0 + kSumRows < a.rows ? r0 + kSumRows : a.rows;
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = blockIdx.y * 64 + 2 * lane;
+  const int64_t r0 = (int64_t)blockIdx.x * kSumRows, r1 = r0 + kSumRows < a.rows ? r0 + kSumRows : a.rows;
   float2 s = make_float2(0.f, 0.f);
   if (c < m.cols) {
 #pragma unroll 8
@@ -111,7 +113,7 @@ __global__ void __launch_bounds__(256) colsum_kernel(const __grid_constant__ Sum
   __syncthreads();
   if (w != 0 || c >= m.cols) return;
   for (int k = 1; k < 8; ++k) s.x += sm[k][lane].x, s.y += sm[k][lane].y;
-  float* o = m.part + (int64_t)blockIdx.y * m.cols + c;
+  float* o = m.part + (int64_t)blockIdx.x * m.cols + c;
   o[0] = s.x;
   if (c + 1 < m.cols) o[1] = s.y;
 }
@@ -133,17 +135,16 @@ __global__ void __launch_bounds__(256) colsum_finish_kernel(const __grid_constan
 }
 int colsums(const Sums& a, cudaStream_t st) {
   if (a.n == 0) return M3B_OK;
-  if (a.chunks > 65535) return fail(M3B_ERR_UNSUPPORTED, "gated_ffn_bwd: bias gradients over more than 8,388,480 rows");
   int cols = 0;
   for (int i = 0; i < a.n; ++i) cols = a.s[i].cols > cols ? a.s[i].cols : cols;
-  const int rc = launch_dependent(colsum_kernel, dim3((cols + 63) / 64, a.chunks, a.n), 256, st, a);
+  const int rc = launch_dependent(colsum_kernel, dim3(a.chunks, (cols + 63) / 64, a.n), 256, st, a);
   return rc != M3B_OK ? rc : launch_dependent(colsum_finish_kernel, dim3((cols + 31) / 32, a.n), 256, st, a);
 }
 
 int check(const m3b_gated_ffn_args* a, bool bwd) {
   if (!a) return fail(M3B_ERR_INVALID_ARG, "gated_ffn: null args");
   if (a->rows < 0 || a->d_model <= 0 || a->d_ff <= 0) return fail(M3B_ERR_INVALID_ARG, "gated_ffn: bad sizes");
-  if (a->rows > (int64_t(1) << 31) - 512 || a->d_model > (1 << 24) || a->d_ff > (1 << 24))
+  if (a->rows > (int64_t(1) << 31) - 512 || a->d_model > kMaxWidth || a->d_ff > kMaxWidth)
     return fail(M3B_ERR_INVALID_ARG, "gated_ffn: sizes past the kernels' limits");
   if (a->dtype != M3B_F32 && a->dtype != M3B_BF16 && a->dtype != M3B_F16)
     return fail(M3B_ERR_INVALID_ARG, "gated_ffn: dtype");

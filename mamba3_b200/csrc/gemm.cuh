@@ -122,6 +122,7 @@ struct GemmParams {
   int64_t part_ld;
   const float* lse2;       // log2 of the row's sum of exponentials
   const float* roww;       // weight per row or null
+  float shift;             // softmax - one-hot times 2^shift
   int col0;                // first vocabulary column of this piece
   int* err;
   uint64_t wait_ns;
@@ -1001,7 +1002,8 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
         if (rok) p.part[(int64_t)(job.nt * 2 + half) * p.part_ld + grow] = make_float2(m, sum);
       } else {
         const int tgt = rok ? p.target[grow] - p.col0 : -1;
-        const float l2 = rok ? p.lse2[grow] : 0.f, w = rok && p.roww ? p.roww[grow] : 1.f;
+        const float l2 = (rok ? p.lse2[grow] : 0.f) - p.shift, one = ex2_fast(p.shift);
+        const float w = rok && p.roww ? p.roww[grow] : 1.f;
         rows.M = 0x7fffffff;  // rows behind the last kept token are K values of the next products: zero
         columns(cfirst, clast, [&](int c, float (&v)[32]) {
           const int col = job.nt * bn + c;
@@ -1011,7 +1013,7 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
           const int to = tgt - col;
           if (to >= 0 && to < 32) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = to == i ? v[i] - 1.f : v[i];
+            for (int i = 0; i < 32; ++i) v[i] = to == i ? v[i] - one : v[i];
           }
           if (p.roww) {
 #pragma unroll

@@ -350,6 +350,9 @@ int backward(const m3b_linear_xent_args* a, void* workspace, size_t* need, bool 
   base.f16 = d.f16;
   base.dyn = s.count;
   base.err = a->err;
+  // fp16 has nothing between 0 and 6e-8, where most of a large vocabulary's probabilities may lie: they are
+  // kept times 2^15 (at most 32768).  With weights per row the range is the caller's.
+  base.shift = d.f16 && a->reduction != 0 ? 15.f : 0.f;
 
   // the two gradients' shares of the piece of n columns from c0 on, side by side
   auto gradients = [&](GemmParams& p, int64_t c0, int64_t n, const GemmOperand* z, const GemmOperand* wp) {
@@ -359,7 +362,7 @@ int backward(const m3b_linear_xent_args* a, void* workspace, size_t* need, bool 
       g.N = d.D;
       g.nk[0] = K;
       g.b_mn = 1;
-      g.alpha = 1.f;
+      g.alpha = base.shift > 0.f ? 1.f / 32768.f : 1.f;
       if (a->reduction != 0) g.alpha_num = a->dloss;
       if (a->reduction == 1) g.alpha_den = s.count;
       g.out.kind = okind;

@@ -85,7 +85,12 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     w_gate, w_up, w_down = w_gate.contiguous(), w_up.contiguous(), w_down.contiguous()
     scale = float(residual_scale)
     if torch.is_grad_enabled() and any([t.requires_grad for t in ts]):
-        y = _GatedFfn.apply(x2, w_gate, w_up, w_down, b_gate, b_up, b_down, r2, scale)
+        args = [x2, w_gate, w_up, w_down, b_gate, b_up, b_down, r2]
+        if torch.compiler.is_compiling():
+            # one tensor in two places (x as its own residual) is one argument to the tracer, which then
+            # loses one of its two gradients: views keep them apart
+            args = [None if t is None else t.view(t.shape) for t in args]
+        y = _GatedFfn.apply(*args, scale)
     else:
         y = ops.gated_ffn_fwd(x2, w_gate, w_up, w_down, b_gate, b_up, b_down, r2, scale, False)[0]
     return y if y.dim() == x.dim() else y.view(x.shape)

@@ -550,3 +550,133 @@ def test_lm_decode_with_the_fused_mlp():
     out = lm.generate(ids, max_new_tokens=12, temperature=0.0)
     dec = GraphDecoder(lm, 3, 12, compact=False)
     assert torch.equal(dec.generate(ids), out)
+
+
+# ---------------------------------------------------------------------------
+# calls at the edges of what the documentation allows
+# ---------------------------------------------------------------------------
+def test_loss_frozen_weight_or_hidden():
+    from mamba3_b200 import linear_cross_entropy
+
+    h, w, t = loss_inputs(90, 64, 300, torch.bfloat16, 0.2)
+    want = ref.loss(h, w, t, dloss=1.0)
+    a = h.clone().requires_grad_(True)
+    linear_cross_entropy(a, w, t).backward()
+    ref.check(a.grad, want["hidden"], "hidden alone")
+    b = w.clone().requires_grad_(True)
+    linear_cross_entropy(h, b, t).backward()
+    ref.check(b.grad, want["weight"], "weight alone")
+
+
+def test_loss_small_probabilities_in_fp16():
+    """A sure prediction over a large vocabulary: the other 19,999 probabilities are near 2e-9, which fp16 alone
+    would drop, but together they are the whole gradient along what the others share."""
+    from mamba3_b200 import linear_cross_entropy
+
+    n, d, v = 64, 64, 20000
+    h, w, t = loss_inputs(n, d, v, torch.float16)
+    w = (w * 0.02).contiguous()
+    h[:, 0], h[:, 1] = 10.0, 0.0
+    w[:, 0], w[:, 1] = 0.0, 1.0
+    w[7] = 0.0
+    w[7, 0] = 2.0  # the target's logit 20 above the rest: 4e-5 of the mass on all others
+    t.fill_(7)
+    h.requires_grad_(True)
+    (linear_cross_entropy(h, w, t) * 1024.0).backward()
+    p = torch.softmax(h.detach().double() @ w.double().t(), 1)
+    p[:, 7] = 0.0
+    want = 1024.0 * p.sum(1) / n
+    # two roundings to fp16 (the scaled probability, the result) and fp32 logits of 20 and their log-sum
+    err = (2 * 2.0 ** -11 + 8 * 2.0 ** -20) * want
+    assert bool(((h.grad[:, 1].double() - want).abs() <= err).all())
+
+
+def test_ffn_offsets_past_32_bits():
+    """act, g and u, dg and du of more than 2^31 values: the last rows against the plain form, and the weight
+    gradient's sum over all rows through a product with few live rows."""
+    from mamba3_b200 import gated_ffn
+
+    n, d, f = 400_200, 32, 5504
+    x = torch.zeros(n, d, device="cuda", dtype=torch.bfloat16)
+    live = torch.tensor([0, 1, 255, 256, 390_167, 390_168, n - 2, n - 1], device="cuda")  # 2^31 / 5504 = 390,167
+    x[live] = rnd(len(live), d, seed=1, dtype=torch.bfloat16)
+    t = ffn_inputs(1, d, f, torch.bfloat16, False, False)
+    leaves = [v.requires_grad_(True) for v in (x, t["w_gate"], t["w_up"], t["w_down"])]
+    y = gated_ffn(*leaves)
+    dout = torch.zeros_like(y)
+    dout[live] = rnd(len(live), d, seed=2, dtype=torch.bfloat16)
+    grads = torch.autograd.grad(y, leaves, dout)
+    small = dict(t, x=x.detach()[live])
+    want = ffn_want(small, dout=dout[live])
+    ref.check(y[live], want["out"], "out")
+    ref.check(grads[0][live], want["x"], "dx")
+    for g, k in zip(grads[1:], ("w_gate", "w_up", "w_down")):
+        value, bound = want[k]
+        ref.check(g, (value, bound * 2), k)  # the other rows add zeros, in more steps than the bound counts
+    dead = torch.ones(n, dtype=torch.bool, device="cuda")
+    dead[live] = False
+    assert not y[dead].any() and not grads[0][dead].any()
+
+
+def test_loss_offsets_past_32_bits():
+    """softmax - onehot of more than 2^31 values in one piece: the last tokens' gradients."""
+    from mamba3_b200 import linear_cross_entropy
+
+    n, d, v = 1_060_000, 16, 2050
+    h, w, _ = loss_inputs(300, d, v, torch.bfloat16)
+    t = torch.randint(0, v, (n,), device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    big = h.repeat(n // 300 + 1, 1)[:n].contiguous().requires_grad_(True)
+    y = linear_cross_entropy(big, w, t, reduction="sum")
+    dh, = torch.autograd.grad(y, big)
+    for s in (slice(0, 300), slice(n - 300, n)):
+        want = ref.loss(big[s], w, t[s], reduction="sum", dloss=1.0)
+        ref.check(dh[s], want["hidden"], f"rows {s}")
+
+
+def test_clip_offsets_past_32_bits():
+    from mamba3_b200 import clip_grads
+
+    n = (1 << 31) + 8200
+    g = torch.zeros(n, device="cuda", dtype=torch.bfloat16)
+    at = torch.tensor([0, 5, (1 << 31) - 1, 1 << 31, n - 1], device="cuda")
+    g[at] = 2.0
+    norm = clip_grads([g], 1.0)
+    assert abs(norm.item() - math.sqrt(20.0)) < 1e-5
+    want = torch.tensor(2.0 / (math.sqrt(20.0) + 1e-6)).bfloat16().item()
+    assert g[at].tolist() == [want] * 5 and int((g != 0).sum()) == 5
+
+
+def test_operators_under_compile():
+    """As opaque nodes of a traced graph, forward and backward: the eager values."""
+    from mamba3_b200 import gated_ffn, linear_cross_entropy
+
+    t = ffn_inputs(40, 64, 72, torch.bfloat16, False, True)
+    _, w, tg = loss_inputs(40, 64, 200, torch.bfloat16, 0.2)
+
+    def step(x, wg, wu, wd, w):
+        y = gated_ffn(x, wg, wu, wd, residual=x, residual_scale=0.5)
+        return linear_cross_entropy(y, w, tg)
+
+    leaves = [v.clone().requires_grad_(True) for v in (t["x"], t["w_gate"], t["w_up"], t["w_down"], w)]
+    eager = step(*leaves)
+    want = torch.autograd.grad(eager, leaves)
+    got = torch.compile(step, backend="aot_eager")(*leaves)
+    assert torch.equal(got, eager)
+    for a, b in zip(torch.autograd.grad(got, leaves), want):
+        assert torch.equal(a, b)
+
+
+def test_gradients_are_the_same_every_time():
+    """Jobs are drawn in an order that changes from run to run; the sums are not."""
+    from mamba3_b200 import gated_ffn, linear_cross_entropy
+
+    t = ffn_inputs(1000, 256, 520, torch.bfloat16, False, False)
+    h, w, tg = loss_inputs(1000, 256, 5000, torch.bfloat16, 0.3)
+    leaves = [v.requires_grad_(True) for v in t.values()] + [h.requires_grad_(True), w.requires_grad_(True)]
+    first = None
+    for _ in range(5):
+        g = torch.autograd.grad(gated_ffn(*leaves[:4]).float().square().sum() + linear_cross_entropy(*leaves[4:], tg),
+                                leaves)
+        if first is None:
+            first = g
+        assert all(torch.equal(a, b) for a, b in zip(g, first))
