@@ -833,8 +833,13 @@ def _call(fn, what, index, *args):
         check_device_errors(torch.device("cuda", index))
 
 
-def _bytes(n, index):
-    return torch.empty(n, dtype=torch.uint8, device=torch.device("cuda", index))
+def _bytes(n, dev):
+    return torch.empty(n, dtype=torch.uint8, device=dev)
+
+
+def _empty_rows(t):
+    """A contiguous tensor of t's shape and dtype."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 def _rows2d(t, d):
@@ -866,22 +871,28 @@ def _ffn_args(x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual, scale):
     return a
 
 
+def ffn_saved_bytes(x, d_ff):
+    """(m3b_gated_ffn_act_bytes, m3b_gated_ffn_gu_bytes) of x (rows, d_model)."""
+    rows, planes = x.shape[0], 3 if x.dtype == torch.float32 else 1
+    return planes * rows * (-(-d_ff // 8) * 8) * 2, -(-rows // 256) * 256 * (-(-d_ff // 32) * 32) * 8
+
+
 def gated_ffn_fwd(x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual, scale, save):
     """Launch the gated feed-forward; x (rows, d_model), weights and biases contiguous, one dtype.
     Returns (out, act, gu): act and gu are what the backward reads (gu None unless `save`)."""
-    index = x.get_device()
+    index, dev = x.get_device(), x.device
     a = _ffn_args(x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual, scale)
     p = C.byref(a)
     L = lib()
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    n = L.m3b_gated_ffn_act_bytes(p)
-    gu = _bytes(L.m3b_gated_ffn_gu_bytes(p), index) if save else None
+    out = _empty_rows(x)
+    n, n_gu = ffn_saved_bytes(x, w_gate.shape[0])
+    gu = _bytes(n_gu, dev) if save else None
     a.saved_gu = _addr(gu)
     need = L.m3b_gated_ffn_fwd_workspace(p)
     # act and the workspace in one allocation where act is not kept
     room = -(-n // 256) * 256
-    act = _bytes(n if save else room + need, index)
-    ws = (_bytes(need, index).data_ptr() if need else None) if save else act.data_ptr() + room
+    act = _bytes(n if save else room + need, dev)
+    ws = (_bytes(need, dev).data_ptr() if need else None) if save else act.data_ptr() + room
     a.saved_act, a.out = act.data_ptr(), out.data_ptr()
     _call(L.m3b_gated_ffn_fwd, "m3b_gated_ffn_fwd", index, p, ws, need)
     return out, act, gu
@@ -893,15 +904,14 @@ def gated_ffn_bwd(x, w_gate, w_up, w_down, b_gate, b_up, b_down, scale, act, gu,
     index = _same_gpu("gated_ffn_bwd", (x, act, dout))
     a = _ffn_args(x, w_gate, w_up, w_down, b_gate, b_up, b_down, None, scale)
     ins = (x, w_gate, w_up, w_down, b_gate, b_up, b_down)
-    g = [torch.empty(t.shape, dtype=x.dtype, device=x.device) if w and t is not None else None
-         for t, w in zip(ins, want)]
+    g = [_empty_rows(t) if w and t is not None else None for t, w in zip(ins, want)]
     a.dout_stride, a.dout = _rows_apart(dout, x.shape[1]), dout.data_ptr()
     a.saved_act, a.saved_gu = act.data_ptr(), gu.data_ptr()
     a.dx, a.dw_gate, a.dw_up, a.dw_down, a.db_gate, a.db_up, a.db_down = [_addr(t) for t in g]
     p = C.byref(a)
     L = lib()
     need = L.m3b_gated_ffn_bwd_workspace(p)
-    ws = _bytes(need, index)
+    ws = _bytes(need, x.device)
     _call(L.m3b_gated_ffn_bwd, "m3b_gated_ffn_bwd", index, p, ws.data_ptr(), need)
     return g
 
@@ -916,21 +926,25 @@ def _xent_args(rows, d, weight, ignore_index, reduction):
     return a
 
 
-def linear_xent_fwd(hidden, weight, target, ignore_index, reduction):
+def linear_xent_fwd(hidden, weight, target, ignore_index, reduction, save=True):
     """Launch the head's cross entropy; hidden (rows, d_model), weight (vocab, d_model) contiguous of
-    the same dtype, target (rows) int64 contiguous.  Returns (loss fp32, saved)."""
+    the same dtype, target (rows) int64 contiguous.  Returns (loss fp32, saved): saved is what the backward
+    reads (nothing of use without `save`)."""
     index = hidden.get_device()
     rows, d = hidden.shape
     a = _xent_args(rows, d, weight, ignore_index, reduction)
     a.hidden_stride, a.hidden, a.target = _rows_apart(hidden, d), hidden.data_ptr(), target.data_ptr()
     p = C.byref(a)
     L = lib()
-    loss = torch.empty((rows,) if reduction == "none" else (), dtype=torch.float32, device=hidden.device)
-    saved = _bytes(max(16, L.m3b_linear_xent_saved(p)), index)
+    dev = hidden.device
+    loss = torch.empty((rows,) if reduction == "none" else (), dtype=torch.float32, device=dev)
+    n, need = max(16, L.m3b_linear_xent_saved(p)), L.m3b_linear_xent_fwd_workspace(p)
+    # what is saved and the workspace in one allocation where nothing is kept
+    room = -(-n // 256) * 256
+    saved = _bytes(n if save else room + need, dev)
+    ws = _bytes(need, dev).data_ptr() if save else saved.data_ptr() + room
     a.saved, a.loss = saved.data_ptr(), loss.data_ptr()
-    need = L.m3b_linear_xent_fwd_workspace(p)
-    ws = _bytes(need, index)
-    _call(L.m3b_linear_xent_fwd, "m3b_linear_xent_fwd", index, p, ws.data_ptr(), need)
+    _call(L.m3b_linear_xent_fwd, "m3b_linear_xent_fwd", index, p, ws, need)
     return loss, saved
 
 
@@ -939,13 +953,13 @@ def linear_xent_bwd(rows, weight, saved, dloss, ignore_index, reduction, want_hi
     index = _same_gpu("linear_xent_bwd", (weight, saved, dloss))
     d = weight.shape[1]
     a = _xent_args(rows, d, weight, ignore_index, reduction)
-    dh = torch.empty(rows, d, dtype=weight.dtype, device=weight.device) if want_hidden else None
+    dh = weight.new_empty(rows, d) if want_hidden else None
     dw = torch.empty_like(weight) if want_weight else None
     a.saved, a.dloss, a.dhidden, a.dweight = saved.data_ptr(), dloss.data_ptr(), _addr(dh), _addr(dw)
     p = C.byref(a)
     L = lib()
     need = L.m3b_linear_xent_bwd_workspace(p)
-    ws = _bytes(need, index)
+    ws = _bytes(need, weight.device)
     _call(L.m3b_linear_xent_bwd, "m3b_linear_xent_bwd", index, p, ws.data_ptr(), need)
     return dh, dw
 
@@ -966,6 +980,6 @@ def grad_clip(ptrs, numel, dtypes, out_ptrs, out_dtypes, max_norm, inf_norm, dev
     a.norm_type, a.max_norm, a.norm = (0 if inf_norm else 2), max_norm, norm.data_ptr()
     L = lib()
     need = L.m3b_grad_clip_workspace(C.byref(a))
-    ws = _bytes(need, dev.index)
+    ws = _bytes(need, dev)
     _call(L.m3b_grad_clip, "m3b_grad_clip", dev.index, C.byref(a), ws.data_ptr(), need)
     return norm

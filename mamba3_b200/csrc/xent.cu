@@ -28,7 +28,7 @@ struct Saved {
   int* row;        // [Tp] where they come from
   int* target;     // [Tp]; -1 behind the last, -2 out of range
   float* lse2;     // [Tp]
-  int* count;      // kept rows
+  int* count;      // kept rows; blocks of the join kernel that are done
   size_t bytes;
 };
 
@@ -60,7 +60,7 @@ Saved saved_of(const m3b_linear_xent_args* a, void* p) {
   s.row = static_cast<int*>(c.take((size_t)d.Tp * 4));
   s.target = static_cast<int*>(c.take((size_t)d.Tp * 4));
   s.lse2 = static_cast<float*>(c.take((size_t)d.Tp * 4));
-  s.count = static_cast<int*>(c.take(4));
+  s.count = static_cast<int*>(c.take(8));
   s.bytes = c.at;
   return s;
 }
@@ -111,7 +111,10 @@ __global__ void __launch_bounds__(1024) keep_kernel(const int64_t* __restrict__ 
     s.row[i] = -1;
     s.target[i] = -1;
   }
-  if (tid == 0) *s.count = total;
+  if (tid == 0) {
+    s.count[0] = total;
+    s.count[1] = 0;
+  }
 }
 
 // One warp per row of the dense operand; rows behind the last kept one are zero up to the tile's end.
@@ -153,16 +156,20 @@ __device__ __forceinline__ void join2(float& m, float& sum, float2 v) {
   sum = sum * ex2_fast(m - top) + v.y * ex2_fast(v.x - top);
   m = top;
 }
+// The block that ends last makes the loss of the rows' losses, summed in a fixed order in fp64; without
+// a reduction each goes to its row's place.
 __global__ void __launch_bounds__(512) join_kernel(const float2* __restrict__ part, int slots, int64_t Tp,
-                                                   const float* __restrict__ target_logit, Saved s,
-                                                   float* __restrict__ row_loss) {
+                                                   const float* __restrict__ target_logit, Saved s, float* row_loss,
+                                                   int reduction, float* __restrict__ loss) {
   __shared__ float2 sm[16][32];
+  __shared__ double sums[16];
+  __shared__ int last;
   pdl_wait_primary();
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int n = *s.count;
-  const int64_t row = (int64_t)blockIdx.x * 32 + lane;
-  if ((int64_t)blockIdx.x * 32 >= n) return;
+  const int n = s.count[0], blocks = n > 0 ? (n + 31) / 32 : 1;
+  const int row = blockIdx.x * 32 + lane;
+  if (blockIdx.x >= blocks) return;
   float m[4] = {-1e30f, -1e30f, -1e30f, -1e30f}, sum[4] = {0.f, 0.f, 0.f, 0.f};
   if (row < n) {
     int k = w;
@@ -179,36 +186,34 @@ __global__ void __launch_bounds__(512) join_kernel(const float2* __restrict__ pa
   }
   sm[w][lane] = make_float2(m[0], sum[0]);
   __syncthreads();
-  if (w != 0 || row >= n) return;
+  if (w == 0 && row < n) {
 #pragma unroll
-  for (int k = 1; k < 16; ++k) join2(m[0], sum[0], sm[k][lane]);
-  const bool ok = s.target[row] >= 0;
-  const float l2 = ok ? m[0] + log2f(sum[0]) : __int_as_float(0x7fffffff);
-  s.lse2[row] = l2;
-  row_loss[row] = l2 * kLn2 - (ok ? target_logit[row] : 0.f);
-}
-
-// The loss from the rows' losses: summed in a fixed order in fp64, or put at the rows' places.
-__global__ void __launch_bounds__(1024) loss_kernel(const float* __restrict__ row_loss, Saved s, int reduction,
-                                                    float* __restrict__ loss) {
-  pdl_wait_primary();
-  const int n = *s.count;
-  if (reduction == 0) {
-    for (int i = threadIdx.x; i < n; i += 1024) loss[s.row[i]] = row_loss[i];
-    return;
+    for (int k = 1; k < 16; ++k) join2(m[0], sum[0], sm[k][lane]);
+    const bool ok = s.target[row] >= 0;
+    const float l2 = ok ? m[0] + log2f(sum[0]) : __int_as_float(0x7fffffff);
+    const float l = l2 * kLn2 - (ok ? target_logit[row] : 0.f);
+    s.lse2[row] = l2;
+    if (reduction == 0) loss[s.row[row]] = l;
+    else __stcg(row_loss + row, l);
+    __threadfence();  // before this block counts as done
   }
-  __shared__ double sm[32];
+  if (reduction == 0) return;
+  __syncthreads();
+  if (threadIdx.x == 0) last = atomicAdd(s.count + 1, 1) == blocks - 1;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
   double x = 0.0;
-  for (int i = threadIdx.x; i < n; i += 1024) x += (double)row_loss[i];
+#pragma unroll 4
+  for (int i = threadIdx.x; i < n; i += 512) x += (double)__ldcg(row_loss + i);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-  if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = x;
+  if (lane == 0) sums[w] = x;
   __syncthreads();
-  if (threadIdx.x < 32) {
-    x = sm[threadIdx.x];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-    if (threadIdx.x == 0) *loss = (float)(reduction == 1 ? x / (double)n : x);
+  if (threadIdx.x == 0) {
+    x = 0.0;
+    for (int k = 0; k < 16; ++k) x += sums[k];
+    *loss = (float)(reduction == 1 ? x / (double)n : x);
   }
 }
 
@@ -315,9 +320,8 @@ int forward(const m3b_linear_xent_args* a, void* workspace, size_t* need, bool r
   M3B_TRY(launch_gemm(p, kEpiLse, pair, nullptr, st));
   if (a->reduction == 0 && cudaMemsetAsync(a->loss, 0, (size_t)d.T * 4, st) != cudaSuccess)
     return check_launch("linear_xent loss");
-  M3B_TRY(launch_dependent(join_kernel, dim3((unsigned)(d.Tp / 32)), 512, st, (const float2*)part, nt * 2, d.Tp,
-                           (const float*)target_logit, s, row_loss));
-  return launch_dependent(loss_kernel, dim3(1), 1024, st, (const float*)row_loss, s, (int)a->reduction, a->loss);
+  return launch_dependent(join_kernel, dim3((unsigned)(d.Tp / 32)), 512, st, (const float2*)part, nt * 2, d.Tp,
+                          (const float*)target_logit, s, row_loss, (int)a->reduction, a->loss);
 }
 
 // Columns of a piece of the vocabulary.

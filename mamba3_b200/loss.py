@@ -16,7 +16,7 @@ from . import _lib, ops
 class _LinearXent(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, target, ignore_index, reduction):
-        loss, saved = ops.linear_xent_fwd(hidden, weight, target, ignore_index, reduction)
+        loss, saved = ops.linear_xent_fwd(hidden, weight, target, ignore_index, reduction, True)
         ctx.save_for_backward(weight, saved)
         ctx.cfg = (hidden.shape[0], ignore_index, reduction)
         return loss
@@ -62,10 +62,13 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     if targets.dtype not in (torch.int64, torch.int32, torch.int16, torch.uint8, torch.int8):
         raise ValueError(f"linear_cross_entropy: integer targets expected, got {targets.dtype}")
     h2 = _lib._rows2d(hidden, weight.shape[1])
-    t1 = (targets if targets.dim() == 1 else targets.reshape(-1)).to(torch.int64).contiguous()
+    t1 = targets if targets.dim() == 1 else targets.reshape(-1)
+    if t1.dtype != torch.int64:
+        t1 = t1.to(torch.int64)
+    t1 = t1.contiguous()
     w = weight.contiguous()
     if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
         loss = _LinearXent.apply(h2, w, t1, int(ignore_index), reduction)
     else:
-        loss = ops.linear_xent_fwd(h2, w, t1, int(ignore_index), reduction)[0]
+        loss = ops.linear_xent_fwd(h2, w, t1, int(ignore_index), reduction, False)[0]
     return loss.view(targets.shape) if reduction == "none" else loss

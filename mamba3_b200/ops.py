@@ -478,14 +478,9 @@ def _gated_ffn_fwd_op(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
     return out, act, _opt(gu, x.device)
 
 
-def _ffn_saved_bytes(x, f):
-    rows, planes = x.shape[0], 3 if x.dtype == torch.float32 else 1
-    return planes * rows * ((f + 7) // 8 * 8) * 2, ((rows + 255) // 256 * 256) * ((f + 31) // 32 * 32) * 8
-
-
 @_gated_ffn_fwd_op.register_fake
 def _(x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual, scale, save):
-    act, gu = _ffn_saved_bytes(x, w_gate.shape[0])
+    act, gu = _lib.ffn_saved_bytes(x, w_gate.shape[0])
     u8 = dict(dtype=torch.uint8, device=x.device)
     return x.new_empty(x.shape), torch.empty(act, **u8), torch.empty(gu if save else 0, **u8)
 
@@ -548,9 +543,10 @@ def _(rows, weight, saved, dloss, ignore_index, reduction, want_hidden, want_wei
             weight.new_empty(weight.shape if want_weight else (0,)))
 
 
-def linear_xent_fwd(hidden, weight, target, ignore_index, reduction):
-    f = _linear_xent_fwd_op if torch.compiler.is_compiling() else _lib.linear_xent_fwd
-    return f(hidden, weight, target, ignore_index, reduction)
+def linear_xent_fwd(hidden, weight, target, ignore_index, reduction, save):
+    if torch.compiler.is_compiling():
+        return _linear_xent_fwd_op(hidden, weight, target, ignore_index, reduction)
+    return _lib.linear_xent_fwd(hidden, weight, target, ignore_index, reduction, save)
 
 
 def linear_xent_bwd(rows, weight, saved, dloss, ignore_index, reduction, want_hidden, want_weight):

@@ -54,6 +54,24 @@ def test_short_workspace_is_refused():
     assert L.m3b_grad_clip(ctypes.byref(c), p, 1 << 12, None) == 1 and b"norm_type" in L.m3b_last_error()
 
 
+@pytest.mark.parametrize("dtype,code", [(torch.float32, 0), (torch.bfloat16, 1), (torch.float16, 2)])
+def test_saved_sizes_agree_with_the_library(dtype, code):
+    L = _lib.lib()
+    for rows, f in ((0, 8), (1, 1), (7, 33), (256, 2112), (257, 100)):
+        a = _lib.GatedFfnArgs(rows, 64, 0, 64, 64, f, code)
+        want = L.m3b_gated_ffn_act_bytes(ctypes.byref(a)), L.m3b_gated_ffn_gu_bytes(ctypes.byref(a))
+        assert _lib.ffn_saved_bytes(torch.empty(rows, 64, dtype=dtype), f) == want
+
+
+def test_sizes_past_the_limits_are_refused():
+    L = _lib.lib()
+    for rows, d, f in ((1 << 31, 64, 64), (4, 1 << 22, 64), (4, 64, 1 << 22)):
+        a = _lib.GatedFfnArgs(rows, d, 0, d, d, f, 1)
+        assert L.m3b_gated_ffn_fwd(ctypes.byref(a), None, 0, None) == 1 and b"limits" in L.m3b_last_error()
+    x = _lib.LinearXentArgs(1 << 31, 64, -100, 64, 1000, 1, 1)
+    assert L.m3b_linear_xent_fwd(ctypes.byref(x), None, 0, None) == 1 and b"limits" in L.m3b_last_error()
+
+
 def test_cpu_tensors_raise():
     x, w = torch.randn(3, 8), torch.randn(16, 8)
     with pytest.raises(m.M3bError, match="CUDA"):
