@@ -213,6 +213,17 @@ __device__ __forceinline__ uint32_t pack16(float a, float b, bool f16) {
   return pack_bf16x2(a, b);
 }
 
+// 1 / (1 + exp(-g)) of a pair: packed arithmetic and the hardware's 2^x and reciprocal (2 and 1 steps);
+// 0 where exp(-g) overflows.
+__device__ __forceinline__ float2 sigmoid2(float2 g) {
+  const float2 t = mul2(g, make_float2(-kLog2e, -kLog2e));
+  const float2 y = fma2(make_float2(ex2_fast(t.x), ex2_fast(t.y)), make_float2(1.f, 1.f), make_float2(1.f, 1.f));
+  float2 r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(y.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(y.y));
+  return r;
+}
+
 // Results leave through a staging box per epilogue warp: a thread owns one row of the accumulator,
 // but a warp's stores should cover whole 32-byte sectors of few rows.  Each thread writes its 32
 // columns into the box (16-byte chunks swizzled by the row, so neither side has bank conflicts) and
@@ -927,7 +938,11 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
             }
           }
 #pragma unroll
-          for (int i = 0; i < 32; ++i) g[i] = g[i] * sigmoid_fast(g[i]) * u[i];
+          for (int i = 0; i < 32; i += 2) {
+            const float2 g2 = make_float2(g[i], g[i + 1]);
+            const float2 a = mul2(mul2(g2, sigmoid2(g2)), make_float2(u[i], u[i + 1]));
+            g[i] = a.x, g[i + 1] = a.y;
+          }
           put_operand<PLANES>(box, s.out, rows, col, s.N, g);
         }
       } else if constexpr (EPI == kEpiDglu) {
@@ -942,19 +957,21 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
             const uint32_t slot = gu_used % kGuSlots;
             if (!__all_sync(0xffffffffu, gm_wait(&gub[slot], (gu_used / kGuSlots) & 1, p.wait_ns))) give_up();
             const float4* run = reinterpret_cast<const float4*>(gus + slot * kGuRun) + lane;
-            const float4 g2[2] = {run[0], run[64]}, u2[2] = {run[32], run[96]};
+            const float4 g4[2] = {run[0], run[64]}, u4[2] = {run[32], run[96]};
             __syncwarp();
             gu_send();
+            const float2 one = make_float2(1.f, 1.f), alpha = make_float2(s.alpha, s.alpha);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float4 gq = g2[i >> 2], uq = u2[i >> 2];
-              const float g = (i & 3) == 0 ? gq.x : (i & 3) == 1 ? gq.y : (i & 3) == 2 ? gq.z : gq.w;
-              const float u = (i & 3) == 0 ? uq.x : (i & 3) == 1 ? uq.y : (i & 3) == 2 ? uq.z : uq.w;
-              const float sg = sigmoid_fast(g), ds = d[8 * h + i] * s.alpha * sg;
-              du[PLANES ? 8 * h + i : i] = ds * g;
-              const float x = ds * u * fmaf(g, 1.f - sg, 1.f);
-              if constexpr (PLANES) d[8 * h + i] = x;
-              else dg[i] = x;
+            for (int i = 0; i < 8; i += 2) {
+              const float4 gq = g4[i >> 2], uq = u4[i >> 2];
+              const float2 g = (i & 2) ? make_float2(gq.z, gq.w) : make_float2(gq.x, gq.y);
+              const float2 u = (i & 2) ? make_float2(uq.z, uq.w) : make_float2(uq.x, uq.y);
+              const float2 sg = sigmoid2(g);
+              const float2 ds = mul2(mul2(make_float2(d[8 * h + i], d[8 * h + i + 1]), alpha), sg);
+              const float2 x = mul2(mul2(ds, u), fma2(g, fma2(sg, make_float2(-1.f, -1.f), one), one)), y = mul2(ds, g);
+              du[(PLANES ? 8 * h : 0) + i] = y.x, du[(PLANES ? 8 * h : 0) + i + 1] = y.y;
+              if constexpr (PLANES) d[8 * h + i] = x.x, d[8 * h + i + 1] = x.y;
+              else dg[i] = x.x, dg[i + 1] = x.y;
             }
             if constexpr (!PLANES) {
 #pragma unroll
@@ -1009,7 +1026,10 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
           const int col = job.nt * bn + c;
           if (col >= s.N) return;
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = ex2_fast(fmaf(v[i], kLog2e, -l2));
+          for (int i = 0; i < 32; i += 2) {
+            const float2 t = fma2(make_float2(v[i], v[i + 1]), make_float2(kLog2e, kLog2e), make_float2(-l2, -l2));
+            v[i] = ex2_fast(t.x), v[i + 1] = ex2_fast(t.y);
+          }
           const int to = tgt - col;
           if (to >= 0 && to < 32) {
 #pragma unroll

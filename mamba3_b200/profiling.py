@@ -117,6 +117,35 @@ def train_step_profile(batch: int = 16, seqlen: int = 4096, rows: int = 24) -> s
     return prof.key_averages().table(sort_by="self_cuda_time_total", row_limit=rows, max_name_column_width=72)
 
 
+def lm_train_step_profile(batch: int = 8, seqlen: int = 2048, rows: int = 30) -> str:
+    """Per-kernel device time of one training step of a 4-layer KulaMambaLM (d_model 768, vocabulary
+    32,000, bf16, random init, synthetic tokens) as the training operators run it: the MLPs by
+    gated_ffn, the loss by linear_cross_entropy without logits, the gradients clipped by their global
+    norm.  From torch's profiler, after three warm-up steps."""
+    import torch
+    from torch.profiler import ProfilerActivity, profile
+
+    from .block import KulaMambaLM
+    from .clip import clip_grad_norm_
+
+    torch.manual_seed(0)
+    lm = KulaMambaLM(vocab_size=32000, d_model=768, n_layers=4, fused_mlp=True).cuda().to(torch.bfloat16).train()
+    ids = torch.randint(0, 32000, (batch, seqlen), device="cuda")
+
+    def step():
+        lm.zero_grad(set_to_none=True)
+        lm(ids, ids, return_logits=False)["loss"].backward()
+        clip_grad_norm_(lm.parameters(), 1.0)
+
+    for _ in range(3):
+        step()
+    torch.cuda.synchronize()
+    with profile(activities=[ProfilerActivity.CUDA]) as prof:
+        step()
+        torch.cuda.synchronize()
+    return prof.key_averages().table(sort_by="self_cuda_time_total", row_limit=rows, max_name_column_width=72)
+
+
 def kernel_workload(case: str, reps: int = 3) -> None:
     """Small fixed workloads for per-kernel captures (ncu -k <kernel> -s <warm-up launches>):
     each runs its kernels once as warm-up and then `reps` times.
@@ -133,6 +162,12 @@ def kernel_workload(case: str, reps: int = 3) -> None:
              chunk_state_kernel, the scan, the tf32 chunk_out_kernel
     in_proj  the config-1 input projection with its B / C 1/rms epilogue: x (16 x 4096, 768) bf16
              -> proj (65536, 3696) (in_proj_kernel)
+    xent     linear_cross_entropy, hidden (4096, 768) x weight (32000, 768) bf16, forward and backward:
+             keep, gather, gemm_kernel (statistics), join, then per piece of the vocabulary gemm_kernel
+             (softmax - onehot) and gemm_kernel (both gradients)
+    ffn      gated_ffn, x (16384, 768) x d_ff 2112 bf16, forward and backward: gemm_kernel four times
+             (gate | up, down, dg and du, dx and the weight gradients)
+    clip     clip_grads of 238 M bf16 gradients in 400 tensors into fp32: norm_kernel, clip_kernel
     decode   config-4 decoding: the 24-layer LM, batch 256, a 16-token prompt, then `reps` token
              steps of the CUDA-graph decoder (every kernel of a token step, in graph order)"""
     import torch
@@ -170,6 +205,30 @@ def kernel_workload(case: str, reps: int = 3) -> None:
                     torch.randn(H, device="cuda", generator=g), r(B, T, H, P, R), r(B, T, H, P, R), f(B, H, P, N),
                     f(B, H, P, N))
             run = lambda: _lib.chunked_ssd_bwd(*args)  # noqa: E731
+        elif case in ("xent", "ffn"):
+            from .ffn import gated_ffn
+            from .loss import linear_cross_entropy
+
+            r = lambda *sh: torch.randn(*sh, device="cuda", generator=g).mul_(sh[-1] ** -0.5).to(torch.bfloat16)  # noqa: E731
+            if case == "xent":
+                leaves = [r(4096, 768) * 28, r(32000, 768) * 2.5]
+                t = torch.randint(0, 32000, (4096,), device="cuda", generator=g)
+                f = lambda: linear_cross_entropy(*leaves, t)  # noqa: E731
+            else:
+                leaves = [r(16384, 768) * 28, r(2112, 768), r(2112, 768), r(768, 2112)]
+                f = lambda: gated_ffn(*leaves).float().sum()  # noqa: E731
+            for v in leaves:
+                v.requires_grad_(True)
+
+            def run():
+                with torch.enable_grad():
+                    torch.autograd.grad(f(), leaves)
+        elif case == "clip":
+            from .clip import clip_grads
+
+            grads = [torch.randn(595_000, device="cuda", generator=g).to(torch.bfloat16) for _ in range(400)]
+            outs = [torch.empty(t.shape, device="cuda") for t in grads]
+            run = lambda: clip_grads(grads, 1.0, out=outs)  # noqa: E731
         elif case == "in_proj":
             m = KulaMamba(d_model=768, d_state=128, headdim=64, mimo_rank=2).cuda().to(torch.bfloat16).eval()
             x = torch.randn(16, 4096, 768, device="cuda", generator=g).to(torch.bfloat16)
@@ -213,12 +272,15 @@ if __name__ == "__main__":
     import argparse
 
     ap = argparse.ArgumentParser(description="profiling helpers")
-    ap.add_argument("what", choices=["train", "cfg3", "chunked", "chunked_bwd", "step", "fp32", "in_proj", "decode"])
-    ap.add_argument("--batch", type=int, default=16)
-    ap.add_argument("--seqlen", type=int, default=4096)
+    ap.add_argument("what", choices=["train", "train_lm", "cfg3", "chunked", "chunked_bwd", "step", "fp32",
+                                     "in_proj", "xent", "ffn", "clip", "decode"])
+    ap.add_argument("--batch", type=int)
+    ap.add_argument("--seqlen", type=int)
     ap.add_argument("--reps", type=int, default=3)
     args = ap.parse_args()
     if args.what == "train":
-        print(train_step_profile(args.batch, args.seqlen))
+        print(train_step_profile(args.batch or 16, args.seqlen or 4096))
+    elif args.what == "train_lm":
+        print(lm_train_step_profile(args.batch or 8, args.seqlen or 2048))
     else:
         kernel_workload(args.what, args.reps)
