@@ -540,7 +540,7 @@ M3B_API int m3b_scaled_add(const void* x, const void* h, float scale, void* out,
  * operands travel as three bf16 planes, which keeps 24 bits.
  *
  * saved_act (m3b_gated_ffn_act_bytes) is always written.  saved_gu (m3b_gated_ffn_gu_bytes; g and
- * u in fp32, private layout) is written when not null; the backward needs both as the forward
+ * u in fp32, or their upper 24 bits where `dtype` has 16; private layout) is written when not null; the backward needs both as the forward
  * left them.  Backward outputs may be null where no gradient is wanted.  16-byte aligned
  * workspace of m3b_gated_ffn_{fwd,bwd}_workspace bytes (may be 0).
  * ------------------------------------------------------------------------ */

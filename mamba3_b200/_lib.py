@@ -874,7 +874,8 @@ def _ffn_args(x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual, scale):
 def ffn_saved_bytes(x, d_ff):
     """(m3b_gated_ffn_act_bytes, m3b_gated_ffn_gu_bytes) of x (rows, d_model)."""
     rows, planes = x.shape[0], 3 if x.dtype == torch.float32 else 1
-    return planes * rows * (-(-d_ff // 8) * 8) * 2, -(-rows // 256) * 256 * (-(-d_ff // 32) * 32) * 8
+    return (planes * rows * (-(-d_ff // 8) * 8) * 2,
+            -(-rows // 256) * 256 * (-(-d_ff // 32) * 32) * (8 if planes == 3 else 6))
 
 
 def gated_ffn_fwd(x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual, scale, save):

@@ -11,7 +11,7 @@
 // dx (one product over two K segments) and the three weight gradients side by side in one launch.
 // Inference on at most kSmallRows rows (a decoding step) runs the matrix-vector form of ffn_small.cu.
 // 18 rows d_model d_ff operations forward and backward, the least there are: g and u are kept in
-// fp32 (8 bytes a value), because the rounding of a 16-bit copy would reach every gradient.
+// 24 bits or more (6 bytes a pair; fp32 8), because the rounding of a 16-bit copy would reach every gradient.
 #include "ffn_small.h"
 #include "gemm.cuh"
 
@@ -232,8 +232,8 @@ int forward(const m3b_gated_ffn_args* a, void* workspace, size_t* need, bool run
   s.bias = a->b_gate;
   s.bias2 = a->b_up;
   s.dt = a->dtype;
-  p.gu = static_cast<float*>(a->saved_gu);
-  p.gu_ld4 = up(d.F, 32) / 4;
+  p.gu = static_cast<uint8_t*>(a->saved_gu);
+  p.gu_ld = up(d.F, 32) / 8;
   plan_gemm(p, kEpiGlu, pair);
 
   GemmParams q = params(d, a, pair ? (d.f32 ? 128 : 256) : 64);
@@ -336,8 +336,8 @@ int backward(const m3b_gated_ffn_args* a, void* workspace, size_t* need, bool ru
     s.alpha = a->residual_scale;
     s.out = operand_out(dg, d.f16);
     s.out2 = operand_out(du, d.f16);
-    p.gu = static_cast<float*>(a->saved_gu);
-    p.gu_ld4 = up(d.F, 32) / 4;
+    p.gu = static_cast<uint8_t*>(a->saved_gu);
+    p.gu_ld = up(d.F, 32) / 8;
     p.clear = ticket;
     plan_gemm(p, kEpiDglu, true);
     M3B_TRY(launch_gemm(p, kEpiDglu, true, nullptr, st));
@@ -367,7 +367,7 @@ size_t m3b_gated_ffn_act_bytes(const m3b_gated_ffn_args* a) {
 
 size_t m3b_gated_ffn_gu_bytes(const m3b_gated_ffn_args* a) {
   if (!m3b::sizes_ok(a)) return 0;
-  return (size_t)m3b::up(a->rows, 256) * m3b::up(a->d_ff, 32) * 8;
+  return (size_t)m3b::up(a->rows, 256) * m3b::up(a->d_ff, 32) * (a->dtype == M3B_F32 ? 8 : 6);
 }
 
 size_t m3b_gated_ffn_fwd_workspace(const m3b_gated_ffn_args* a) {

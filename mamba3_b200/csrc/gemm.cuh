@@ -46,7 +46,12 @@ constexpr uint32_t kGmStageA = 128 * kGmBK * 2;     // 16 KB
 constexpr uint32_t kGmStage = 2 * kGmStageA;        // + B: at most 128 rows of 64
 constexpr uint32_t kGmBox = 32 * 128;               // staging of an epilogue warp: 32 rows x 32 fp32
 constexpr int kGuSlots = 4;                         // kEpiDglu: runs of 8 columns of g and u per epilogue warp
-constexpr uint32_t kGuRun = 8 * 2 * 32 * 4;         // 2 KB
+// What the forward pass keeps of g and u, in runs of 32 rows x 8 columns: in fp32, [g, u][column / 4][row][4],
+// or, where 16-bit operands follow, their upper 24 bits: the upper halves of g and u beside each other,
+// [column / 4][row][4], then the next 8 bits of both, [row][column][g, u].  (A 16-bit copy's rounding would
+// reach every gradient; the last 8 bits of fp32 do not, and a quarter of the bytes is theirs.)
+template <bool PLANES>
+constexpr uint32_t kGuRun = PLANES ? 2048 : 1536;
 constexpr uint32_t kGmBarOff = 6 * kGmStage + 8 * kGmBox;
 constexpr uint32_t kGmSmem = kGmBarOff + 768 + 1024;  // barriers, job queue, TMEM slot; alignment
 static_assert(kGmSmem <= 227 * 1024, "shared memory plan");
@@ -111,10 +116,9 @@ struct GemmParams {
   const int* dyn;
   int* ticket;  // zeroed counter that jobs are drawn from, or null: dealt in turn
   int* clear;   // a counter to zero for the launch that follows
-  // kEpiGlu / kEpiDglu: g and u in fp32, [row / 32][col / 4][g, u][row % 32][4], ld4 = column quads (of
-  // whole runs of 32 columns)
-  float* gu;
-  int64_t gu_ld4;
+  // kEpiGlu / kEpiDglu: g and u in runs (kGuRun), gu_ld of them (whole 32 columns) for every 32 rows
+  uint8_t* gu;
+  int64_t gu_ld;
   // kEpiLse / kEpiDlogit
   const int* target;       // per row
   float* target_logit;
@@ -478,7 +482,7 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
   // six stages; kEpiDglu gives two of them to the runs of g and u
   constexpr int kGmStages = EPI == kEpiDglu ? 4 : 6;
   constexpr uint32_t kGmBoxOff = kGmStages * kGmStage, kGuOff = kGmBoxOff + 8 * kGmBox;
-  static_assert(kGuOff + (EPI == kEpiDglu ? 8 * kGuSlots * kGuRun : 0) <= kGmBarOff, "shared memory plan");
+  static_assert(kGuOff + (EPI == kEpiDglu ? 8 * kGuSlots * kGuRun<PLANES> : 0) <= kGmBarOff, "shared memory plan");
   constexpr bool kDraws = EPI == kEpiStore || EPI == kEpiAcc;  // forms with several products a launch
   extern __shared__ uint8_t smraw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smraw) + 1023) & ~uintptr_t(1023));
@@ -730,16 +734,16 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
     // kEpiDglu: this warp's runs of g and u, in the order it will use them (the jobs are dealt, so the
     // next tile's are known), kGuSlots of them on their way or in shared memory
     uint64_t* gub = gufull + (warp - 2) * kGuSlots;
-    const uint8_t* gus = sm + kGuOff + (uint32_t)(warp - 2) * kGuSlots * kGuRun;
+    const uint8_t* gus = sm + kGuOff + (uint32_t)(warp - 2) * kGuSlots * kGuRun<PLANES>;
     uint32_t gu_used = 0, gu_sent = 0, gu_tile = 0;
     int gu_run = 0, gu_runs = 0;
-    const float4* gu_at = nullptr;
+    const uint8_t* gu_at = nullptr;
     auto gu_enter = [&](const GemmJob& j) {  // the runs of tile j
       const int64_t row = (int64_t)j.mt * kTileM + (int64_t)rank * 128 + q * 32;
       const int col = j.nt * bn + half * (bn / 2), n = p.sub[0].N - col < bn / 2 ? p.sub[0].N - col : bn / 2;
       gu_run = 0;
       gu_runs = n > 0 ? (n + 31) / 32 * 4 : 0;
-      gu_at = reinterpret_cast<const float4*>(p.gu) + ((row >> 5) * p.gu_ld4 + (col >> 2)) * 64;
+      gu_at = p.gu + ((row >> 5) * p.gu_ld + (col >> 3)) * kGuRun<PLANES>;
     };
     auto gu_send = [&]() {
       while (gu_run >= gu_runs) {
@@ -752,10 +756,10 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
       }
       const uint32_t slot = gu_sent++ % kGuSlots;
       if (lane == 0) {
-        mbar_arrive_expect_tx(&gub[slot], kGuRun);
+        mbar_arrive_expect_tx(&gub[slot], kGuRun<PLANES>);
         asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                         smem_u32(gus + slot * kGuRun)),
-                     "l"(gu_at + (int64_t)gu_run * 128), "r"(kGuRun), "r"(smem_u32(&gub[slot]))
+                         smem_u32(gus + slot * kGuRun<PLANES>)),
+                     "l"(gu_at + (int64_t)gu_run * kGuRun<PLANES>), "r"(kGuRun<PLANES>), "r"(smem_u32(&gub[slot]))
                      : "memory");
       }
       ++gu_run;
@@ -930,11 +934,30 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
             }
           }
           if (p.gu) {
-            float4* gp = reinterpret_cast<float4*>(p.gu) + ((grow >> 5) * p.gu_ld4 + (col >> 2)) * 64 + lane;
+            uint8_t* run = p.gu + ((grow >> 5) * p.gu_ld + (col >> 3)) * kGuRun<PLANES> + lane * 16;
 #pragma unroll
-            for (int i = 0; i < 8; ++i, gp += 64) {
-              gp[0] = make_float4(g[4 * i], g[4 * i + 1], g[4 * i + 2], g[4 * i + 3]);
-              gp[32] = make_float4(u[4 * i], u[4 * i + 1], u[4 * i + 2], u[4 * i + 3]);
+            for (int k = 0; k < 4; ++k, run += kGuRun<PLANES>) {
+              if constexpr (PLANES) {
+#pragma unroll
+                for (int q4 = 0; q4 < 2; ++q4) {
+                  const int i = 8 * k + 4 * q4;
+                  *reinterpret_cast<float4*>(run + q4 * 512) = make_float4(g[i], g[i + 1], g[i + 2], g[i + 3]);
+                  *reinterpret_cast<float4*>(run + 1024 + q4 * 512) = make_float4(u[i], u[i + 1], u[i + 2], u[i + 3]);
+                }
+              } else {
+                uint32_t hi[8], lo[4];
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) {
+                  const uint32_t g0 = __float_as_uint(g[8 * k + i]), g1 = __float_as_uint(g[8 * k + i + 1]);
+                  const uint32_t u0 = __float_as_uint(u[8 * k + i]), u1 = __float_as_uint(u[8 * k + i + 1]);
+                  hi[i] = __byte_perm(g0, u0, 0x7632);
+                  hi[i + 1] = __byte_perm(g1, u1, 0x7632);
+                  lo[i >> 1] = __byte_perm(__byte_perm(g0, u0, 0x0051), __byte_perm(g1, u1, 0x0051), 0x5410);
+                }
+                *reinterpret_cast<uint4*>(run) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                *reinterpret_cast<uint4*>(run + 512) = make_uint4(hi[4], hi[5], hi[6], hi[7]);
+                *reinterpret_cast<uint4*>(run + 1024) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+              }
             }
           }
 #pragma unroll
@@ -956,16 +979,30 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
           for (int h = 0; h < 4; ++h, ++gu_used) {
             const uint32_t slot = gu_used % kGuSlots;
             if (!__all_sync(0xffffffffu, gm_wait(&gub[slot], (gu_used / kGuSlots) & 1, p.wait_ns))) give_up();
-            const float4* run = reinterpret_cast<const float4*>(gus + slot * kGuRun) + lane;
-            const float4 g4[2] = {run[0], run[64]}, u4[2] = {run[32], run[96]};
+            const uint4* run = reinterpret_cast<const uint4*>(gus + slot * kGuRun<PLANES>) + lane;
+            const uint4 r0 = run[0], r1 = run[32], r2 = run[64];
+            uint32_t w[16];  // g and u of eight columns: fp32 words, or halves and their next bits
+            w[0] = r0.x, w[1] = r0.y, w[2] = r0.z, w[3] = r0.w, w[4] = r1.x, w[5] = r1.y, w[6] = r1.z, w[7] = r1.w;
+            w[8] = r2.x, w[9] = r2.y, w[10] = r2.z, w[11] = r2.w;
+            if constexpr (PLANES) {
+              const uint4 r3 = run[96];
+              w[12] = r3.x, w[13] = r3.y, w[14] = r3.z, w[15] = r3.w;
+            }
             __syncwarp();
             gu_send();
             const float2 one = make_float2(1.f, 1.f), alpha = make_float2(s.alpha, s.alpha);
 #pragma unroll
             for (int i = 0; i < 8; i += 2) {
-              const float4 gq = g4[i >> 2], uq = u4[i >> 2];
-              const float2 g = (i & 2) ? make_float2(gq.z, gq.w) : make_float2(gq.x, gq.y);
-              const float2 u = (i & 2) ? make_float2(uq.z, uq.w) : make_float2(uq.x, uq.y);
+              float2 g, u;
+              if constexpr (PLANES) {
+                g = make_float2(__uint_as_float(w[i]), __uint_as_float(w[i + 1]));
+                u = make_float2(__uint_as_float(w[8 + i]), __uint_as_float(w[9 + i]));
+              } else {
+                // the bits below stand twice: any do, and these need no instruction of their own
+                const uint32_t lo = w[8 + (i >> 1)];
+                g = make_float2(__uint_as_float(__byte_perm(w[i], lo, 0x1044)), __uint_as_float(__byte_perm(w[i + 1], lo, 0x1066)));
+                u = make_float2(__uint_as_float(__byte_perm(w[i], lo, 0x3255)), __uint_as_float(__byte_perm(w[i + 1], lo, 0x3277)));
+              }
               const float2 sg = sigmoid2(g);
               const float2 ds = mul2(mul2(make_float2(d[8 * h + i], d[8 * h + i + 1]), alpha), sg);
               const float2 x = mul2(mul2(ds, u), fma2(g, fma2(sg, make_float2(-1.f, -1.f), one), one)), y = mul2(ds, g);

@@ -69,6 +69,8 @@ def ffn(x, wg, wu, wd, bg=None, bu=None, bd=None, residual=None, scale=1.0, dout
     da = scale * (dy @ D)
     eda = abs(scale) * (sum_error(d, dt) + 2.0 ** -22) * (dy.abs() @ D.abs())
     pg, pu = u * sig * (1 + g * (1 - sig)), act
+    if dt != torch.float32:  # the forward keeps the upper 24 bits of g and u, 16 of them significant: off by less than one step, 2^-15 of 1..2
+        eg, eu = eg + 2.0 ** -15 * g.abs(), eu + 2.0 ** -15 * u.abs()
     # d/dg of u sig (1 + g (1 - sig)) is at most u / 2 in magnitude; 1 - sig and the sum are within 3 steps
     epg = 0.5 * u.abs() * eg + 1.1 * eu + 4 * es * u.abs() * sig * (1 + g.abs())
     epu = 1.1 * eg + es * act.abs()

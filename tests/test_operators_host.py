@@ -17,7 +17,7 @@ def test_entry_points_reject_bad_arguments():
     a = _lib.GatedFfnArgs(4, 64, 0, 64, 64, 128, 1)
     assert L.m3b_gated_ffn_fwd(ctypes.byref(a), None, 0, None) == 1 and b"null" in L.m3b_last_error()
     assert L.m3b_gated_ffn_act_bytes(ctypes.byref(a)) == 4 * 128 * 2
-    assert L.m3b_gated_ffn_gu_bytes(ctypes.byref(a)) == 256 * 128 * 8
+    assert L.m3b_gated_ffn_gu_bytes(ctypes.byref(a)) == 256 * 128 * 6
     for bad in (_lib.GatedFfnArgs(-1, 64, 0, 64, 64, 128, 1), _lib.GatedFfnArgs(4, 64, 0, 64, 0, 128, 1),
                 _lib.GatedFfnArgs(4, 64, 0, 64, 64, 128, 9)):
         assert L.m3b_gated_ffn_fwd(ctypes.byref(bad), None, 0, None) == 1
