@@ -63,16 +63,6 @@ GemmOut result(void* p, int64_t ld, int dtype) {
   return o;
 }
 
-GemmOut operand_out(const GemmOperand& o, bool f16) {
-  GemmOut r{};
-  r.p = const_cast<void*>(o.p);
-  r.ld = o.ld;
-  r.plane = o.plane;
-  r.kind = o.planes > 1 ? kOutPlanes : f16 ? kOutF16 : kOutBf16;
-  r.vec = 1;
-  return r;
-}
-
 // Sums over the rows of up to three operands, times `scale`, in a fixed order.  A block takes 64 columns (two a
 // lane) and kSumRows rows, its warps every eighth row, and leaves one partial; the chunks' partials
 // are added by a second kernel.
@@ -228,7 +218,6 @@ int forward(const m3b_gated_ffn_args* a, void* workspace, size_t* need, bool run
   s.M = (int)d.M;
   s.N = d.F;
   s.nk[0] = blocks_of(d.D);
-  s.out = operand_out(act, d.f16);
   s.bias = a->b_gate;
   s.bias2 = a->b_up;
   s.dt = a->dtype;
@@ -257,6 +246,7 @@ int forward(const m3b_gated_ffn_args* a, void* workspace, size_t* need, bool run
   M3B_MAP(&s.a[0], x, false, 128, d.f16);
   M3B_MAP(&s.b[0], wg, false, gemm_box_b(pair, p.bn, kEpiGlu), d.f16);
   M3B_MAP(&s.b[1], wu, false, gemm_box_b(pair, p.bn, kEpiGlu), d.f16);
+  M3B_TRY(gemm_out_map(&p.o[0], act, d.f16));
   M3B_TRY(launch_gemm(p, kEpiGlu, pair, nullptr, st));
   M3B_MAP(&t.a[0], act, false, 128, d.f16);
   M3B_MAP(&t.b[0], wd, false, gemm_box_b(pair, q.bn, kEpiFinal), d.f16);
@@ -334,8 +324,8 @@ int backward(const m3b_gated_ffn_args* a, void* workspace, size_t* need, bool ru
     s.N = d.F;
     s.nk[0] = blocks_of(d.D);
     s.alpha = a->residual_scale;
-    s.out = operand_out(dg, d.f16);
-    s.out2 = operand_out(du, d.f16);
+    M3B_TRY(gemm_out_map(&p.o[0], dg, d.f16));
+    M3B_TRY(gemm_out_map(&p.o[1], du, d.f16));
     p.gu = static_cast<uint8_t*>(a->saved_gu);
     p.gu_ld = up(d.F, 32) / 8;
     p.clear = ticket;

@@ -108,18 +108,19 @@ int device_setup(int* pairs) {
 
 }  // namespace
 
-int gemm_map(CUtensorMap* m, const GemmOperand& o, bool mn_major, int box_rows, bool f16) {
+namespace {
+int encode(CUtensorMap* m, const GemmOperand& o, int box_cols, int box_rows, CUtensorMapSwizzle swizzle, bool f16) {
   const EncodeTiledFn enc = encode_tiled();
   if (!enc) return fail(M3B_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
   const cuuint64_t dims[3] = {(cuuint64_t)o.cols, (cuuint64_t)o.rows, (cuuint64_t)o.planes};
   const cuuint64_t strides[2] = {(cuuint64_t)o.ld * 2, (cuuint64_t)(o.planes > 1 ? o.plane : o.rows * o.ld) * 2};
-  const cuuint32_t box[3] = {(cuuint32_t)kGmBK, (cuuint32_t)(mn_major ? kGmBK : box_rows), 1};
+  const cuuint32_t box[3] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1};
   const cuuint32_t estr[3] = {1, 1, 1};
   CUresult r = CUDA_SUCCESS;
   for (int attempt = 0; attempt < 2; ++attempt) {
     r = enc(m, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(o.p),
-            dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+            dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_ERROR_INVALID_CONTEXT) break;
     // a host thread that has made no runtime call yet (autograd's): bind the device's context to it
     int dev = 0;
@@ -128,6 +129,15 @@ int gemm_map(CUtensorMap* m, const GemmOperand& o, bool mn_major, int box_rows, 
   if (r == CUDA_SUCCESS) return M3B_OK;
   return fail(M3B_ERR_CUDA, "cuTensorMapEncodeTiled refused %p: %lld x %lld, rows %lld apart, %d planes (%d)", o.p,
               (long long)o.rows, (long long)o.cols, (long long)o.ld, o.planes, (int)r);
+}
+}  // namespace
+
+int gemm_map(CUtensorMap* m, const GemmOperand& o, bool mn_major, int box_rows, bool f16) {
+  return encode(m, o, kGmBK, mn_major ? kGmBK : box_rows, CU_TENSOR_MAP_SWIZZLE_128B, f16);
+}
+
+int gemm_out_map(CUtensorMap* m, const GemmOperand& o, bool f16) {
+  return encode(m, o, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B, f16);
 }
 
 int gemm_columns(int64_t M, int64_t N, bool planes) {

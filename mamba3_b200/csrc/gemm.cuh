@@ -60,12 +60,11 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
 // How a product's result is stored.
-enum GemmOutKind { kOutBf16 = 0, kOutF16 = 1, kOutF32 = 2, kOutPlanes = 3 };
+enum GemmOutKind { kOutBf16 = 0, kOutF16 = 1, kOutF32 = 2 };
 
 struct GemmOut {
   void* p;
   int64_t ld;     // elements between rows
-  int64_t plane;  // elements between planes (kOutPlanes)
   int kind;
   int vec;        // rows and columns allow 16-byte stores
 };
@@ -92,7 +91,7 @@ struct GemmSub {
   int m_dyn, k_dyn;
   int split;       // jobs along K of each tile
   float* part;     // [split][row / 32][col / 4][row % 32][4] fp32 when split > 1
-  GemmOut out, out2;
+  GemmOut out;     // final results (kEpiStore, kEpiFinal, kEpiAcc)
   // kEpiStore, kEpiFinal, kEpiAcc
   float alpha;
   const float* alpha_num;  // alpha *= alpha_num[0]
@@ -109,6 +108,7 @@ struct GemmSub {
 
 struct GemmParams {
   GemmSub sub[kGmSubs];
+  CUtensorMap o[2];  // kEpiGlu, kEpiDglu, kEpiDlogit: the first product's results (out, out2), 32 x 32 boxes
   int nsub;
   int bn;       // accumulator columns of a tile
   int npass;    // plane pairs: 1, or 6 for fp32 operands
@@ -297,20 +297,47 @@ __device__ __forceinline__ void put32(uint8_t* box, const GemmOut& o, const Gemm
   }
 }
 
+// A following product's operand leaves by TMA instead: the warp fills one of its two boxes (the same
+// swizzle is the tensor map's 64-byte one) and one thread sends it, while the warp goes on.  (Stored row by
+// row, dg and du cost the warp 24 us of 104 at 16384 x 768 x 2112.)
+struct GemmSend {
+  uint8_t* box;
+  uint32_t side;
+  __device__ __forceinline__ void operator()(const CUtensorMap* map, int col, int64_t row, int plane,
+                                             const uint32_t (&w)[16]) {
+    const int lane = threadIdx.x & 31;
+    uint8_t* b = box + side * (kGmBox / 2);
+    side ^= 1;
+    if (lane == 0) bulk_wait_group_read<1>();  // the box sent before last has been read
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      *reinterpret_cast<uint4*>(b + lane * 64 + ((k ^ ((lane >> 1) & 3)) << 4)) =
+          make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+    fence_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(map), "r"(col),
+                   "r"((int)row), "r"(plane), "r"(smem_u32(b))
+                   : "memory");
+      bulk_commit_group();
+    }
+  }
+};
+
 // 32 columns of a following product's operand: a 16-bit type, or the planes of fp32 values (each plane
 // takes the upper halves and leaves the remainders; a value that is not finite lies in the first alone).
 template <bool PLANES>
-__device__ __forceinline__ void put_operand(uint8_t* box, const GemmOut& o, const GemmRows& rows, int col, int N,
+__device__ __forceinline__ void put_operand(GemmSend& send, const CUtensorMap* map, bool f16, int col, int64_t row,
                                             float (&v)[32]) {
-  uint16_t* base = static_cast<uint16_t*>(o.p);
   if constexpr (!PLANES) {
     uint32_t w[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) w[i] = pack16(v[2 * i], v[2 * i + 1], o.kind == kOutF16);
-    put16(box, o, base, rows, col, N, w);
+    for (int i = 0; i < 16; ++i) w[i] = pack16(v[2 * i], v[2 * i + 1], f16);
+    send(map, col, row, 0, w);
   } else {
 #pragma unroll 1
-    for (int pl = 0; pl < 3; ++pl, base += o.plane) {
+    for (int pl = 0; pl < 3; ++pl) {
       uint32_t w[16];
 #pragma unroll
       for (int i = 0; i < 32; ++i) {
@@ -321,9 +348,17 @@ __device__ __forceinline__ void put_operand(uint8_t* box, const GemmOut& o, cons
         if (i & 1) w[i >> 1] |= top << 16;
         else w[i >> 1] = top;
       }
-      put16(box, o, base, rows, col, N, w);
+      send(map, col, row, pl, w);
     }
   }
+}
+// 32 columns of a 16-bit final result.
+__device__ __forceinline__ void put_narrow(uint8_t* box, const GemmOut& o, const GemmRows& rows, int col, int N,
+                                           const float (&v)[32]) {
+  uint32_t w[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) w[i] = pack16(v[2 * i], v[2 * i + 1], o.kind == kOutF16);
+  put16(box, o, static_cast<uint16_t*>(o.p), rows, col, N, w);
 }
 
 // 32 columns as final results, (v + bias) alpha + residual, fp32 until the one rounding.
@@ -767,6 +802,7 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
     if constexpr (EPI == kEpiDglu)
       for (int i = 0; i < kGuSlots; ++i) gu_send();
     uint32_t jn = 0;
+    GemmSend send{sm + kGmBoxOff + (uint32_t)(warp - 2) * kGmBox, 0};
     GemmJob job = next_job(0);
     for (; job.sub >= 0; job = next_job(++jn)) {
       const GemmSub& s = p.sub[job.sub];
@@ -853,7 +889,7 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] *= alpha;
         if (s.out.kind == kOutF32) put32(box, s.out, rows, col, s.N, v);
-        else put_operand<false>(box, s.out, rows, col, s.N, v);
+        else put_narrow(box, s.out, rows, col, s.N, v);
       };
       // a part of a split product, as it is
       auto put_part = [&](int col, const float (&v)[32]) {
@@ -966,7 +1002,7 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
             const float2 a = mul2(mul2(g2, sigmoid2(g2)), make_float2(u[i], u[i + 1]));
             g[i] = a.x, g[i + 1] = a.y;
           }
-          put_operand<PLANES>(box, s.out, rows, col, s.N, g);
+          if (rows.row0 < M) put_operand<PLANES>(send, &p.o[0], p.f16, col, rows.row0, g);
         }
       } else if constexpr (EPI == kEpiDglu) {
         columns(cfirst, clast, [&](int c, float (&d)[32]) {
@@ -1013,17 +1049,19 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
             if constexpr (!PLANES) {
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                wg[4 * h + i] = pack16(dg[2 * i], dg[2 * i + 1], s.out.kind == kOutF16);
-                wu[4 * h + i] = pack16(du[2 * i], du[2 * i + 1], s.out.kind == kOutF16);
+                wg[4 * h + i] = pack16(dg[2 * i], dg[2 * i + 1], p.f16);
+                wu[4 * h + i] = pack16(du[2 * i], du[2 * i + 1], p.f16);
               }
             }
           }
           if constexpr (PLANES) {
-            put_operand<true>(box, s.out, rows, col, s.N, d);
-            put_operand<true>(box, s.out2, rows, col, s.N, du);
-          } else {
-            put16(box, s.out, static_cast<uint16_t*>(s.out.p), rows, col, s.N, wg);
-            put16(box, s.out2, static_cast<uint16_t*>(s.out2.p), rows, col, s.N, wu);
+            if (rows.row0 < M) {
+              put_operand<true>(send, &p.o[0], false, col, rows.row0, d);
+              put_operand<true>(send, &p.o[1], false, col, rows.row0, du);
+            }
+          } else if (rows.row0 < M) {
+            send(&p.o[0], col, rows.row0, 0, wg);
+            send(&p.o[1], col, rows.row0, 0, wu);
           }
         });
       } else if constexpr (EPI == kEpiLse) {
@@ -1058,7 +1096,7 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
         const int tgt = rok ? p.target[grow] - p.col0 : -1;
         const float l2 = (rok ? p.lse2[grow] : 0.f) - p.shift, one = ex2_fast(p.shift);
         const float w = rok && p.roww ? p.roww[grow] : 1.f;
-        rows.M = 0x7fffffff;  // rows behind the last kept token are K values of the next products: zero
+        // rows behind the last kept token are K values of the next products: zero
         columns(cfirst, clast, [&](int c, float (&v)[32]) {
           const int col = job.nt * bn + c;
           if (col >= s.N) return;
@@ -1080,12 +1118,13 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = 0.f;
           }
-          put_operand<PLANES>(box, s.out, rows, col, s.N, v);
+          put_operand<PLANES>(send, &p.o[0], p.f16, col, rows.row0, v);
         });
       }
       if constexpr (!PLANES) release();
     }
     if (job.sub == -2) give_up();
+    if (lane == 0) bulk_wait_group_all();  // boxes stay until they have been sent
     if constexpr (EPI == kEpiDglu)  // an aborted run leaves once its copies have landed
       for (; gu_used < gu_sent; ++gu_used) mbar_wait(&gub[gu_used % kGuSlots], (gu_used / kGuSlots) & 1, 10000000ull);
   }
@@ -1180,7 +1219,7 @@ __global__ void __launch_bounds__(256) gemm_join_kernel(const __grid_constant__ 
 #pragma unroll
       for (int k = 0; k < 32; ++k) v[k] *= alpha;
       if (s.out.kind == kOutF32) put32(box, s.out, rows, col, s.N, v);
-      else put_operand<false>(box, s.out, rows, col, s.N, v);
+      else put_narrow(box, s.out, rows, col, s.N, v);
     }
   }
 }
@@ -1201,6 +1240,8 @@ inline bool tma_ok(const void* p, int64_t ld_elems) { return aligned16(p) && ld_
 // Tensor map of an operand; box_rows counts the other dimension's box when K is along the rows
 // (K-major), MN-major maps always use 64 x 64 boxes.
 int gemm_map(CUtensorMap* m, const GemmOperand& o, bool mn_major, int box_rows, bool f16);
+// Tensor map of an operand that a kernel's epilogue writes.
+int gemm_out_map(CUtensorMap* m, const GemmOperand& o, bool f16);
 // Fills mt, nt and split from M, N, nk, npass and bn, and orders the products longest job first;
 // returns the bytes of fp32 parts the split ones need (to be carved and given to launch_gemm).
 size_t plan_gemm(GemmParams& p, int epi, bool pair);

@@ -428,11 +428,7 @@ int backward(const m3b_linear_xent_args* a, void* workspace, size_t* need, bool 
       g.m_dyn = 1;
       g.N = (int)n;
       g.nk[0] = (d.D + kGmBK - 1) / kGmBK;
-      g.out.p = dz;
-      g.out.ld = ldz;
-      g.out.plane = z.plane;
-      g.out.kind = d.f32 ? kOutPlanes : okind;
-      g.out.vec = 1;
+      M3B_TRY(gemm_out_map(&p.o[0], z, d.f16));
       p.target = s.target;
       p.lse2 = s.lse2;
       p.roww = roww;
