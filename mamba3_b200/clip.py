@@ -75,9 +75,13 @@ def clip_grads(grads: Iterable[torch.Tensor], max_norm: float, norm_type: float 
         if numel != list(map(_numel, os)):
             raise ValueError("clip_grads: each output needs its gradient's length")
         out_ptrs = list(map(_data_ptr, os))
-        if dtypes != out_dtypes and any(n and p == q and a != b
-                                        for n, p, q, a, b in zip(numel, ptrs, out_ptrs, dtypes, out_dtypes)):
-            raise ValueError("clip_grads: an output in its gradient's place needs its dtype")
+        if not {p for p, n in zip(out_ptrs, numel) if n}.isdisjoint(ptrs):
+            for n, p, q, a, b in zip(numel, ptrs, out_ptrs, dtypes, out_dtypes):
+                if n and p == q and a != b:
+                    raise ValueError("clip_grads: an output in its gradient's place needs its dtype")
+                if n and p != q and q in ptrs:  # (an empty gradient may have any address)
+                    if any(q == r and k for r, k in zip(ptrs, numel)):
+                        raise ValueError("clip_grads: an output in another gradient's place")
     used = [p for p, n in zip(out_ptrs, numel) if n]
     if len(set(used)) != len(used):
         raise ValueError("clip_grads: the same tensor twice")

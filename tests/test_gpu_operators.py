@@ -315,6 +315,9 @@ def test_loss_shapes_strides_and_integer_types():
     assert math.isnan(e.item())
     assert linear_cross_entropy(h[:0], w, t[:0], reduction="sum").item() == 0.0
     assert linear_cross_entropy(h[:0], w, t[:0], reduction="none").shape == (0,)
+    a, b = h[:0].clone().requires_grad_(True), w.clone().requires_grad_(True)
+    linear_cross_entropy(a, b, t[:0], reduction="sum").backward()
+    assert a.grad.shape == (0, 64) and not b.grad.any()
 
 
 def test_loss_gradient_against_differences():

@@ -135,7 +135,9 @@ def test_clip_refuses(monkeypatch):
     for call in (lambda: m.clip_grads([_Cuda(g)], -1.0), lambda: m.clip_grads([_Cuda(g)], math.nan),
                  lambda: m.clip_grads([_Cuda(g)], 1.0, 1.0), lambda: m.clip_grads([_Cuda(g), _Cuda(g)], 1.0),
                  lambda: m.clip_grads([_Cuda(g)], 1.0, out=[]), lambda: m.clip_grads([_Cuda(g[::2])], 1.0),
-                 lambda: m.clip_grads([_Cuda(g)], 1.0, out=[fake(11)])):
+                 lambda: m.clip_grads([_Cuda(g)], 1.0, out=[fake(11)]),
+                 lambda: m.clip_grads([_Cuda(g), fake(10)], 1.0, out=[fake(10), _Cuda(g)]),
+                 lambda: m.clip_grads([_Cuda(g)], 1.0, out=[_Cuda(g.view(torch.bfloat16)[:10])])):
         with pytest.raises(ValueError):
             call()
     with pytest.raises(m.M3bError, match="unsupported dtype"):
