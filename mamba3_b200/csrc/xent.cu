@@ -13,6 +13,7 @@
 // pieces in fp32.  8 rows d_model vocab operations forward and backward, 2 more than with the
 // logits kept.
 #include "gemm.cuh"
+#include "xent_small.h"
 
 namespace m3b {
 
@@ -277,6 +278,7 @@ GemmOperand piece_of(const GemmOperand& w, int64_t c0, int64_t cols) {
 
 int forward(const m3b_linear_xent_args* a, void* workspace, size_t* need, bool run, cudaStream_t st) {
   const Dims d(a);
+  if (d.T <= kSmallXentRows) return small_xent_fwd(a, workspace, need, run, st);
   Carve ws(workspace);
   const bool pair = d.T > 128;
   const int bn = pair ? gemm_columns(d.T, d.V, d.f32) : d.f32 ? 64 : 128;
@@ -333,6 +335,7 @@ int64_t piece_cols(const Dims& d) {
 
 int backward(const m3b_linear_xent_args* a, void* workspace, size_t* need, bool run, cudaStream_t st) {
   const Dims d(a);
+  if (d.T <= kSmallXentRows) return small_xent_bwd(a, workspace, need, run, st);
   Carve ws(workspace);
   const int64_t cols = piece_cols(d), ldz = up(cols, 8);
   const int bn = d.f32 ? 128 : 256, pieces = (int)((d.V + cols - 1) / cols);
@@ -464,7 +467,8 @@ __global__ void empty_loss_kernel(float* loss, int reduction) {
 extern "C" {
 
 size_t m3b_linear_xent_saved(const m3b_linear_xent_args* a) {
-  return m3b::sizes_ok(a) ? m3b::saved_of(a, nullptr).bytes : 0;
+  if (!m3b::sizes_ok(a)) return 0;
+  return a->rows <= m3b::kSmallXentRows ? m3b::small_xent_saved(a) : m3b::saved_of(a, nullptr).bytes;
 }
 
 size_t m3b_linear_xent_fwd_workspace(const m3b_linear_xent_args* a) {

@@ -683,3 +683,122 @@ def test_gradients_are_the_same_every_time():
         if first is None:
             first = g
         assert all(torch.equal(a, b) for a, b in zip(g, first))
+
+
+# ---------------------------------------------------------------------------
+# cross entropy of a few rows
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("n,d,v,ignored", [(1, 8, 5, ()), (1, 513, 2000, ()), (2, 1100, 33, (1,)), (3, 1, 1000, ()),
+                                           (4, 512, 19000, (0,)), (5, 2052, 700, (2, 3)), (6, 130, 40003, ()),
+                                           (8, 768, 4097, ()), (8, 67, 515, (0, 1, 2, 4, 5, 6, 7)), (9, 512, 515, (8,))])
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_loss_of_few_rows(n, d, v, ignored, reduction, dtype):
+    from mamba3_b200 import linear_cross_entropy
+
+    h, w, t = loss_inputs(n, d, v, dtype)
+    clean = h.clone()
+    for r in ignored:
+        t[r] = -100
+        h[r] = float("nan")
+    kept = [r for r in range(n) if r not in ignored]
+    t[kept[0]], t[kept[-1]] = 0, v - 1
+    h.requires_grad_(True), w.requires_grad_(True)
+    y = linear_cross_entropy(h, w, t, reduction=reduction)
+    dl = rnd(n, seed=9) if reduction == "none" else torch.tensor(-1.5, device="cuda")
+    dh, dw = torch.autograd.grad(y, (h, w), dl, retain_graph=True)
+    want = ref.loss(clean, w, t, reduction=reduction, dloss=dl)
+    ref.check(y, want["loss"], "loss")
+    ref.check(dh, want["hidden"], "dhidden")
+    ref.check(dw, want["weight"], "dweight")
+    again = torch.autograd.grad(linear_cross_entropy(h, w, t, reduction=reduction), (h, w), dl)
+    assert torch.equal(again[0], dh) and torch.equal(again[1], dw)
+    # one gradient alone.  (Nine rows take the general form, which may split a product's sum in other places
+    # when it runs alone: other orders of the same terms, each within the bound of every order.)
+    only_h, = torch.autograd.grad(linear_cross_entropy(h, w.detach(), t, reduction=reduction), h, dl)
+    only_w, = torch.autograd.grad(linear_cross_entropy(h.detach(), w, t, reduction=reduction), w, dl)
+    ref.check(only_h, want["hidden"], "dhidden alone")
+    ref.check(only_w, want["weight"], "dweight alone")
+    if n <= 8:
+        assert torch.equal(only_h, dh) and torch.equal(only_w, dw)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_loss_of_few_rows_at_its_edges(dtype):
+    """No kept row, targets out of range, infinite and large logits, rows and weights that start anywhere."""
+    from mamba3_b200 import M3bError, check_device_errors, linear_cross_entropy
+
+    h, w, t = loss_inputs(6, 64, 300, dtype)
+    none = torch.full_like(t, -100)
+    for reduction, want in (("mean", math.nan), ("sum", 0.0)):
+        a, b = h.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        y = linear_cross_entropy(a, b, none, reduction=reduction)
+        assert y.item() == want or (math.isnan(want) and math.isnan(y.item()))
+        y.backward()
+        assert not a.grad.any() and not b.grad.any()
+    assert not linear_cross_entropy(h, w, none, reduction="none").any()
+    for bad in (300, -1, 2 ** 40):
+        s = t.clone()
+        s[4] = bad
+        a = h.clone().requires_grad_(True)
+        y = linear_cross_entropy(a, w, s, reduction="none")
+        assert torch.isnan(y).nonzero().flatten().tolist() == [4]
+        g, = torch.autograd.grad(y.sum(), a)
+        assert torch.isnan(g).any(1).nonzero().flatten().tolist() == [4]
+        with pytest.raises(M3bError, match="invalid argument"):
+            check_device_errors()
+    # columns of -infinity leave the others as they are; a row of them, or one of +infinity, has no loss
+    a, b = h.abs(), w.clone()
+    b[7] = float("-inf")
+    s = t.clone()
+    s[s == 7] = 8
+    keep = torch.arange(300, device="cuda") != 7
+    want = ref.loss(a, b[keep], s - (s > 7).long(), reduction="none")["loss"]
+    ref.check(linear_cross_entropy(a, b, s, reduction="none"), want, "a column of -infinity")
+    for x in (float("inf"), float("-inf")):
+        assert torch.isnan(linear_cross_entropy(a, torch.full_like(b, x), s, reduction="none")).all()
+    ref.check(linear_cross_entropy(h * 512, w, t, reduction="none"), ref.loss(h * 512, w, t, reduction="none")["loss"], "large")
+    want = ref.loss(h, w, t, dloss=1.0)
+    for off, width in ((8, 80), (3, 71)):
+        buf = torch.full((6, width), float("nan"), device="cuda", dtype=dtype)
+        buf[:, off:off + 64] = h
+        flat = torch.empty(300 * 64 + 8, device="cuda", dtype=dtype)
+        moved = flat[off:off + 300 * 64].view(300, 64) if off == 3 else w.clone()
+        moved.copy_(w)
+        a, b = buf[:, off:off + 64].detach().requires_grad_(True), moved.detach().requires_grad_(True)
+        y = linear_cross_entropy(a, b, t)
+        ref.check(y, want["loss"], f"rows at {off}")
+        dh, dw = torch.autograd.grad(y, (a, b))
+        ref.check(dh, want["hidden"], "dhidden")
+        ref.check(dw, want["weight"], "dweight")
+
+
+def test_loss_of_few_rows_captured():
+    from mamba3_b200 import linear_cross_entropy
+
+    h, w, t = loss_inputs(5, 200, 3001, torch.bfloat16)
+    h.requires_grad_(True), w.requires_grad_(True)
+
+    def step():
+        y = linear_cross_entropy(h, w, t)
+        return (y,) + torch.autograd.grad(y, (h, w))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for seed in (1, 2):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        with torch.no_grad():
+            h.copy_(torch.randn(5, 200, device="cuda", generator=g))
+            t.copy_(torch.randint(0, 3001, (5,), device="cuda", generator=g))
+            t[seed] = -100
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b)
