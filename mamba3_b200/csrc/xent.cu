@@ -11,7 +11,12 @@
 // joins the tiles' statistics.  Backward: a piece of the vocabulary at a time, the logits once more
 // with the softmax as their epilogue, and the piece's share of both gradients; dh is summed over the
 // pieces in fp32.  8 rows d_model vocab operations forward and backward, 2 more than with the
-// logits kept.
+// logits kept.  At most kSmallXentRows rows take the matrix-vector form of xent_small.cu.
+//
+// Bound by the tensor cores, and in long runs by the power they draw.  4096 x 768 x 32000 bf16: the forward
+// product 132 us (tensor pipe 92 % active, 1.53 PFLOP/s), softmax - onehot 142 us (84 %; what else it takes is
+// its 262 MB on their way out), both gradients 269 us (87 %, 1.50 PFLOP/s); the copy of the rows, the join and
+// the gradients' join are 30 us together.  With four tenths of the targets ignored, 451 us in all.
 #include "gemm.cuh"
 #include "xent_small.h"
 

@@ -10,6 +10,10 @@
 // and never made twice.  fp32 multiply-adds on CUDA cores from the operands as they are: 8 rows of 1408 x
 // 21251 are 240 M of them a product, 7 us, beside 120 MB, 18 us, in fp32, where the tensor cores' six plane
 // products of padded rows and the planes themselves cost far more.  Every sum has a fixed order.
+// Measured, forward and backward: those 8 fp32 rows 143 us (the tensor-core form 583), of them 45 the logits
+// and 51 the gradients (4.7 TB/s); 8 rows of 2048 x 50257 bf16 244 us, 81 and 147 (2.8 TB/s: eight products
+// of every 16-bit weight and their conversions, 128 registers a thread); 1 row of 768 x 32000 bf16 is bound
+// by the host's calls (140 us; on the device 9, 7, 30).
 #include "xent_small.h"
 
 #include <float.h>
@@ -23,7 +27,8 @@ namespace {
 
 constexpr int kWarps = 4;        // of the logits' and gradients' blocks
 constexpr int kRowsWarp = 4;     // weight rows of a warp: their loads are in flight together
-constexpr int kRun = 32;         // weight rows whose dz are made at once
+constexpr int kRun = 128;        // weight rows whose dz are made at once
+constexpr int kSliceStep = 32;   // weight rows of a block: a multiple of this
 constexpr int kAhead = 8;        // of them, rows loaded ahead
 constexpr int kGroups = 16;      // dh: groups of shares summed side by side
 constexpr float kToLog2 = 1.4426950408889634f;
@@ -117,7 +122,7 @@ __device__ __forceinline__ float2 join(float2 a, float2 b) {
 }
 
 template <typename T, int M>
-__global__ void __launch_bounds__(32 * kWarps) logits_rows_kernel(SmallXent p) {
+__global__ void __launch_bounds__(32 * kWarps, 4) logits_rows_kernel(SmallXent p) {
   __shared__ float2 stat[kWarps][M];
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -249,19 +254,20 @@ __global__ void __launch_bounds__(1024) loss_rows_kernel(SmallXent p) {
 // A thread owns four columns of d_model: its part of the kept rows and of dh stay in registers while the
 // block walks its slice of the vocabulary, kRun rows' dz at a time in shared memory.
 template <typename T, int M>
-__global__ void __launch_bounds__(32 * kWarps) grads_rows_kernel(SmallXent p) {
+__global__ void __launch_bounds__(32 * kWarps, 4) grads_rows_kernel(SmallXent p) {
   __shared__ alignas(16) float dz[kRun][M];
   pdl_launch_dependents();
   const int tid = threadIdx.x, n = *p.count;
   const int64_t c0 = ((int64_t)blockIdx.x * (32 * kWarps) + tid) * 4;
   const bool in = c0 < p.D;
-  float h[M][4], acc[M][4];
+  float2 h[M][2], acc[M][2];  // pairs: packed fp32 arithmetic halves the multiply-adds' instructions
+  auto kept_at = [&](int m, int e) { return m < n && c0 + e < p.D ? p.hs[(int64_t)m * p.D + c0 + e] : 0.f; };
 #pragma unroll
   for (int m = 0; m < M; ++m)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      h[m][e] = m < n && c0 + e < p.D ? p.hs[(int64_t)m * p.D + c0 + e] : 0.f;
-      acc[m][e] = 0.f;
+    for (int e = 0; e < 2; ++e) {
+      h[m][e] = make_float2(kept_at(m, 2 * e), kept_at(m, 2 * e + 1));
+      acc[m][e] = make_float2(0.f, 0.f);
     }
   const T* w = static_cast<const T*>(p.w);
   T* dw = static_cast<T*>(p.dw);
@@ -306,14 +312,16 @@ __global__ void __launch_bounds__(32 * kWarps) grads_rows_kernel(SmallXent p) {
 #pragma unroll
           for (int m = 0; m < M; ++m)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[m][e] = fmaf(z[m], wv[i][e], acc[m][e]);
+            for (int e = 0; e < 2; ++e)
+              acc[m][e] = fma2(make_float2(z[m], z[m]), make_float2(wv[i][2 * e], wv[i][2 * e + 1]), acc[m][e]);
         }
         if (p.dw) {
-          float g[4] = {0.f, 0.f, 0.f, 0.f};
+          float2 q[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
           for (int m = 0; m < M; ++m)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) g[e] = fmaf(z[m], h[m][e], g[e]);
+            for (int e = 0; e < 2; ++e) q[e] = fma2(make_float2(z[m], z[m]), h[m][e], q[e]);
+          const float g[4] = {q[0].x, q[0].y, q[1].x, q[1].y};
           T* dst = dw + (r0 + k + i) * p.D + c0;
           if (p.vec) {
             store_row4(dst, g);
@@ -331,7 +339,8 @@ __global__ void __launch_bounds__(32 * kWarps) grads_rows_kernel(SmallXent p) {
   for (int m = 0; m < M; ++m)
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (m < n && c0 + e < p.D) p.share[((int64_t)blockIdx.y * M + m) * p.D + c0 + e] = acc[m][e];
+      if (m < n && c0 + e < p.D)
+        p.share[((int64_t)blockIdx.y * M + m) * p.D + c0 + e] = e & 1 ? acc[m][e / 2].y : acc[m][e / 2].x;
 }
 
 // 32 columns of one row per block: the slices' shares, kGroups sums side by side.
@@ -422,10 +431,10 @@ int small_xent_fwd(const m3b_linear_xent_args* a, void* workspace, size_t* need,
 int small_xent_bwd(const m3b_linear_xent_args* a, void* workspace, size_t* need, bool run, cudaStream_t st) {
   SmallXent p{};
   carve_saved(a, &p);
-  // four blocks a SM, slices of whole runs
+  // four blocks a SM: all resident
   const int64_t blocks = (p.D + 128 * kWarps - 1) / (128 * kWarps), want = (int64_t)num_sms() * 4 / blocks;
   const int64_t rows = (p.V + (want > 1 ? want : 1) - 1) / (want > 1 ? want : 1);
-  p.slice_rows = (int)((rows + kRun - 1) / kRun * kRun);
+  p.slice_rows = (int)((rows + kSliceStep - 1) / kSliceStep * kSliceStep);
   p.slices = (int)((p.V + (int64_t)p.slice_rows - 1) / p.slice_rows);
   *need = a->dhidden ? (size_t)p.slices * form_of(p.T) * p.D * 4 : 4;
   if (!run) return M3B_OK;
