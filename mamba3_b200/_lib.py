@@ -968,15 +968,16 @@ def linear_xent_bwd(rows, weight, saved, dloss, ignore_index, reduction, want_hi
 def grad_clip(ptrs, numel, dtypes, out_ptrs, out_dtypes, max_norm, inf_norm, dev):
     """Launch the global norm over tensors on `dev`, given as lists of addresses, lengths and dtypes, and,
     with out_ptrs (the same list for in place), the clipped values.  Returns the norm (fp32, on `dev`)."""
-    code = _DT.__getitem__
-    gp, num = array.array("Q", ptrs), array.array("q", numel)
-    gd = array.array("i", map(code, dtypes))
+    def codes(dts):  # mostly one dtype, hundreds of times
+        return array.array("i", [_DT[dts[0]]]) * len(dts) if len(set(dts)) == 1 else array.array("i", map(_DT.get, dts))
+
+    gp, num, gd = array.array("Q", ptrs), array.array("q", numel), codes(dtypes)
     op, od = gp, gd
     norm = torch.empty((), dtype=torch.float32, device=dev)
     a = GradClipArgs(len(ptrs))
     a.grads, a.numel, a.grad_dtype = gp.buffer_info()[0], num.buffer_info()[0], gd.buffer_info()[0]
     if out_ptrs is not ptrs:
-        op, od = array.array("Q", out_ptrs), array.array("i", map(code, out_dtypes))
+        op, od = array.array("Q", out_ptrs), codes(out_dtypes)
     a.outs, a.out_dtype = op.buffer_info()[0], od.buffer_info()[0]
     a.norm_type, a.max_norm, a.norm = (0 if inf_norm else 2), max_norm, norm.data_ptr()
     L = lib()

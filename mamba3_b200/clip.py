@@ -71,20 +71,22 @@ def clip_grads(grads: Iterable[torch.Tensor], max_norm: float, norm_type: float 
                 raise ValueError("clip_grads: each output needs its gradient's shape and memory order")
     ptrs = list(map(_data_ptr, gs))
     out_ptrs = ptrs
+    full = 0 not in numel  # an empty tensor may have any address: it is in nobody's place
     if os is not gs:
         if numel != list(map(_numel, os)):
             raise ValueError("clip_grads: each output needs its gradient's length")
         out_ptrs = list(map(_data_ptr, os))
-        if not {p for p, n in zip(out_ptrs, numel) if n}.isdisjoint(ptrs):
-            for n, p, q, a, b in zip(numel, ptrs, out_ptrs, dtypes, out_dtypes):
-                if n and p == q and a != b:
-                    raise ValueError("clip_grads: an output in its gradient's place needs its dtype")
-                if n and p != q and q in ptrs:  # (an empty gradient may have any address)
-                    if any(q == r and k for r, k in zip(ptrs, numel)):
-                        raise ValueError("clip_grads: an output in another gradient's place")
-    used = [p for p, n in zip(out_ptrs, numel) if n]
-    if len(set(used)) != len(used):
+    written = out_ptrs if full else [p for p, n in zip(out_ptrs, numel) if n]
+    places = set(written)
+    if len(places) != len(written):
         raise ValueError("clip_grads: the same tensor twice")
+    if os is not gs and not places.isdisjoint(ptrs):
+        read = set(ptrs if full else (p for p, n in zip(ptrs, numel) if n))
+        for n, p, q, a, b in zip(numel, ptrs, out_ptrs, dtypes, out_dtypes):
+            if n and p == q and a != b:
+                raise ValueError("clip_grads: an output in its gradient's place needs its dtype")
+            if n and p != q and q in read:
+                raise ValueError("clip_grads: an output in another gradient's place")
     return _lib.grad_clip(ptrs, numel, dtypes, out_ptrs, out_dtypes, max_norm, norm_type == math.inf, gs[0].device)
 
 
