@@ -15,7 +15,8 @@
 //
 // 16384 x 768 x 2112 bf16, forward and backward, 509 us: gate | up 93 us (tensor pipe 66 % active; it writes
 // 277 MB of act, g and u), down 48 us (71 %), dg and du 96 us (34 %: 12 K blocks a tile beside its g and u on
-// their way in, dg and du out: 250 and 106 MB, 45 % of HBM's time), dx and the three weight gradients 192 us (87 %, 1.39 PFLOP/s).
+// their way in, dg and du out: 250 and 106 MB, 45 % of HBM's time), dx and the three weight gradients 192 us
+// (87 %, 1.39 PFLOP/s).
 #include "ffn_small.h"
 #include "gemm.cuh"
 

@@ -24,6 +24,8 @@ def test_entry_points_reject_bad_arguments():
         assert L.m3b_gated_ffn_fwd_workspace(ctypes.byref(bad)) == 0
     x = _lib.LinearXentArgs(4, 64, -100, 64, 1000, 1, 1)
     assert L.m3b_linear_xent_fwd(ctypes.byref(x), None, 0, None) == 1 and b"null" in L.m3b_last_error()
+    assert L.m3b_linear_xent_saved(ctypes.byref(x)) >= 4 * 64 * 4 + 4 * 1000 * 4  # few rows: in fp32, and the logits
+    x.rows = 40
     assert L.m3b_linear_xent_saved(ctypes.byref(x)) >= 256 * 64 * 2 + 3 * 256 * 4
     x.reduction = 3
     assert L.m3b_linear_xent_fwd(ctypes.byref(x), None, 0, None) == 1 and b"reduction" in L.m3b_last_error()
@@ -45,6 +47,11 @@ def test_short_workspace_is_refused():
     assert L.m3b_gated_ffn_fwd(ctypes.byref(a), p, need, None) == 4
     x = _lib.LinearXentArgs(4, 64, -100, 64, 1000, 1, 1, p, p, p, p, p)
     assert L.m3b_linear_xent_fwd(ctypes.byref(x), None, 0, None) == 6
+    need = L.m3b_linear_xent_fwd_workspace(ctypes.byref(x))
+    assert L.m3b_linear_xent_fwd(ctypes.byref(x), p, need - 1, None) == 6
+    x.dloss = x.dhidden = x.dweight = p
+    need = L.m3b_linear_xent_bwd_workspace(ctypes.byref(x))
+    assert need >= 4 * 64 * 4 and L.m3b_linear_xent_bwd(ctypes.byref(x), p, need - 1, None) == 6
     one = (ctypes.c_void_p * 1)(p)
     num, dt = (ctypes.c_int64 * 1)(10), (ctypes.c_int32 * 1)(0)
     c = _lib.GradClipArgs(1, ctypes.addressof(one), ctypes.addressof(one), ctypes.addressof(num), ctypes.addressof(dt),
