@@ -927,6 +927,16 @@ def _xent_args(rows, d, weight, ignore_index, reduction):
     return a
 
 
+def xent_saved_bytes(hidden, vocab):
+    """m3b_linear_xent_saved of hidden (rows, d_model)."""
+    rows, d = hidden.shape
+    up = lambda n: (n + 255) // 256 * 256  # noqa: E731
+    if rows <= 8:
+        return up(rows * d * 4) + up(rows * vocab * 4) + 5 * 256
+    tp, planes = up(rows), 3 if hidden.dtype == torch.float32 else 1
+    return up(planes * tp * ((d + 7) // 8 * 8) * 2) + 3 * up(tp * 4) + 256
+
+
 def linear_xent_fwd(hidden, weight, target, ignore_index, reduction, save=True):
     """Launch the head's cross entropy; hidden (rows, d_model), weight (vocab, d_model) contiguous of
     the same dtype, target (rows) int64 contiguous.  Returns (loss fp32, saved): saved is what the backward

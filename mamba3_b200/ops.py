@@ -521,10 +521,7 @@ def _linear_xent_fwd_op(hidden: torch.Tensor, weight: torch.Tensor, target: torc
 
 @_linear_xent_fwd_op.register_fake
 def _(hidden, weight, target, ignore_index, reduction):
-    rows, d = hidden.shape
-    tp, planes = (rows + 255) // 256 * 256, 3 if hidden.dtype == torch.float32 else 1
-    up = lambda n: (n + 255) // 256 * 256  # noqa: E731
-    saved = up(planes * tp * ((d + 7) // 8 * 8) * 2) + 3 * up(tp * 4) + 256
+    saved = _lib.xent_saved_bytes(hidden, weight.shape[0])
     return (torch.empty((rows,) if reduction == "none" else (), dtype=torch.float32, device=hidden.device),
             torch.empty(saved, dtype=torch.uint8, device=hidden.device))
 

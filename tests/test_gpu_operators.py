@@ -802,3 +802,47 @@ def test_loss_of_few_rows_captured():
         torch.cuda.synchronize()
         for a, b in zip(got, step()):
             assert torch.equal(a, b)
+
+
+def test_loss_of_few_rows_offsets_past_32_bits():
+    """A weight of more than 2^31 values, zero but for a few rows: the sums have closed forms."""
+    from mamba3_b200 import linear_cross_entropy
+
+    d, v = 2048, (1 << 20) + 77
+    w = torch.zeros(v, d, device="cuda", dtype=torch.bfloat16)
+    at = torch.tensor([0, 5, 1 << 20, v - 1], device="cuda")
+    w[at] = rnd(4, d, seed=2, std=2.0 * d ** -0.5, dtype=torch.bfloat16)
+    h = rnd(3, d, seed=1, dtype=torch.bfloat16).requires_grad_(True)
+    t = torch.tensor([v - 1, 1 << 20, 9], device="cuda")
+    y = linear_cross_entropy(h, w.requires_grad_(True), t, reduction="sum")
+    dh, dw = torch.autograd.grad(y, (h, w))
+    H, W = h.detach().double(), w.detach()[at].double()
+    z = H @ W.t()
+    lse = (z.exp().sum(1) + (v - 4)).log()
+    loss = lse.sum() - z[0, 3] - z[1, 2]
+    # 600 steps of 2^-23 for the statistics (as in the plain form), 2^-14 with the logits' sums
+    assert abs(y.item() - loss.item()) <= 2.0 ** -14 * 3 + 2.0 ** -23 * abs(loss.item())
+    p = (z - lse[:, None]).exp()
+    rest = (-lse).exp()  # of every zero row
+    dz = p.clone()
+    dz[0, 3] -= 1.0
+    dz[1, 2] -= 1.0
+    want, by = dz @ W, dz.abs() @ W.abs()
+    assert bool(((dh.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -13 * by + 2.0 ** -60).all())
+    for row, c in ((0, dz[:, 0]), (5, dz[:, 1]), (1 << 20, dz[:, 2]), (v - 1, dz[:, 3]), (9, rest - torch.tensor(
+            [0.0, 0.0, 1.0], device="cuda", dtype=torch.float64)), (v - 2, rest)):
+        want, by = c @ H, c.abs() @ H.abs()
+        assert bool(((dw[row].double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -13 * by).all()), row
+
+
+def test_loss_of_few_rows_under_compile():
+    from mamba3_b200 import linear_cross_entropy
+
+    h, w, t = loss_inputs(6, 64, 333, torch.bfloat16)
+    leaves = [h.requires_grad_(True), w.requires_grad_(True)]
+    eager = linear_cross_entropy(*leaves, t)
+    want = torch.autograd.grad(eager, leaves)
+    got = torch.compile(lambda a, b: linear_cross_entropy(a, b, t), backend="aot_eager")(*leaves)
+    assert torch.equal(got, eager)
+    for a, b in zip(torch.autograd.grad(got, leaves), want):
+        assert torch.equal(a, b)

@@ -64,10 +64,13 @@ def test_short_workspace_is_refused():
 @pytest.mark.parametrize("dtype,code", [(torch.float32, 0), (torch.bfloat16, 1), (torch.float16, 2)])
 def test_saved_sizes_agree_with_the_library(dtype, code):
     L = _lib.lib()
-    for rows, f in ((0, 8), (1, 1), (7, 33), (256, 2112), (257, 100)):
+    for rows, f in ((0, 8), (1, 1), (7, 33), (8, 64), (9, 64), (256, 2112), (257, 100)):
         a = _lib.GatedFfnArgs(rows, 64, 0, 64, 64, f, code)
         want = L.m3b_gated_ffn_act_bytes(ctypes.byref(a)), L.m3b_gated_ffn_gu_bytes(ctypes.byref(a))
         assert _lib.ffn_saved_bytes(torch.empty(rows, 64, dtype=dtype), f) == want
+        for d in (64, 33):
+            x = _lib.LinearXentArgs(rows, d, -100, d, 1003, code, 1)
+            assert _lib.xent_saved_bytes(torch.empty(rows, d, dtype=dtype), 1003) == L.m3b_linear_xent_saved(ctypes.byref(x))
 
 
 def test_sizes_past_the_limits_are_refused():
