@@ -31,6 +31,8 @@ class SwiGLU(nn.Module):
     """w_down(silu(w_gate x) * w_up x)  (mamba3/block.py:16-26).  With ``fused`` it runs as the
     gated_ffn operator, forward and backward, and can take the block's scaled residual along."""
 
+    fused = False  # of modules pickled without the attribute
+
     def __init__(self, d_model: int, d_ff: int | None = None, bias: bool = False, *, fused: bool = False):
         super().__init__()
         self.fused = bool(fused)
@@ -107,7 +109,8 @@ class KulaMambaBlock(nn.Module):
         if self.use_mlp:
             if self.gradient_checkpointing and self.training:
                 m = grad_checkpoint(lambda t: self.mlp(self.mlp_norm(t)), x, use_reentrant=False)
-            elif self.mlp.fused and not torch.is_autocast_enabled("cuda"):  # autocast keeps the stream's dtype
+            elif getattr(self.mlp, "fused", False) and not torch.is_autocast_enabled("cuda"):
+                # (under autocast the residual stream keeps a dtype of its own)
                 return self.mlp(self.mlp_norm(x), x, self.residual_scale)
             else:
                 m = self.mlp(self.mlp_norm(x))
@@ -221,6 +224,8 @@ class KulaMambaLM(nn.Module):
         if not return_logits:
             if labels is None:
                 raise ValueError("return_logits=False needs labels")
+            if not isinstance(self.lm_head, nn.Linear) or self.lm_head.bias is not None:
+                raise ValueError("return_logits=False needs an nn.Linear without bias as lm_head")
             h = self._hidden(input_ids)
             # token t predicts label t + 1; the last one predicts nothing
             targets = F.pad(labels[:, 1:], (0, 1), value=-100)

@@ -846,3 +846,15 @@ def test_loss_of_few_rows_under_compile():
     assert torch.equal(got, eager)
     for a, b in zip(torch.autograd.grad(got, leaves), want):
         assert torch.equal(a, b)
+
+
+def test_block_with_another_module_as_its_mlp():
+    from mamba3_b200 import KulaMambaBlock
+
+    blk = KulaMambaBlock(64, d_state=16, headdim=16).cuda().bfloat16()
+    blk.mlp = torch.nn.Linear(64, 64).cuda().bfloat16()
+    x = rnd(2, 64, 64, seed=1, dtype=torch.bfloat16)
+    assert blk(x).shape == x.shape
+    blk.train()
+    blk(x.requires_grad_(True)).float().sum().backward()
+    assert blk.mlp.weight.grad.any()

@@ -1,6 +1,7 @@
 """Refusals and host logic of the training and serving operators (no kernel launches)."""
 
 import ctypes
+import pickle
 import math
 
 import pytest
@@ -164,3 +165,22 @@ def test_lm_options():
     assert set(lm.state_dict()) == set(plain.state_dict())
     with pytest.raises(ValueError, match="labels"):
         lm(torch.zeros(1, 4, dtype=torch.long), return_logits=False)
+
+
+def test_modules_pickled_without_the_fused_attribute():
+    mlp = m.SwiGLU(8, 16, fused=True)
+    del mlp.__dict__["fused"]
+    old = pickle.loads(pickle.dumps(mlp))
+    assert old.fused is False
+
+
+def test_loss_without_logits_needs_a_plain_head():
+    """Only its weight is read: a head that does more is refused, before anything runs."""
+    lm = m.KulaMambaLM(vocab_size=50, d_model=64, n_layers=1, d_state=16, headdim=16)
+    ids = torch.zeros(1, 4, dtype=torch.long)
+    with pytest.raises(ValueError, match="labels"):
+        lm(ids, return_logits=False)
+    for head in (torch.nn.Linear(64, 50), torch.nn.Sequential(torch.nn.Linear(64, 50, bias=False))):
+        lm.lm_head = head
+        with pytest.raises(ValueError, match="lm_head"):
+            lm(ids, ids, return_logits=False)
