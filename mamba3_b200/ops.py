@@ -522,7 +522,7 @@ def _linear_xent_fwd_op(hidden: torch.Tensor, weight: torch.Tensor, target: torc
 @_linear_xent_fwd_op.register_fake
 def _(hidden, weight, target, ignore_index, reduction):
     saved = _lib.xent_saved_bytes(hidden, weight.shape[0])
-    return (torch.empty((rows,) if reduction == "none" else (), dtype=torch.float32, device=hidden.device),
+    return (torch.empty(hidden.shape[:1] if reduction == "none" else (), dtype=torch.float32, device=hidden.device),
             torch.empty(saved, dtype=torch.uint8, device=hidden.device))
 
 
