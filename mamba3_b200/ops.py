@@ -475,14 +475,14 @@ def _gated_ffn_fwd_op(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
                       residual: Optional[torch.Tensor], scale: float,
                       save: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     out, act, gu = _lib.gated_ffn_fwd(x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual, scale, save)
-    return out, act, _opt(gu, x.device)
+    return out, _opt(act if save else None, x.device), _opt(gu, x.device)
 
 
 @_gated_ffn_fwd_op.register_fake
 def _(x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual, scale, save):
     act, gu = _lib.ffn_saved_bytes(x, w_gate.shape[0])
     u8 = dict(dtype=torch.uint8, device=x.device)
-    return x.new_empty(x.shape), torch.empty(act, **u8), torch.empty(gu if save else 0, **u8)
+    return x.new_empty(x.shape), torch.empty(act if save else 0, **u8), torch.empty(gu if save else 0, **u8)
 
 
 @torch.library.custom_op("mamba3_b200::gated_ffn_bwd", mutates_args=())
