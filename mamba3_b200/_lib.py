@@ -893,7 +893,8 @@ def gated_ffn_fwd(x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual, scale
     # act and the workspace in one allocation where act is not kept
     room = -(-n // 256) * 256
     act = _bytes(n if save else room + need, dev)
-    ws = (_bytes(need, dev).data_ptr() if need else None) if save else act.data_ptr() + room
+    own = _bytes(need, dev) if save and need else None  # held until the launches are made
+    ws = _addr(own) if save else act.data_ptr() + room
     a.saved_act, a.out = act.data_ptr(), out.data_ptr()
     _call(L.m3b_gated_ffn_fwd, "m3b_gated_ffn_fwd", index, p, ws, need)
     return out, act, gu
@@ -953,7 +954,8 @@ def linear_xent_fwd(hidden, weight, target, ignore_index, reduction, save=True):
     # what is saved and the workspace in one allocation where nothing is kept
     room = -(-n // 256) * 256
     saved = _bytes(n if save else room + need, dev)
-    ws = _bytes(need, dev).data_ptr() if save else saved.data_ptr() + room
+    own = _bytes(need, dev) if save else None  # held until the launches are made
+    ws = _addr(own) if save else saved.data_ptr() + room
     a.saved, a.loss = saved.data_ptr(), loss.data_ptr()
     _call(L.m3b_linear_xent_fwd, "m3b_linear_xent_fwd", index, p, ws, need)
     return loss, saved

@@ -1,5 +1,7 @@
 """The Python side of the training and serving operators: traced forms, workspaces, modules (no kernel launches)."""
 
+import weakref
+
 import pytest
 import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
@@ -38,3 +40,33 @@ def test_traced_ffn_returns_what_the_call_returns(rows, dtype, save, no_launches
     assert len(no_launches) == 1
     for a, b in zip(got, want):
         assert a.shape == b.shape and a.dtype == b.dtype and a.stride() == b.stride()
+
+
+@pytest.mark.parametrize("rows", [3, 40])
+@pytest.mark.parametrize("save", [True, False])
+def test_workspaces_live_until_the_launches_are_made(rows, save, monkeypatch, no_launches):
+    """A block that is given back before the call could be handed to another thread between its launches."""
+    given, dead = [], []
+    real = _lib._bytes
+
+    def counted(n, dev):
+        t = real(n, dev)
+        given.append(weakref.ref(t))
+        return t
+
+    monkeypatch.setattr(_lib, "_bytes", counted)
+    monkeypatch.setattr(_lib, "_call", lambda fn, what, *a: dead.append((what, sum(r() is None for r in given))))
+    z = lambda *s: torch.zeros(s)  # noqa: E731
+    x, wg, wu, wd = z(rows, 33), z(24, 33), z(24, 33), z(33, 24)
+    out, act, gu = _lib.gated_ffn_fwd(x, wg, wu, wd, None, None, None, None, 1.0, save)
+    if save:
+        given.clear()
+        _lib.gated_ffn_bwd(x, wg, wu, wd, None, None, None, 1.0, act, gu, x, [True] * 7)
+    given.clear()
+    loss, saved = _lib.linear_xent_fwd(x, wg, torch.zeros(rows, dtype=torch.long), -100, "mean", save)
+    if save:
+        given.clear()
+        _lib.linear_xent_bwd(rows, wg, saved, loss, -100, "mean", True, True)
+    given.clear()
+    _lib.grad_clip([x.data_ptr()], [x.numel()], [x.dtype], [x.data_ptr()], [x.dtype], 1.0, False, x.device)
+    assert len(dead) == (5 if save else 3) and not any(n for _, n in dead), dead
