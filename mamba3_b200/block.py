@@ -228,7 +228,7 @@ class KulaMambaLM(nn.Module):
                 raise ValueError("return_logits=False needs an nn.Linear without bias as lm_head")
             h = self._hidden(input_ids)
             # token t predicts label t + 1; the last one predicts nothing
-            targets = F.pad(labels[:, 1:], (0, 1), value=-100)
+            targets = F.pad(labels[:, 1:].long(), (0, 1), value=-100)
             return {"loss": linear_cross_entropy(h, self.lm_head.weight, targets)}
         logits = self.lm_head(self._hidden(input_ids))
         result = {"logits": logits}

@@ -6,7 +6,7 @@ import pytest
 import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
 
-from mamba3_b200 import _lib
+from mamba3_b200 import _lib, block
 
 
 @pytest.mark.parametrize("reduction,per_row", [("none", True), ("mean", False), ("sum", False)])
@@ -70,3 +70,15 @@ def test_workspaces_live_until_the_launches_are_made(rows, save, monkeypatch, no
     given.clear()
     _lib.grad_clip([x.data_ptr()], [x.numel()], [x.dtype], [x.data_ptr()], [x.dtype], 1.0, False, x.device)
     assert len(dead) == (5 if save else 3) and not any(n for _, n in dead), dead
+
+
+def test_labels_of_any_integer_type(monkeypatch):
+    """The last token predicts nothing: its label is the ignored one also where the labels' type cannot hold it."""
+    seen = []
+    monkeypatch.setattr(block, "linear_cross_entropy", lambda h, w, t: seen.append(t) or h.sum())
+    lm = block.KulaMambaLM(vocab_size=50, d_model=64, n_layers=1, d_state=16, headdim=16)
+    monkeypatch.setattr(lm, "_hidden", lambda ids: torch.zeros(*ids.shape, 64))
+    ids = torch.tensor([[3, 4, 5]])
+    for dt in (torch.int64, torch.int32, torch.int16, torch.uint8):
+        lm(ids, ids.to(dt), return_logits=False)
+        assert seen.pop().tolist() == [[4, 5, -100]]
