@@ -27,9 +27,16 @@ def _residual(x, h, scale):
     return ops.scaled_add(x, h, scale) if ops.kernel_ok(x, h) else x + h * scale
 
 
+def _unhooked(m, cls):
+    """Calling m runs cls.forward and nothing around it: no override, no forward of its own, no hooks."""
+    return (isinstance(m, cls) and type(m).forward is cls.forward and "forward" not in m.__dict__
+            and not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks))
+
+
 class SwiGLU(nn.Module):
     """w_down(silu(w_gate x) * w_up x)  (mamba3/block.py:16-26).  With ``fused`` it runs as the
-    gated_ffn operator, forward and backward, and can take the block's scaled residual along."""
+    gated_ffn operator, forward and backward, and can take the block's scaled residual along; projections
+    that do more than a Linear (an adapter, a hook) run as modules all the same."""
 
     fused = False  # of modules pickled without the attribute
 
@@ -54,13 +61,13 @@ class SwiGLU(nn.Module):
 
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None, scale: float = 1.0) -> torch.Tensor:
         """The MLP of x; with `residual`, residual + scale * MLP(x) (in the operator's epilogue when fused)."""
-        if self.fused:
+        plain = _unhooked(self.w_gate, nn.Linear) and _unhooked(self.w_up, nn.Linear)
+        if self.fused and plain and _unhooked(self.w_down, nn.Linear):
             return gated_ffn(x, self.w_gate.weight, self.w_up.weight, self.w_down.weight, b_gate=self.w_gate.bias,
                              b_up=self.w_up.bias, b_down=self.w_down.bias, residual=residual, residual_scale=scale)
         if residual is not None:
             return _residual(residual, self.forward(x), scale)
-        d_ff = self.w_gate.out_features
-        if (ops.kernel_ok(x) and d_ff % 8 == 0
+        if (ops.kernel_ok(x) and plain and self.w_gate.out_features % 8 == 0
                 and not (torch.is_grad_enabled() and any(p.requires_grad for p in self.parameters()))):
             # inference: the gate and up projections as one GEMM over the stacked weights
             w, b = self._stacked()
@@ -109,8 +116,8 @@ class KulaMambaBlock(nn.Module):
         if self.use_mlp:
             if self.gradient_checkpointing and self.training:
                 m = grad_checkpoint(lambda t: self.mlp(self.mlp_norm(t)), x, use_reentrant=False)
-            elif getattr(self.mlp, "fused", False) and not torch.is_autocast_enabled("cuda"):
-                # (under autocast the residual stream keeps a dtype of its own)
+            elif _unhooked(self.mlp, SwiGLU) and self.mlp.fused and not torch.is_autocast_enabled("cuda"):
+                # (under autocast the residual stream keeps a dtype of its own; a hook is for the MLP's own output)
                 return self.mlp(self.mlp_norm(x), x, self.residual_scale)
             else:
                 m = self.mlp(self.mlp_norm(x))
@@ -224,8 +231,8 @@ class KulaMambaLM(nn.Module):
         if not return_logits:
             if labels is None:
                 raise ValueError("return_logits=False needs labels")
-            if not isinstance(self.lm_head, nn.Linear) or self.lm_head.bias is not None:
-                raise ValueError("return_logits=False needs an nn.Linear without bias as lm_head")
+            if not _unhooked(self.lm_head, nn.Linear) or self.lm_head.bias is not None:
+                raise ValueError("return_logits=False needs a plain nn.Linear without bias or hooks as lm_head")
             h = self._hidden(input_ids)
             # token t predicts label t + 1; the last one predicts nothing
             targets = F.pad(labels[:, 1:].long(), (0, 1), value=-100)

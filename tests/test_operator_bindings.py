@@ -4,6 +4,7 @@ import weakref
 
 import pytest
 import torch
+import torch.nn.utils.parametrize
 from torch._subclasses.fake_tensor import FakeTensorMode
 
 from mamba3_b200 import _lib, block
@@ -82,3 +83,79 @@ def test_labels_of_any_integer_type(monkeypatch):
     for dt in (torch.int64, torch.int32, torch.int16, torch.uint8):
         lm(ids, ids.to(dt), return_logits=False)
         assert seen.pop().tolist() == [[4, 5, -100]]
+
+
+class _Adapter(torch.nn.Linear):
+    def forward(self, x):
+        return super().forward(x) + 1.0
+
+
+def _altered(linear, how):
+    """`linear` doing more than its weight and bias say."""
+    if how == "subclass":
+        other = _Adapter(linear.in_features, linear.out_features, bias=linear.bias is not None)
+        other.load_state_dict(linear.state_dict())
+        return other
+    if how == "wrapped":
+        return torch.nn.Sequential(linear)
+    if how == "forward hook":
+        linear.register_forward_hook(lambda mod, args, out: out + 1.0)
+    elif how == "pre-hook":
+        linear.register_forward_pre_hook(lambda mod, args: (args[0] + 1.0,))
+    elif how == "backward hook":
+        linear.register_full_backward_hook(lambda mod, gi, go: None)
+    else:
+        linear.forward = lambda x: torch.nn.functional.linear(x, linear.weight, linear.bias) + 1.0
+    return linear
+
+
+ALTERED = ["subclass", "wrapped", "forward hook", "pre-hook", "backward hook", "own forward"]
+
+
+@pytest.mark.parametrize("how", ALTERED)
+@pytest.mark.parametrize("name", ["w_gate", "w_up", "w_down"])
+def test_fused_mlp_runs_projections_that_do_more_as_modules(name, how):
+    """The operator reads weights only (and refuses CPU tensors, so what returns here ran as modules)."""
+    mlp = block.SwiGLU(8, 16, bias=True, fused=True)
+    x, r = torch.randn(3, 8), torch.randn(3, 8)
+    with pytest.raises(_lib.M3bError, match="CUDA"):
+        mlp(x)
+    setattr(mlp, name, _altered(getattr(mlp, name), how))
+    want = mlp.w_down(torch.nn.functional.silu(mlp.w_gate(x)) * mlp.w_up(x))
+    assert torch.equal(mlp(x), want) and torch.allclose(mlp(x, r, 0.5), r + 0.5 * want)
+
+
+@pytest.mark.parametrize("how", ALTERED)
+def test_fused_mlp_with_a_parametrised_or_hooked_module(how, monkeypatch):
+    """A parametrised Linear is its computed weight: the operator takes that.  A hook on the MLP itself sees the
+    MLP's output, without the residual."""
+    calls = []
+    monkeypatch.setattr(block, "gated_ffn", lambda x, *w, residual=None, residual_scale=1.0, **b:
+                        calls.append((w, residual)) or x)
+    blk = block.KulaMambaBlock(64, d_state=16, headdim=16, fused_mlp=True)
+    x = torch.randn(2, 3, 64)
+    blk._mlp_residual(x)
+    assert calls.pop()[1] is x and not calls
+    torch.nn.utils.parametrize.register_parametrization(blk.mlp.w_up, "weight", _Doubled())
+    blk._mlp_residual(x)
+    (w, r), = calls
+    assert r is x and torch.equal(w[1], blk.mlp.w_up.weight)
+    calls.clear()
+    if how in ("forward hook", "pre-hook", "backward hook"):
+        _altered(blk.mlp, how)
+        blk._mlp_residual(x)
+        assert calls.pop()[1] is None and not calls
+
+
+class _Doubled(torch.nn.Module):
+    def forward(self, w):
+        return 2 * w
+
+
+@pytest.mark.parametrize("how", ALTERED)
+def test_loss_without_logits_refuses_heads_that_do_more(how):
+    lm = block.KulaMambaLM(vocab_size=50, d_model=64, n_layers=1, d_state=16, headdim=16)
+    ids = torch.zeros(1, 4, dtype=torch.long)
+    lm.lm_head = _altered(lm.lm_head, how)
+    with pytest.raises(ValueError, match="lm_head"):
+        lm(ids, ids, return_logits=False)
