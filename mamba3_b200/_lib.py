@@ -13,6 +13,7 @@ import threading
 from pathlib import Path
 
 import torch
+import torch.autograd.forward_ad as fwAD
 
 _PKG = Path(__file__).resolve().parent
 LIB_PATH = _PKG / "libmamba3_b200.so"
@@ -819,6 +820,12 @@ def _same_gpu(name, ts):
             elif t.get_device() != dev:
                 raise M3bError(f"{name}: tensors on different devices: cuda:{dev} vs {t.device}")
     return dev
+
+
+def _no_tangent(name, ts):
+    """Refuse forward-mode derivatives, which a call of the library would drop without a word."""
+    if fwAD._current_level >= 0 and any(t is not None and fwAD.unpack_dual(t).tangent is not None for t in ts):
+        raise M3bError(f"{name}: forward-mode derivatives (jvp) are not supported")
 
 
 def _call(fn, what, index, *args):

@@ -57,6 +57,7 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
             for t in (x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual)]
     ts = [t for t in (x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual) if t is not None]
     _lib._same_gpu("gated_ffn", ts)
+    _lib._no_tangent("gated_ffn", ts)
     dt = x.dtype
     for t in ts:
         if t.dtype != dt:

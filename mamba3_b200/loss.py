@@ -47,6 +47,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
         dt = torch.get_autocast_dtype("cuda")
         hidden, weight = hidden.to(dt), weight.to(dt)
     _lib._same_gpu("linear_cross_entropy", (hidden, weight, targets))
+    _lib._no_tangent("linear_cross_entropy", (hidden, weight))
     if hidden.dtype != weight.dtype:
         raise _lib.M3bError(f"linear_cross_entropy: one dtype expected, got {hidden.dtype} and {weight.dtype}")
     _lib.dtype_code(hidden.dtype)

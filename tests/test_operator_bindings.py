@@ -4,10 +4,11 @@ import weakref
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 import torch.nn.utils.parametrize
 from torch._subclasses.fake_tensor import FakeTensorMode
 
-from mamba3_b200 import _lib, block
+from mamba3_b200 import _lib, block, ffn, loss, ops
 
 
 @pytest.mark.parametrize("reduction,per_row", [("none", True), ("mean", False), ("sum", False)])
@@ -159,3 +160,21 @@ def test_loss_without_logits_refuses_heads_that_do_more(how):
     lm.lm_head = _altered(lm.lm_head, how)
     with pytest.raises(ValueError, match="lm_head"):
         lm(ids, ids, return_logits=False)
+
+
+def test_forward_mode_derivatives_are_refused(monkeypatch):
+    """No operator here has a forward-mode derivative: a tangent raises, also where nothing requires grad."""
+    monkeypatch.setattr(_lib, "_same_gpu", lambda name, ts: 0)
+    monkeypatch.setattr(ops, "gated_ffn_fwd", lambda x, *a: (x + 0.0, x.detach(), x.detach()))
+    monkeypatch.setattr(ops, "linear_xent_fwd", lambda h, *a: (h.sum().detach(), h.detach()))
+    x, w, wd = torch.randn(3, 8), torch.randn(16, 8), torch.randn(8, 16)
+    t = torch.zeros(3, dtype=torch.long)
+    calls = [lambda a: ffn.gated_ffn(a, w, w, wd), lambda a: ffn.gated_ffn(x, w, w, wd, residual=a),
+             lambda a: loss.linear_cross_entropy(a, w, t)]
+    for call in calls:
+        call(x)
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad), fwAD.dual_level(), pytest.raises(RuntimeError, match="jvp|forward"):
+                call(fwAD.make_dual(x, torch.ones_like(x)))
+            with torch.set_grad_enabled(grad), fwAD.dual_level():
+                call(x)  # no tangent among the arguments
