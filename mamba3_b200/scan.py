@@ -11,7 +11,7 @@ from __future__ import annotations
 
 import torch
 
-from . import ops
+from . import _lib, ops
 
 
 def _flat(chunk_decay, h_chunk, h_init):
@@ -51,6 +51,7 @@ class SSDScanFn(torch.autograd.Function):
 def ssd_scan(chunk_decay, h_chunk, h_init=None):
     """h_states[:,0] = h_init (or 0), h_states[:,k+1] = decay[:,k] h_states[:,k] + h_chunk[:,k]
     (mamba3/scan.py:143-144); differentiable through SSDScanFn when an input requires grad."""
+    _lib._no_tangent("ssd_scan", (chunk_decay, h_chunk, h_init))
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (chunk_decay, h_chunk, h_init)):
         return SSDScanFn.apply(chunk_decay, h_chunk, h_init)
     hc, hi = _flat(chunk_decay, h_chunk, h_init)

@@ -10,7 +10,7 @@ from dataclasses import dataclass
 
 import torch
 
-from . import ops
+from . import _lib, ops
 
 
 @dataclass
@@ -54,6 +54,7 @@ def chunked_ssd(x_g, x_b, B_g, B_b, C, dt, A, D, x_raw, chunk_size=64, h_init=No
     not change the result beyond fp32 rounding.  Returns SSDOutput(y in x_g.dtype, h_final fp32).
     """
     ins = (x_g, x_b, B_g, B_b, C, dt, A, D, x_raw, h_init)
+    _lib._no_tangent("chunked_ssd", ins)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ins):
         y, hf = ChunkedSSDFn.apply(*ins, return_final_state)
     else:

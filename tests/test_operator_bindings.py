@@ -178,3 +178,14 @@ def test_forward_mode_derivatives_are_refused(monkeypatch):
                 call(fwAD.make_dual(x, torch.ones_like(x)))
             with torch.set_grad_enabled(grad), fwAD.dual_level():
                 call(x)  # no tangent among the arguments
+
+
+def test_forward_mode_derivatives_of_the_scans_are_refused():
+    from mamba3_b200 import chunked_ssd, ssd_scan
+
+    with fwAD.dual_level():
+        a = fwAD.make_dual(torch.zeros(1, 2, 3), torch.ones(1, 2, 3))
+        with pytest.raises(_lib.M3bError, match="forward-mode"):
+            ssd_scan(a, torch.zeros(1, 2, 3, 4, 5))
+        with pytest.raises(_lib.M3bError, match="forward-mode"):
+            chunked_ssd(None, None, None, None, None, a, None, None, None)
