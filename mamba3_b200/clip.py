@@ -87,7 +87,9 @@ def clip_grads(grads: Iterable[torch.Tensor], max_norm: float, norm_type: float 
                 raise ValueError("clip_grads: an output in its gradient's place needs its dtype")
             if n and p != q and q in read:
                 raise ValueError("clip_grads: an output in another gradient's place")
-    return _lib.grad_clip(ptrs, numel, dtypes, out_ptrs, out_dtypes, max_norm, norm_type == math.inf, gs[0].device)
+    norm = _lib.grad_clip(ptrs, numel, dtypes, out_ptrs, out_dtypes, max_norm, norm_type == math.inf, gs[0].device)
+    torch.autograd.graph.increment_version(os)  # written by address: autograd must hear of it
+    return norm
 
 
 def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0,

@@ -8,7 +8,7 @@ import torch.autograd.forward_ad as fwAD
 import torch.nn.utils.parametrize
 from torch._subclasses.fake_tensor import FakeTensorMode
 
-from mamba3_b200 import _lib, block, ffn, loss, ops
+from mamba3_b200 import _lib, block, clip, ffn, loss, ops
 
 
 @pytest.mark.parametrize("reduction,per_row", [("none", True), ("mean", False), ("sum", False)])
@@ -189,3 +189,18 @@ def test_forward_mode_derivatives_of_the_scans_are_refused():
             ssd_scan(a, torch.zeros(1, 2, 3, 4, 5))
         with pytest.raises(_lib.M3bError, match="forward-mode"):
             chunked_ssd(None, None, None, None, None, a, None, None, None)
+
+
+@pytest.mark.parametrize("other", [False, True])
+def test_clipping_is_a_write_that_autograd_knows_of(monkeypatch, other):
+    """A tensor kept for a backward pass and then clipped: the backward pass raises, as after any write in place."""
+    monkeypatch.setattr(clip, "_get_device", lambda t: 0)
+    monkeypatch.setattr(_lib, "grad_clip", lambda *a: torch.zeros(()))
+    w, g = torch.ones(3, requires_grad=True), torch.ones(3)
+    y = (w * g).sum()
+    clip.clip_grads([torch.ones(3)] if other else [g], 1.0, out=[g] if other else None)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    y = (w * g).sum()
+    clip.clip_grads([g], 1.0, out=[torch.ones(3)])  # only read
+    y.backward()
