@@ -7,9 +7,11 @@
 //   operand may be stored with K along its rows (K-major) or across them (MN-major, for the
 //   products of the backward passes); the tile then arrives as 64 x 64 boxes and the UMMA
 //   descriptor reads it transposed.
-// * fp32 operands travel as three bf16 planes whose sum is the value exactly (each plane takes
-//   the next 8 significant bits by truncation).  The product runs over the six plane pairs with
-//   2^-16 or more of the leading one's weight, smallest first; the dropped pairs are below 2^-24.  The
+// * fp32 operands travel as three bf16 planes whose sum is the value exactly (each plane is what the
+//   planes before it leave, rounded to nearest: at most 2^-8 and 2^-17 of the value, of either sign).  The
+//   product runs over six plane pairs, smallest first; each of the two largest that are left out is
+//   at most 2^-25 of the product.  (Planes cut off instead of rounded leave out up to 2^-21, always of the
+//   product's sign.)  The
 //   tensor core cuts its sums off instead of rounding them, a bias of half a step per addition that
 //   fp32 results would show (3e-6 of a 323 x 897 product): so every kGmGroup K blocks are a sum of
 //   their own, and the epilogue adds them, rounded, in registers (8e-7).
@@ -197,19 +199,22 @@ struct GemmSched {
 // element helpers
 // ---------------------------------------------------------------------------
 
-// The three bf16 planes of an fp32 value; a value that is not finite lies in the first alone.
-__device__ __forceinline__ void split_planes(float v, uint16_t (&w)[3]) {
+// The next bf16 plane of an fp32 value: v keeps what is left.  Infinity and NaN lie in the last plane, which
+// meets only the other operand's first, beside a first plane of +-1: so their products are those of the
+// value itself (in the first plane they would meet the zeros of the other's second and third).
+__device__ __forceinline__ uint32_t next_plane(float& v, int plane) {
   const uint32_t b = __float_as_uint(v);
-  if ((b & 0x7f800000u) == 0x7f800000u) {
-    w[0] = (b & 0x007fffffu) ? 0x7fff : (uint16_t)(b >> 16);
-    w[1] = w[2] = 0;
-    return;
-  }
-  const float hi = __uint_as_float(b & 0xffff0000u), r = v - hi;
-  const uint32_t m = __float_as_uint(r) & 0xffff0000u;
-  w[0] = (uint16_t)(b >> 16);
-  w[1] = (uint16_t)(m >> 16);
-  w[2] = (uint16_t)(__float_as_uint(r - __uint_as_float(m)) >> 16);
+  const bool fin = (b & 0x7f800000u) != 0x7f800000u;
+  uint32_t r = (b + 0x7fffu + (b >> 16 & 1u)) & 0xffff0000u;
+  if ((r & 0x7f800000u) == 0x7f800000u) r = b & 0xffff0000u;  // would round to infinity: cut off
+  const uint32_t last = v != v ? 0x7fffu : b >> 16;           // a NaN whose set bits are all below stays one
+  const uint32_t odd = plane == 2 ? last : plane == 1 ? 0u : (b >> 16 & 0x8000u) | 0x3f80u;
+  if (fin) v -= __uint_as_float(r);
+  return fin ? r >> 16 : odd;
+}
+__device__ __forceinline__ void split_planes(float v, uint16_t (&w)[3]) {
+#pragma unroll
+  for (int k = 0; k < 3; ++k) w[k] = (uint16_t)next_plane(v, k);
 }
 
 __device__ __forceinline__ uint32_t pack16(float a, float b, bool f16) {
@@ -328,8 +333,7 @@ struct GemmSend {
   }
 };
 
-// 32 columns of a following product's operand: a 16-bit type, or the planes of fp32 values (each plane
-// takes the upper halves and leaves the remainders; a value that is not finite lies in the first alone).
+// 32 columns of a following product's operand: a 16-bit type, or the planes of fp32 values.
 template <bool PLANES>
 __device__ __forceinline__ void put_operand(GemmSend& send, const CUtensorMap* map, bool f16, int col, int64_t row,
                                             float (&v)[32]) {
@@ -344,10 +348,7 @@ __device__ __forceinline__ void put_operand(GemmSend& send, const CUtensorMap* m
       uint32_t w[16];
 #pragma unroll
       for (int i = 0; i < 32; ++i) {
-        const uint32_t b = __float_as_uint(v[i]);
-        const bool fin = (b & 0x7f800000u) != 0x7f800000u;
-        const uint32_t top = v[i] != v[i] ? 0x7fffu : b >> 16;  // a NaN whose set bits are all below stays one
-        v[i] = fin ? v[i] - __uint_as_float(b & 0xffff0000u) : 0.f;
+        const uint32_t top = next_plane(v[i], pl);
         if (i & 1) w[i >> 1] |= top << 16;
         else w[i >> 1] = top;
       }

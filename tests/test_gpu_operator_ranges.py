@@ -100,3 +100,83 @@ def test_custom_ops_as_torch_checks_them(rows, dtype):
         for a, b in ((True, True), (True, False), (False, True)):
             check(ops.linear_xent_bwd.default, (rows, w, saved, torch.ones_like(loss), -100, reduction, a, b),
                   test_utils=utils)
+
+
+# ---------------------------------------------------------------------------
+# large logits
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("n", [6, 40, 300])
+def test_loss_of_infinite_logits(n, dtype):
+    """Vocabulary rows of -infinity leave the others as they are; a token all of whose logits are, or one of
+    +infinity, has no loss."""
+    from mamba3_b200 import linear_cross_entropy
+
+    h, w, t = loss_inputs(n, 64, 300, dtype)
+    a, b = h.abs() + 0.5, w.clone()
+    b[7], b[150] = float("-inf"), float("-inf")
+    t[(t == 7) | (t == 150)] = 8
+    keep = torch.ones(300, dtype=torch.bool, device="cuda")
+    keep[7] = keep[150] = False
+    want = ref.loss(a, b[keep], t - (t > 7).long() - (t > 150).long(), reduction="sum", dloss=1.0)
+    b.requires_grad_(True)
+    y = linear_cross_entropy(a, b, t, reduction="sum")
+    ref.check(y, want["loss"], "loss")
+    dw, = torch.autograd.grad(y, b)
+    assert not dw[~keep].any()
+    ref.check(dw[keep], want["weight"], "dweight")
+    t[0] = 7
+    assert linear_cross_entropy(a, b, t, reduction="none")[0].item() == math.inf
+    for x in (math.inf, -math.inf):
+        assert torch.isnan(linear_cross_entropy(a, torch.full_like(w, x), t, reduction="none")).all()
+        c = w.clone()
+        c[9] = x
+        y = linear_cross_entropy(a, c, t, reduction="none")
+        assert bool(torch.isnan(y).all() if x > 0 else torch.isfinite(y[t != 9]).all())
+
+
+# ---------------------------------------------------------------------------
+# fp32 operands
+# ---------------------------------------------------------------------------
+def test_fp32_products_of_one_sign():
+    """Sums of sixteen equal products of values with all 24 bits set, in every remainder's sign: no error averages
+    out.  Two steps for the last sum of sixteen products (in two halves; the passes before it are 2^-8 of it and less),
+    half a step for the loss's own rounding, and 2^-24 for the plane pairs that are left out.  The loss of two logits z > 16 and 0 is z for the second
+    to within e^-16."""
+    from mamba3_b200 import linear_cross_entropy
+
+    n = 600
+    v = 1.0 + torch.rand(n, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)) * 0.99
+    v[:6] = torch.tensor([1 + 2.0 ** -7 - 2.0 ** -23, 1 + 2.0 ** -7 - 2.0 ** -15 - 2.0 ** -23, 2 - 2.0 ** -23,
+                          1 + 2.0 ** -8, 1 + 2.0 ** -8 - 2.0 ** -23, 1.0], device="cuda")
+    h = v[:, None].expand(n, 16).contiguous()
+    t = torch.ones(n, dtype=torch.long, device="cuda")
+    for c in (1 + 2.0 ** -7 - 2.0 ** -23, 2 - 2.0 ** -23, 1 + 2.0 ** -8 - 2.0 ** -16 + 2.0 ** -23, 1.0):
+        w = torch.zeros(2, 16, device="cuda")
+        w[0] = c
+        y = linear_cross_entropy(h, w, t, reduction="none").double()
+        z = 16 * v.double() * float(w[0, 0])
+        want = z + torch.log1p(torch.exp(-z))
+        bound = 3 * 2.0 ** -23 * want
+        off = (y - want).abs()
+        assert bool((off <= bound).all()), (c, float((off / want).max()))
+
+
+@pytest.mark.parametrize("n", [6, 40, 300])
+def test_fp32_infinities_are_those_of_the_sums(n):
+    """Infinite inputs of the fp32 feed-forward: as in plain fp32 arithmetic, infinite where one sign meets
+    finite values that are not zero, and nothing else touched."""
+    from mamba3_b200 import gated_ffn
+
+    d, f = 64, 72
+    x, w = rnd(n, d, seed=1).abs() + 0.5, rnd(f, d, seed=2).abs() * d ** -0.5 + 0.01
+    wd = rnd(d, f, seed=3).abs() * f ** -0.5 + 0.01
+    wd[5] = -wd[5]
+    x[2, 3] = math.inf
+    y = gated_ffn(x, w, w, wd)
+    rows = torch.arange(n, device="cuda") != 2
+    assert torch.isfinite(y[rows]).all()
+    assert bool((y[2][torch.arange(d, device="cuda") != 5] == math.inf).all()) and y[2, 5].item() == -math.inf
+    x[2, 3] = math.nan
+    y = gated_ffn(x, w, w, wd)
+    assert torch.isfinite(y[rows]).all() and torch.isnan(y[2]).all()
