@@ -590,7 +590,7 @@ M3B_API int m3b_gated_ffn_bwd(const m3b_gated_ffn_args* a, void* workspace, size
  * the two gradient products); fp32 operands travel as three bf16 planes.
  *
  * saved (m3b_linear_xent_saved bytes, 16-byte aligned): the kept rows in operand form, their row
- * numbers, targets and log-sums; of at most 8 rows the values in fp32 and the logits, which are then not
+ * numbers, targets, maxima and log-sums; of at most 8 rows the values in fp32 and the logits, which are then not
  * computed again.  The backward needs it as the forward left it.  Backward
  * outputs may be null.  Workspaces as the query functions say.
  * ------------------------------------------------------------------------ */

@@ -942,7 +942,7 @@ def xent_saved_bytes(hidden, vocab):
     if rows <= 8:
         return up(rows * d * 4) + up(rows * vocab * 4) + 5 * 256
     tp, planes = up(rows), 3 if hidden.dtype == torch.float32 else 1
-    return up(planes * tp * ((d + 7) // 8 * 8) * 2) + 3 * up(tp * 4) + 256
+    return up(planes * tp * ((d + 7) // 8 * 8) * 2) + 2 * up(tp * 4) + up(tp * 8) + 256
 
 
 def linear_xent_fwd(hidden, weight, target, ignore_index, reduction, save=True):

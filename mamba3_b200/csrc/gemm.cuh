@@ -36,6 +36,8 @@
 // of that size 1.51 - 1.55).  With K short the epilogue's stores show: the pipe is 66 - 92 % active at K = 768.
 #pragma once
 
+#include <float.h>
+
 #include "launch.h"
 #include "pair.cuh"
 #include "tmap.h"
@@ -127,9 +129,9 @@ struct GemmParams {
   // kEpiLse / kEpiDlogit
   const int* target;       // per row
   float* target_logit;
-  float2* part;            // (slots, rows): maximum and sum in powers of two
+  float2* part;            // (slots, rows): maximum, and sum of exp(logit - maximum)
   int64_t part_ld;
-  const float* lse2;       // log2 of the row's sum of exponentials
+  const float2* stat;      // per row: maximum, and log2 of the sum of exp(logit - maximum)
   const float* roww;       // weight per row or null
   float shift;             // softmax - one-hot times 2^shift
   int col0;                // first vocabulary column of this piece
@@ -1070,7 +1072,9 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
         });
       } else if constexpr (EPI == kEpiLse) {
         const int tgt = rok ? p.target[grow] : -1;
-        float m = -1e30f, sum = 0.f;  // m in powers of two
+        // the maximum as it is: a product with log2(e) would be rounded to 2^-24 of it, and with it the loss.
+        // It starts at the least finite value, so that a set of -infinities has a sum of 0.
+        float m = -FLT_MAX, sum = 0.f;
         columns(cfirst, clast, [&](int c, float (&v)[32]) {
           const int col = job.nt * bn + c;
           if (col >= s.N) return;
@@ -1088,17 +1092,21 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
           float t[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
           for (int i = 4; i < 32; ++i) t[i & 3] = fmaxf(t[i & 3], v[i]);
-          const float top = fmaxf(m, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * kLog2e);
-          float e[4] = {sum * ex2_fast(m - top), 0.f, 0.f, 0.f};
+          const float top = fmaxf(m, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])));
+          float e[4] = {sum * ex2_fast((m - top) * kLog2e), 0.f, 0.f, 0.f};
           m = top;
 #pragma unroll
-          for (int i = 0; i < 32; ++i) e[i & 3] += ex2_fast(fmaf(v[i], kLog2e, -top));
+          for (int i = 0; i < 32; i += 2) {
+            const float2 x = mul2(add2(make_float2(v[i], v[i + 1]), make_float2(-top, -top)), make_float2(kLog2e, kLog2e));
+            e[i & 3] += ex2_fast(x.x), e[(i & 3) + 1] += ex2_fast(x.y);
+          }
           sum = (e[0] + e[1]) + (e[2] + e[3]);
         });
         if (rok) p.part[(int64_t)(job.nt * 2 + half) * p.part_ld + grow] = make_float2(m, sum);
       } else {
         const int tgt = rok ? p.target[grow] - p.col0 : -1;
-        const float l2 = (rok ? p.lse2[grow] : 0.f) - p.shift, one = ex2_fast(p.shift);
+        const float2 st = rok ? p.stat[grow] : make_float2(0.f, 0.f);
+        const float ls = st.y - p.shift, one = ex2_fast(p.shift);
         const float w = rok && p.roww ? p.roww[grow] : 1.f;
         // rows behind the last kept token are K values of the next products: zero
         columns(cfirst, clast, [&](int c, float (&v)[32]) {
@@ -1106,7 +1114,8 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
           if (col >= s.N) return;
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
-            const float2 t = fma2(make_float2(v[i], v[i + 1]), make_float2(kLog2e, kLog2e), make_float2(-l2, -l2));
+            const float2 t = fma2(add2(make_float2(v[i], v[i + 1]), make_float2(-st.x, -st.x)), make_float2(kLog2e, kLog2e),
+                                  make_float2(-ls, -ls));
             v[i] = ex2_fast(t.x), v[i + 1] = ex2_fast(t.y);
           }
           const int to = tgt - col;

@@ -7,7 +7,7 @@
 // The kept rows are first gathered into a dense operand, so ignored tokens cost nothing in any
 // product (and what they hold, NaN included, reaches no sum); how many remain is read on the device.
 // Forward: one product over all vocabulary tiles whose epilogue keeps each row's running maximum
-// and sum (in powers of two) and the target's logit; the logits never leave the SM.  A small kernel
+// and sum and the target's logit; the logits never leave the SM.  A small kernel
 // joins the tiles' statistics.  Backward: a piece of the vocabulary at a time, the logits once more
 // with the softmax as their epilogue, and the piece's share of both gradients; dh is summed over the
 // pieces in fp32.  8 rows d_model vocab operations forward and backward, 2 more than with the
@@ -33,7 +33,7 @@ struct Saved {
   uint16_t* h;     // [planes][Tp][Dp] kept rows
   int* row;        // [Tp] where they come from
   int* target;     // [Tp]; -1 behind the last, -2 out of range
-  float* lse2;     // [Tp]
+  float2* stat;    // [Tp] maximum, and log2 of the sum of exp(z - maximum)
   int* count;      // kept rows; blocks of the join kernel that are done
   size_t bytes;
 };
@@ -65,7 +65,7 @@ Saved saved_of(const m3b_linear_xent_args* a, void* p) {
   s.h = static_cast<uint16_t*>(c.take((size_t)d.np * d.Tp * d.Dp * 2));
   s.row = static_cast<int*>(c.take((size_t)d.Tp * 4));
   s.target = static_cast<int*>(c.take((size_t)d.Tp * 4));
-  s.lse2 = static_cast<float*>(c.take((size_t)d.Tp * 4));
+  s.stat = static_cast<float2*>(c.take((size_t)d.Tp * 8));
   s.count = static_cast<int*>(c.take(8));
   s.bytes = c.at;
   return s;
@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(256) gather_kernel(const void* __restrict__ h,
 // flight (one after the other, their latencies and exponentials made 30 us of 16384 rows x 394 pairs).
 __device__ __forceinline__ void join2(float& m, float& sum, float2 v) {
   const float top = fmaxf(m, v.x);
-  sum = sum * ex2_fast(m - top) + v.y * ex2_fast(v.x - top);
+  sum = sum * ex2_fast((m - top) * kLog2e) + v.y * ex2_fast((v.x - top) * kLog2e);
   m = top;
 }
 // The block that ends last makes the loss of the rows' losses, summed in a fixed order in fp64; without
@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(512) join_kernel(const float2* __restrict__ pa
   const int n = s.count[0], blocks = n > 0 ? (n + 31) / 32 : 1;
   const int row = blockIdx.x * 32 + lane;
   if (blockIdx.x >= blocks) return;
-  float m[4] = {-1e30f, -1e30f, -1e30f, -1e30f}, sum[4] = {0.f, 0.f, 0.f, 0.f};
+  float m[4] = {-FLT_MAX, -FLT_MAX, -FLT_MAX, -FLT_MAX}, sum[4] = {0.f, 0.f, 0.f, 0.f};
   if (row < n) {
     int k = w;
     for (; k + 48 < slots; k += 64) {
@@ -196,9 +196,11 @@ __global__ void __launch_bounds__(512) join_kernel(const float2* __restrict__ pa
 #pragma unroll
     for (int k = 1; k < 16; ++k) join2(m[0], sum[0], sm[k][lane]);
     const bool ok = s.target[row] >= 0;
-    const float l2 = ok ? m[0] + log2f(sum[0]) : __int_as_float(0x7fffffff);
-    const float l = l2 * kLn2 - (ok ? target_logit[row] : 0.f);
-    s.lse2[row] = l2;
+    // the maximum and the logarithm apart: their sum is rounded to 2^-24 of the maximum, which a sure token's loss
+    // and the probabilities of large logits do not bear
+    const float l2 = ok ? log2f(sum[0]) : __int_as_float(0x7fffffff);
+    const float l = fmaf(l2, kLn2, ok ? m[0] - target_logit[row] : 0.f);
+    s.stat[row] = make_float2(m[0], l2);
     if (reduction == 0) loss[s.row[row]] = l;
     else __stcg(row_loss + row, l);
     __threadfence();  // before this block counts as done
@@ -438,7 +440,7 @@ int backward(const m3b_linear_xent_args* a, void* workspace, size_t* need, bool 
       g.nk[0] = (d.D + kGmBK - 1) / kGmBK;
       M3B_TRY(gemm_out_map(&p.o[0], z, d.f16));
       p.target = s.target;
-      p.lse2 = s.lse2;
+      p.stat = s.stat;
       p.roww = roww;
       p.col0 = (int)c0;
       p.clear = ticket;

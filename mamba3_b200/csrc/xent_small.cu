@@ -45,7 +45,7 @@ struct SmallXent {
   // saved, kept rows in order
   float* hs;     // [kept][D]
   float* z;      // [kept][V]
-  float* lse;    // [kept]
+  float2* stat;  // [kept] maximum, and log of the sum of exp(z - maximum)
   int* row;      // [kept]
   int* tgt;      // [kept]; -2 out of range
   int* pos;      // [T]: place among the kept, -1 ignored
@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(1024) loss_rows_kernel(SmallXent p) {
     if (!ok) record_error(p.err, M3B_ERR_INVALID_ARG);
     const float nan = __int_as_float(0x7fffffff), ln = logf(s.y);
     const float l = ok ? (s.x - __ldcg(p.z + (int64_t)m * p.V + t)) + ln : nan;
-    p.lse[m] = ok ? s.x + ln : nan;
+    p.stat[m] = make_float2(s.x, ok ? ln : nan);
     p.row[m] = r;
     p.tgt[m] = ok ? (int)t : -2;
     row_loss[m] = l;
@@ -281,7 +281,8 @@ __global__ void __launch_bounds__(32 * kWarps, 4) grads_rows_kernel(SmallXent p)
       float x = 0.f;
       if (m < n && r < rows) {
         const float weight = p.reduction == 0 ? p.dloss[p.row[m]] : p.reduction == 1 ? *p.dloss / (float)n : *p.dloss;
-        x = exp2f((p.z[(int64_t)m * p.V + r0 + r] - p.lse[m]) * kToLog2);
+        const float2 st = p.stat[m];  // apart: the maximum would cost their sum its last bits
+        x = exp2f(((p.z[(int64_t)m * p.V + r0 + r] - st.x) - st.y) * kToLog2);
         x = weight * (p.tgt[m] == r0 + r ? x - 1.f : x);
       }
       dz[r][m] = x;
@@ -368,7 +369,7 @@ size_t carve_saved(const m3b_linear_xent_args* a, SmallXent* p) {
   p->T = (int)a->rows, p->D = a->d_model, p->V = a->vocab, p->reduction = a->reduction;
   p->hs = static_cast<float*>(c.take((size_t)a->rows * a->d_model * 4));
   p->z = static_cast<float*>(c.take((size_t)a->rows * a->vocab * 4));
-  p->lse = static_cast<float*>(c.take(kSmallXentRows * 4));
+  p->stat = static_cast<float2*>(c.take(kSmallXentRows * 8));
   p->row = static_cast<int*>(c.take(kSmallXentRows * 4));
   p->tgt = static_cast<int*>(c.take(kSmallXentRows * 4));
   p->pos = static_cast<int*>(c.take(kSmallXentRows * 4));

@@ -105,6 +105,83 @@ def test_custom_ops_as_torch_checks_them(rows, dtype):
 # ---------------------------------------------------------------------------
 # large logits
 # ---------------------------------------------------------------------------
+def ladder(n, v, d, top, gap, dtype):
+    """Hidden states and weights whose logits are exact: `top` at column i % v of row i, top - gap elsewhere
+    (products of powers of two in two columns)."""
+    h, w = torch.zeros(n, d, device="cuda"), torch.zeros(v, d, device="cuda")
+    i = torch.arange(n, device="cuda") % v
+    w[:, 0] = 1.0
+    h[:, 0] = top - gap
+    at = 1 + i % (d - 1)
+    h[torch.arange(n, device="cuda"), at] = gap
+    w[torch.arange(1, d, device="cuda") - 1, torch.arange(1, d, device="cuda")] = 1.0
+    return h.to(dtype), w.to(dtype), at - 1
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("n", [4, 40, 300])
+@pytest.mark.parametrize("top,gap", [(128.0, 16.0), (4096.0, 16.0), (16384.0, 128.0), (-4096.0, 32.0)])
+def test_sure_tokens_with_large_logits(n, top, gap, dtype):
+    """One logit `gap` above 399 equal ones: loss log(1 + 399 e^-gap) for it and gap more for another, whatever the
+    logits' size; never below zero.  Each term that is added to the 1 of the largest is rounded to 2^-24 of it: at
+    most 48 of them (128 columns a thread, a quarter of them one after the other, and the joins), its logarithm and
+    the loss to half a step each; the exponentials' 2 steps and the exponent's rounding (2^-24 of up to 185) weigh
+    e^-gap."""
+    from mamba3_b200 import linear_cross_entropy
+
+    v, d = 400, 64
+    h, w, best = ladder(n, v, d, top, gap, dtype)
+    z = h.double() @ w.double().t()
+    assert bool((z.amax(1) == top).all()) and bool((z.sort(1)[0][:, -2] == top - gap).all())
+    rest = 399 * math.exp(-gap)
+    want = math.log1p(rest)
+    err = 48 * 2.0 ** -24 + (3 * 2.0 ** -23 + 185 * 2.0 ** -24) * rest
+    y = linear_cross_entropy(h, w, best, reduction="none")
+    assert bool((y >= 0).all()) and bool(((y.double() - want).abs() <= err + 2.0 ** -23 * want).all())
+    y = linear_cross_entropy(h, w, best + 100, reduction="none")
+    assert bool(((y.double() - want - gap).abs() <= err + 2.0 ** -23 * (want + gap)).all())
+
+
+@pytest.mark.parametrize("n", [4, 40, 300])
+def test_probabilities_of_large_logits_sum_to_one(n):
+    """fp32, logits of 4096 and more and 399 others up to 2 below: the sum over the vocabulary of softmax - onehot, read off a
+    weight column of ones, is 0.  Each probability is off by its exponent's roundings (2^-24 of up to 3, and of the
+    sum's logarithm, up to 9 in powers of two), the hardware exponential (2^-22) and what its sum had (16 steps);
+    the product's sum adds sum_error: 64 steps of 2^-23 of the 2 that all magnitudes sum to."""
+    from mamba3_b200 import linear_cross_entropy
+
+    v, d = 400, 16
+    h, w = torch.zeros(n, d, device="cuda"), torch.zeros(v, d, device="cuda")
+    h[:, 0], h[:, 1] = 4096.0 + torch.arange(n, device="cuda"), 1.0
+    w[:, 0], w[:, 1] = 1.0, -torch.arange(v, device="cuda") / 256.0
+    w[:, 2] = 1.0  # times 0 in the logits
+    h.requires_grad_(True)
+    t = torch.full((n,), 399, device="cuda")
+    dh, = torch.autograd.grad(linear_cross_entropy(h, w, t, reduction="sum"), h)
+    assert bool((dh[:, 2].abs() <= 64 * 2.0 ** -23 * 2).all()), float(dh[:, 2].abs().max())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("n", [4, 40, 300])
+def test_loss_of_very_negative_logits(n, dtype):
+    """Rows whose logits all lie near -1e35: differences of 1e32 and more, so the loss is that to the best one."""
+    from mamba3_b200 import linear_cross_entropy
+
+    v, d = 300, 64
+    h, w = torch.zeros(n, d, device="cuda", dtype=dtype), torch.zeros(v, d, device="cuda", dtype=dtype)
+    h[:, 0] = 2.0 ** 60
+    w[:, 0] = -(2.0 ** 56) * (1 + (torch.arange(v, device="cuda") % 100 + 1) / 128.0)
+    w[7, 0] = -(2.0 ** 56)
+    z = h.double() @ w.double().t()
+    for t in (torch.full((n,), 7, device="cuda"), torch.arange(n, device="cuda") % v):
+        want = z.amax(1) - z[torch.arange(n, device="cuda"), t]
+        a = h.clone().requires_grad_(True)
+        y = linear_cross_entropy(a, w, t, reduction="none")
+        assert bool(((y.double() - want).abs() <= 2.0 ** -23 * z.abs().amax(1) * (want > 0)).all())
+        g, = torch.autograd.grad(y.sum(), a)
+        assert bool(torch.isfinite(g).all())
+
+
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 @pytest.mark.parametrize("n", [6, 40, 300])
 def test_loss_of_infinite_logits(n, dtype):
