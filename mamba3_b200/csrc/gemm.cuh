@@ -134,6 +134,11 @@ struct GemmParams {
   const float2* stat;      // per row: maximum, and log2 of the sum of exp(logit - maximum)
   const float* roww;       // weight per row or null
   float shift;             // softmax - one-hot times 2^shift
+  // fp16: a power of two that brings values into its range (peak_scale), from the largest magnitude of each
+  // of npeaks blocks, or null; *peak_out: that power, for the products that read the scaled values
+  const float* peaks;
+  int npeaks;
+  float* peak_out;
   int col0;                // first vocabulary column of this piece
   int* err;
   uint64_t wait_ns;
@@ -447,6 +452,17 @@ __device__ __forceinline__ void put_final(uint8_t* box, const GemmOut& o, const 
       stf(o.p, row * o.ld + c + e, o.kind == kOutF32 ? M3B_F32 : o.kind == kOutF16 ? M3B_F16 : M3B_BF16, x);
     }
   }
+}
+
+// The power of two at or below the largest of n magnitudes, for whole warps; 2^-100 .. 2^100, so that it and
+// its reciprocal are normal (all zero: 2^-100, which scales zeros).
+__device__ __forceinline__ float peak_scale(const float* peaks, int n) {
+  float x = 0.f;
+  for (int i = threadIdx.x & 31; i < n; i += 32) x = fmaxf(x, peaks[i]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+  x = fminf(fmaxf(x, 0x1p-100f), 0x1p100f);
+  return __uint_as_float(__float_as_uint(x) & 0x7f800000u);
 }
 
 // Waits of all roles: the plain test in a loop (the sleeping form of mbar_wait may wake late for a
@@ -807,6 +823,13 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
     };
     if constexpr (EPI == kEpiDglu)
       for (int i = 0; i < kGuSlots; ++i) gu_send();
+    float peak = 1.f;
+    if constexpr (EPI == kEpiDlogit) {
+      if (p.peaks) {
+        peak = peak_scale(p.peaks, p.npeaks);
+        if (blockIdx.x == 0 && threadIdx.x == 64) *p.peak_out = peak;
+      }
+    }
     uint32_t jn = 0;
     GemmSend send{sm + kGmBoxOff + (uint32_t)(warp - 2) * kGmBox, 0};
     GemmJob job = next_job(0);
@@ -1107,7 +1130,7 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
         const int tgt = rok ? p.target[grow] - p.col0 : -1;
         const float2 st = rok ? p.stat[grow] : make_float2(0.f, 0.f);
         const float ls = st.y - p.shift, one = ex2_fast(p.shift);
-        const float w = rok && p.roww ? p.roww[grow] : 1.f;
+        const float w = rok && p.roww ? p.roww[grow] / peak : 1.f;
         // rows behind the last kept token are K values of the next products: zero
         columns(cfirst, clast, [&](int c, float (&v)[32]) {
           const int col = job.nt * bn + c;

@@ -225,9 +225,25 @@ __global__ void __launch_bounds__(512) join_kernel(const float2* __restrict__ pa
   }
 }
 
-__global__ void roww_kernel(const float* __restrict__ dloss, Saved s, float* __restrict__ roww) {
+// The kept rows' weights, and each block's largest finite magnitude of them.
+constexpr int kRowwBlocks = 64;
+__global__ void __launch_bounds__(256) roww_kernel(const float* __restrict__ dloss, Saved s, float* __restrict__ roww,
+                                                   float* __restrict__ peaks) {
+  __shared__ float sm[8];
   const int n = *s.count;
-  for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < n; i += gridDim.x * blockDim.x) roww[i] = dloss[s.row[i]];
+  float top = 0.f;
+  for (int i = blockIdx.x * 256 + threadIdx.x; i < n; i += kRowwBlocks * 256) {
+    const float w = dloss[s.row[i]];
+    roww[i] = w;
+    if (isfinite(w)) top = fmaxf(top, fabsf(w));
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = top;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int k = 1; k < 8; ++k) top = fmaxf(top, sm[k]);
+  peaks[blockIdx.x] = top;
 }
 
 bool sizes_ok(const m3b_linear_xent_args* a) {
@@ -350,8 +366,12 @@ int backward(const m3b_linear_xent_args* a, void* workspace, size_t* need, bool 
   uint16_t* dz = static_cast<uint16_t*>(ws.take((size_t)d.np * d.Tp * ldz * 2));
   float* acc = nullptr;
   if (a->dhidden && pieces > 1) acc = static_cast<float*>(ws.take((size_t)d.Tp * up(d.D, bn) * 4));
-  float* roww = nullptr;
-  if (a->reduction == 0) roww = static_cast<float*>(ws.take((size_t)d.Tp * 4));
+  float *roww = nullptr, *peaks = nullptr, *peak = nullptr;
+  if (a->reduction == 0) {
+    roww = static_cast<float*>(ws.take((size_t)d.Tp * 4));
+    peaks = static_cast<float*>(ws.take((kRowwBlocks + 1) * 4));
+    peak = peaks ? peaks + kRowwBlocks : nullptr;
+  }
   int* ticket = static_cast<int*>(ws.take(4));
   const GemmOperand w = weight_of(a, ws, run, st, &rc);
   const Saved s = saved_of(a, a->saved);
@@ -365,8 +385,11 @@ int backward(const m3b_linear_xent_args* a, void* workspace, size_t* need, bool 
   base.dyn = s.count;
   base.err = a->err;
   // fp16 has nothing between 0 and 6e-8, where most of a large vocabulary's probabilities may lie: they are
-  // kept times 2^15 (at most 32768).  With weights per row the range is the caller's.
-  base.shift = d.f16 && a->reduction != 0 ? 15.f : 0.f;
+  // kept times 2^15 (at most 32768).  Weights per row, which may be a loss scaler's 65536 or one token's share of
+  // a mean, are divided by the power of two at or below the largest of them (then below 2, so times 2^14), and
+  // the two products multiply it back in fp32.
+  const bool rowf16 = d.f16 && a->reduction == 0;
+  base.shift = rowf16 ? 14.f : d.f16 ? 15.f : 0.f;
 
   // the two gradients' shares of the piece of n columns from c0 on, side by side
   auto gradients = [&](GemmParams& p, int64_t c0, int64_t n, const GemmOperand* z, const GemmOperand* wp) {
@@ -376,8 +399,9 @@ int backward(const m3b_linear_xent_args* a, void* workspace, size_t* need, bool 
       g.N = d.D;
       g.nk[0] = K;
       g.b_mn = 1;
-      g.alpha = base.shift > 0.f ? 1.f / 32768.f : 1.f;
+      g.alpha = rowf16 ? 0x1p-14f : d.f16 ? 0x1p-15f : 1.f;
       if (a->reduction != 0) g.alpha_num = a->dloss;
+      else if (d.f16) g.alpha_num = peak;
       if (a->reduction == 1) g.alpha_den = s.count;
       g.out.kind = okind;
       g.out.ld = d.D;
@@ -420,7 +444,7 @@ int backward(const m3b_linear_xent_args* a, void* workspace, size_t* need, bool 
   if (a->dhidden && cudaMemsetAsync(a->dhidden, 0, (size_t)d.T * d.D * es, st) != cudaSuccess)
     return check_launch("linear_xent_bwd");
   if (roww) {
-    roww_kernel<<<64, 256, 0, st>>>(a->dloss, s, roww);
+    roww_kernel<<<kRowwBlocks, 256, 0, st>>>(a->dloss, s, roww, peaks);
     M3B_TRY(check_launch("linear_xent roww"));
   }
   for (int64_t c0 = 0; c0 < d.V; c0 += cols) {
@@ -442,6 +466,11 @@ int backward(const m3b_linear_xent_args* a, void* workspace, size_t* need, bool 
       p.target = s.target;
       p.stat = s.stat;
       p.roww = roww;
+      if (rowf16) {
+        p.peaks = peaks;
+        p.npeaks = kRowwBlocks;
+        p.peak_out = peak;
+      }
       p.col0 = (int)c0;
       p.clear = ticket;
       plan_gemm(p, kEpiDlogit, true);

@@ -103,6 +103,56 @@ def test_custom_ops_as_torch_checks_them(rows, dtype):
 
 
 # ---------------------------------------------------------------------------
+# fp16's range
+# ---------------------------------------------------------------------------
+def scaled(want, by, dtype):
+    """(value, bound) of a result that is linear in a factor `by` (a power of two): the bound's own least step
+    is one of the unscaled result, so the result's is added."""
+    return want[0] * by, want[1] * by + ref.least(dtype)
+
+
+@pytest.mark.parametrize("scale,size", [(2.0 ** -10, 1.0), (2.0 ** -18, 256.0), (2.0 ** 16, 2.0 ** -5), (1.0, 1.0)])
+def test_fp16_loss_per_token_keeps_small_weights(scale, size):
+    """The caller's mean over 1000 tokens (weights near 1e-3, or smaller) and a loss scaler's 65536: softmax times
+    weight is 5e-8 and less, or its one-hot part past 65504, and the gradients are within fp16 all the same."""
+    from mamba3_b200 import linear_cross_entropy
+
+    n, d, v = 1000, 64, 20000
+    h = ((rnd(n, d, seed=1) * 0.5 + 1.0) * size).half().requires_grad_(True)
+    w = (rnd(v, d, seed=2) * 0.02 / max(size, 1.0) + 0.01).half().requires_grad_(True)
+    t = torch.randint(0, v, (n,), device="cuda", generator=torch.Generator(device="cuda").manual_seed(3))
+    t[::7] = -100
+    dl = (1.0 + 0.5 * rnd(n, seed=4).tanh()) * scale
+    dl[::14] = 2.0 ** 40 * scale  # of ignored tokens: no part in the range
+    dl[3] = -dl[3]
+    dh, dw = torch.autograd.grad(linear_cross_entropy(h, w, t, reduction="none"), (h, w), dl)
+    want = ref.loss(h, w, t, reduction="none", dloss=dl / scale)
+    ref.check(dh, scaled(want["hidden"], scale, torch.float16), "dhidden")
+    ref.check(dw, scaled(want["weight"], scale, torch.float16), "dweight")
+
+
+def test_fp16_loss_per_token_with_weights_that_are_no_numbers():
+    """Zero weights alone; an infinite or NaN weight stays in its own token's row of the hidden gradient."""
+    from mamba3_b200 import linear_cross_entropy
+
+    h, w, t = loss_inputs(40, 64, 300, torch.float16)
+    h.requires_grad_(True)
+    y = linear_cross_entropy(h, w, t, reduction="none")
+    dl = torch.zeros(40, device="cuda")
+    dh, = torch.autograd.grad(y, h, dl, retain_graph=True)
+    assert not dh.any()
+    dl = rnd(40, seed=5) * 2.0 ** -12
+    want = ref.loss(h, w, t, reduction="none", dloss=dl * 2.0 ** 12)
+    want = scaled(want["hidden"], 2.0 ** -12, torch.float16)
+    for bad in (math.inf, math.nan):
+        dl[7] = bad
+        dh, = torch.autograd.grad(y, h, dl, retain_graph=True)
+        assert not torch.isfinite(dh[7]).any()
+        keep = torch.arange(40, device="cuda") != 7
+        ref.check(dh[keep], (want[0][keep], want[1][keep]), "the others")
+
+
+# ---------------------------------------------------------------------------
 # large logits
 # ---------------------------------------------------------------------------
 def ladder(n, v, d, top, gap, dtype):
