@@ -536,7 +536,8 @@ M3B_API int m3b_scaled_add(const void* x, const void* h, float scale, void* out,
  * x, residual, out and their gradients (rows, d_model), w_gate / w_up (d_ff, d_model), w_down
  * (d_model, d_ff), all of `dtype`; x, residual and dout with rows *_stride elements apart, the
  * rest contiguous; biases and residual may be null.  Sums are kept in fp32; act, and in the
- * backward dg and du, are rounded to 16-bit `dtype` once (operands of the next product); fp32
+ * backward dg and du, are rounded to 16-bit `dtype` once (operands of the next product; fp16 dg and du
+ * over a power of two that keeps small output gradients' bits); fp32
  * operands travel as three bf16 planes, which keeps 24 bits.
  *
  * saved_act (m3b_gated_ffn_act_bytes) is always written.  saved_gu (m3b_gated_ffn_gu_bytes; g and

@@ -80,6 +80,7 @@ struct Sums {
     int64_t plane, ld;
     int cols;
     float scale;
+    const float* num;  // scale *= *num, or null
     void* out;
     float* part;
   } s[3];
@@ -128,7 +129,7 @@ __global__ void __launch_bounds__(256) colsum_finish_kernel(const __grid_constan
   __syncthreads();
   if (w != 0 || c >= m.cols) return;
   for (int k = 1; k < 8; ++k) s += sm[k][lane];
-  stf(m.out, c, a.dt, s * m.scale);
+  stf(m.out, c, a.dt, s * (m.num ? m.scale * *m.num : m.scale));
 }
 int colsums(const Sums& a, cudaStream_t st) {
   if (a.n == 0) return M3B_OK;
@@ -136,6 +137,41 @@ int colsums(const Sums& a, cudaStream_t st) {
   for (int i = 0; i < a.n; ++i) cols = a.s[i].cols > cols ? a.s[i].cols : cols;
   const int rc = launch_dependent(colsum_kernel, dim3(a.chunks, (cols + 63) / 64, a.n), 256, st, a);
   return rc != M3B_OK ? rc : launch_dependent(colsum_finish_kernel, dim3((cols + 31) / 32, a.n), 256, st, a);
+}
+
+// fp16's smallest step is 6e-8: dg and du of an unscaled mean loss, near 1e-5, would lose most of their bits.  They
+// are kept divided by a power of two that brings the largest |s dout| up to 2^-8 (larger ones stay as they are),
+// and the products that read them multiply it back in fp32.  Not further up: with g and u within
+// fp16 themselves, dg and du can then pass 65504 only where a column of w_down has a sum of magnitudes above 100,
+// so no step that was finite becomes infinite, as a loss scaler that lowers its scale in vain would see it.
+// Largest finite |s dout| of each block's rows; rows start on 16 bytes.
+constexpr int kPeakBlocks = 128;
+__global__ void __launch_bounds__(512) peak_kernel(const uint16_t* __restrict__ x, int64_t rows, int D, int64_t ld,
+                                                   float scale, float* __restrict__ peaks) {
+  __shared__ uint32_t sm[16];
+  pdl_wait_primary();
+  pdl_launch_dependents();
+  uint32_t top = 0;
+  auto take = [&](uint32_t h) {
+    h &= 0x7fffu;
+    if (h < 0x7c00u && h > top) top = h;
+  };
+  const int eights = D / 8, tail = D - 8 * eights, lane = threadIdx.x & 31;
+  for (int64_t r = blockIdx.x * 16 + (threadIdx.x >> 5); r < rows; r += kPeakBlocks * 16) {
+    const uint4* row = reinterpret_cast<const uint4*>(x + r * ld);
+#pragma unroll 4
+    for (int c = lane; c < eights; c += 32) {
+      const uint4 w = __ldg(row + c);
+      take(w.x), take(w.x >> 16), take(w.y), take(w.y >> 16), take(w.z), take(w.z >> 16), take(w.w), take(w.w >> 16);
+    }
+    if (lane < tail) take(x[r * ld + 8 * eights + lane]);
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  if (lane == 0) sm[threadIdx.x >> 5] = top;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int k = 1; k < 16; ++k) top = sm[k] > top ? sm[k] : top;
+  peaks[blockIdx.x] = __half2float(__ushort_as_half((unsigned short)top)) * fabsf(scale);
 }
 
 int check(const m3b_gated_ffn_args* a, bool bwd) {
@@ -275,14 +311,16 @@ int backward(const m3b_gated_ffn_args* a, void* workspace, size_t* need, bool ru
   Sums sums{};
   sums.f16 = d.f16, sums.planes = d.np, sums.dt = a->dtype, sums.rows = d.M;
   sums.chunks = (int)((d.M + kSumRows - 1) / kSumRows);
-  auto sum = [&](const GemmOperand& o, float scale, void* out) {
+  float* peaks = d.f16 ? static_cast<float*>(ws.take((kPeakBlocks + 1) * 4)) : nullptr;
+  float* peak = peaks ? peaks + kPeakBlocks : nullptr;
+  auto sum = [&](const GemmOperand& o, float scale, const float* num, void* out) {
     if (!out) return;
     float* part = static_cast<float*>(ws.take((size_t)sums.chunks * o.cols * 4));
-    sums.s[sums.n++] = {static_cast<const uint16_t*>(o.p), o.plane, o.ld, (int)o.cols, scale, out, part};
+    sums.s[sums.n++] = {static_cast<const uint16_t*>(o.p), o.plane, o.ld, (int)o.cols, scale, num, out, part};
   };
-  sum(dg, 1.f, a->db_gate);
-  sum(du, 1.f, a->db_up);
-  sum(dy, a->residual_scale, a->db_down);
+  sum(dg, 1.f, peak, a->db_gate);
+  sum(du, 1.f, peak, a->db_up);
+  sum(dy, a->residual_scale, nullptr, a->db_down);
   int* ticket = static_cast<int*>(ws.take(4));
 
   // dx and the three weight gradients, side by side
@@ -294,11 +332,12 @@ int backward(const m3b_gated_ffn_args* a, void* workspace, size_t* need, bool ru
     bool a_mn;
     int64_t M, N, K;
     float alpha;
+    const float* num;
   };
-  const Product all[4] = {{a->dx, {&dg, &du}, {&wg, &wu}, false, d.M, d.D, d.F, 1.f},
-                          {a->dw_gate, {&dg, nullptr}, {&x, nullptr}, true, d.F, d.D, d.M, 1.f},
-                          {a->dw_up, {&du, nullptr}, {&x, nullptr}, true, d.F, d.D, d.M, 1.f},
-                          {a->dw_down, {&dy, nullptr}, {&act, nullptr}, true, d.D, d.F, d.M, a->residual_scale}};
+  const Product all[4] = {{a->dx, {&dg, &du}, {&wg, &wu}, false, d.M, d.D, d.F, 1.f, peak},
+                          {a->dw_gate, {&dg, nullptr}, {&x, nullptr}, true, d.F, d.D, d.M, 1.f, peak},
+                          {a->dw_up, {&du, nullptr}, {&x, nullptr}, true, d.F, d.D, d.M, 1.f, peak},
+                          {a->dw_down, {&dy, nullptr}, {&act, nullptr}, true, d.D, d.F, d.M, a->residual_scale, nullptr}};
   for (const Product& e : all) {
     if (!e.out) continue;
     GemmSub& s = q.sub[q.nsub++];
@@ -314,12 +353,16 @@ int backward(const m3b_gated_ffn_args* a, void* workspace, size_t* need, bool ru
     s.M = (int)e.M;
     s.N = (int)e.N;
     s.alpha = e.alpha;
+    s.alpha_num = e.num;
     s.out = result(e.out, e.N, a->dtype);
   }
   void* parts = ws.take(plan_gemm(q, kEpiStore, true));
   *need = ws.at;
   if (!run) return M3B_OK;
   M3B_TRY(launch_pack(packs, a->dtype, st));
+  if (d.f16)
+    M3B_TRY(launch_dependent(peak_kernel, dim3(kPeakBlocks), 512, st, static_cast<const uint16_t*>(dy.p), d.M, d.D, dy.ld,
+                             a->residual_scale, peaks));
   {  // da -> dg, du
     GemmParams p = params(d, a, gemm_columns(d.M, d.F, d.f32));
     GemmSub& s = p.sub[0];
@@ -336,6 +379,11 @@ int backward(const m3b_gated_ffn_args* a, void* workspace, size_t* need, bool ru
     p.gu = static_cast<uint8_t*>(a->saved_gu);
     p.gu_ld = up(d.F, 32) / 8;
     p.clear = ticket;
+    if (d.f16) {
+      p.peaks = peaks;
+      p.npeaks = kPeakBlocks;
+      p.peak_out = peak;
+    }
     plan_gemm(p, kEpiDglu, true);
     M3B_TRY(launch_gemm(p, kEpiDglu, true, nullptr, st));
   }

@@ -823,10 +823,11 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
     };
     if constexpr (EPI == kEpiDglu)
       for (int i = 0; i < kGuSlots; ++i) gu_send();
-    float peak = 1.f;
-    if constexpr (EPI == kEpiDlogit) {
+    float peak = 1.f;  // fp16: values are kept divided by it
+    if constexpr (EPI == kEpiDlogit || EPI == kEpiDglu) {
       if (p.peaks) {
         peak = peak_scale(p.peaks, p.npeaks);
+        if constexpr (EPI == kEpiDglu) peak = fminf(peak * 256.f, 1.f);  // up to 2^-8, never down: see ffn.cu
         if (blockIdx.x == 0 && threadIdx.x == 64) *p.peak_out = peak;
       }
     }
@@ -1034,6 +1035,7 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
           if (rows.row0 < M) put_operand<PLANES>(send, &p.o[0], p.f16, col, rows.row0, g);
         }
       } else if constexpr (EPI == kEpiDglu) {
+        const float factor = s.alpha / peak;
         columns(cfirst, clast, [&](int c, float (&d)[32]) {
           const int col = job.nt * bn + c;
           if (col >= s.N) return;
@@ -1055,7 +1057,7 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
             }
             __syncwarp();
             gu_send();
-            const float2 one = make_float2(1.f, 1.f), alpha = make_float2(s.alpha, s.alpha);
+            const float2 one = make_float2(1.f, 1.f), alpha = make_float2(factor, factor);
 #pragma unroll
             for (int i = 0; i < 8; i += 2) {
               float2 g, u;

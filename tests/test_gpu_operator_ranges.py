@@ -152,6 +152,72 @@ def test_fp16_loss_per_token_with_weights_that_are_no_numbers():
         ref.check(dh[keep], (want[0][keep], want[1][keep]), "the others")
 
 
+@pytest.mark.parametrize("n,d,f", [(100, 64, 72), (300, 128, 264), (20, 40, 24)])
+@pytest.mark.parametrize("scale", [1.0, 2.0 ** -5])
+def test_fp16_ffn_keeps_small_output_gradients(n, d, f, scale):
+    """Output gradients of a few of fp16's smallest steps (an unscaled mean loss): dg and du keep their 11 bits.  They
+    are brought up until the largest output gradient, 4 steps here, is 2^-8: half a smallest step there, 2^-25,
+    is 2^-15 of the steps that the plain form below counts in, in each of dg and du."""
+    from test_gpu_operators import ffn_call, ffn_want
+
+    t = ffn_inputs(n, d, f, torch.float16, True, False)
+    t["x"] = t["x"].abs()
+    for v in t.values():
+        v.requires_grad_(True)
+    steps = torch.randint(-4, 5, (n, d), device="cuda", generator=torch.Generator(device="cuda").manual_seed(8))
+    dout = (steps.double() * 2.0 ** -24).half()
+    grads = torch.autograd.grad(ffn_call(t, scale), list(t.values()), dout)
+    want = ffn_want(t, scale, (steps.double() / scale).half())  # the largest near 1 after the factor
+    x, wg, wu = (t[k].detach().double().abs() for k in ("x", "w_gate", "w_up"))
+    least = {"x": (wg.sum(0) + wu.sum(0)).expand(n, d), "w_gate": x.sum(0).expand(f, d), "w_up": x.sum(0).expand(f, d),
+             "b_gate": torch.full((f,), float(n), device="cuda"), "b_up": torch.full((f,), float(n), device="cuda")}
+    for k, g in zip(t, grads):
+        value, bound = want[k]
+        ref.check(g, scaled((value, bound + 2.0 ** -15 * least.get(k, 0)), 2.0 ** -24 * scale, torch.float16), f"d{k}")
+
+
+def test_fp16_ffn_output_gradients_at_their_ends():
+    """All zero, and one that is not finite: its row's gradients alone (and the sums over rows) are no numbers."""
+    from test_gpu_operators import ffn_call, ffn_want
+
+    t = ffn_inputs(30, 64, 72, torch.float16, False, False)
+    x = t["x"].requires_grad_(True)
+    y = ffn_call(t)
+    g, = torch.autograd.grad(y, x, torch.zeros_like(y), retain_graph=True)
+    assert not g.any()
+    steps = torch.randint(-4, 5, (30, 64), device="cuda", generator=torch.Generator(device="cuda").manual_seed(8))
+    value, bound = ffn_want(t, 1.0, steps.half())["x"]
+    both = (t["w_gate"].double().abs() + t["w_up"].double().abs()).sum(0)  # 2^-15 of dg and du, as above
+    want = scaled((value, bound + 2.0 ** -15 * both), 2.0 ** -24, torch.float16)
+    for bad in (math.inf, math.nan):
+        dout = (steps.double() * 2.0 ** -24).half()
+        dout[11, 5] = bad
+        g, = torch.autograd.grad(y, x, dout, retain_graph=True)
+        keep = torch.arange(30, device="cuda") != 11
+        assert not torch.isfinite(g[11]).any()
+        ref.check(g[keep], (want[0][keep], want[1][keep]), "the others")
+
+
+@pytest.mark.parametrize("d,width", [(13, 13), (13, 16), (24, 24), (21, 40), (5, 8), (264, 264)])
+def test_fp16_ffn_finds_the_largest_output_gradient(d, width):
+    """Small output gradients but for one of 100 in the last column of a row: a factor for the small ones alone would
+    make its row infinite."""
+    from test_gpu_operators import ffn_call, ffn_want
+
+    n, f = 70, 40
+    t = ffn_inputs(n, d, f, torch.float16, False, False)
+    for v in t.values():
+        v.requires_grad_(True)
+    buf = torch.full((n, width), 7.0, device="cuda", dtype=torch.float16)  # what lies between the rows has no part
+    buf[:, :d] = rnd(n, d, seed=3) * 2.0 ** -18
+    buf[n - 1, d - 1] = 100.0
+    dout = buf[:, :d]
+    grads = torch.autograd.grad(ffn_call(t), list(t.values()), dout)
+    want = ffn_want(t, 1.0, dout)
+    for k, g in zip(t, grads):
+        ref.check(g, want[k], f"d{k}")
+
+
 # ---------------------------------------------------------------------------
 # large logits
 # ---------------------------------------------------------------------------
