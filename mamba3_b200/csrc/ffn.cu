@@ -17,6 +17,7 @@
 // 277 MB of act, g and u), down 48 us (71 %), dg and du 96 us (34 %: 12 K blocks a tile beside its g and u on
 // their way in, dg and du out: 250 and 106 MB, 45 % of HBM's time), dx and the three weight gradients 192 us
 // (87 %, 1.39 PFLOP/s).
+#include "carve.h"
 #include "ffn_small.h"
 #include "gemm.cuh"
 
@@ -25,19 +26,6 @@ namespace m3b {
 namespace {
 
 constexpr int kMaxWidth = (1 << 22) - 64;  // column blocks of the bias gradients' grid
-
-inline int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
-
-struct Carve {
-  uint8_t* base;
-  size_t at = 0;
-  explicit Carve(void* p) : base(static_cast<uint8_t*>(p)) {}
-  void* take(size_t bytes) {
-    void* r = base ? base + at : nullptr;
-    at += (bytes + 255) / 256 * 256;
-    return r;
-  }
-};
 
 struct Dims {
   int64_t M;
@@ -209,11 +197,6 @@ GemmOperand act_operand(const m3b_gated_ffn_args* a, void* p) {
   return GemmOperand{p, d.M, d.F, ld, d.M * ld, d.np};
 }
 
-#define M3B_TRY(x)                     \
-  do {                                 \
-    const int rc_ = (x);               \
-    if (rc_ != M3B_OK) return rc_;     \
-  } while (0)
 #define M3B_MAP(...) M3B_TRY(gemm_map(__VA_ARGS__))
 
 GemmParams params(const Dims& d, const m3b_gated_ffn_args* a, int bn) {

@@ -63,10 +63,13 @@ __global__ void pack_kernel(const __grid_constant__ PackList l) {
 
 using KernelFn = void (*)(const GemmParams);
 
+// Single CTAs are for forward passes of at most 128 rows; the other forms are null.
 template <int EPI>
 KernelFn pick(bool pair, bool planes) {
-  if (planes) return pair ? (KernelFn)gemm_kernel<EPI, true, true> : (KernelFn)gemm_kernel<EPI, false, true>;
-  return pair ? (KernelFn)gemm_kernel<EPI, true, false> : (KernelFn)gemm_kernel<EPI, false, false>;
+  if (pair) return planes ? (KernelFn)gemm_kernel<EPI, true, true> : (KernelFn)gemm_kernel<EPI, true, false>;
+  if constexpr (EPI == kEpiFinal || EPI == kEpiGlu || EPI == kEpiLse)
+    return planes ? (KernelFn)gemm_kernel<EPI, false, true> : (KernelFn)gemm_kernel<EPI, false, false>;
+  return nullptr;
 }
 
 KernelFn kernel_of(int epi, bool pair, bool planes) {
@@ -112,8 +115,9 @@ int device_setup(int* pairs) {
   }
   for (int epi = 0; epi < kEpiCount; ++epi)
     for (int k = 0; k < 4; ++k) {
-      const cudaError_t e = cudaFuncSetAttribute((const void*)kernel_of(epi, (k & 1) != 0, k >= 2),
-                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kGmSmem);
+      const KernelFn fn = kernel_of(epi, (k & 1) != 0, k >= 2);
+      if (!fn) continue;
+      const cudaError_t e = cudaFuncSetAttribute((const void*)fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kGmSmem);
       if (e != cudaSuccess) return fail(M3B_ERR_CUDA, "gemm: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
     }
   cudaLaunchAttribute at[2];
@@ -242,12 +246,14 @@ int launch_gemm(GemmParams& p, int epi, bool pair, void* parts, cudaStream_t st)
   }
   if (jobs == 0) return M3B_OK;
   if (jobs > (int64_t(1) << 30)) return fail(M3B_ERR_UNSUPPORTED, "gemm: too many tiles");
+  const KernelFn fn = kernel_of(epi, pair, p.npass > 1);
+  if (!fn) return fail(M3B_ERR_UNSUPPORTED, "gemm: no single-CTA kernel of this form");
   if (p.wait_ns == 0) p.wait_ns = kWaitLimitNs;
   const int64_t most = pair ? pairs : num_sms();
   const unsigned workers = (unsigned)(jobs < most ? jobs : most);
   cudaLaunchAttribute attr[2];
   const cudaLaunchConfig_t cfg = config(pair ? 2 * workers : workers, pair, st, attr);
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel_of(epi, pair, p.npass > 1), p);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, p);
   if (e != cudaSuccess) return fail(M3B_ERR_CUDA, "gemm_kernel: %s", cudaGetErrorString(e));
   if (pieces) {
     int split = 1, warps = 1;  // warps to a piece

@@ -17,6 +17,7 @@
 // product 132 us (tensor pipe 92 % active, 1.53 PFLOP/s), softmax - onehot 142 us (84 %; what else it takes is
 // its 262 MB on their way out), both gradients 269 us (87 %, 1.50 PFLOP/s); the copy of the rows, the join and
 // the gradients' join are 30 us together.  With four tenths of the targets ignored, 451 us in all.
+#include "carve.h"
 #include "gemm.cuh"
 #include "xent_small.h"
 
@@ -26,8 +27,6 @@ namespace {
 
 constexpr size_t kPieceBytes = size_t(256) << 20;  // of softmax - onehot in memory at once
 constexpr int kPieceLeast = 2048;                   // columns of a piece at least
-
-inline int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 
 struct Saved {
   uint16_t* h;     // [planes][Tp][Dp] kept rows
@@ -45,17 +44,6 @@ struct Dims {
   explicit Dims(const m3b_linear_xent_args* a)
       : T(a->rows), Tp(up(a->rows, 256)), Dp(up(a->d_model, 8)), D(a->d_model), V(a->vocab),
         np(a->dtype == M3B_F32 ? 3 : 1), f16(a->dtype == M3B_F16), f32(a->dtype == M3B_F32) {}
-};
-
-struct Carve {
-  uint8_t* base;
-  size_t at = 0;
-  explicit Carve(void* p) : base(static_cast<uint8_t*>(p)) {}
-  void* take(size_t bytes) {
-    void* r = base ? base + at : nullptr;
-    at += (bytes + 255) / 256 * 256;
-    return r;
-  }
 };
 
 Saved saved_of(const m3b_linear_xent_args* a, void* p) {
@@ -292,11 +280,6 @@ GemmOperand piece_of(const GemmOperand& w, int64_t c0, int64_t cols) {
   return o;
 }
 
-#define M3B_TRY(x)                     \
-  do {                                 \
-    const int rc_ = (x);               \
-    if (rc_ != M3B_OK) return rc_;     \
-  } while (0)
 #define M3B_MAP(...) M3B_TRY(gemm_map(__VA_ARGS__))
 
 int forward(const m3b_linear_xent_args* a, void* workspace, size_t* need, bool run, cudaStream_t st) {

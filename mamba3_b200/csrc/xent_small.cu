@@ -18,6 +18,7 @@
 
 #include <float.h>
 
+#include "carve.h"
 #include "common.cuh"
 #include "launch.h"
 
@@ -56,17 +57,6 @@ struct SmallXent {
   float* share;  // [slice][M][D] of dh
   int slices, slice_rows;
   int vec;       // rows start on, and are, whole vectors
-};
-
-struct Carve {
-  uint8_t* base;
-  size_t at = 0;
-  explicit Carve(void* p) : base(static_cast<uint8_t*>(p)) {}
-  void* take(size_t bytes) {
-    void* r = base ? base + at : nullptr;
-    at += (bytes + 255) / 256 * 256;
-    return r;
-  }
 };
 
 // Rows of a kernel's form: 1, 2, 4 or 8.
