@@ -63,13 +63,20 @@ __global__ void pack_kernel(const __grid_constant__ PackList l) {
 
 using KernelFn = void (*)(const GemmParams);
 
-// Single CTAs are for forward passes of at most 128 rows; the other forms are null.
+// Single CTAs are for forward passes of at most 128 rows, kEpi*Sums for 16-bit operands; other forms are null.
 template <int EPI>
 KernelFn pick(bool pair, bool planes) {
-  if (pair) return planes ? (KernelFn)gemm_kernel<EPI, true, true> : (KernelFn)gemm_kernel<EPI, true, false>;
-  if constexpr (EPI == kEpiFinal || EPI == kEpiGlu || EPI == kEpiLse)
-    return planes ? (KernelFn)gemm_kernel<EPI, false, true> : (KernelFn)gemm_kernel<EPI, false, false>;
-  return nullptr;
+  if constexpr (EPI == kEpiLseSums || EPI == kEpiDlogitSums) {
+    if (planes) return nullptr;
+    if (pair) return (KernelFn)gemm_kernel<EPI, true, false>;
+    if constexpr (EPI == kEpiLseSums) return (KernelFn)gemm_kernel<EPI, false, false>;
+    return nullptr;
+  } else {
+    if (pair) return planes ? (KernelFn)gemm_kernel<EPI, true, true> : (KernelFn)gemm_kernel<EPI, true, false>;
+    if constexpr (EPI == kEpiFinal || EPI == kEpiGlu || EPI == kEpiLse)
+      return planes ? (KernelFn)gemm_kernel<EPI, false, true> : (KernelFn)gemm_kernel<EPI, false, false>;
+    return nullptr;
+  }
 }
 
 KernelFn kernel_of(int epi, bool pair, bool planes) {
@@ -80,6 +87,8 @@ KernelFn kernel_of(int epi, bool pair, bool planes) {
     case kEpiGlu: return pick<kEpiGlu>(pair, planes);
     case kEpiDglu: return pick<kEpiDglu>(pair, planes);
     case kEpiLse: return pick<kEpiLse>(pair, planes);
+    case kEpiLseSums: return pick<kEpiLseSums>(pair, planes);
+    case kEpiDlogitSums: return pick<kEpiDlogitSums>(pair, planes);
     default: return pick<kEpiDlogit>(pair, planes);
   }
 }

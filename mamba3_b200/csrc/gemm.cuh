@@ -14,7 +14,8 @@
 //   product's sign.)  The
 //   tensor core cuts its sums off instead of rounding them, a bias of half a step per addition that
 //   fp32 results would show (3e-6 of a 323 x 897 product): so every kGmGroup K blocks are a sum of
-//   their own, and the epilogue adds them, rounded, in registers (8e-7).
+//   their own, and the epilogue adds them, rounded, in registers (8e-7).  The loss's logits of 16-bit operands
+//   are sums of groups too (kGmSums).
 // * A launch holds up to four products ("subs"), so that products that are too small to fill the
 //   GPU run side by side, and a product has up to two K segments with operands of their own.
 // * Row or K counts may come from device memory (`dyn`): the loss drops ignored tokens without
@@ -49,6 +50,12 @@ constexpr int kGmSubs = 4;      // products of a launch at most
 constexpr int kGmQueue = 4;     // drawn jobs that the producer may be ahead of the epilogue
 constexpr int kGmBK = 64;
 constexpr int kGmGroup = 4;     // K blocks of fp32 operands summed in one accumulator
+// K blocks of 16-bit operands summed in one accumulator where the result is the loss.  The tensor core's cut-off
+// sums make a loss too small, by 5.5e-7 of it at K = 1024, 1.06e-6 at 2048 and 2.3e-6 at 4096 (fp16; a library
+// product's fp32 logits likewise); in sums of 16 blocks by 5.0e-7 at 2048 and 5.9e-7 at 4096.  16384 x 2048 x
+// 50257 bf16, forward and backward, takes 10.5 ms with either.  (Sums of 8 blocks: 2.9e-7 at 2048; of 4: 1.5e-7, and
+// the forward pass 2.58 ms for 2.41.)  K up to 16 blocks is one sum: the registers between cost K = 128 a tenth.
+constexpr int kGmSums = 16;
 constexpr uint32_t kGmStageA = 128 * kGmBK * 2;     // 16 KB
 constexpr uint32_t kGmStage = 2 * kGmStageA;        // + B: at most 128 rows of 64
 constexpr uint32_t kGmBox = 32 * 128;               // staging of an epilogue warp: 32 rows x 32 fp32
@@ -86,8 +93,10 @@ enum GemmEpi {
   kEpiDglu = 4,    // d(silu(g) u) -> dg, du
   kEpiLse = 5,     // running maximum and sum of each row, and the target's logit
   kEpiDlogit = 6,  // softmax - one-hot
+  kEpiLseSums = 7,     // kEpiLse and kEpiDlogit of 16-bit operands and more than kGmSums K blocks, in sums of at
+  kEpiDlogitSums = 8,  // most that many
 };
-constexpr int kEpiCount = 7;
+constexpr int kEpiCount = 9;
 
 struct GemmSub {
   CUtensorMap a[2], b[2];
@@ -119,6 +128,7 @@ struct GemmParams {
   int nsub;
   int bn;       // accumulator columns of a tile
   int npass;    // plane pairs: 1, or 6 for fp32 operands
+  int group;    // kEpiLseSums, kEpiDlogitSums: K blocks of a sum
   int f16;      // operand type: fp16 instead of bf16
   const int* dyn;
   int* ticket;  // zeroed counter that jobs are drawn from, or null: dealt in turn
@@ -126,7 +136,7 @@ struct GemmParams {
   // kEpiGlu / kEpiDglu: g and u in runs (kGuRun), gu_ld of them (whole 32 columns) for every 32 rows
   uint8_t* gu;
   int64_t gu_ld;
-  // kEpiLse / kEpiDlogit
+  // kEpiLse, kEpiLseSums, kEpiDlogit
   const int* target;       // per row
   float* target_logit;
   float2* part;            // (slots, rows): maximum, and sum of exp(logit - maximum)
@@ -540,6 +550,9 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
   constexpr int kGmStages = EPI == kEpiDglu ? 4 : 6;
   constexpr uint32_t kGmBoxOff = kGmStages * kGmStage, kGuOff = kGmBoxOff + 8 * kGmBox;
   static_assert(kGuOff + (EPI == kEpiDglu ? 8 * kGuSlots * kGuRun<PLANES> : 0) <= kGmBarOff, "shared memory plan");
+  constexpr bool kSums = EPI == kEpiLseSums || EPI == kEpiDlogitSums;
+  constexpr bool GROUPS = PLANES || kSums;  // sums of groups of K blocks, added in registers
+  constexpr int kPart = kSums ? 4 : 2;
   constexpr bool kDraws = EPI == kEpiStore || EPI == kEpiAcc;  // forms with several products a launch
   extern __shared__ uint8_t smraw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smraw) + 1023) & ~uintptr_t(1023));
@@ -612,8 +625,8 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
     if (lane == 0) gm_arrive_first<PAIR>(&jempty[slot]);
     return o;
   };
-  auto group_end = [](const GemmJob& j, int i) {
-    const int e = (i / (6 * kGmGroup) + 1) * 6 * kGmGroup;
+  auto group_end = [&](const GemmJob& j, int i) {
+    const int n = PLANES ? 6 * kGmGroup : p.group, e = (i / n + 1) * n;
     return e < j.ke ? e : j.ke;
   };
   // The first CTA's producer, one thread: job n into both CTAs' queues.
@@ -748,9 +761,9 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
         const uint32_t la = (s.a_mn ? 8192u >> 4 : 1u) << 16, lb = (s.b_mn ? 8192u >> 4 : 1u) << 16;
         const uint32_t hi = (1024u >> 4) | (1u << 14) | (2u << 29);
         int i = job.kb;
-        do {  // one accumulator a job, with planes one a group of K blocks
-          const int e = PLANES ? group_end(job, i) : job.ke;
-          if (PLANES && i == e) break;
+        do {  // one accumulator a job, or one a group of K blocks
+          const int e = GROUPS ? group_end(job, i) : job.ke;
+          if (GROUPS && i == e) break;
           const uint32_t acc = sc & 1;
           ok = __all_sync(0xffffffffu, gm_wait(&acce[acc], ((sc >> 1) & 1) ^ 1, p.wait_ns));
           if (!ok) break;
@@ -780,7 +793,7 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
           }
           if (ok && leader) gm_commit<PAIR>(&accf[acc]);
           ++sc;
-        } while (PLANES && ok && i < job.ke);
+        } while (GROUPS && ok && i < job.ke);
       }
       if (!ok || job.sub == -2) give_up();
     }
@@ -824,7 +837,7 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
     if constexpr (EPI == kEpiDglu)
       for (int i = 0; i < kGuSlots; ++i) gu_send();
     float peak = 1.f;  // fp16: values are kept divided by it
-    if constexpr (EPI == kEpiDlogit || EPI == kEpiDglu) {
+    if constexpr (EPI == kEpiDlogit || EPI == kEpiDlogitSums || EPI == kEpiDglu) {
       if (p.peaks) {
         peak = peak_scale(p.peaks, p.npeaks);
         if constexpr (EPI == kEpiDglu) peak = fminf(peak * 256.f, 1.f);  // up to 2^-8, never down: see ffn.cu
@@ -856,10 +869,10 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
         if (lane == 0) gm_arrive_first<PAIR>(&acce[sc & 1]);
         ++sc;
       };
-      float part[2][32];  // with planes: 64 columns (GLU: 32 of either half), summed over the groups
-      if constexpr (PLANES) {
+      float part[kPart][32];  // the columns (GLU: 32 of either half), summed over the groups
+      if constexpr (GROUPS) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
+        for (int k = 0; k < kPart; ++k)
 #pragma unroll
           for (int i = 0; i < 32; ++i) part[k][i] = 0.f;
         bool fine = true;
@@ -867,14 +880,24 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
           fine = await();
           if (!fine) break;
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            if (k == 1 && EPI != kEpiGlu && bn < 128) break;
-            uint32_t ra[32];
-            __syncwarp();
-            tmem_ld32_async(tc + (EPI == kEpiGlu ? half * (bn / 4) + k * (bn / 2) : cfirst + 32 * k), ra);
-            tmem_wait_ld(ra);
+          for (int k = 0; k < kPart; ++k) {
+            if (EPI != kEpiGlu && 32 * k >= bn / 2) break;
+            constexpr int kRun = kPart == 4 ? 16 : 32;  // beside 128 sums, 32 more registers would spill
 #pragma unroll
-            for (int e = 0; e < 32; ++e) part[k][e] += __uint_as_float(ra[e]);
+            for (int h = 0; h < 32; h += kRun) {
+              uint32_t ra[kRun];
+              __syncwarp();
+              const uint32_t at = tc + (EPI == kEpiGlu ? half * (bn / 4) + k * (bn / 2) : cfirst + 32 * k) + h;
+              if constexpr (kRun == 16) tmem_ld16_async(at, ra);
+              else tmem_ld32_async(at, ra);
+              tmem_wait_ld(ra);
+#pragma unroll
+              for (int e = 0; e < kRun; e += 2) {
+                const float2 x = add2(make_float2(part[k][h + e], part[k][h + e + 1]),
+                                      make_float2(__uint_as_float(ra[e]), __uint_as_float(ra[e + 1])));
+                part[k][h + e] = x.x, part[k][h + e + 1] = x.y;
+              }
+            }
           }
           release();
         }
@@ -892,21 +915,21 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
       // an asynchronous load still writes must not be moved or spilled, and the second warp of the
       // same lanes covers the wait.
       auto columns = [&](int c0, int c1, auto&& f) {
-        if constexpr (PLANES) {
+        if constexpr (GROUPS) {
 #pragma unroll
-          for (int k = 0; k < 2; ++k)
+          for (int k = 0; k < kPart; ++k)
             if (c0 + 32 * k < c1) f(c0 + 32 * k, part[k]);
-          return;
-        }
-        for (int c = c0; c < c1; c += 32) {
-          uint32_t ra[32];
-          __syncwarp();
-          tmem_ld32_async(tc + c, ra);
-          tmem_wait_ld(ra);
-          float v[32];
+        } else {
+          for (int c = c0; c < c1; c += 32) {
+            uint32_t ra[32];
+            __syncwarp();
+            tmem_ld32_async(tc + c, ra);
+            tmem_wait_ld(ra);
+            float v[32];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = none ? 0.f : __uint_as_float(ra[i]);
-          f(c, v);
+            for (int i = 0; i < 32; ++i) v[i] = none ? 0.f : __uint_as_float(ra[i]);
+            f(c, v);
+          }
         }
       };
       auto scale_of = [&]() {
@@ -1095,7 +1118,7 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
             send(&p.o[1], col, rows.row0, 0, wu);
           }
         });
-      } else if constexpr (EPI == kEpiLse) {
+      } else if constexpr (EPI == kEpiLse || EPI == kEpiLseSums) {
         const int tgt = rok ? p.target[grow] : -1;
         // the maximum as it is: a product with log2(e) would be rounded to 2^-24 of it, and with it the loss.
         // It starts at the least finite value, so that a set of -infinities has a sum of 0.
@@ -1159,7 +1182,7 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
           put_operand<PLANES>(send, &p.o[0], p.f16, col, rows.row0, v);
         });
       }
-      if constexpr (!PLANES) release();
+      if constexpr (!GROUPS) release();
     }
     if (job.sub == -2) give_up();
     if (lane == 0) bulk_wait_group_all();  // boxes stay until they have been sent

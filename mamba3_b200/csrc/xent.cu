@@ -282,6 +282,12 @@ GemmOperand piece_of(const GemmOperand& w, int64_t c0, int64_t cols) {
 
 #define M3B_MAP(...) M3B_TRY(gemm_map(__VA_ARGS__))
 
+// K blocks of the logits' sums of 16-bit operands (kGmSums), of equal length; 0: one sum.
+int group_of(const Dims& d) {
+  const int nk = (d.D + kGmBK - 1) / kGmBK, groups = d.f32 ? 1 : (nk + kGmSums - 1) / kGmSums;
+  return groups > 1 ? (nk + groups - 1) / groups : 0;
+}
+
 int forward(const m3b_linear_xent_args* a, void* workspace, size_t* need, bool run, cudaStream_t st) {
   const Dims d(a);
   if (d.T <= kSmallXentRows) return small_xent_fwd(a, workspace, need, run, st);
@@ -320,12 +326,14 @@ int forward(const m3b_linear_xent_args* a, void* workspace, size_t* need, bool r
   g.m_dyn = 1;
   g.N = d.V;
   g.nk[0] = (d.D + kGmBK - 1) / kGmBK;
+  p.group = group_of(d);
   p.target = s.target;
   p.target_logit = target_logit;
   p.part = part;
   p.part_ld = d.Tp;
-  plan_gemm(p, kEpiLse, pair);
-  M3B_TRY(launch_gemm(p, kEpiLse, pair, nullptr, st));
+  const int epi = p.group ? kEpiLseSums : kEpiLse;
+  plan_gemm(p, epi, pair);
+  M3B_TRY(launch_gemm(p, epi, pair, nullptr, st));
   if (a->reduction == 0 && cudaMemsetAsync(a->loss, 0, (size_t)d.T * 4, st) != cudaSuccess)
     return check_launch("linear_xent loss");
   return launch_dependent(join_kernel, dim3((unsigned)(d.Tp / 32)), 512, st, (const float2*)part, nt * 2, d.Tp,
@@ -456,8 +464,10 @@ int backward(const m3b_linear_xent_args* a, void* workspace, size_t* need, bool 
       }
       p.col0 = (int)c0;
       p.clear = ticket;
-      plan_gemm(p, kEpiDlogit, true);
-      M3B_TRY(launch_gemm(p, kEpiDlogit, true, nullptr, st));
+      p.group = group_of(d);  // the logits of the forward pass: a sure token's gradient is their difference
+      const int epi = p.group ? kEpiDlogitSums : kEpiDlogit;
+      plan_gemm(p, epi, true);
+      M3B_TRY(launch_gemm(p, epi, true, nullptr, st));
     }
     GemmParams p = base;
     M3B_TRY(gradients(p, c0, n, &z, &wp));

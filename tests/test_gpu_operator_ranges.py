@@ -373,3 +373,53 @@ def test_fp32_infinities_are_those_of_the_sums(n):
     x[2, 3] = math.nan
     y = gated_ffn(x, w, w, wd)
     assert torch.isfinite(y[rows]).all() and torch.isnan(y[2]).all()
+
+
+# ---------------------------------------------------------------------------
+# long sums of 16-bit operands
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", DTYPES[:2], ids=IDS[:2])
+@pytest.mark.parametrize("n", [40, 300])
+@pytest.mark.parametrize("k", [1024, 4096, 8192, 8200])
+def test_loss_of_long_sums_of_one_sign(k, n, dtype):
+    """The tensor core cuts off each sum of sixteen products (perhaps in two halves), always downwards where all are
+    positive: at most two steps of 2^-23 of the sum so far, half of the whole on average over the 64 of a group
+    of 1024: 65 steps.  The groups' sums and the loss's own rounding, five.  The loss of two logits z and 0 is z for the
+    second."""
+    from mamba3_b200 import linear_cross_entropy
+
+    h = 1.0 + torch.rand(n, k, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    w = torch.zeros(2, k, device="cuda")
+    w[0] = (1.0 + torch.rand(k, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2))) / 16
+    h, w = h.to(dtype), w.to(dtype)
+    t = torch.ones(n, dtype=torch.long, device="cuda")
+    z = h.double() @ w[0].double()
+    y = linear_cross_entropy(h, w, t, reduction="none").double()
+    assert bool(((y - z).abs() <= 70 * 2.0 ** -23 * z).all()), float(((y - z).abs() / z).max())
+
+
+@pytest.mark.parametrize("dtype", DTYPES[:2], ids=IDS[:2])
+@pytest.mark.parametrize("n", [40, 300])
+def test_gradient_of_sure_tokens_uses_the_loss_s_logits(n, dtype):
+    """d_model 4096: exp(loss) is 1 / p of the target, and the gradient along a weight column of ones that no logit
+    reads is 0: the backward pass makes the same logits as the forward pass, or the probabilities' sum would be off by
+    the cut-off sums' bias.  399 other logits about 8 below: dz is rounded to 16 bits (2^-8, 2^-11 of each), the sums
+    to 2^-18 of all magnitudes; the gradient of the target's own column is p - 1 within the same."""
+    from mamba3_b200 import linear_cross_entropy
+
+    v, d = 400, 4096
+    g = torch.Generator(device="cuda").manual_seed(3)
+    h = (1.0 + torch.rand(n, d, device="cuda", generator=g)) / 32
+    w = (torch.rand(v, d, device="cuda", generator=g) * 0.5 + 0.5) * 0.1
+    w[5] = w[5] + 0.04
+    h[:, 0] = 0.0
+    w[:, 0] = 1.0
+    h, w = h.to(dtype).requires_grad_(True), w.to(dtype)
+    t = torch.full((n,), 5, device="cuda")
+    y = linear_cross_entropy(h, w, t, reduction="none")
+    p = torch.softmax(h.detach().double() @ w.double().t(), 1)
+    rest = 1.0 - p[:, 5]
+    dh, = torch.autograd.grad(y.sum(), h)
+    assert bool((rest < 0.5).all()) and bool((rest > 1e-6).all())
+    bound = 2 * rest * (2 * ref.half_step(dtype) + 2.0 ** -18) + 2 * 2.0 ** -22 + ref.least(dtype)
+    assert bool((dh[:, 0].double().abs() <= bound).all()), float((dh[:, 0].double().abs() / bound).max())
