@@ -423,3 +423,125 @@ def test_gradient_of_sure_tokens_uses_the_loss_s_logits(n, dtype):
     assert bool((rest < 0.5).all()) and bool((rest > 1e-6).all())
     bound = 2 * rest * (2 * ref.half_step(dtype) + 2.0 ** -18) + 2 * 2.0 ** -22 + ref.least(dtype)
     assert bool((dh[:, 0].double().abs() <= bound).all()), float((dh[:, 0].double().abs() / bound).max())
+
+
+# ---------------------------------------------------------------------------
+# captured, and from several threads
+# ---------------------------------------------------------------------------
+def captured(step):
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    return graph, out
+
+
+@pytest.mark.parametrize("d", [64, 2000])
+def test_fp16_steps_captured_follow_their_gradients_range(d):
+    """The factors of the fp16 backward passes are made on the device: a replay with output gradients and weights of
+    another size gives the eager call's values."""
+    from mamba3_b200 import gated_ffn, linear_cross_entropy
+
+    n, f, v = 70, 72, 500
+    t = ffn_inputs(n, d, f, torch.float16, True, False)
+    h, w, tg = loss_inputs(n, d, v, torch.float16, 0.2)
+    leaves = [q.requires_grad_(True) for q in (*t.values(), h, w)]
+    dout, dl = torch.zeros(n, d, device="cuda", dtype=torch.float16), torch.zeros(n, device="cuda")
+
+    def step():
+        y = gated_ffn(*leaves[:4], b_gate=leaves[4], b_up=leaves[5], b_down=leaves[6])
+        loss = linear_cross_entropy(leaves[7], leaves[8], tg, reduction="none")
+        return (y.detach(), loss.detach(), *torch.autograd.grad((y, loss), leaves, (dout, dl)))
+
+    graph, got = captured(step)
+    for seed, scale in ((1, 1.0), (2, 2.0 ** -18), (3, 0.0), (4, 2.0 ** 6)):
+        dout.copy_(rnd(n, d, seed=seed) * scale)
+        dl.copy_(rnd(n, seed=seed + 9) * scale)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b) and bool(torch.isfinite(a).all())
+
+
+def test_calls_from_several_threads_on_one_stream():
+    """Each thread's workspaces are its own until its kernels are launched: all get the values of a call alone."""
+    import threading
+
+    from mamba3_b200 import clip_grads, gated_ffn, linear_cross_entropy
+
+    jobs = []
+    for i, (n, d, f, v, dtype) in enumerate([(40, 130, 72, 333, torch.float32), (300, 65, 130, 777, torch.bfloat16),
+                                             (9, 33, 40, 1000, torch.float16), (5, 64, 72, 2000, torch.bfloat16)]):
+        t = ffn_inputs(n, d, f, dtype, True, True, seed=10 * i)
+        h, w, tg = loss_inputs(n, d, v, dtype, 0.1, seed=10 * i)
+        tg[0] = 1
+        jobs.append(([q.requires_grad_(True) for q in (*t.values(), h, w)], tg))
+
+    def step(leaves, tg):
+        y = gated_ffn(*leaves[:4], b_gate=leaves[4], b_up=leaves[5], b_down=leaves[6], residual=leaves[7])
+        loss = linear_cross_entropy(leaves[8], leaves[9], tg)
+        grads = torch.autograd.grad(y.float().square().sum() + loss, leaves)
+        outs = [torch.empty_like(g) for g in grads]
+        return [y.detach(), loss.detach(), *grads, clip_grads(grads, 0.1, out=outs), *outs]
+
+    want = [step(*j) for j in jobs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        try:
+            for _ in range(30):
+                got = step(*jobs[i])
+                wrong.extend((i, k) for k, (a, b) in enumerate(zip(got, want[i])) if not torch.equal(a, b))
+        except Exception as e:  # noqa: BLE001 - reported by the test
+            wrong.append((i, e))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(jobs))]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not wrong, wrong[:5]
+
+
+@pytest.mark.parametrize("ckpt", [False, True])
+@pytest.mark.parametrize("cast", [None, torch.bfloat16, torch.float16])
+def test_lm_without_logits_under_autocast_and_checkpointing(cast, ckpt):
+    from mamba3_b200 import KulaMambaLM
+
+    torch.manual_seed(0)
+    lm = KulaMambaLM(vocab_size=203, d_model=64, n_layers=2, d_state=16, headdim=16, fused_mlp=True,
+                     gradient_checkpointing=ckpt).cuda().train()
+    ids = torch.randint(0, 203, (2, 40), device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    losses, grads = [], []
+    for logits in (True, False):
+        lm.zero_grad()
+        with torch.autocast("cuda", cast or torch.bfloat16, enabled=cast is not None):
+            loss = lm(ids, ids, return_logits=logits)["loss"]
+        loss.backward()
+        losses.append(loss.detach())
+        grads.append([p.grad.clone() for p in lm.parameters()])
+    torch.testing.assert_close(losses[1].float(), losses[0].float(), rtol=2e-3, atol=0)
+    for a, b in zip(*grads):
+        assert b.dtype == torch.float32 and (a - b).norm() <= 3e-2 * a.norm()
+
+
+def test_loss_of_small_integer_targets_and_expanded_weights():
+    """int8 and uint8 targets, an expanded incoming gradient, one row of hidden states for every token."""
+    from mamba3_b200 import linear_cross_entropy
+
+    h, w, t = loss_inputs(60, 64, 100, torch.bfloat16)
+    want = ref.loss(h, w, t, reduction="none", dloss=torch.full((60,), 0.5, device="cuda"))
+    for dt in (torch.int8, torch.uint8):
+        a = h.clone().requires_grad_(True)
+        y = linear_cross_entropy(a, w, t.to(dt), reduction="none")
+        ref.check(y, want["loss"], str(dt))
+        g, = torch.autograd.grad(y, a, torch.tensor(0.5, device="cuda").expand(60))
+        ref.check(g, want["hidden"], str(dt))
+    row = h[:1].clone().requires_grad_(True)
+    g, = torch.autograd.grad(linear_cross_entropy(row.expand(60, 64), w, t, reduction="sum"), row)
+    same = ref.loss(h[:1].expand(60, 64), w, t, reduction="sum", dloss=1.0)["hidden"]
+    ref.check(g, (same[0].sum(0, keepdim=True), same[1].sum(0, keepdim=True) * 2 + 60 * 2.0 ** -8 * same[0].abs().sum(0, keepdim=True)), "one row")
