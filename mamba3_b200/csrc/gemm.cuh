@@ -14,7 +14,7 @@
 //   product's sign.)  The
 //   tensor core cuts its sums off instead of rounding them, a bias of half a step per addition that
 //   fp32 results would show (3e-6 of a 323 x 897 product): so every kGmGroup K blocks are a sum of
-//   their own, and the epilogue adds them, rounded, in registers (8e-7).  The loss's logits of 16-bit operands
+//   their own, and the epilogue adds them, rounded, in registers (7e-7).  The loss's logits of 16-bit operands
 //   are sums of groups too (kGmSums).
 // * A launch holds up to four products ("subs"), so that products that are too small to fill the
 //   GPU run side by side, and a product has up to two K segments with operands of their own.

@@ -13,10 +13,11 @@
 // pieces in fp32.  8 rows d_model vocab operations forward and backward, 2 more than with the
 // logits kept.  At most kSmallXentRows rows take the matrix-vector form of xent_small.cu.
 //
-// Bound by the tensor cores, and in long runs by the power they draw.  4096 x 768 x 32000 bf16: the forward
-// product 132 us (tensor pipe 92 % active, 1.53 PFLOP/s), softmax - onehot 142 us (84 %; what else it takes is
-// its 262 MB on their way out), both gradients 269 us (87 %, 1.50 PFLOP/s); the copy of the rows, the join and
-// the gradients' join are 30 us together.  With four tenths of the targets ignored, 451 us in all.
+// Bound by the tensor cores, and in long runs by the power they draw.  4096 x 768 x 32000 bf16, each launch by
+// itself at 1.6 - 1.7 GHz: the forward product 113 us (tensor pipe 92 % active, 1.77 PFLOP/s), softmax - onehot
+// 127 us (80 %; what else it takes is its 262 MB on their way out), both gradients 244 us (87 %, 1.65 PFLOP/s); the
+// kept rows' numbers, their copy, the join and the gradients' join 5, 6, 9 and 16 us.  With four tenths of the
+// targets ignored 71, 85, 152 and 5, 6, 9 and 14 us, and 441 us a call of a long run, whose clock is lower.
 #include "carve.h"
 #include "gemm.cuh"
 #include "xent_small.h"

@@ -165,6 +165,7 @@ def kernel_workload(case: str, reps: int = 3) -> None:
     xent     linear_cross_entropy, hidden (4096, 768) x weight (32000, 768) bf16, forward and backward:
              keep, gather, gemm_kernel (statistics), join, then per piece of the vocabulary gemm_kernel
              (softmax - onehot) and gemm_kernel (both gradients)
+    xent_masked  the same with four tenths of the targets ignored
     ffn      gated_ffn, x (16384, 768) x d_ff 2112 bf16, forward and backward: gemm_kernel four times
              (gate | up, down, dg and du, dx and the weight gradients)
     clip     clip_grads of 238 M bf16 gradients in 400 tensors into fp32: norm_kernel, clip_kernel
@@ -205,14 +206,16 @@ def kernel_workload(case: str, reps: int = 3) -> None:
                     torch.randn(H, device="cuda", generator=g), r(B, T, H, P, R), r(B, T, H, P, R), f(B, H, P, N),
                     f(B, H, P, N))
             run = lambda: _lib.chunked_ssd_bwd(*args)  # noqa: E731
-        elif case in ("xent", "ffn"):
+        elif case in ("xent", "xent_masked", "ffn"):
             from .ffn import gated_ffn
             from .loss import linear_cross_entropy
 
             r = lambda *sh: torch.randn(*sh, device="cuda", generator=g).mul_(sh[-1] ** -0.5).to(torch.bfloat16)  # noqa: E731
-            if case == "xent":
+            if case != "ffn":
                 leaves = [r(4096, 768) * 28, r(32000, 768) * 2.5]
                 t = torch.randint(0, 32000, (4096,), device="cuda", generator=g)
+                if case == "xent_masked":
+                    t[torch.rand(4096, device="cuda", generator=g) < 0.4] = -100
                 f = lambda: linear_cross_entropy(*leaves, t)  # noqa: E731
             else:
                 leaves = [r(16384, 768) * 28, r(2112, 768), r(2112, 768), r(768, 2112)]
@@ -273,7 +276,7 @@ if __name__ == "__main__":
 
     ap = argparse.ArgumentParser(description="profiling helpers")
     ap.add_argument("what", choices=["train", "train_lm", "cfg3", "chunked", "chunked_bwd", "step", "fp32",
-                                     "in_proj", "xent", "ffn", "clip", "decode"])
+                                     "in_proj", "xent", "xent_masked", "ffn", "clip", "decode"])
     ap.add_argument("--batch", type=int)
     ap.add_argument("--seqlen", type=int)
     ap.add_argument("--reps", type=int, default=3)
