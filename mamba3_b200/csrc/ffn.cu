@@ -58,9 +58,10 @@ GemmOut result(void* p, int64_t ld, int dtype) {
 
 // Sums over the rows of up to three operands, times `scale`, in a fixed order.  A block takes 64 columns (two a
 // lane) and kSumRows rows, its warps every eighth row, and leaves one partial; the chunks' partials
-// are added by a second kernel.  The bias gradients are sums of dg and du as the products read them: in 16 bits
-// their rounding, a random half step a row, leaves the sum as far off as its own rounding does (2.1e-3 and
-// 1.3e-3 of 10505 rows in bf16); summed before it, in the epilogue, it would cost registers that spill there.
+// are added by a second kernel.  dg and du of 16 bits are summed before they are rounded, by the epilogue that
+// makes them (kEpiDgluSums), which leaves the partials of 32 rows: 16384 x 768 x 2112 bf16 with biases, forward and
+// backward, 730 - 780 us, and 805 with the rounded dg and du read once more (2.1e-3 off, where the result's own
+// rounding is 1.3e-3).
 constexpr int kSumRows = 128;
 struct Sums {
   struct {
@@ -70,9 +71,11 @@ struct Sums {
     float scale;
     const float* num;  // scale *= *num, or null
     void* out;
-    float* part;
+    float* part;       // [parts][cols]
+    int parts;
   } s[3];
-  int n, f16, planes, dt, chunks;
+  int n, f16, planes, dt;
+  int made;            // of the n, the first ones whose partials colsum_kernel makes
   int64_t rows;
 };
 __global__ void __launch_bounds__(256) colsum_kernel(const __grid_constant__ Sums a) {
@@ -111,7 +114,7 @@ __global__ void __launch_bounds__(256) colsum_finish_kernel(const __grid_constan
   float s = 0.f;
   if (c < m.cols) {
 #pragma unroll 4
-    for (int k = w; k < a.chunks; k += 8) s += m.part[(int64_t)k * m.cols + c];
+    for (int k = w; k < m.parts; k += 8) s += m.part[(int64_t)k * m.cols + c];
   }
   sm[w][lane] = s;
   __syncthreads();
@@ -123,7 +126,10 @@ int colsums(const Sums& a, cudaStream_t st) {
   if (a.n == 0) return M3B_OK;
   int cols = 0;
   for (int i = 0; i < a.n; ++i) cols = a.s[i].cols > cols ? a.s[i].cols : cols;
-  const int rc = launch_dependent(colsum_kernel, dim3(a.chunks, (cols + 63) / 64, a.n), 256, st, a);
+  int rc = M3B_OK;
+  if (a.made)
+    rc = launch_dependent(colsum_kernel, dim3((unsigned)((a.rows + kSumRows - 1) / kSumRows), (cols + 63) / 64, a.made), 256,
+                          st, a);
   return rc != M3B_OK ? rc : launch_dependent(colsum_finish_kernel, dim3((cols + 31) / 32, a.n), 256, st, a);
 }
 
@@ -294,17 +300,22 @@ int backward(const m3b_gated_ffn_args* a, void* workspace, size_t* need, bool ru
   const GemmOperand act = act_operand(a, a->saved_act);
   Sums sums{};
   sums.f16 = d.f16, sums.planes = d.np, sums.dt = a->dtype, sums.rows = d.M;
-  sums.chunks = (int)((d.M + kSumRows - 1) / kSumRows);
   float* peaks = d.f16 ? static_cast<float*>(ws.take((kPeakBlocks + 1) * 4)) : nullptr;
   float* peak = peaks ? peaks + kPeakBlocks : nullptr;
-  auto sum = [&](const GemmOperand& o, float scale, const float* num, void* out) {
-    if (!out) return;
-    float* part = static_cast<float*>(ws.take((size_t)sums.chunks * o.cols * 4));
-    sums.s[sums.n++] = {static_cast<const uint16_t*>(o.p), o.plane, o.ld, (int)o.cols, scale, num, out, part};
+  // of an operand, or of the partials that the epilogue leaves of it
+  auto sum = [&](const GemmOperand& o, bool made, float scale, const float* num, void* out) {
+    const int64_t rows = made ? kSumRows : 32;
+    const int parts = (int)((d.M + rows - 1) / rows);
+    float* part = static_cast<float*>(ws.take((size_t)parts * o.cols * 4));
+    if (out) sums.s[sums.n++] = {static_cast<const uint16_t*>(o.p), o.plane, o.ld, (int)o.cols, scale, num, out, part, parts};
+    if (out && made) ++sums.made;
+    return part;
   };
-  sum(dg, 1.f, peak, a->db_gate);
-  sum(du, 1.f, peak, a->db_up);
-  sum(dy, a->residual_scale, nullptr, a->db_down);
+  if (a->db_down) sum(dy, true, a->residual_scale, nullptr, a->db_down);
+  const bool in_epilogue = !d.f32 && (a->db_gate || a->db_up);
+  float *sum_g = nullptr, *sum_u = nullptr;
+  if (in_epilogue || a->db_gate) sum_g = sum(dg, !in_epilogue, 1.f, peak, a->db_gate);
+  if (in_epilogue || a->db_up) sum_u = sum(du, !in_epilogue, 1.f, peak, a->db_up);
   int* ticket = static_cast<int*>(ws.take(4));
 
   // dx and the three weight gradients, side by side
@@ -368,8 +379,11 @@ int backward(const m3b_gated_ffn_args* a, void* workspace, size_t* need, bool ru
       p.npeaks = kPeakBlocks;
       p.peak_out = peak;
     }
-    plan_gemm(p, kEpiDglu, true);
-    M3B_TRY(launch_gemm(p, kEpiDglu, true, nullptr, st));
+    p.sum_g = sum_g;
+    p.sum_u = sum_u;
+    const int epi = in_epilogue ? kEpiDgluSums : kEpiDglu;
+    plan_gemm(p, epi, true);
+    M3B_TRY(launch_gemm(p, epi, true, nullptr, st));
   }
   if (q.nsub) M3B_TRY(launch_gemm(q, kEpiStore, true, parts, st));
   return colsums(sums, st);

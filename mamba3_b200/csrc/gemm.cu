@@ -66,7 +66,7 @@ using KernelFn = void (*)(const GemmParams);
 // Single CTAs are for forward passes of at most 128 rows, kEpi*Sums for 16-bit operands; other forms are null.
 template <int EPI>
 KernelFn pick(bool pair, bool planes) {
-  if constexpr (EPI == kEpiLseSums || EPI == kEpiDlogitSums) {
+  if constexpr (EPI == kEpiLseSums || EPI == kEpiDlogitSums || EPI == kEpiDgluSums) {
     if (planes) return nullptr;
     if (pair) return (KernelFn)gemm_kernel<EPI, true, false>;
     if constexpr (EPI == kEpiLseSums) return (KernelFn)gemm_kernel<EPI, false, false>;
@@ -89,6 +89,7 @@ KernelFn kernel_of(int epi, bool pair, bool planes) {
     case kEpiLse: return pick<kEpiLse>(pair, planes);
     case kEpiLseSums: return pick<kEpiLseSums>(pair, planes);
     case kEpiDlogitSums: return pick<kEpiDlogitSums>(pair, planes);
+    case kEpiDgluSums: return pick<kEpiDgluSums>(pair, planes);
     default: return pick<kEpiDlogit>(pair, planes);
   }
 }

@@ -95,8 +95,9 @@ enum GemmEpi {
   kEpiDlogit = 6,  // softmax - one-hot
   kEpiLseSums = 7,     // kEpiLse and kEpiDlogit of 16-bit operands and more than kGmSums K blocks, in sums of at
   kEpiDlogitSums = 8,  // most that many
+  kEpiDgluSums = 9,    // kEpiDglu of 16-bit operands, with the column sums of dg and du before they are rounded
 };
-constexpr int kEpiCount = 9;
+constexpr int kEpiCount = 10;
 
 struct GemmSub {
   CUtensorMap a[2], b[2];
@@ -136,6 +137,7 @@ struct GemmParams {
   // kEpiGlu / kEpiDglu: g and u in runs (kGuRun), gu_ld of them (whole 32 columns) for every 32 rows
   uint8_t* gu;
   int64_t gu_ld;
+  float *sum_g, *sum_u;  // kEpiDgluSums: [row / 32][column of sub[0].N], sums over 32 rows
   // kEpiLse, kEpiLseSums, kEpiDlogit
   const int* target;       // per row
   float* target_logit;
@@ -547,9 +549,10 @@ template <int EPI, bool PAIR, bool PLANES>
 __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_constant__ GemmParams p) {
   constexpr int kTileM = PAIR ? 256 : 128;
   // six stages; kEpiDglu gives two of them to the runs of g and u
-  constexpr int kGmStages = EPI == kEpiDglu ? 4 : 6;
+  constexpr bool kDglu = EPI == kEpiDglu || EPI == kEpiDgluSums;
+  constexpr int kGmStages = kDglu ? 4 : 6;
   constexpr uint32_t kGmBoxOff = kGmStages * kGmStage, kGuOff = kGmBoxOff + 8 * kGmBox;
-  static_assert(kGuOff + (EPI == kEpiDglu ? 8 * kGuSlots * kGuRun<PLANES> : 0) <= kGmBarOff, "shared memory plan");
+  static_assert(kGuOff + (kDglu ? 8 * kGuSlots * kGuRun<PLANES> : 0) <= kGmBarOff, "shared memory plan");
   constexpr bool kSums = EPI == kEpiLseSums || EPI == kEpiDlogitSums;
   constexpr bool GROUPS = PLANES || kSums;  // sums of groups of K blocks, added in registers
   constexpr int kPart = kSums ? 4 : 2;
@@ -834,13 +837,13 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
       }
       ++gu_run;
     };
-    if constexpr (EPI == kEpiDglu)
+    if constexpr (kDglu)
       for (int i = 0; i < kGuSlots; ++i) gu_send();
     float peak = 1.f;  // fp16: values are kept divided by it
-    if constexpr (EPI == kEpiDlogit || EPI == kEpiDlogitSums || EPI == kEpiDglu) {
+    if constexpr (EPI == kEpiDlogit || EPI == kEpiDlogitSums || kDglu) {
       if (p.peaks) {
         peak = peak_scale(p.peaks, p.npeaks);
-        if constexpr (EPI == kEpiDglu) peak = fminf(peak * 256.f, 1.f);  // up to 2^-8, never down: see ffn.cu
+        if constexpr (kDglu) peak = fminf(peak * 256.f, 1.f);  // up to 2^-8, never down: see ffn.cu
         if (blockIdx.x == 0 && threadIdx.x == 64) *p.peak_out = peak;
       }
     }
@@ -1057,7 +1060,7 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
           }
           if (rows.row0 < M) put_operand<PLANES>(send, &p.o[0], p.f16, col, rows.row0, g);
         }
-      } else if constexpr (EPI == kEpiDglu) {
+      } else if constexpr (kDglu) {
         const float factor = s.alpha / peak;
         columns(cfirst, clast, [&](int c, float (&d)[32]) {
           const int col = job.nt * bn + c;
@@ -1106,6 +1109,25 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
                 wg[4 * h + i] = pack16(dg[2 * i], dg[2 * i + 1], p.f16);
                 wu[4 * h + i] = pack16(du[2 * i], du[2 * i + 1], p.f16);
               }
+            }
+            if constexpr (EPI == kEpiDgluSums) {
+              // sums of 16 columns over the warp's rows in 16 shuffles: each step sends the half that the other
+              // lane keeps, until lanes 2i and 2i + 1 have column i
+              float a[16];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) a[i] = rok ? dg[i] : 0.f, a[8 + i] = rok ? du[i] : 0.f;
+#pragma unroll
+              for (int o = 16, n = 8; n > 0; o >>= 1, n >>= 1) {
+                const bool upper = (lane & o) != 0;
+#pragma unroll
+                for (int i = 0; i < n; ++i) {
+                  const float other = __shfl_xor_sync(0xffffffffu, upper ? a[i] : a[i + n], o);
+                  a[i] = (upper ? a[i + n] : a[i]) + other;
+                }
+              }
+              a[0] += __shfl_xor_sync(0xffffffffu, a[0], 1);
+              const int v = lane >> 1, c8 = col + 8 * h + (v & 7);
+              if (!(lane & 1) && rows.row0 < M && c8 < s.N) (v < 8 ? p.sum_g : p.sum_u)[(rows.row0 >> 5) * s.N + c8] = a[0];
             }
           }
           if constexpr (PLANES) {
@@ -1186,7 +1208,7 @@ __global__ void __launch_bounds__(kGmThreads, 1) gemm_kernel(const __grid_consta
     }
     if (job.sub == -2) give_up();
     if (lane == 0) bulk_wait_group_all();  // boxes stay until they have been sent
-    if constexpr (EPI == kEpiDglu)  // an aborted run leaves once its copies have landed
+    if constexpr (kDglu)  // an aborted run leaves once its copies have landed
       for (; gu_used < gu_sent; ++gu_used) mbar_wait(&gub[gu_used % kGuSlots], (gu_used / kGuSlots) & 1, 10000000ull);
   }
   tc_fence_before();

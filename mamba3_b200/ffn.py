@@ -49,7 +49,7 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     autocast dtype first.  Any sizes and strides: operands that the copies cannot read in place
     (widths that are no multiple of 8, a last dimension with a stride, fp32) are laid out once per
     call.  Differentiable in every tensor argument; sums in fp32, and the activation (forward) and its
-    two factors' gradients (backward, the bias gradients' summands too) rounded to a 16-bit dtype once
+    two factors' gradients (backward) rounded to a 16-bit dtype once, as operands of the next products
     (fp16: relative to the largest incoming gradient, so that small ones keep their bits)."""
     if x.is_cuda and torch.is_autocast_enabled("cuda"):
         dt = torch.get_autocast_dtype("cuda")

@@ -426,6 +426,39 @@ def test_gradient_of_sure_tokens_uses_the_loss_s_logits(n, dtype):
 
 
 # ---------------------------------------------------------------------------
+# sums over the rows
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("n", [1, 20, 33, 300])
+@pytest.mark.parametrize("frozen", [(), ("b_gate",), ("b_up",), ("b_down",)])
+def test_bias_gradients_are_sums_of_what_is_not_rounded(n, frozen, dtype):
+    """Inputs whose products are exact in any type (steps of 2^-5, sums of 16): the bias gradients are then off by their
+    one rounding and 2^-18 of the summands' magnitudes (the hardware's exponential and reciprocal, a few steps of
+    2^-22 each, and the fp32 sums)."""
+    from mamba3_b200 import gated_ffn
+
+    d, f = 16, 200
+    g = torch.Generator(device="cuda").manual_seed(n)
+    ints = lambda *s, top: torch.randint(-top, top + 1, s, device="cuda", generator=g).to(dtype)  # noqa: E731
+    t = {"x": ints(n, d, top=1), "w_gate": ints(f, d, top=7) / 32, "w_up": ints(f, d, top=7) / 32,
+         "w_down": ints(d, f, top=7) / 32, "b_gate": ints(f, top=7) / 32, "b_up": ints(f, top=7) / 32,
+         "b_down": ints(d, top=7) / 32}
+    for k, v in t.items():
+        v.requires_grad_(k not in frozen)
+    y = gated_ffn(t["x"], t["w_gate"], t["w_up"], t["w_down"], b_gate=t["b_gate"], b_up=t["b_up"], b_down=t["b_down"])
+    dout = ints(n, d, top=3) / 4
+    names = [k for k in ("b_gate", "b_up", "b_down") if k not in frozen]
+    grads = torch.autograd.grad(y, [t[k] for k in names], dout)
+    q = {k: v.detach().double() for k, v in t.items()}
+    a, b, da = q["x"] @ q["w_gate"].t() + q["b_gate"], q["x"] @ q["w_up"].t() + q["b_up"], dout.double() @ q["w_down"]
+    s = torch.sigmoid(a)
+    terms = {"b_gate": da * b * s * (1 + a * (1 - s)), "b_up": da * a * s, "b_down": dout.double()}
+    for k, got in zip(names, grads):
+        want = terms[k].sum(0)
+        ref.check(got, (want, ref.rounded(want, 2.0 ** -18 * terms[k].abs().sum(0), dtype)), k)
+
+
+# ---------------------------------------------------------------------------
 # captured, and from several threads
 # ---------------------------------------------------------------------------
 def captured(step):
